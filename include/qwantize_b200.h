@@ -273,6 +273,40 @@ QZ_API int qz_output_error_sums(const uint16_t* X, int64_t T, int64_t K, const u
                          const uint16_t* W_dq, int64_t M, double* sums, void* stream);
 
 /*
+ * qz_fp4_scale_layout -- the scale bytes (N, K / bs) of a packed FP4 weight in
+ * the order that the block-scaled tensor cores read (once per weight, for
+ * qz_fp4_linear).  format QZ_FMT_NVFP4 (bs = 16) or QZ_FMT_MXFP4 (bs = 32);
+ * out has qz_fp4_scale_layout_bytes bytes, 16-byte aligned.  No counterpart in the reference, which keeps fp32 results only.
+ */
+QZ_API int qz_fp4_scale_layout_bytes(int64_t N, int64_t K, int format, int64_t* bytes);
+QZ_API int qz_fp4_scale_layout(const uint8_t* scale_codes, int64_t N, int64_t K, int format, uint8_t* out,
+                               void* stream);
+
+/*
+ * qz_fp4_linear -- out = x W^T (+ bias), W (N, K) in packed FP4 and each row of
+ * x (T, K) quantized to the same format on the way in; products on the
+ * block-scaled tensor cores, fp32 accumulation, one rounding to out_dtype.  No
+ * counterpart in the reference, whose quantized weights are only dequantized.
+ *   x            rows ldx elements apart, 16-byte aligned.  A row is quantized
+ *                by the naive rule of qz_quantize; for NVFP4 after division by
+ *                the smallest power of two p with max|row| <= 448 * 6 * p.
+ *   packed       N rows of up(K, 32) / 2 bytes, ldp bytes apart (a multiple of
+ *                16; codes beyond K zero); element 2i in the low nibble
+ *   scales       from qz_fp4_scale_layout
+ *   tensor_scale W is tensor_scale times the value of its codes and scales
+ *   bias         N elements of bias_dtype, or NULL
+ *   out          rows ldo elements apart
+ *   workspace    qz_fp4_linear_workspace bytes (for the current device),
+ *                256-byte aligned, not shared by calls that can overlap
+ * A row with an infinity or NaN gives NaN (MXFP4: NaN or infinities).
+ */
+QZ_API int qz_fp4_linear_workspace(int64_t T, int64_t K, int64_t N, int format, int64_t* bytes);
+QZ_API int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T, int64_t K, int64_t N, int format,
+                         const uint8_t* packed, int64_t ldp, const uint8_t* scales, float tensor_scale,
+                         const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
  * qz_poll_device_error -- reads (and with clear != 0 resets) the flags that
  * bounded device-side waits set when they give up (bit 0: bulk-load wait,
  * bit 1: tensor-core pipeline wait, bit 2: epilogue wait).  Synchronous.

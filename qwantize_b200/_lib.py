@@ -27,7 +27,8 @@ EXPORTS = [
     "qz_weight_error_sums", "qz_output_error_sums", "qz_scale_table", "qz_last_error",
     "qz_version", "qz_device_ok", "qz_poll_device_error", "qz_gram_full_noalloc", "qz_admm",
     "qz_quantize_table", "qz_selftest_wait", "qz_quantize_grouped", "qz_gptq", "qz_spd_inverse",
-    "qz_gram_unpack",
+    "qz_gram_unpack", "qz_fp4_scale_layout_bytes", "qz_fp4_scale_layout", "qz_fp4_linear_workspace",
+    "qz_fp4_linear",
 ]
 
 
@@ -71,10 +72,13 @@ def load():
     L.qz_spd_inverse.argtypes = [vp, i64, vp, vp, vp]
     L.qz_gram_unpack.argtypes = [vp, i64, vp, vp]
     L.qz_gptq.argtypes = [vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp, vp, vp]
-    L.qz_last_error.restype = ctypes.c_char_p
+    L.qz_fp4_scale_layout_bytes.argtypes = [i64, i64, i32, vp]
+    L.qz_fp4_scale_layout.argtypes = [vp, i64, i64, i32, vp, vp]
+    L.qz_fp4_linear_workspace.argtypes = [i64, i64, i64, i32, vp]
+    L.qz_fp4_linear.argtypes = [vp, i32, i64, i64, i64, i64, i32, vp, i64, vp, ctypes.c_float, vp, i32, vp, i32, i64,
+                                vp, i64, vp]
     for name in EXPORTS:
-        if name not in ("qz_last_error",):
-            getattr(L, name).restype = ctypes.c_int
+        getattr(L, name).restype = ctypes.c_int
     L.qz_last_error.restype = ctypes.c_char_p
     _lib = L
     return L

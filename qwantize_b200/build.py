@@ -29,6 +29,7 @@ UNITS = {
     "qz_quantize.cu": ["-fmad=false"],
     "qz_elementwise.cu": ["-fmad=false"],
     "qz_int.cu": ["-fmad=false"],
+    "qz_linear.cu": ["-fmad=false"],
     "qz_abi.cu": [],
     "qz_gemm.cu": [],
 }

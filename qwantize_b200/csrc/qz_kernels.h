@@ -95,5 +95,6 @@ cudaError_t launch_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 cudaError_t read_device_error_quantize(unsigned* out, bool clear);
 cudaError_t read_device_error_gemm(unsigned* out, bool clear);
 cudaError_t read_device_error_int(unsigned* out, bool clear);
+cudaError_t read_device_error_linear(unsigned* out, bool clear);
 
 }  // namespace qz
