@@ -307,6 +307,38 @@ QZ_API int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T, int
                          int64_t workspace_bytes, void* stream);
 
 /*
+ * qz_moe_layout -- the packed FP4 weights of E experts, (E, rows, K) with scale
+ * codes (E, rows, K / bs) and nibbles (E, rows, K / 2), in the order qz_moe reads
+ * (once per weight; rows and K multiples of 32).  gate_up != 0: rows are the
+ * gate rows, then as many up rows.  codes_out: E * rows * up(K, 64) / 2 bytes,
+ * scales_out: E * rows * up(K, 64) / bs bytes, both 16-byte aligned.
+ */
+QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int64_t E, int64_t rows, int64_t K,
+                         int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, void* stream);
+
+/*
+ * qz_moe -- a mixture-of-experts layer for at most 64 tokens: router logits
+ * x R^T in fp32, the top_k largest per token (ties: lowest index), the softmax
+ * over them (renormalize != 0) or over all experts as weights c, and
+ * out = sum c * D_e (silu(G_e x) * (U_e x)), fp32 sums, one rounding to x's type.
+ *   x        (T, H) bf16 or fp16, rows ldx elements apart, 16-byte aligned
+ *   router   (E, H) fp32, bf16 or fp16;  E <= 512, top_k <= 16
+ *   *_codes, *_scales, *_tensor_scale: from qz_moe_layout; gate / up (2 I, H) and
+ *            down (H, I), I and H multiples of 32
+ *   out      (T, H) of x's type;  ids (T, top_k) and weights (T, top_k): the
+ *            routing, descending logits (NULL: not written)
+ *   workspace  qz_moe_workspace bytes, 256-byte aligned, not shared by calls
+ *            that can overlap
+ * The second launch is cooperative: it needs the whole GPU's SMs to become free.
+ */
+QZ_API int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k, int64_t* bytes);
+QZ_API int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k,
+                  int renormalize, const void* router, int router_dtype, int format, const uint8_t* up_codes,
+                  const uint8_t* up_scales, float up_tensor_scale, const uint8_t* down_codes,
+                  const uint8_t* down_scales, float down_tensor_scale, void* out, int* ids, float* weights,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * qz_poll_device_error -- reads (and with clear != 0 resets) the flags that
  * bounded device-side waits set when they give up (bit 0: bulk-load wait,
  * bit 1: tensor-core pipeline wait, bit 2: epilogue wait).  Synchronous.

@@ -10,6 +10,7 @@ from .fp4 import fp4_unpack
 from .int8 import int8_dequantize, int8_naive, int8_optimal, int8_optimal_hessian, int8_quantize_packed
 from .linear import FP4Weight, fp4_linear
 from .metrics import compute_metrics
+from .moe import FP4Experts, fp4_moe
 from .mxfp4 import (mxfp4_dequantize, mxfp4_dequantize_packed, mxfp4_naive, mxfp4_naive_torch,
                     mxfp4_naive_triton, mxfp4_optimal, mxfp4_optimal_hessian, mxfp4_optimal_torch,
                     mxfp4_optimal_triton, mxfp4_quantize_packed)

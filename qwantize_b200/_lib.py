@@ -28,7 +28,7 @@ EXPORTS = [
     "qz_version", "qz_device_ok", "qz_poll_device_error", "qz_gram_full_noalloc", "qz_admm",
     "qz_quantize_table", "qz_selftest_wait", "qz_quantize_grouped", "qz_gptq", "qz_spd_inverse",
     "qz_gram_unpack", "qz_fp4_scale_layout_bytes", "qz_fp4_scale_layout", "qz_fp4_linear_workspace",
-    "qz_fp4_linear",
+    "qz_fp4_linear", "qz_moe_layout", "qz_moe_workspace", "qz_moe",
 ]
 
 
@@ -77,6 +77,11 @@ def load():
     L.qz_fp4_linear_workspace.argtypes = [i64, i64, i64, i32, vp]
     L.qz_fp4_linear.argtypes = [vp, i32, i64, i64, i64, i64, i32, vp, i64, vp, ctypes.c_float, vp, i32, vp, i32, i64,
                                 vp, i64, vp]
+    f32 = ctypes.c_float
+    L.qz_moe_layout.argtypes = [vp, vp, i64, i64, i64, i32, i32, vp, vp, vp]
+    L.qz_moe_workspace.argtypes = [i64, i64, i64, i64, i64, vp]
+    L.qz_moe.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, i32, i32, vp, vp, f32, vp, vp, f32, vp, vp,
+                         vp, vp, i64, vp]
     for name in EXPORTS:
         getattr(L, name).restype = ctypes.c_int
     L.qz_last_error.restype = ctypes.c_char_p

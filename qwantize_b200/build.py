@@ -30,6 +30,7 @@ UNITS = {
     "qz_elementwise.cu": ["-fmad=false"],
     "qz_int.cu": ["-fmad=false"],
     "qz_linear.cu": ["-fmad=false"],
+    "qz_moe.cu": [],
     "qz_abi.cu": [],
     "qz_gemm.cu": [],
 }
