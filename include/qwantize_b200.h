@@ -339,6 +339,59 @@ QZ_API int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t H, i
                   void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * Paged key / value cache in 8 bits.  Pages of 64 tokens; k and v hold
+ * (num_pages, Hkv) blocks of 64 * D bytes, k_scale and v_scale one fp32 scale for
+ * each block (a value is code * scale); D is 64 or 128.  Inside a block, key
+ * token n = 16 t + 2 j + e, value d at byte ((j * D/64 + d/64) * 8 + 2 t + e) * 64 +
+ * d % 64 (t < 4, j < 8, e < 2), value token n, value d at byte 64 d + n.
+ * table (B, max_pages): the page of each sequence's tokens 64 i .. 64 i + 63 (rows
+ * ld_table apart); an entry outside [0, num_pages) is skipped.  No counterpart in
+ * the reference.
+ */
+#define QZ_KV_INT8 0
+#define QZ_KV_E4M3 1
+
+/*
+ * qz_kv_append -- new tokens at positions lengths[b], lengths[b] + 1, ... of each
+ * sequence.  new_k, new_v: N tokens (Hkv, D) of dtype (bf16, fp16), strides
+ * in elements, rows 16-byte aligned; sequence b takes tokens cu_new[b] ..
+ * cu_new[b + 1] - 1 (at most max_new of them are written), or token b if cu_new is
+ * NULL (N = B).  A page's scale becomes max(scale, max|new| * r), r = 1 / 127 (E4M3:
+ * 1 / 448) rounded to fp32; the codes of its older tokens are rescaled if it grew (a page without older
+ * tokens starts from scale 0), slots behind the last token are zeroed.  A value
+ * that is not finite makes the page's scale NaN.  Pages written must belong to
+ * one sequence each; lengths is not changed.
+ */
+QZ_API int qz_kv_append(uint8_t* k, float* k_scale, uint8_t* v, float* v_scale, int kv_dtype, int64_t num_pages,
+                        int64_t Hkv, int64_t D, const void* new_k, int64_t k_tok, int64_t k_head, const void* new_v,
+                        int64_t v_tok, int64_t v_head, int dtype, int64_t N, const int* table, int64_t ld_table,
+                        int64_t max_pages, const int* lengths, const int* cu_new, int64_t max_new, int64_t B,
+                        void* stream);
+
+/*
+ * qz_kv_read -- the values of n pages, out_k and out_v (n, Hkv, 64, D) of
+ * out_dtype (either may be NULL); NaN for an entry outside [0, num_pages).
+ */
+QZ_API int qz_kv_read(const uint8_t* k, const float* k_scale, const uint8_t* v, const float* v_scale, int kv_dtype,
+                      int64_t num_pages, int64_t Hkv, int64_t D, const int* pages, int64_t n, void* out_k,
+                      void* out_v, int out_dtype, void* stream);
+
+/*
+ * qz_kv_attention -- out (B, Hq, D) = softmax(scale q k^T) v over the first
+ * lengths[b] tokens of each sequence (at most 64 * max_pages; zeros for none), Hq /
+ * Hkv query heads sharing one cache head.  q (B, Hq, D) bf16 or fp16, strides
+ * in elements, rows 16-byte aligned; out of q's type, contiguous.  B <= 4096.
+ * workspace: qz_kv_attention_workspace bytes, 16-byte aligned, not shared by
+ * calls that can overlap.
+ */
+QZ_API int qz_kv_attention_workspace(int64_t D, int64_t* bytes);
+QZ_API int qz_kv_attention(const uint8_t* k, const float* k_scale, const uint8_t* v, const float* v_scale, int kv_dtype,
+                           int64_t num_pages, int64_t Hkv, int64_t D, const void* q, int64_t q_seq, int64_t q_head,
+                           int dtype, int64_t B, int64_t Hq, const int* table, int64_t ld_table, int64_t max_pages,
+                           const int* lengths, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
+/*
  * qz_poll_device_error -- reads (and with clear != 0 resets) the flags that
  * bounded device-side waits set when they give up (bit 0: bulk-load wait,
  * bit 1: tensor-core pipeline wait, bit 2: epilogue wait).  Synchronous.

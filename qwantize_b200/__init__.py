@@ -8,6 +8,7 @@ bit-identical to the reference's pure-PyTorch path."""
 from .core import quantize_many
 from .fp4 import fp4_unpack
 from .int8 import int8_dequantize, int8_naive, int8_optimal, int8_optimal_hessian, int8_quantize_packed
+from .kv_cache import KVCache8, kv_cache_append, kv_cache_attention, kv_cache_read
 from .linear import FP4Weight, fp4_linear
 from .metrics import compute_metrics
 from .moe import FP4Experts, fp4_moe

@@ -19,6 +19,7 @@ DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 FMT_NVFP4, FMT_MXFP4 = 0, 1
 FMT_NVINT4, FMT_INT8 = 3, 4  # symmetric integer grids (nvint4/, int8/ of the reference)
 METHOD_NAIVE, METHOD_SSE, METHOD_HESSIAN, METHOD_NAIVE_ARGMIN, METHOD_TWO_ARGMIN = 0, 1, 2, 3, 4
+KV_INT8, KV_E4M3 = 0, 1
 GRAM_FULL, GRAM_BLOCKDIAG, GRAM_FULL_UPPER_TILES = 0, 1, 2
 
 # every symbol include/qwantize_b200.h declares
@@ -28,7 +29,8 @@ EXPORTS = [
     "qz_version", "qz_device_ok", "qz_poll_device_error", "qz_gram_full_noalloc", "qz_admm",
     "qz_quantize_table", "qz_selftest_wait", "qz_quantize_grouped", "qz_gptq", "qz_spd_inverse",
     "qz_gram_unpack", "qz_fp4_scale_layout_bytes", "qz_fp4_scale_layout", "qz_fp4_linear_workspace",
-    "qz_fp4_linear", "qz_moe_layout", "qz_moe_workspace", "qz_moe",
+    "qz_fp4_linear", "qz_moe_layout", "qz_moe_workspace", "qz_moe", "qz_kv_append", "qz_kv_read",
+    "qz_kv_attention_workspace", "qz_kv_attention",
 ]
 
 
@@ -82,6 +84,12 @@ def load():
     L.qz_moe_workspace.argtypes = [i64, i64, i64, i64, i64, vp]
     L.qz_moe.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, i32, i32, vp, vp, f32, vp, vp, f32, vp, vp,
                          vp, vp, i64, vp]
+    L.qz_kv_append.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, vp, i64, i64, vp,
+                               vp, i64, i64, vp]
+    L.qz_kv_read.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp, vp, i32, vp]
+    L.qz_kv_attention_workspace.argtypes = [i64, vp]
+    L.qz_kv_attention.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, i64, i32, i64, i64, vp, i64, i64, vp, f32,
+                                  vp, vp, i64, vp]
     for name in EXPORTS:
         getattr(L, name).restype = ctypes.c_int
     L.qz_last_error.restype = ctypes.c_char_p

@@ -31,6 +31,7 @@ UNITS = {
     "qz_int.cu": ["-fmad=false"],
     "qz_linear.cu": ["-fmad=false"],
     "qz_moe.cu": [],
+    "qz_kv.cu": [],
     "qz_abi.cu": [],
     "qz_gemm.cu": [],
 }

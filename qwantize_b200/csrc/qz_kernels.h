@@ -97,5 +97,6 @@ cudaError_t read_device_error_gemm(unsigned* out, bool clear);
 cudaError_t read_device_error_int(unsigned* out, bool clear);
 cudaError_t read_device_error_linear(unsigned* out, bool clear);
 cudaError_t read_device_error_moe(unsigned* out, bool clear);
+cudaError_t read_device_error_kv(unsigned* out, bool clear);
 
 }  // namespace qz

@@ -1,0 +1,791 @@
+// qz_kv.cu -- a paged key / value cache held in 8 bits (int8 or E4M3) with one
+// fp32 scale per page of 64 tokens and head: append, read back, and attention
+// of one query token per sequence over it.
+//
+//   append     s' = max(s, max|new| * fp32(1 / top)), s = 0 for a page without
+//              tokens; codes of the page's older tokens are taken over by s / s', new
+//              ones are x / s'; slots behind the last token are zero   (top = 127 / 448)
+//   attention  o_h = sum_n p_n v_n, p = softmax_n(scale q_h . k_n), the query heads
+//              of a group sharing one head of the cache
+//
+// The attention reads each code once and is bound by HBM: 2 D bytes per token and
+// head.  Layout inside a (page, head) block of 64 D bytes, so that a warp's
+// 16-byte loads are contiguous and are the B fragments of mma.m16n8k16 after an
+// exact conversion to fp16 (int8 and E4M3 both fit):
+//   keys    token n = 16 t + 2 j + e, value d at ((j D/64 + d/64) 8 + 2 t + e) 64 + d % 64
+//   values  transposed: token n, value d at 64 d + n
+// The score fragment of 8-token tiles 2i, 2i + 1 is then the probability fragment of
+// the value product's step i, with no exchange between lanes.
+//
+// Work: the pages of all (sequence, head) pairs, in order, are cut into equal
+// runs, one per warp of the grid (lengths live on the device, so the cut is made
+// there); a warp streams its run through its own ring of bulk copies with a
+// running maximum and sum, and never waits for another warp.  A pair that one warp
+// covers is written at once; of the others each warp leaves a partial result and
+// a second kernel joins them in order.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/qwantize_b200.h"
+#include "qz_common.cuh"
+#include "qz_kernels.h"
+#include "qz_ptx.cuh"
+
+namespace qz {
+
+int fail(int code, const char* fmt, ...);
+int cuda_status(cudaError_t e, const char* what);
+int current_sms(int* sms);
+
+constexpr int kPage = 64;           // tokens per page
+constexpr int kKvInt8 = 0, kKvE4M3 = 1;
+constexpr int kKvMaxSeqs = 4096;    // sequences per attention call (their prefix sums sit in shared memory)
+
+// Byte offsets inside a (page, head) block.
+__host__ __device__ __forceinline__ int key_at(int n, int d, int D) {
+  return (((n >> 1 & 7) * (D / 64) + d / 64) * 8 + (n >> 4) * 2 + (n & 1)) * 64 + d % 64;
+}
+__host__ __device__ __forceinline__ int value_at(int n, int d) { return d * 64 + n; }
+// The token of byte `at` of a key block.
+__device__ __forceinline__ int key_token(int at, int D) {
+  const int j = at / (D * 8), g = at / 64 % 8;
+  return (g >> 1) * 16 + 2 * j + (g & 1);
+}
+
+template <int KV>
+__device__ __forceinline__ float decode8(uint32_t b) {
+  if (KV == kKvInt8) return (float)(int8_t)b;
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)b));
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xffffu)));
+}
+
+template <int KV>
+__device__ __forceinline__ uint32_t encode8(float y) {
+  if (KV == kKvInt8) return (uint32_t)(int)fminf(fmaxf(rintf(y), -127.0f), 127.0f) & 255u;
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(y));
+  return r & 255u;
+}
+
+__device__ __forceinline__ float load16(const uint16_t* p, int dtype, int64_t i) {
+  return dtype == kDtBF16 ? bf16_bits_to_float(p[i]) : f16_bits_to_float(p[i]);
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct AppendParams {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int64_t num_pages;
+  int Hkv, D, dtype;
+  const uint16_t *nk, *nv;      // new tokens: (token, head, D), strides in elements
+  int64_t k_tok, k_head, v_tok, v_head, N;
+  const int* table;             // (B, max_pages)
+  int64_t ld_table;
+  int max_pages;
+  const int* lengths;           // tokens before the append
+  const int* cu;                // (B + 1) prefix sums of the new tokens, or NULL: one per sequence
+  int64_t max_new;
+};
+
+// One CTA per (page a sequence touches, head, sequence); keys, then values.  The
+// page's block is rebuilt in shared memory and written whole.  Memory-bound for
+// prompts, one round trip for a decode step.
+template <int KV>
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  extern __shared__ __align__(16) uint8_t s_block[];  // 64 D bytes
+  __shared__ uint32_t s_max[8];
+  const int tid = threadIdx.x, D = p.D, head = blockIdx.y, b = blockIdx.z;
+  int64_t first = b, end = b + 1;
+  if (p.cu) { first = p.cu[b]; end = p.cu[b + 1]; }
+  const int64_t old = p.lengths[b];
+  if (old < 0 || first < 0 || end > p.N || end <= first) return;
+  if (end - first > p.max_new) end = first + p.max_new;
+  const int64_t blk = old / kPage + blockIdx.x;
+  if (blk >= p.max_pages) return;
+  const int64_t t0 = blk * kPage > old ? blk * kPage : old;   // position of the first new token in this page
+  int64_t t1 = old + (end - first);
+  if (t1 > (blk + 1) * kPage) t1 = (blk + 1) * kPage;
+  if (t0 >= t1) return;
+  const int64_t page = p.table[b * p.ld_table + blk];
+  if (page < 0 || page >= p.num_pages) return;
+  const int off = (int)(t0 - blk * kPage), count = (int)(t1 - t0);
+  const int64_t src = first + (t0 - old), at = page * p.Hkv + head;
+  const float per_top = KV == kKvInt8 ? 1.0f / 127.0f : 1.0f / 448.0f;  // rounded once, a constant
+  const int vecs = count * (D / 8);  // 8 values each
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const uint16_t* x = which ? p.nv + src * p.v_tok + head * p.v_head : p.nk + src * p.k_tok + head * p.k_head;
+    const int64_t tok = which ? p.v_tok : p.k_tok;
+    float* scale_p = (which ? p.vs : p.ks) + at;
+    uint8_t* block = (which ? p.v : p.k) + at * (int64_t)(kPage * D);
+    uint32_t m = 0;
+    for (int i = tid; i < vecs; i += 256) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + i / (D / 8) * tok + i % (D / 8) * 8));
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float lo = p.dtype == kDtBF16 ? bf16_bits_to_float(ww[q] & 0xffffu) : f16_bits_to_float(ww[q] & 0xffffu);
+        const float hi = p.dtype == kDtBF16 ? bf16_bits_to_float(ww[q] >> 16) : f16_bits_to_float(ww[q] >> 16);
+        m = max(m, max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu));
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    const float before = off > 0 ? *scale_p : 0.0f;
+    __syncthreads();  // the previous half's block has been written out
+    if ((tid & 31) == 0) s_max[tid >> 5] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, s_max[w]);
+    const float need = __fmul_rn(__uint_as_float(m), per_top);
+    float s = before > need ? before : need;
+    // a value that is not finite, now or earlier, leaves the page's scale NaN and its codes 0
+    const bool fine = m < 0x7f800000u && before <= 3.0e38f;
+    if (!fine) s = __uint_as_float(0x7fc00000u);
+    const float ratio = s > 0.0f ? __fdiv_rn(before, s) : 0.0f;
+    // older tokens (slots below off), zeros elsewhere
+    for (int i = tid * 16; i < kPage * D; i += 256 * 16) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (off > 0 && fine && before > 0.0f) {
+        w = *reinterpret_cast<const uint4*>(block + i);
+        uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        const int kt = key_token(i, D);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t r = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int n = which ? (i + 4 * q + c) % 64 : kt;
+            uint32_t code = ww[q] >> (8 * c) & 255u;
+            if (ratio != 1.0f) code = encode8<KV>(__fmul_rn(decode8<KV>(code), ratio));
+            if (n < off) r |= code << (8 * c);
+          }
+          ww[q] = r;
+        }
+        w = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+      }
+      *reinterpret_cast<uint4*>(s_block + i) = w;
+    }
+    __syncthreads();
+    if (fine && s > 0.0f) {
+      for (int i = tid; i < vecs; i += 256) {
+        const int n = i / (D / 8), d0 = i % (D / 8) * 8;
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + n * tok + d0));
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t h = ww[q / 2] >> (16 * (q & 1)) & 0xffffu;
+          const float f = p.dtype == kDtBF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
+          s_block[which ? value_at(off + n, d0 + q) : key_at(off + n, d0 + q, D)] = (uint8_t)encode8<KV>(__fdiv_rn(f, s));
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = tid * 16; i < kPage * D; i += 256 * 16)
+      *reinterpret_cast<uint4*>(block + i) = *reinterpret_cast<const uint4*>(s_block + i);
+    if (tid == 0) *scale_p = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+// One CTA per (page of the list, head): codes times scale, (n, Hkv, 64, D).
+template <int KV>
+__global__ void __launch_bounds__(256) kv_read_kernel(const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
+                                                      const float* __restrict__ ks, const float* __restrict__ vs,
+                                                      int64_t num_pages, int Hkv, int D, const int* __restrict__ pages,
+                                                      void* __restrict__ ok, void* __restrict__ ov, int dtype) {
+  extern __shared__ __align__(16) uint8_t s_block[];  // 68 D bytes
+  const int tid = threadIdx.x, head = blockIdx.x;
+  const int64_t n = blockIdx.y, page = pages[n];
+  const bool there = page >= 0 && page < num_pages;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    void* out = which ? ov : ok;
+    if (!out) continue;
+    const int64_t at = page * Hkv + head;
+    const uint8_t* block = (which ? v : k) + at * (int64_t)(kPage * D);
+    const float s = there ? (which ? vs : ks)[at] : __uint_as_float(0x7fc00000u);
+    __syncthreads();
+    for (int i = tid * 16; i < kPage * D; i += 256 * 16) {
+      const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(block + i)) : make_uint4(0, 0, 0, 0);
+      uint32_t* d = reinterpret_cast<uint32_t*>(s_block + (which ? i / 64 * 68 + i % 64 : i));
+      d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
+    }
+    __syncthreads();
+    const int64_t o0 = (n * Hkv + head) * kPage * D;
+    for (int i = tid * 4; i < kPage * D; i += 256 * 4) {
+      const int tkn = i / D, d = i % D;
+      float f[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        f[q] = __fmul_rn(decode8<KV>(s_block[which ? (d + q) * 68 + tkn : key_at(tkn, d + q, D)]), s);
+      if (dtype == kDtF32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + o0 + i) = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+        uint32_t a, c;
+        if (dtype == kDtBF16) {
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(f[1]), "f"(f[0]));
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(c) : "f"(f[3]), "f"(f[2]));
+        } else {
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(f[1]), "f"(f[0]));
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(c) : "f"(f[3]), "f"(f[2]));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o0 + i) = make_uint2(a, c);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+struct AttnParams {
+  const uint8_t *k, *v;
+  const float *ks, *vs;
+  int64_t num_pages;
+  int B, Hkv, G, row_tiles;      // G query heads per cache head, in row_tiles tiles of 16
+  const uint16_t* q;             // (B, Hkv * G, D), strides in elements
+  int64_t q_seq, q_head;
+  int dtype;
+  const int* table;
+  int64_t ld_table;
+  int max_pages;
+  const int* lengths;
+  float scale_log2;              // softmax scale * log2(e)
+  float* part_o;                 // (warps, 2, 16, D) partial sums
+  float* part_ml;                // (warps, 2, 16, 2) maximum (base 2) and sum
+  void* out;                     // (B, Hkv * G, D), contiguous
+};
+
+__device__ __forceinline__ int pages_of(const AttnParams& p, int b) {
+  const int len = p.lengths[b];
+  if (len <= 0) return 0;
+  const int nb = (len + kPage - 1) / kPage;
+  return nb < p.max_pages ? nb : p.max_pages;
+}
+
+// prefix[b] = pages of the sequences before b, b = 0 .. B (all threads of the CTA)
+__device__ __forceinline__ void page_prefix(const AttnParams& p, int* prefix) {
+  if (threadIdx.x < 32) {
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + threadIdx.x;
+      int n = b < p.B ? pages_of(p, b) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int m = __shfl_up_sync(0xffffffffu, n, o);
+        if ((int)threadIdx.x >= o) n += m;
+      }
+      if (b < p.B) prefix[b + 1] = base + n;
+      base += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (threadIdx.x == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+}
+
+template <int KV>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (KV == kKvInt8) {
+    // 0x6400 | (code + 128) is 1024 + code + 128 in fp16
+    w ^= 0x80808080u;
+    lo = __byte_perm(w, 0x64646464u, 0x4140);
+    hi = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), c), b = __hsub2(*reinterpret_cast<__half2*>(&hi), c);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+  } else {
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D>
+struct AttnGeo {
+  static constexpr int kBlock = kPage * D;               // bytes of keys (or values) of one page and head
+  static constexpr int kWarps = D == 128 ? 6 : 8;
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kRing = kWarps * kStages * 2 * kBlock;
+  static int smem(int B) { return kRing + kWarps * kStages * 2 * 8 + (B + 1) * 4; }
+};
+
+template <int D, int KV>
+__global__ void __launch_bounds__(AttnGeo<D>::kWarps * 32, 1) kv_attention_kernel(const __grid_constant__ AttnParams p) {
+  using G = AttnGeo<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kRing) + warp * G::kStages * 2;  // keys, values per stage
+  int* prefix = reinterpret_cast<int*>(smem + G::kRing + G::kWarps * G::kStages * 16);
+  uint8_t* ring = smem + warp * G::kStages * 2 * G::kBlock;
+  if (lane == 0) {
+    for (int i = 0; i < G::kStages * 2; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  page_prefix(p, prefix);
+  const int HR = p.Hkv * p.row_tiles;
+  const int64_t total = (int64_t)prefix[p.B] * HR, warps = (int64_t)gridDim.x * G::kWarps;
+  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours in work on different SMs
+  const int64_t u0 = me * total / warps, u1 = (me + 1) * total / warps;
+  if (u0 >= u1) return;
+
+  // position in the work list: sequence b, head and row tile hr, page pg of nb
+  struct Pos { int b, hr, pg, nb; };
+  auto locate = [&](int64_t u) {
+    int lo = 0, hi = p.B;  // last b with prefix[b] * HR <= u
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)prefix[mid] * HR <= u) lo = mid; else hi = mid;
+    }
+    Pos x;
+    x.b = lo;
+    x.nb = prefix[lo + 1] - prefix[lo];
+    const int64_t r = u - (int64_t)prefix[lo] * HR;
+    x.hr = (int)(r / x.nb);
+    x.pg = (int)(r % x.nb);
+    return x;
+  };
+  auto advance = [&](Pos& x) {
+    if (++x.pg < x.nb) return;
+    x.pg = 0;
+    if (++x.hr < HR) return;
+    x.hr = 0;
+    do ++x.b; while (x.b < p.B && prefix[x.b + 1] == prefix[x.b]);
+    x.nb = x.b < p.B ? prefix[x.b + 1] - prefix[x.b] : 1;
+  };
+  auto issue = [&](const Pos& x, int stage) {  // lane 0
+    const int64_t page = p.table[(int64_t)x.b * p.ld_table + x.pg];
+    uint64_t* bk = bars + stage * 2;
+    if (page < 0 || page >= p.num_pages) {  // no such page: nothing is read, its tokens are masked
+      mbar_arrive(bk);
+      mbar_arrive(bk + 1);
+      return;
+    }
+    const int64_t at = (page * p.Hkv + x.hr / p.row_tiles) * (int64_t)G::kBlock;
+    mbar_arrive_expect_tx(bk, G::kBlock);
+    bulk_load(ring + stage * 2 * G::kBlock, p.k + at, G::kBlock, bk);
+    mbar_arrive_expect_tx(bk + 1, G::kBlock);
+    bulk_load(ring + stage * 2 * G::kBlock + G::kBlock, p.v + at, G::kBlock, bk + 1);
+  };
+
+  Pos cur = locate(u0), ahead = cur;
+  int64_t next = u0;  // next unit to load
+  if (lane == 0)
+    for (int s = 0; s < G::kStages && next < u1; ++s, ++next) { issue(ahead, s); advance(ahead); }
+
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4];
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, qs0 = 1.0f, qs1 = 1.0f;
+  bool fresh = true;
+  int64_t seg_begin = u0;
+  bool ok = true;
+  uint32_t it = 0;
+  for (int64_t u = u0; u < u1; ++u, ++it) {
+    const int stage = it % G::kStages;
+    const uint32_t parity = it / G::kStages & 1;
+    const int head = cur.hr / p.row_tiles, r0 = cur.hr % p.row_tiles * 16;
+    if (fresh) {
+      // this pair's query rows as fp16, each on the power of two that puts its
+      // largest magnitude in [2^14, 2^15) (fp16 rows as they are)
+      fresh = false;
+      const bool h0 = r0 + g < p.G, h1 = r0 + g + 8 < p.G;
+      const uint16_t* q0 = p.q + cur.b * p.q_seq + (int64_t)(head * p.G + r0 + (h0 ? g : 0)) * p.q_head;
+      const uint16_t* q1 = p.q + cur.b * p.q_seq + (int64_t)(head * p.G + r0 + (h1 ? g + 8 : 0)) * p.q_head;
+      uint32_t raw[D / 16][4];
+      uint32_t x0 = 0, x1 = 0;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        // lane t takes values 64 h + 16 t .. + 15 of its two rows
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const uint4 a = h0 ? __ldg(reinterpret_cast<const uint4*>(q0 + 64 * h + 16 * t + 8 * v)) : make_uint4(0, 0, 0, 0);
+          const uint4 c = h1 ? __ldg(reinterpret_cast<const uint4*>(q1 + 64 * h + 16 * t + 8 * v)) : make_uint4(0, 0, 0, 0);
+          raw[4 * h + 2 * v][0] = a.x; raw[4 * h + 2 * v][2] = a.y;
+          raw[4 * h + 2 * v + 1][0] = a.z; raw[4 * h + 2 * v + 1][2] = a.w;
+          raw[4 * h + 2 * v][1] = c.x; raw[4 * h + 2 * v][3] = c.y;
+          raw[4 * h + 2 * v + 1][1] = c.z; raw[4 * h + 2 * v + 1][3] = c.w;
+        }
+      }
+      qs0 = qs1 = 1.0f;
+      if (p.dtype == kDtBF16) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t hi = raw[s][i] & 0x7fff0000u, lo = raw[s][i] << 16 & 0x7fff0000u;
+            if (i & 1) x1 = max(x1, max(hi, lo)); else x0 = max(x0, max(hi, lo));
+          }
+        x0 = max(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+        x0 = max(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+        x1 = max(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+        x1 = max(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const int e0 = x0 == 0 || x0 >= 0x7f800000u ? 0 : max((int)(x0 >> 23) - 141, -112);
+        const int e1 = x1 == 0 || x1 >= 0x7f800000u ? 0 : max((int)(x1 >> 23) - 141, -112);
+        qs0 = pow2f(e0);
+        qs1 = pow2f(e1);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float inv = pow2f(i & 1 ? -e1 : -e0);
+            const __half2 h = __floats2half2_rn(bf16_bits_to_float(raw[s][i] & 0xffffu) * inv, bf16_bits_to_float(raw[s][i] >> 16) * inv);
+            qf[s][i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qf[s][i] = raw[s][i];
+      }
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
+    }
+    const int64_t page = p.table[(int64_t)cur.b * p.ld_table + cur.pg];
+    const bool there = page >= 0 && page < p.num_pages;
+    const float ks = there ? __ldg(p.ks + page * p.Hkv + head) : 0.0f, vs = there ? __ldg(p.vs + page * p.Hkv + head) : 0.0f;
+    int valid = there ? p.lengths[cur.b] - cur.pg * kPage : 0;
+    if (valid > kPage) valid = kPage;
+    const uint8_t* sk = ring + stage * 2 * G::kBlock + lane * 16;
+    const uint8_t* sv = sk + G::kBlock;
+    if (!mbar_wait_bounded(bars + stage * 2, parity, kDevErrLoadTimeout)) { ok = false; break; }
+    // scores of 64 tokens: 8 tiles of 8
+    float s[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[j][c] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        const uint4 w = *reinterpret_cast<const uint4*>(sk + (j * (D / 64) + h) * 512);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t b0, b1;
+          codes_to_f16<KV>(ww[q], b0, b1);
+          mma_16816(s[j], qf[4 * h + q], b0, b1);
+        }
+      }
+    }
+    const float f0 = ks * qs0 * p.scale_log2, f1 = ks * qs1 * p.scale_log2;
+    float n0 = m0, n1 = m1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[j][c] *= c < 2 ? f0 : f1;
+        if (valid < kPage && 16 * t + 2 * j + (c & 1) >= valid) s[j][c] = -INFINITY;
+      }
+      n0 = fmaxf(n0, fmaxf(s[j][0], s[j][1]));
+      n1 = fmaxf(n1, fmaxf(s[j][2], s[j][3]));
+    }
+    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+    const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;  // nothing unmasked yet
+    const float c0 = exp2f(m0 - z0), c1 = exp2f(m1 - z1);
+    m0 = n0;
+    m1 = n1;
+    float a0 = 0.0f, a1 = 0.0f;
+    uint32_t pf[4][4];  // probabilities, fp16: the A fragments of the value product
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[j][c] = exp2f(s[j][c] - (c < 2 ? z0 : z1));
+      a0 += s[j][0] + s[j][1];
+      a1 += s[j][2] + s[j][3];
+      const __half2 x = __floats2half2_rn(s[j][0], s[j][1]), y = __floats2half2_rn(s[j][2], s[j][3]);
+      pf[j >> 1][(j & 1) * 2] = *reinterpret_cast<const uint32_t*>(&x);
+      pf[j >> 1][(j & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    l0 = fmaf(l0, c0, a0);
+    l1 = fmaf(l1, c1, a1);
+    if (!mbar_wait_bounded(bars + stage * 2 + 1, parity, kDevErrLoadTimeout)) { ok = false; break; }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      uint4 w = *reinterpret_cast<const uint4*>(sv + i * 512);
+      uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (valid < kPage) {  // what lies behind the last token may decode to NaN
+          const int left = valid - (16 * t + 4 * q);
+          ww[q] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        }
+        uint32_t b0, b1;
+        codes_to_f16<KV>(ww[q], b0, b1);
+        mma_16816(d, pf[q], b0, b1);
+      }
+      o[i][0] = fmaf(d[0], vs, o[i][0] * c0);
+      o[i][1] = fmaf(d[1], vs, o[i][1] * c0);
+      o[i][2] = fmaf(d[2], vs, o[i][2] * c1);
+      o[i][3] = fmaf(d[3], vs, o[i][3] * c1);
+    }
+    __syncwarp();
+    if (lane == 0 && next < u1) {
+      issue(ahead, stage);
+      advance(ahead);
+      ++next;
+    }
+    const bool pair_ends = cur.pg + 1 == cur.nb;
+    if (pair_ends || u + 1 == u1) {
+      // the sums of a row lie in its four lanes
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      const bool whole = pair_ends && u + 1 - seg_begin == cur.nb;
+      const bool h0 = r0 + g < p.G, h1 = r0 + g + 8 < p.G;
+      if (whole) {
+        const float i0 = l0 > 0.0f ? 1.0f / l0 : (l0 == 0.0f ? 0.0f : l0), i1 = l1 > 0.0f ? 1.0f / l1 : (l1 == 0.0f ? 0.0f : l1);
+        uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)cur.b * p.Hkv + head) * p.G * D;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t x, y;
+          if (p.dtype == kDtBF16) {
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(o[i][1] * i0), "f"(o[i][0] * i0));
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(o[i][3] * i1), "f"(o[i][2] * i1));
+          } else {
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(o[i][1] * i0), "f"(o[i][0] * i0));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(o[i][3] * i1), "f"(o[i][2] * i1));
+          }
+          if (h0) *reinterpret_cast<uint32_t*>(out + (int64_t)(r0 + g) * D + 8 * i + 2 * t) = x;
+          if (h1) *reinterpret_cast<uint32_t*>(out + (int64_t)(r0 + g + 8) * D + 8 * i + 2 * t) = y;
+        }
+      } else {
+        const int64_t slot = me * 2 + (seg_begin == u0 ? 0 : 1);
+        float* po = p.part_o + slot * 16 * D;
+        float* ml = p.part_ml + slot * 32;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          if (h0) *reinterpret_cast<float2*>(po + g * D + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
+          if (h1) *reinterpret_cast<float2*>(po + (g + 8) * D + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
+        }
+        if (t == 0) {
+          ml[g * 2] = m0;
+          ml[g * 2 + 1] = l0;
+          ml[g * 2 + 16] = m1;
+          ml[g * 2 + 17] = l1;
+        }
+      }
+      fresh = true;
+      seg_begin = u + 1;
+    }
+    advance(cur);
+  }
+  if (!ok) {
+    // copies in flight must land before the CTA exits (bounded)
+    for (int i = 0; i < G::kStages * 2; ++i) {
+      const uint32_t k = it + (i / 2 + G::kStages - it % G::kStages) % G::kStages;  // the last unit loaded into stage i / 2
+      if (u0 + k < u1) mbar_wait_bounded(bars + i, k / G::kStages & 1, kDevErrLoadTimeout);
+    }
+  }
+}
+
+// Joins the partial results of the (sequence, head, row tile) pairs that several
+// warps share, in the order of their pages; writes zeros for empty sequences.
+// One CTA per query row.
+template <int D>
+__global__ void __launch_bounds__(D) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps, int attn_warps) {
+  extern __shared__ int prefix[];
+  const int HR = p.Hkv * p.row_tiles;
+  const int row = blockIdx.x % p.G, bh = blockIdx.x / p.G, head = bh % p.Hkv, b = bh / p.Hkv, d = threadIdx.x;
+  page_prefix(p, prefix);
+  const int64_t total = (int64_t)prefix[p.B] * HR;
+  const int nb = prefix[b + 1] - prefix[b], hr = head * p.row_tiles + row / 16;
+  float v = 0.0f;
+  if (nb > 0) {
+    const int64_t u0 = (int64_t)prefix[b] * HR + (int64_t)hr * nb, u1 = u0 + nb;
+    // the warp of unit u: the last w with w * total / warps <= u
+    const int64_t w0 = ((u0 + 1) * warps - 1) / total, w1 = (u1 * warps - 1) / total;
+    if (w0 == w1) return;  // one warp had all of it
+    float m = -INFINITY, l = 0.0f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t begin = w * total / warps;
+      if (begin == (w + 1) * total / warps) continue;  // more warps than units
+      const int64_t slot = w * 2 + (begin >= u0 ? 0 : 1);
+      const float mw = __ldg(p.part_ml + slot * 32 + row % 16 * 2), lw = __ldg(p.part_ml + slot * 32 + row % 16 * 2 + 1);
+      const float ow = __ldg(p.part_o + slot * 16 * D + row % 16 * D + d);
+      const float n = fmaxf(m, mw), z = n == -INFINITY ? 0.0f : n;
+      const float c = exp2f(m - z), cw = exp2f(mw - z);
+      v = v * c + ow * cw;
+      l = l * c + lw * cw;
+      m = n;
+    }
+    v = l > 0.0f ? v / l : (l == 0.0f ? 0.0f : l);
+  }
+  const int64_t at = ((int64_t)bh * p.G + row) * D + d;
+  uint16_t r;
+  if (p.dtype == kDtBF16) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+  else r = __half_as_ushort(__float2half_rn(v));
+  static_cast<uint16_t*>(p.out)[at] = r;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+cudaError_t read_device_error_kv(unsigned* out, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, qz_device_error, sizeof(unsigned));
+  if (e != cudaSuccess || !clear) return e;
+  unsigned zero = 0;
+  return cudaMemcpyToSymbol(qz_device_error, &zero, sizeof(unsigned));
+}
+
+static int check_cache(int kv_dtype, int64_t num_pages, int64_t Hkv, int64_t D) {
+  if (kv_dtype != QZ_KV_INT8 && kv_dtype != QZ_KV_E4M3) return fail(QZ_ERR_INVALID, "unknown cache type %d", kv_dtype);
+  if (D != 64 && D != 128) return fail(QZ_ERR_INVALID, "head dimension %lld, expected 64 or 128", (long long)D);
+  if (Hkv < 1 || Hkv > 1024) return fail(QZ_ERR_INVALID, "%lld cache heads, expected 1 to 1024", (long long)Hkv);
+  if (num_pages < 0 || num_pages > 2147483647LL) return fail(QZ_ERR_INVALID, "num_pages must fit in int32");
+  return QZ_OK;
+}
+
+static bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+template <int D, int KV>
+static int launch_attention(const AttnParams& p, int sms, cudaStream_t st) {
+  using G = AttnGeo<D>;
+  static int attr_smem[64] = {0};  // per device (a benign race: the value only grows and is set again if it was lost)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
+  const int smem = G::smem(p.B), most = G::smem(kKvMaxSeqs);
+  if (dev < 0 || dev >= 64 || attr_smem[dev] == 0) {
+    e = cudaFuncSetAttribute(kv_attention_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
+    if (dev >= 0 && dev < 64) attr_smem[dev] = most;
+  }
+  kv_attention_kernel<D, KV><<<sms, G::kWarps * 32, smem, st>>>(p);
+  int s = cuda_status(cudaGetLastError(), "kv attention launch");
+  if (s != QZ_OK) return s;
+  kv_join_kernel<D><<<(unsigned)((int64_t)p.B * p.Hkv * p.G), D, (p.B + 1) * 4, st>>>(p, (int64_t)sms * G::kWarps, G::kWarps);
+  return cuda_status(cudaGetLastError(), "kv join launch");
+}
+
+}  // namespace qz
+
+using namespace qz;
+
+extern "C" int qz_kv_append(uint8_t* k, float* k_scale, uint8_t* v, float* v_scale, int kv_dtype, int64_t num_pages,
+                            int64_t Hkv, int64_t D, const void* new_k, int64_t k_tok, int64_t k_head, const void* new_v,
+                            int64_t v_tok, int64_t v_head, int dtype, int64_t N, const int* table, int64_t ld_table,
+                            int64_t max_pages, const int* lengths, const int* cu_new, int64_t max_new, int64_t B,
+                            void* stream) {
+  int s = check_cache(kv_dtype, num_pages, Hkv, D);
+  if (s != QZ_OK) return s;
+  if (dtype != QZ_DTYPE_BF16 && dtype != QZ_DTYPE_F16) return fail(QZ_ERR_INVALID, "new tokens must be bf16 or fp16, got dtype %d", dtype);
+  if (B < 0 || B > 65535 || N < 0 || N > 2147483647LL || max_new < 0 || max_pages < 0 || max_pages > 2147483647LL || ld_table < max_pages)
+    return fail(QZ_ERR_INVALID, "need 0 <= B <= 65535, 0 <= N < 2^31, max_new >= 0 and table rows of max_pages");
+  if (!cu_new && N != B) return fail(QZ_ERR_INVALID, "without cu_new there is one new token per sequence: N=%lld, B=%lld", (long long)N, (long long)B);
+  if (B == 0 || N == 0 || max_new == 0 || max_pages == 0) return QZ_OK;
+  if (!k || !v || !k_scale || !v_scale || !new_k || !new_v || !table || !lengths) return fail(QZ_ERR_INVALID, "NULL pointer");
+  if (off16(k) || off16(v) || off16(new_k) || off16(new_v) || k_tok % 8 || k_head % 8 || v_tok % 8 || v_head % 8)
+    return fail(QZ_ERR_INVALID, "caches and rows of new tokens must be 16-byte aligned");
+  int sms = 0;
+  if ((s = current_sms(&sms)) != QZ_OK) return s;
+  // a run of max_new tokens touches at most this many pages, wherever it starts
+  int64_t touched = (max_new + kPage - 2) / kPage + 1;
+  if (touched > max_pages) touched = max_pages;
+  AppendParams p{k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, dtype, static_cast<const uint16_t*>(new_k),
+                 static_cast<const uint16_t*>(new_v), k_tok, k_head, v_tok, v_head, N, table, ld_table, (int)max_pages,
+                 lengths, cu_new, max_new};
+  const dim3 grid((unsigned)touched, (unsigned)Hkv, (unsigned)B);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv_dtype == QZ_KV_INT8) kv_append_kernel<kKvInt8><<<grid, 256, kPage * D, st>>>(p);
+  else kv_append_kernel<kKvE4M3><<<grid, 256, kPage * D, st>>>(p);
+  return cuda_status(cudaGetLastError(), "kv append launch");
+}
+
+extern "C" int qz_kv_read(const uint8_t* k, const float* k_scale, const uint8_t* v, const float* v_scale, int kv_dtype,
+                          int64_t num_pages, int64_t Hkv, int64_t D, const int* pages, int64_t n, void* out_k,
+                          void* out_v, int out_dtype, void* stream) {
+  int s = check_cache(kv_dtype, num_pages, Hkv, D);
+  if (s != QZ_OK) return s;
+  if (out_dtype != QZ_DTYPE_F32 && out_dtype != QZ_DTYPE_BF16 && out_dtype != QZ_DTYPE_F16)
+    return fail(QZ_ERR_INVALID, "unknown dtype %d", out_dtype);
+  if (n < 0) return fail(QZ_ERR_INVALID, "n must be >= 0");
+  if (n == 0) return QZ_OK;
+  if (!k || !v || !k_scale || !v_scale || !pages) return fail(QZ_ERR_INVALID, "NULL pointer");
+  if (off16(k) || off16(v) || off16(out_k) || off16(out_v)) return fail(QZ_ERR_INVALID, "caches and outputs must be 16-byte aligned");
+  int sms = 0;
+  if ((s = current_sms(&sms)) != QZ_OK) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t out_page = (size_t)Hkv * kPage * D * (out_dtype == QZ_DTYPE_F32 ? 4 : 2);
+  for (int64_t n0 = 0; n0 < n; n0 += 65535) {  // the grid's y dimension
+    const unsigned ny = (unsigned)(n - n0 < 65535 ? n - n0 : 65535);
+    uint8_t *ok = out_k ? static_cast<uint8_t*>(out_k) + n0 * out_page : nullptr, *ov = out_v ? static_cast<uint8_t*>(out_v) + n0 * out_page : nullptr;
+    const dim3 grid((unsigned)Hkv, ny);
+    if (kv_dtype == QZ_KV_INT8)
+      kv_read_kernel<kKvInt8><<<grid, 256, 68 * D, st>>>(k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, pages + n0, ok, ov, out_dtype);
+    else
+      kv_read_kernel<kKvE4M3><<<grid, 256, 68 * D, st>>>(k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, pages + n0, ok, ov, out_dtype);
+    s = cuda_status(cudaGetLastError(), "kv read launch");
+    if (s != QZ_OK) return s;
+  }
+  return QZ_OK;
+}
+
+extern "C" int qz_kv_attention_workspace(int64_t D, int64_t* bytes) {
+  int sms = 0;
+  const int s = check_cache(QZ_KV_INT8, 0, 1, D);
+  if (s != QZ_OK) return s;
+  if (!bytes) return fail(QZ_ERR_INVALID, "NULL pointer");
+  const int r = current_sms(&sms);
+  if (r != QZ_OK) return r;
+  const int64_t warps = (int64_t)sms * (D == 128 ? AttnGeo<128>::kWarps : AttnGeo<64>::kWarps);
+  *bytes = warps * 2 * (16 * D + 32) * 4;
+  return QZ_OK;
+}
+
+extern "C" int qz_kv_attention(const uint8_t* k, const float* k_scale, const uint8_t* v, const float* v_scale, int kv_dtype,
+                               int64_t num_pages, int64_t Hkv, int64_t D, const void* q, int64_t q_seq, int64_t q_head,
+                               int dtype, int64_t B, int64_t Hq, const int* table, int64_t ld_table, int64_t max_pages,
+                               const int* lengths, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  int s = check_cache(kv_dtype, num_pages, Hkv, D);
+  if (s != QZ_OK) return s;
+  if (dtype != QZ_DTYPE_BF16 && dtype != QZ_DTYPE_F16) return fail(QZ_ERR_INVALID, "q must be bf16 or fp16, got dtype %d", dtype);
+  if (Hq < 1 || Hq % Hkv || Hq > 65536) return fail(QZ_ERR_INVALID, "%lld query heads are not a multiple of %lld cache heads", (long long)Hq, (long long)Hkv);
+  if (B < 0 || B > kKvMaxSeqs) return fail(QZ_ERR_INVALID, "%lld sequences, expected at most %d", (long long)B, kKvMaxSeqs);
+  if (max_pages < 0 || ld_table < max_pages || max_pages * (B ? B : 1) > 2147483647LL)
+    return fail(QZ_ERR_INVALID, "need table rows of max_pages entries, B * max_pages < 2^31");
+  if (B == 0) return QZ_OK;
+  if (!k || !v || !k_scale || !v_scale || !q || !lengths || !out || !workspace || (!table && max_pages)) return fail(QZ_ERR_INVALID, "NULL pointer");
+  if (off16(k) || off16(v) || off16(q) || off16(out) || off16(workspace) || q_seq % 8 || q_head % 8)
+    return fail(QZ_ERR_INVALID, "caches, q, out and workspace must be 16-byte aligned");
+  int sms = 0;
+  if ((s = current_sms(&sms)) != QZ_OK) return s;
+  const int64_t warps = (int64_t)sms * (D == 128 ? AttnGeo<128>::kWarps : AttnGeo<64>::kWarps);
+  const int64_t need = warps * 2 * (16 * D + 32) * 4;
+  if (workspace_bytes < need) return fail(QZ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  AttnParams p{};
+  p.k = k; p.v = v; p.ks = k_scale; p.vs = v_scale; p.num_pages = num_pages;
+  p.B = (int)B; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.row_tiles = (p.G + 15) / 16;
+  p.q = static_cast<const uint16_t*>(q); p.q_seq = q_seq; p.q_head = q_head; p.dtype = dtype;
+  p.table = table; p.ld_table = ld_table; p.max_pages = (int)max_pages; p.lengths = lengths;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + warps * 2 * 16 * D;
+  p.out = out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (D == 128) return kv_dtype == QZ_KV_INT8 ? launch_attention<128, kKvInt8>(p, sms, st) : launch_attention<128, kKvE4M3>(p, sms, st);
+  return kv_dtype == QZ_KV_INT8 ? launch_attention<64, kKvInt8>(p, sms, st) : launch_attention<64, kKvE4M3>(p, sms, st);
+}
