@@ -10,12 +10,12 @@
 //
 // The attention reads each code once and is bound by HBM: 2 D bytes per token and
 // head.  Layout inside a (page, head) block of 64 D bytes, so that a warp's
-// 16-byte loads are contiguous and are the B fragments of mma.m16n8k16 after an
+// 16-byte loads are contiguous and are the A fragments of mma.m16n8k16 after an
 // exact conversion to fp16 (int8 and E4M3 both fit):
 //   keys    token n = 16 t + 2 j + e, value d at ((j D/64 + d/64) 8 + 2 t + e) 64 + d % 64
 //   values  transposed: token n, value d at 64 d + n
-// The score fragment of 8-token tiles 2i, 2i + 1 is then the probability fragment of
-// the value product's step i, with no exchange between lanes.
+// Key tiles 2i and 2i + 1 (8 tokens each) are the 16 rows of score tile i, and a
+// lane's 4 bytes of a value row are its part of the value product's step i.
 //
 // Work: the pages of all (sequence, head) pairs, in order, are cut into equal
 // runs, one per warp of the grid (lengths live on the device, so the cut is made
@@ -250,7 +250,8 @@ struct AttnParams {
   const uint8_t *k, *v;
   const float *ks, *vs;
   int64_t num_pages;
-  int B, Hkv, G, row_tiles;      // G query heads per cache head, in row_tiles tiles of 16
+  int B, Hkv, G;                 // G query heads per cache head ...
+  int row_tiles, rows_per_tile;  // ... in row_tiles tiles of 8 or 16
   const uint16_t* q;             // (B, Hkv * G, D), strides in elements
   int64_t q_seq, q_head;
   int dtype;
@@ -309,31 +310,55 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          const uint32_t (&b)[2]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
 
-template <int D>
+// Transpose of an 8 x 8 tile of 16-bit values (row g, columns 2t, 2t + 1 per lane).
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units of the last place; 0 for -inf
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// NH tiles of 8 query heads share the warp's pass over a page.  Warps per SM:
+// what the registers allow (D = 128: 12 of at most 168 with one tile; two tiles
+// keep twice the sums: 8) and the ring, one page of keys and values per warp.
+template <int D, int NH>
 struct AttnGeo {
   static constexpr int kBlock = kPage * D;               // bytes of keys (or values) of one page and head
-  static constexpr int kWarps = D == 128 ? 6 : 8;
-  static constexpr int kStages = D == 128 ? 2 : 3;
-  static constexpr int kRing = kWarps * kStages * 2 * kBlock;
-  static int smem(int B) { return kRing + kWarps * kStages * 2 * 8 + (B + 1) * 4; }
+  static constexpr int kWarps = D == 128 ? (NH == 1 ? 12 : 8) : (NH == 1 ? 16 : 12);
+  static constexpr int kRing = kWarps * 2 * kBlock;
+  static int smem(int B) { return kRing + kWarps * 2 * 8 + (B + 1) * 4; }
 };
+constexpr int kAttnMaxWarps = 16;
 
-template <int D, int KV>
-__global__ void __launch_bounds__(AttnGeo<D>::kWarps * 32, 1) kv_attention_kernel(const __grid_constant__ AttnParams p) {
-  using G = AttnGeo<D>;
+// Scores as S^T = K Q^T and sums as O^T = V^T P^T: the cache is the 16-row A
+// operand, 8 query heads the N side, so a group of up to 8 heads wastes nothing
+// and a page costs 4 D/16 + 4 D/16 matrix instructions.  The codes' conversion to
+// fp16 (2 instructions per 4 E4M3 codes, 5 per 4 int8) is the largest part of
+// the rest.
+template <int D, int KV, int NH>
+__global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_kernel(const __grid_constant__ AttnParams p) {
+  using G = AttnGeo<D, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kRing) + warp * G::kStages * 2;  // keys, values per stage
-  int* prefix = reinterpret_cast<int*>(smem + G::kRing + G::kWarps * G::kStages * 16);
-  uint8_t* ring = smem + warp * G::kStages * 2 * G::kBlock;
+  uint64_t* bar_k = reinterpret_cast<uint64_t*>(smem + G::kRing) + warp * 2;
+  uint64_t* bar_v = bar_k + 1;
+  int* prefix = reinterpret_cast<int*>(smem + G::kRing + G::kWarps * 16);
+  uint8_t* ring = smem + warp * 2 * G::kBlock;
   if (lane == 0) {
-    for (int i = 0; i < G::kStages * 2; ++i) mbar_init(bars + i, 1);
+    mbar_init(bar_k, 1);
+    mbar_init(bar_v, 1);
     fence_barrier_init();
   }
   __syncwarp();
@@ -342,24 +367,24 @@ __global__ void __launch_bounds__(AttnGeo<D>::kWarps * 32, 1) kv_attention_kerne
   const int64_t total = (int64_t)prefix[p.B] * HR, warps = (int64_t)gridDim.x * G::kWarps;
   const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours in work on different SMs
   const int64_t u0 = me * total / warps, u1 = (me + 1) * total / warps;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (u0 >= u1) return;
 
   // position in the work list: sequence b, head and row tile hr, page pg of nb
   struct Pos { int b, hr, pg, nb; };
-  auto locate = [&](int64_t u) {
-    int lo = 0, hi = p.B;  // last b with prefix[b] * HR <= u
+  Pos cur;
+  {
+    int lo = 0, hi = p.B;  // last b with prefix[b] * HR <= u0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((int64_t)prefix[mid] * HR <= u) lo = mid; else hi = mid;
+      if ((int64_t)prefix[mid] * HR <= u0) lo = mid; else hi = mid;
     }
-    Pos x;
-    x.b = lo;
-    x.nb = prefix[lo + 1] - prefix[lo];
-    const int64_t r = u - (int64_t)prefix[lo] * HR;
-    x.hr = (int)(r / x.nb);
-    x.pg = (int)(r % x.nb);
-    return x;
-  };
+    cur.b = lo;
+    cur.nb = prefix[lo + 1] - prefix[lo];
+    const int64_t r = u0 - (int64_t)prefix[lo] * HR;
+    cur.hr = (int)(r / cur.nb);
+    cur.pg = (int)(r % cur.nb);
+  }
   auto advance = [&](Pos& x) {
     if (++x.pg < x.nb) return;
     x.pg = 0;
@@ -368,270 +393,317 @@ __global__ void __launch_bounds__(AttnGeo<D>::kWarps * 32, 1) kv_attention_kerne
     do ++x.b; while (x.b < p.B && prefix[x.b + 1] == prefix[x.b]);
     x.nb = x.b < p.B ? prefix[x.b + 1] - prefix[x.b] : 1;
   };
-  auto issue = [&](const Pos& x, int stage) {  // lane 0
-    const int64_t page = p.table[(int64_t)x.b * p.ld_table + x.pg];
-    uint64_t* bk = bars + stage * 2;
-    if (page < 0 || page >= p.num_pages) {  // no such page: nothing is read, its tokens are masked
-      mbar_arrive(bk);
-      mbar_arrive(bk + 1);
+  // the cache block of a position, -1 if the table names no page of the cache
+  auto block_of = [&](const Pos& x) -> int64_t {
+    const int64_t page = __ldg(p.table + (int64_t)x.b * p.ld_table + x.pg);
+    return page < 0 || page >= p.num_pages ? -1 : page * p.Hkv + x.hr / p.row_tiles;
+  };
+  int issued_k = 0, issued_v = 0;
+  auto issue = [&](const uint8_t* base, int64_t block, uint8_t* dst, uint64_t* bar) {  // lane 0
+    if (block < 0) {  // nothing is read, the tokens are masked
+      mbar_arrive(bar);
       return;
     }
-    const int64_t at = (page * p.Hkv + x.hr / p.row_tiles) * (int64_t)G::kBlock;
-    mbar_arrive_expect_tx(bk, G::kBlock);
-    bulk_load(ring + stage * 2 * G::kBlock, p.k + at, G::kBlock, bk);
-    mbar_arrive_expect_tx(bk + 1, G::kBlock);
-    bulk_load(ring + stage * 2 * G::kBlock + G::kBlock, p.v + at, G::kBlock, bk + 1);
+    mbar_arrive_expect_tx(bar, G::kBlock);
+    bulk_load(dst, base + block * G::kBlock, G::kBlock, bar);
   };
 
-  Pos cur = locate(u0), ahead = cur;
-  int64_t next = u0;  // next unit to load
-  if (lane == 0)
-    for (int s = 0; s < G::kStages && next < u1; ++s, ++next) { issue(ahead, s); advance(ahead); }
+  Pos next = cur;
+  int64_t blk = block_of(cur), blk_next = -1;
+  if (lane == 0) {
+    issue(p.k, blk, ring, bar_k);
+    issue(p.v, blk, ring + G::kBlock, bar_v);
+  }
+  issued_k = issued_v = 1;
+  float ks = blk >= 0 ? __ldg(p.ks + blk) : 0.0f, vs = blk >= 0 ? __ldg(p.vs + blk) : 0.0f;
+  advance(next);
+  if (u0 + 1 < u1) blk_next = block_of(next);
 
-  uint32_t qf[D / 16][4];
-  float o[D / 8][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, qs0 = 1.0f, qs1 = 1.0f;
-  bool fresh = true;
+  uint32_t qb[NH][D / 16][2];
+  float o[D / 16][NH][4], m[NH][2], l[NH][2], qs[NH][2];
+  bool fresh = true, ok = true;
   int64_t seg_begin = u0;
-  bool ok = true;
-  uint32_t it = 0;
-  for (int64_t u = u0; u < u1; ++u, ++it) {
-    const int stage = it % G::kStages;
-    const uint32_t parity = it / G::kStages & 1;
-    const int head = cur.hr / p.row_tiles, r0 = cur.hr % p.row_tiles * 16;
+  uint32_t parity = 0;
+  for (int64_t u = u0; u < u1; ++u, parity ^= 1) {
+    const int head = cur.hr / p.row_tiles, r0 = cur.hr % p.row_tiles * (8 * NH);
+    const bool more = u + 1 < u1;
+    // one page ahead: its scales; two ahead: its place in the table
+    float ks_next = 0.0f, vs_next = 0.0f;
+    if (more && blk_next >= 0) {
+      ks_next = __ldg(p.ks + blk_next);
+      vs_next = __ldg(p.vs + blk_next);
+    }
+    Pos after = next;
+    int64_t blk_after = -1;
+    if (u + 2 < u1) {
+      advance(after);
+      blk_after = block_of(after);
+    }
+    int valid = blk >= 0 ? __ldg(p.lengths + cur.b) - cur.pg * kPage : 0;
+    if (valid > kPage) valid = kPage;
     if (fresh) {
-      // this pair's query rows as fp16, each on the power of two that puts its
-      // largest magnitude in [2^14, 2^15) (fp16 rows as they are)
+      // this pair's query heads as fp16, each on the power of two that puts its
+      // largest magnitude in [2^14, 2^15) (fp16 heads as they are)
       fresh = false;
-      const bool h0 = r0 + g < p.G, h1 = r0 + g + 8 < p.G;
-      const uint16_t* q0 = p.q + cur.b * p.q_seq + (int64_t)(head * p.G + r0 + (h0 ? g : 0)) * p.q_head;
-      const uint16_t* q1 = p.q + cur.b * p.q_seq + (int64_t)(head * p.G + r0 + (h1 ? g + 8 : 0)) * p.q_head;
-      uint32_t raw[D / 16][4];
-      uint32_t x0 = 0, x1 = 0;
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h) {
-        // lane t takes values 64 h + 16 t .. + 15 of its two rows
+      for (int n = 0; n < NH; ++n) {
+        const int row = r0 + 8 * n + g;
+        const uint16_t* qp = p.q + cur.b * p.q_seq + (int64_t)(head * p.G + (row < p.G ? row : 0)) * p.q_head;
+        uint32_t x = 0;
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const uint4 a = h0 ? __ldg(reinterpret_cast<const uint4*>(q0 + 64 * h + 16 * t + 8 * v)) : make_uint4(0, 0, 0, 0);
-          const uint4 c = h1 ? __ldg(reinterpret_cast<const uint4*>(q1 + 64 * h + 16 * t + 8 * v)) : make_uint4(0, 0, 0, 0);
-          raw[4 * h + 2 * v][0] = a.x; raw[4 * h + 2 * v][2] = a.y;
-          raw[4 * h + 2 * v + 1][0] = a.z; raw[4 * h + 2 * v + 1][2] = a.w;
-          raw[4 * h + 2 * v][1] = c.x; raw[4 * h + 2 * v][3] = c.y;
-          raw[4 * h + 2 * v + 1][1] = c.z; raw[4 * h + 2 * v + 1][3] = c.w;
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {  // lane t takes values 64 h + 16 t .. + 15 of head g
+            const uint4 w = row < p.G ? __ldg(reinterpret_cast<const uint4*>(qp + 64 * h + 16 * t + 8 * v)) : make_uint4(0, 0, 0, 0);
+            qb[n][4 * h + 2 * v][0] = w.x; qb[n][4 * h + 2 * v][1] = w.y;
+            qb[n][4 * h + 2 * v + 1][0] = w.z; qb[n][4 * h + 2 * v + 1][1] = w.w;
+          }
+        float sc = 1.0f;
+        if (p.dtype == kDtBF16) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) x = max(x, max(qb[n][i][c] & 0x7fff0000u, qb[n][i][c] << 16 & 0x7fff0000u));
+          x = max(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = max(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          const int e = x == 0 || x >= 0x7f800000u ? 0 : max((int)(x >> 23) - 141, -112);
+          const float inv = pow2f(-e);
+          sc = pow2f(e);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const __half2 h = __floats2half2_rn(bf16_bits_to_float(qb[n][i][c] & 0xffffu) * inv, bf16_bits_to_float(qb[n][i][c] >> 16) * inv);
+              qb[n][i][c] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        // the sums' columns are heads 2t and 2t + 1
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          qs[n][c] = __shfl_sync(0xffffffffu, sc, (2 * t + c) * 4) * p.scale_log2;
+          m[n][c] = -INFINITY;
+          l[n][c] = 0.0f;
         }
       }
-      qs0 = qs1 = 1.0f;
-      if (p.dtype == kDtBF16) {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t hi = raw[s][i] & 0x7fff0000u, lo = raw[s][i] << 16 & 0x7fff0000u;
-            if (i & 1) x1 = max(x1, max(hi, lo)); else x0 = max(x0, max(hi, lo));
-          }
-        x0 = max(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x0 = max(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = max(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x1 = max(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        const int e0 = x0 == 0 || x0 >= 0x7f800000u ? 0 : max((int)(x0 >> 23) - 141, -112);
-        const int e1 = x1 == 0 || x1 >= 0x7f800000u ? 0 : max((int)(x1 >> 23) - 141, -112);
-        qs0 = pow2f(e0);
-        qs1 = pow2f(e1);
+        for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float inv = pow2f(i & 1 ? -e1 : -e0);
-            const __half2 h = __floats2half2_rn(bf16_bits_to_float(raw[s][i] & 0xffffu) * inv, bf16_bits_to_float(raw[s][i] >> 16) * inv);
-            qf[s][i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-      } else {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) qf[s][i] = raw[s][i];
-      }
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
+          for (int c = 0; c < 4; ++c) o[i][n][c] = 0.0f;
     }
-    const int64_t page = p.table[(int64_t)cur.b * p.ld_table + cur.pg];
-    const bool there = page >= 0 && page < p.num_pages;
-    const float ks = there ? __ldg(p.ks + page * p.Hkv + head) : 0.0f, vs = there ? __ldg(p.vs + page * p.Hkv + head) : 0.0f;
-    int valid = there ? p.lengths[cur.b] - cur.pg * kPage : 0;
-    if (valid > kPage) valid = kPage;
-    const uint8_t* sk = ring + stage * 2 * G::kBlock + lane * 16;
-    const uint8_t* sv = sk + G::kBlock;
-    if (!mbar_wait_bounded(bars + stage * 2, parity, kDevErrLoadTimeout)) { ok = false; break; }
-    // scores of 64 tokens: 8 tiles of 8
-    float s[8][4];
+    if (!mbar_wait_bounded(bar_k, parity, kDevErrLoadTimeout)) { ok = false; break; }
+    // scores: 4 tiles of 16 tokens; row g (g + 8) of tile i is token 16 (g / 2) + 4 i + g % 2 (+ 2)
+    float s[4][NH][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[j][c] = 0.0f;
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[i][n][c] = 0.0f;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {
-        const uint4 w = *reinterpret_cast<const uint4*>(sk + (j * (D / 64) + h) * 512);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        const uint4 w0 = *reinterpret_cast<const uint4*>(ring + (2 * i * (D / 64) + h) * 512 + lane * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(ring + ((2 * i + 1) * (D / 64) + h) * 512 + lane * 16);
+        const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t b0, b1;
-          codes_to_f16<KV>(ww[q], b0, b1);
-          mma_16816(s[j], qf[4 * h + q], b0, b1);
+          uint32_t a0, a1, a2, a3;
+          codes_to_f16<KV>(x0[q], a0, a2);
+          codes_to_f16<KV>(x1[q], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_16816(s[i][n], a0, a1, a2, a3, qb[n][4 * h + q]);
         }
       }
     }
-    const float f0 = ks * qs0 * p.scale_log2, f1 = ks * qs1 * p.scale_log2;
-    float n0 = m0, n1 = m1;
+    __syncwarp();  // every lane has read its keys
+    if (more) {
+      if (lane == 0) issue(p.k, blk_next, ring, bar_k);
+      ++issued_k;
+    }
+    float corr[NH][2];
+    uint32_t pb[4][NH][2];  // probabilities, fp16: the B fragments of the value product
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int n = 0; n < NH; ++n) {
+      float z[2], sum[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[j][c] *= c < 2 ? f0 : f1;
-        if (valid < kPage && 16 * t + 2 * j + (c & 1) >= valid) s[j][c] = -INFINITY;
+      for (int c = 0; c < 2; ++c) {
+        const float f = ks * qs[n][c];
+        float x = m[n][c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[i][n][c] *= f;
+          s[i][n][c + 2] *= f;
+          if (valid < kPage) {
+            const int tok = 16 * (g >> 1) + 4 * i + (g & 1);
+            if (tok >= valid) s[i][n][c] = -INFINITY;
+            if (tok + 2 >= valid) s[i][n][c + 2] = -INFINITY;
+          }
+          x = fmaxf(x, fmaxf(s[i][n][c], s[i][n][c + 2]));
+        }
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        z[c] = x == -INFINITY ? 0.0f : x;  // nothing unmasked yet
+        corr[n][c] = exp2_fast(m[n][c] - z[c]);
+        m[n][c] = x;
       }
-      n0 = fmaxf(n0, fmaxf(s[j][0], s[j][1]));
-      n1 = fmaxf(n1, fmaxf(s[j][2], s[j][3]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[i][n][c] = exp2_fast(s[i][n][c] - z[c & 1]);
+        sum[0] += s[i][n][0] + s[i][n][2];
+        sum[1] += s[i][n][1] + s[i][n][3];
+        const __half2 x = __floats2half2_rn(s[i][n][0], s[i][n][1]), y = __floats2half2_rn(s[i][n][2], s[i][n][3]);
+        pb[i][n][0] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
+        pb[i][n][1] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
+      }
+      l[n][0] = fmaf(l[n][0], corr[n][0], sum[0]);
+      l[n][1] = fmaf(l[n][1], corr[n][1], sum[1]);
     }
-    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-    const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;  // nothing unmasked yet
-    const float c0 = exp2f(m0 - z0), c1 = exp2f(m1 - z1);
-    m0 = n0;
-    m1 = n1;
-    float a0 = 0.0f, a1 = 0.0f;
-    uint32_t pf[4][4];  // probabilities, fp16: the A fragments of the value product
+    if (!mbar_wait_bounded(bar_v, parity, kDevErrLoadTimeout)) { ok = false; break; }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < D / 16; ++i) {
+      const uint4 w0 = *reinterpret_cast<const uint4*>(ring + G::kBlock + i * 1024 + lane * 16);
+      const uint4 w1 = *reinterpret_cast<const uint4*>(ring + G::kBlock + i * 1024 + 512 + lane * 16);
+      uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+      float d[NH][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[j][c] = exp2f(s[j][c] - (c < 2 ? z0 : z1));
-      a0 += s[j][0] + s[j][1];
-      a1 += s[j][2] + s[j][3];
-      const __half2 x = __floats2half2_rn(s[j][0], s[j][1]), y = __floats2half2_rn(s[j][2], s[j][3]);
-      pf[j >> 1][(j & 1) * 2] = *reinterpret_cast<const uint32_t*>(&x);
-      pf[j >> 1][(j & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&y);
-    }
-    l0 = fmaf(l0, c0, a0);
-    l1 = fmaf(l1, c1, a1);
-    if (!mbar_wait_bounded(bars + stage * 2 + 1, parity, kDevErrLoadTimeout)) { ok = false; break; }
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      uint4 w = *reinterpret_cast<const uint4*>(sv + i * 512);
-      uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < 4; ++c) d[n][c] = 0.0f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (valid < kPage) {  // what lies behind the last token may decode to NaN
           const int left = valid - (16 * t + 4 * q);
-          ww[q] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          x0[q] &= mask;
+          x1[q] &= mask;
         }
-        uint32_t b0, b1;
-        codes_to_f16<KV>(ww[q], b0, b1);
-        mma_16816(d, pf[q], b0, b1);
+        uint32_t a0, a1, a2, a3;
+        codes_to_f16<KV>(x0[q], a0, a2);
+        codes_to_f16<KV>(x1[q], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma_16816(d[n], a0, a1, a2, a3, pb[q][n]);
       }
-      o[i][0] = fmaf(d[0], vs, o[i][0] * c0);
-      o[i][1] = fmaf(d[1], vs, o[i][1] * c0);
-      o[i][2] = fmaf(d[2], vs, o[i][2] * c1);
-      o[i][3] = fmaf(d[3], vs, o[i][3] * c1);
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][n][c] = fmaf(d[n][c], vs, o[i][n][c] * corr[n][c & 1]);
     }
-    __syncwarp();
-    if (lane == 0 && next < u1) {
-      issue(ahead, stage);
-      advance(ahead);
-      ++next;
+    __syncwarp();  // every lane has read its values
+    if (more) {
+      if (lane == 0) issue(p.v, blk_next, ring + G::kBlock, bar_v);
+      ++issued_v;
     }
     const bool pair_ends = cur.pg + 1 == cur.nb;
-    if (pair_ends || u + 1 == u1) {
-      // the sums of a row lie in its four lanes
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (pair_ends || !more) {
       const bool whole = pair_ends && u + 1 - seg_begin == cur.nb;
-      const bool h0 = r0 + g < p.G, h1 = r0 + g + 8 < p.G;
-      if (whole) {
-        const float i0 = l0 > 0.0f ? 1.0f / l0 : (l0 == 0.0f ? 0.0f : l0), i1 = l1 > 0.0f ? 1.0f / l1 : (l1 == 0.0f ? 0.0f : l1);
-        uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)cur.b * p.Hkv + head) * p.G * D;
+      const int64_t slot = me * 2 + (seg_begin == u0 ? 0 : 1);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint32_t x, y;
-          if (p.dtype == kDtBF16) {
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(o[i][1] * i0), "f"(o[i][0] * i0));
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(o[i][3] * i1), "f"(o[i][2] * i1));
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // a head's sum lies in the eight lanes of its column
+          float sum = l[n][c];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = 8 * n + 2 * t + c;  // of the row tile
+          if (r0 + row >= p.G) continue;
+          if (whole) {
+            const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            uint16_t* out = static_cast<uint16_t*>(p.out) + (((int64_t)cur.b * p.Hkv + head) * p.G + r0 + row) * D;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float v = o[i][n][2 * h + c] * inv;
+                uint16_t r;
+                if (p.dtype == kDtBF16) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+                else r = __half_as_ushort(__float2half_rn(v));
+                out[16 * i + 8 * h + g] = r;
+              }
           } else {
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(o[i][1] * i0), "f"(o[i][0] * i0));
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(o[i][3] * i1), "f"(o[i][2] * i1));
-          }
-          if (h0) *reinterpret_cast<uint32_t*>(out + (int64_t)(r0 + g) * D + 8 * i + 2 * t) = x;
-          if (h1) *reinterpret_cast<uint32_t*>(out + (int64_t)(r0 + g + 8) * D + 8 * i + 2 * t) = y;
-        }
-      } else {
-        const int64_t slot = me * 2 + (seg_begin == u0 ? 0 : 1);
-        float* po = p.part_o + slot * 16 * D;
-        float* ml = p.part_ml + slot * 32;
+            float* po = p.part_o + (slot * 16 + row) * D;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          if (h0) *reinterpret_cast<float2*>(po + g * D + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
-          if (h1) *reinterpret_cast<float2*>(po + (g + 8) * D + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
+            for (int i = 0; i < D / 16; ++i) {
+              po[16 * i + g] = o[i][n][c];
+              po[16 * i + 8 + g] = o[i][n][2 + c];
+            }
+            if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 16 + row) * 2) = make_float2(m[n][c], sum);
+          }
         }
-        if (t == 0) {
-          ml[g * 2] = m0;
-          ml[g * 2 + 1] = l0;
-          ml[g * 2 + 16] = m1;
-          ml[g * 2 + 17] = l1;
-        }
-      }
       fresh = true;
       seg_begin = u + 1;
     }
-    advance(cur);
+    cur = next;
+    next = after;
+    blk = blk_next;
+    blk_next = blk_after;
+    ks = ks_next;
+    vs = vs_next;
   }
-  if (!ok) {
-    // copies in flight must land before the CTA exits (bounded)
-    for (int i = 0; i < G::kStages * 2; ++i) {
-      const uint32_t k = it + (i / 2 + G::kStages - it % G::kStages) % G::kStages;  // the last unit loaded into stage i / 2
-      if (u0 + k < u1) mbar_wait_bounded(bars + i, k / G::kStages & 1, kDevErrLoadTimeout);
-    }
+  if (!ok) {  // copies in flight must land before the CTA exits (bounded)
+    mbar_wait_bounded(bar_k, (issued_k - 1) & 1, kDevErrLoadTimeout);
+    mbar_wait_bounded(bar_v, (issued_v - 1) & 1, kDevErrLoadTimeout);
   }
 }
 
 // Joins the partial results of the (sequence, head, row tile) pairs that several
 // warps share, in the order of their pages; writes zeros for empty sequences.
-// One CTA per query row.
+// One CTA per query row, kJoinSplit groups of D threads taking every
+// kJoinSplit-th partial result.
+constexpr int kJoinSplit = 4;
 template <int D>
-__global__ void __launch_bounds__(D) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps, int attn_warps) {
+__global__ void __launch_bounds__(D * kJoinSplit) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps) {
   extern __shared__ int prefix[];
-  const int HR = p.Hkv * p.row_tiles;
-  const int row = blockIdx.x % p.G, bh = blockIdx.x / p.G, head = bh % p.Hkv, b = bh / p.Hkv, d = threadIdx.x;
+  __shared__ float s_o[kJoinSplit][D], s_m[kJoinSplit], s_l[kJoinSplit];
+  const int HR = p.Hkv * p.row_tiles, tile = p.rows_per_tile;
+  const int row = blockIdx.x % p.G, bh = blockIdx.x / p.G, head = bh % p.Hkv, b = bh / p.Hkv;
+  const int d = threadIdx.x % D, part = threadIdx.x / D;
   page_prefix(p, prefix);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every CTA: this grid ends after the one before it
   const int64_t total = (int64_t)prefix[p.B] * HR;
-  const int nb = prefix[b + 1] - prefix[b], hr = head * p.row_tiles + row / 16;
-  float v = 0.0f;
+  const int nb = prefix[b + 1] - prefix[b], hr = head * p.row_tiles + row / tile;
+  float v = 0.0f, m = -INFINITY, l = 0.0f;
   if (nb > 0) {
     const int64_t u0 = (int64_t)prefix[b] * HR + (int64_t)hr * nb, u1 = u0 + nb;
-    // the warp of unit u: the last w with w * total / warps <= u
+    // the warp of unit u is the last w with w * total / warps <= u; with fewer
+    // units than warps every unit has a warp of its own
     const int64_t w0 = ((u0 + 1) * warps - 1) / total, w1 = (u1 * warps - 1) / total;
     if (w0 == w1) return;  // one warp had all of it
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t begin = w * total / warps;
-      if (begin == (w + 1) * total / warps) continue;  // more warps than units
-      const int64_t slot = w * 2 + (begin >= u0 ? 0 : 1);
-      const float mw = __ldg(p.part_ml + slot * 32 + row % 16 * 2), lw = __ldg(p.part_ml + slot * 32 + row % 16 * 2 + 1);
-      const float ow = __ldg(p.part_o + slot * 16 * D + row % 16 * D + d);
-      const float n = fmaxf(m, mw), z = n == -INFINITY ? 0.0f : n;
-      const float c = exp2f(m - z), cw = exp2f(mw - z);
+    const int count = total >= warps ? (int)(w1 - w0 + 1) : nb;
+#pragma unroll 4
+    for (int i = part; i < count; i += kJoinSplit) {
+      const int64_t w = total >= warps ? w0 + i : ((u0 + i + 1) * warps - 1) / total;
+      const int64_t slot = w * 2 + (i > 0 || w0 * total / warps >= u0 ? 0 : 1);
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot * 16 + row % tile) * 2));
+      const float ow = __ldcg(p.part_o + (slot * 16 + row % tile) * D + d);
+      const float n = fmaxf(m, ml.x), z = n == -INFINITY ? 0.0f : n;
+      const float c = exp2_fast(m - z), cw = exp2_fast(ml.x - z);
       v = v * c + ow * cw;
-      l = l * c + lw * cw;
+      l = l * c + ml.y * cw;
+      m = n;
+    }
+    s_o[part][d] = v;
+    if (d == 0) {
+      s_m[part] = m;
+      s_l[part] = l;
+    }
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int i = 1; i < kJoinSplit; ++i) {
+      const float n = fmaxf(m, s_m[i]), z = n == -INFINITY ? 0.0f : n;
+      const float c = exp2_fast(m - z), cw = exp2_fast(s_m[i] - z);
+      v = v * c + s_o[i][d] * cw;
+      l = l * c + s_l[i] * cw;
       m = n;
     }
     v = l > 0.0f ? v / l : (l == 0.0f ? 0.0f : l);
+  } else if (part > 0) {
+    return;
   }
   const int64_t at = ((int64_t)bh * p.G + row) * D + d;
   uint16_t r;
@@ -660,24 +732,40 @@ static int check_cache(int kv_dtype, int64_t num_pages, int64_t Hkv, int64_t D) 
 
 static bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
-template <int D, int KV>
-static int launch_attention(const AttnParams& p, int sms, cudaStream_t st) {
-  using G = AttnGeo<D>;
-  static int attr_smem[64] = {0};  // per device (a benign race: the value only grows and is set again if it was lost)
+template <int D, int KV, int NH>
+static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
+  using G = AttnGeo<D, NH>;
+  static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
-  const int smem = G::smem(p.B), most = G::smem(kKvMaxSeqs);
-  if (dev < 0 || dev >= 64 || attr_smem[dev] == 0) {
-    e = cudaFuncSetAttribute(kv_attention_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(kv_attention_kernel<D, KV, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(kKvMaxSeqs));
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
-    if (dev >= 0 && dev < 64) attr_smem[dev] = most;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  kv_attention_kernel<D, KV><<<sms, G::kWarps * 32, smem, st>>>(p);
+  p.rows_per_tile = 8 * NH;
+  p.row_tiles = (p.G + 8 * NH - 1) / (8 * NH);
+  kv_attention_kernel<D, KV, NH><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
   int s = cuda_status(cudaGetLastError(), "kv attention launch");
   if (s != QZ_OK) return s;
-  kv_join_kernel<D><<<(unsigned)((int64_t)p.B * p.Hkv * p.G), D, (p.B + 1) * 4, st>>>(p, (int64_t)sms * G::kWarps, G::kWarps);
-  return cuda_status(cudaGetLastError(), "kv join launch");
+  // the join may begin while the last pages are read; it waits for the kernel's end before it reads results
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.Hkv * p.G));
+  cfg.blockDim = dim3(D * kJoinSplit);
+  cfg.dynamicSmemBytes = (size_t)(p.B + 1) * 4;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kv_join_kernel<D>, p, (int64_t)sms * G::kWarps), "kv join launch");
+}
+
+template <int D, int KV>
+static int run_attention(const AttnParams& p, int sms, cudaStream_t st) {
+  return p.G <= 8 ? launch_attention<D, KV, 1>(p, sms, st) : launch_attention<D, KV, 2>(p, sms, st);
 }
 
 }  // namespace qz
@@ -750,7 +838,7 @@ extern "C" int qz_kv_attention_workspace(int64_t D, int64_t* bytes) {
   if (!bytes) return fail(QZ_ERR_INVALID, "NULL pointer");
   const int r = current_sms(&sms);
   if (r != QZ_OK) return r;
-  const int64_t warps = (int64_t)sms * (D == 128 ? AttnGeo<128>::kWarps : AttnGeo<64>::kWarps);
+  const int64_t warps = (int64_t)sms * kAttnMaxWarps;
   *bytes = warps * 2 * (16 * D + 32) * 4;
   return QZ_OK;
 }
@@ -773,12 +861,12 @@ extern "C" int qz_kv_attention(const uint8_t* k, const float* k_scale, const uin
     return fail(QZ_ERR_INVALID, "caches, q, out and workspace must be 16-byte aligned");
   int sms = 0;
   if ((s = current_sms(&sms)) != QZ_OK) return s;
-  const int64_t warps = (int64_t)sms * (D == 128 ? AttnGeo<128>::kWarps : AttnGeo<64>::kWarps);
+  const int64_t warps = (int64_t)sms * kAttnMaxWarps;
   const int64_t need = warps * 2 * (16 * D + 32) * 4;
   if (workspace_bytes < need) return fail(QZ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   AttnParams p{};
   p.k = k; p.v = v; p.ks = k_scale; p.vs = v_scale; p.num_pages = num_pages;
-  p.B = (int)B; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.row_tiles = (p.G + 15) / 16;
+  p.B = (int)B; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
   p.q = static_cast<const uint16_t*>(q); p.q_seq = q_seq; p.q_head = q_head; p.dtype = dtype;
   p.table = table; p.ld_table = ld_table; p.max_pages = (int)max_pages; p.lengths = lengths;
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -786,6 +874,6 @@ extern "C" int qz_kv_attention(const uint8_t* k, const float* k_scale, const uin
   p.part_ml = p.part_o + warps * 2 * 16 * D;
   p.out = out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (D == 128) return kv_dtype == QZ_KV_INT8 ? launch_attention<128, kKvInt8>(p, sms, st) : launch_attention<128, kKvE4M3>(p, sms, st);
-  return kv_dtype == QZ_KV_INT8 ? launch_attention<64, kKvInt8>(p, sms, st) : launch_attention<64, kKvE4M3>(p, sms, st);
+  if (D == 128) return kv_dtype == QZ_KV_INT8 ? run_attention<128, kKvInt8>(p, sms, st) : run_attention<128, kKvE4M3>(p, sms, st);
+  return kv_dtype == QZ_KV_INT8 ? run_attention<64, kKvInt8>(p, sms, st) : run_attention<64, kKvE4M3>(p, sms, st);
 }
