@@ -652,21 +652,33 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
 
 // Joins the partial results of the (sequence, head, row tile) pairs that several
 // warps share, in the order of their pages; writes zeros for empty sequences.
-// One CTA per query row, kJoinSplit groups of D threads taking every
-// kJoinSplit-th partial result.
-constexpr int kJoinSplit = 4;
+// One CTA per pair: a thread owns four values of one row and one of `split`
+// interleaved shares of the partial results (a long sequence has hundreds),
+// which then meet in shared memory.
+constexpr int kJoinThreads = 512;
 template <int D>
-__global__ void __launch_bounds__(D * kJoinSplit) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps) {
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps) {
   extern __shared__ int prefix[];
-  __shared__ float s_o[kJoinSplit][D], s_m[kJoinSplit], s_l[kJoinSplit];
-  const int HR = p.Hkv * p.row_tiles, tile = p.rows_per_tile;
-  const int row = blockIdx.x % p.G, bh = blockIdx.x / p.G, head = bh % p.Hkv, b = bh / p.Hkv;
-  const int d = threadIdx.x % D, part = threadIdx.x / D;
+  __shared__ float4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
+  const int HR = p.Hkv * p.row_tiles;
+  const int b = blockIdx.x / HR, hr = blockIdx.x % HR, head = hr / p.row_tiles, r0 = hr % p.row_tiles * p.rows_per_tile;
+  const int rows = p.G - r0 < p.rows_per_tile ? p.G - r0 : p.rows_per_tile;
+  const int per = rows * (D / 4), split = kJoinThreads / per;
+  const int part = threadIdx.x / per, row = threadIdx.x % per / (D / 4), d4 = threadIdx.x % (D / 4);
   page_prefix(p, prefix);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // in every CTA: this grid ends after the one before it
   const int64_t total = (int64_t)prefix[p.B] * HR;
-  const int nb = prefix[b + 1] - prefix[b], hr = head * p.row_tiles + row / tile;
-  float v = 0.0f, m = -INFINITY, l = 0.0f;
+  const int nb = prefix[b + 1] - prefix[b];
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -INFINITY, l = 0.0f;
+  auto take = [&](const float2 ml, const float4 o) {
+    const float n = fmaxf(m, ml.x), z = n == -INFINITY ? 0.0f : n;
+    const float c = exp2_fast(m - z), cw = exp2_fast(ml.x - z);
+    v = make_float4(v.x * c + o.x * cw, v.y * c + o.y * cw, v.z * c + o.z * cw, v.w * c + o.w * cw);
+    l = l * c + ml.y * cw;
+    m = n;
+  };
   if (nb > 0) {
     const int64_t u0 = (int64_t)prefix[b] * HR + (int64_t)hr * nb, u1 = u0 + nb;
     // the warp of unit u is the last w with w * total / warps <= u; with fewer
@@ -674,42 +686,35 @@ __global__ void __launch_bounds__(D * kJoinSplit) kv_join_kernel(const __grid_co
     const int64_t w0 = ((u0 + 1) * warps - 1) / total, w1 = (u1 * warps - 1) / total;
     if (w0 == w1) return;  // one warp had all of it
     const int count = total >= warps ? (int)(w1 - w0 + 1) : nb;
+    const int first = w0 * total / warps >= u0 ? 0 : 1;  // w0 began with an earlier pair
+    if (part < split) {
 #pragma unroll 4
-    for (int i = part; i < count; i += kJoinSplit) {
-      const int64_t w = total >= warps ? w0 + i : ((u0 + i + 1) * warps - 1) / total;
-      const int64_t slot = w * 2 + (i > 0 || w0 * total / warps >= u0 ? 0 : 1);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot * 16 + row % tile) * 2));
-      const float ow = __ldcg(p.part_o + (slot * 16 + row % tile) * D + d);
-      const float n = fmaxf(m, ml.x), z = n == -INFINITY ? 0.0f : n;
-      const float c = exp2_fast(m - z), cw = exp2_fast(ml.x - z);
-      v = v * c + ow * cw;
-      l = l * c + ml.y * cw;
-      m = n;
+      for (int i = part; i < count; i += split) {
+        const int64_t w = total >= warps ? w0 + i : ((u0 + i + 1) * warps - 1) / total;
+        const int64_t at = (w * 2 + (i == 0 ? first : 0)) * 16 + row;
+        take(__ldcg(reinterpret_cast<const float2*>(p.part_ml) + at), __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4));
+      }
     }
-    s_o[part][d] = v;
-    if (d == 0) {
-      s_m[part] = m;
-      s_l[part] = l;
-    }
+    s_o[threadIdx.x] = v;
+    s_ml[threadIdx.x] = make_float2(m, l);
     __syncthreads();
     if (part > 0) return;
-#pragma unroll
-    for (int i = 1; i < kJoinSplit; ++i) {
-      const float n = fmaxf(m, s_m[i]), z = n == -INFINITY ? 0.0f : n;
-      const float c = exp2_fast(m - z), cw = exp2_fast(s_m[i] - z);
-      v = v * c + s_o[i][d] * cw;
-      l = l * c + s_l[i] * cw;
-      m = n;
-    }
-    v = l > 0.0f ? v / l : (l == 0.0f ? 0.0f : l);
+    for (int i = 1; i < split; ++i) take(s_ml[i * per + threadIdx.x], s_o[i * per + threadIdx.x]);
+    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
   } else if (part > 0) {
     return;
   }
-  const int64_t at = ((int64_t)bh * p.G + row) * D + d;
-  uint16_t r;
-  if (p.dtype == kDtBF16) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
-  else r = __half_as_ushort(__float2half_rn(v));
-  static_cast<uint16_t*>(p.out)[at] = r;
+  uint32_t x, y;
+  if (p.dtype == kDtBF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w), "f"(v.z));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w), "f"(v.z));
+  }
+  const int64_t at = (((int64_t)b * p.Hkv + head) * p.G + r0 + row) * D + d4 * 4;
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(x, y);
 }
 
 // ---------------------------------------------------------------------------
@@ -754,8 +759,8 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.Hkv * p.G));
-  cfg.blockDim = dim3(D * kJoinSplit);
+  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.Hkv * p.row_tiles));
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = (size_t)(p.B + 1) * 4;
   cfg.stream = st;
   cfg.attrs = &at;
