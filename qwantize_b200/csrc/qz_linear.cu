@@ -13,16 +13,21 @@
 //
 // Two launches: quantize_rows_kernel (one CTA per row), then linear_kernel.
 //
-// linear_kernel, one persistent CTA per SM, 192 threads: warp 0 feeds a ring of
+// linear_kernel, one persistent CTA per SM, 224 threads: warp 0 feeds a ring of
 // stages (256 values of K: 128-byte swizzled rows of A and B by TMA, their
-// scales by bulk copies), warp 1 copies the stage's scales to TMEM
-// (tcgen05.cp) and issues four block-scaled MMAs of K = 64, warps 2-5 drain the
-// accumulator.  The wide form (BN = 256) has 128 token rows as A and 256 rows
+// scales by bulk copies), warp 6 copies a stage's scales to TMEM (tcgen05.cp),
+// warp 1 issues its four block-scaled MMAs of K = 64, warps 2-5 drain the
+// accumulator.  A stage of the wide form is 12 copies and 4 MMAs, and issuing an
+// instruction takes about 30 clocks, so one warp issuing both (700 clocks a
+// stage) could not keep up with the MMAs (543).  The wide form (BN = 256) has 128 token rows as A and 256 rows
 // of W as B.  The narrow forms (BN = 16 .. 128) swap the operands: 128 rows of
 // W are A and BN tokens are B, so that a decode step multiplies few padded
-// rows, and W streams through the ring once.  With few tiles K is cut into
-// splits; the last CTA of a tile adds the splits' fp32 partials in split order
-// (the order of arrival changes nothing).
+// rows, and W streams through the ring once.  Tiles that do not fill a wave of
+// the SMs (all of a decode step's, the last ones of a prompt's) are cut along K:
+// their stages form one list that a number of CTAs share evenly; the last CTA
+// to finish a tile adds the CTAs' fp32 partials in order (the order of arrival
+// changes nothing).  The second launch starts before the first has ended and
+// fetches its first stages of W meanwhile.
 //
 // Scales in memory, for both operands: row tiles of 128 rows (x, narrow form:
 // BN rows), groups of 4 blocks of K; a group is 512 bytes, row r at
@@ -57,37 +62,80 @@ struct Fmt {
 // ---------------------------------------------------------------------------
 // activations to FP4
 // ---------------------------------------------------------------------------
-// One CTA per row, one thread per block of BS values.  Bound by HBM for many
-// rows and by one DRAM round trip for few; the second read of the row (after
-// its maximum is known) comes from L1 / L2.
-template <int BS, int DT>
-__global__ void __launch_bounds__(512) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t K,
-                                                            uint8_t* __restrict__ packed, int64_t ldp,
-                                                            uint8_t* __restrict__ sf, int gran, int64_t n_steps,
-                                                            float* __restrict__ row_scale, int* __restrict__ counters,
-                                                            int n_counters) {
+// The largest magnitude of 16 bytes of elements, as bits that order like it:
+// fp32 bits (bf16 and fp32 input) or fp16 bits.
+template <int DT>
+__device__ __forceinline__ uint32_t abs_max(const uint4& w) {
+  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (DT == kDtF32) m = max(m, ww[k] & 0x7fffffffu);
+    else if (DT == kDtBF16) m = max(m, max(ww[k] & 0x7fff0000u, ww[k] << 16 & 0x7fff0000u));
+    else m = max(m, max(ww[k] >> 16 & 0x7fffu, ww[k] & 0x7fffu));
+  }
+  return m;
+}
+
+template <int DT, int VEC, int BS>
+__device__ __forceinline__ void unpack(const uint4 (&w)[VEC], float (&v)[BS]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DT == kDtF32) {
+        v[4 * i + k] = __uint_as_float(ww[k]);
+      } else {
+        v[8 * i + 2 * k] = DT == kDtBF16 ? bf16_bits_to_float(ww[k] & 0xffffu) : f16_bits_to_float(ww[k] & 0xffffu);
+        v[8 * i + 2 * k + 1] = DT == kDtBF16 ? bf16_bits_to_float(ww[k] >> 16) : f16_bits_to_float(ww[k] >> 16);
+      }
+    }
+  }
+}
+
+// One CTA per row.  A thread keeps its first R blocks of BS values in registers
+// between the row's maximum and the rounding (later ones of very long rows
+// are read again, from L2): R = 1 for few rows, where the latency of one row
+// counts, R = 4 for many, where loads in flight do.
+template <int BS, int DT, int R>
+__global__ void __launch_bounds__(R == 1 ? 512 : 256)
+    quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t K, uint8_t* __restrict__ packed, int64_t ldp,
+                         uint8_t* __restrict__ sf, int gran, int64_t n_steps, float* __restrict__ row_scale,
+                         int* __restrict__ counters, int n_counters) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ uint32_t s_max[16];
+  constexpr int kVec = BS * Elem<DT>::kSize / 16;  // 16-byte loads per block
   const int64_t row = blockIdx.x;
-  const char* base = static_cast<const char*>(x) + row * ldx * Elem<DT>::kSize;
+  const uint4* base = reinterpret_cast<const uint4*>(static_cast<const char*>(x) + row * ldx * Elem<DT>::kSize);
   const int64_t nb = K / BS, nb_pad = n_steps * Fmt<BS>::kBlocks, nb_packed = ldp * 2 / BS;
   const int tid = threadIdx.x, nt = blockDim.x;
   if (row == 0)
     for (int i = tid; i < n_counters; i += nt) counters[i] = 0;
+  uint4 raw[R][kVec];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const int64_t b = tid + (int64_t)r * nt;
+      raw[r][v] = b < nb ? __ldg(base + b * kVec + v) : make_uint4(0, 0, 0, 0);
+    }
   float inv = 1.0f, p = 1.0f;
   if (BS == 16) {
     uint32_t m = 0;
-    for (int64_t b = tid; b < nb; b += nt) {
-      float v[BS];
-      load_block<BS, DT>(base, b, v);
 #pragma unroll
-      for (int i = 0; i < BS; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int v = 0; v < kVec; ++v) m = max(m, abs_max<DT>(raw[r][v]));
+    for (int64_t b = tid + (int64_t)R * nt; b < nb; b += nt)
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) m = max(m, abs_max<DT>(__ldg(base + b * kVec + v)));
+    m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
     m = 0;
     for (int w = 0; w < (nt >> 5); ++w) m = max(m, s_max[w]);
+    if (DT == kDtF16) m = __float_as_uint(f16_bits_to_float(m));
     // smallest e with max <= 1.3125 * 2^(11 + e); 0 for an all-zero row and for inf / NaN
     int e = 0;
     if (m != 0 && m < 0x7f800000u) {
@@ -99,13 +147,12 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const void* __restri
   }
   if (tid == 0) row_scale[row] = p;
   uint8_t* sf_row = sf + (row / gran) * n_steps * Fmt<BS>::kSfBytes + (row % gran % 32) * 16 + (row % gran / 32) * 4;
-  for (int64_t b0 = 0; b0 < nb_pad; b0 += nt) {
-    const int64_t b = b0 + tid;
+  auto block = [&](int64_t b, const uint4 (&w)[kVec]) {
     uint32_t code = 0;
     uint32_t words[BS / 8] = {};
     if (b < nb) {
       float v[BS];
-      load_block<BS, DT>(base, b, v);
+      unpack<DT, kVec>(w, v);
       uint32_t am = 0;
 #pragma unroll
       for (int i = 0; i < BS; ++i) {
@@ -146,9 +193,18 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const void* __restri
       else *reinterpret_cast<uint4*>(packed + row * ldp + b * 16) = make_uint4(words[0], words[1], words[BS / 16], words[BS / 8 - 1]);
     }
     // four neighbouring blocks share one scale word
-    uint32_t w = code | __shfl_down_sync(0xffffffffu, code, 1) << 8;
-    w |= __shfl_down_sync(0xffffffffu, w, 2) << 16;
-    if ((tid & 3) == 0 && b < nb_pad) *reinterpret_cast<uint32_t*>(sf_row + (b >> 2) * kGroupBytes) = w;
+    uint32_t sw = code | __shfl_down_sync(0xffffffffu, code, 1) << 8;
+    sw |= __shfl_down_sync(0xffffffffu, sw, 2) << 16;
+    if ((tid & 3) == 0 && b < nb_pad) *reinterpret_cast<uint32_t*>(sf_row + (b >> 2) * kGroupBytes) = sw;
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if ((int64_t)r * nt < nb_pad) block(tid + (int64_t)r * nt, raw[r]);
+  for (int64_t b0 = (int64_t)R * nt; b0 < nb_pad; b0 += nt) {
+    uint4 w[kVec];
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) w[v] = b0 + tid < nb ? __ldg(base + (b0 + tid) * kVec + v) : make_uint4(0, 0, 0, 0);
+    block(b0 + tid, w);
   }
 }
 
@@ -175,11 +231,13 @@ __global__ void scale_layout_kernel(const uint8_t* __restrict__ codes, int64_t N
 struct LinearParams {
   int64_t T, N;                       // tokens, output features
   int64_t tiles_a, tiles_b;           // 128-row A tiles, BN-row B tiles
-  int splits, n_steps;                // K splits, stages over the whole of K
-  int64_t n_units;
+  int64_t whole;                      // tiles run whole, tile i by CTA i % grid
+  int64_t shared_steps;               // stages of the tiles after them, in tile order,
+  int sharers;                        // which the CTAs below `sharers` take in equal runs
+  int n_steps;                        // stages over the whole of K
   const uint8_t *sf_a, *sf_b;         // scales: tile-major, n_steps * kSfBytes each
-  float* partial;                     // splits > 1: (tile, split, column, 128) fp32
-  int* counters;                      // splits > 1: arrivals per tile, zeroed by the quantization launch
+  float* partial;                     // (sharer, 2, column, 128) fp32
+  int* counters;                      // arrivals per shared tile, zeroed by the quantization launch
   const float* row_scale;             // p_t
   float w_scale;
   const void* bias;
@@ -187,7 +245,7 @@ struct LinearParams {
   void* out;
   int out_dtype;
   int64_t ldo;
-  int vec;                            // 16-byte stores are aligned (wide form, 16-bit outputs)
+  int tma_out;                        // map_out is valid (wide form, 16-bit output, 16-byte rows)
 };
 
 template <int BN, int BS>
@@ -197,33 +255,39 @@ struct LinGeo {
   static constexpr int kBTiles = BN > 128 ? BN / 128 : 1;  // 128-row scale tiles of B
   static constexpr int kSf = Fmt<BS>::kSfBytes;
   static constexpr int kStageBytes = kABytes + kBBytes + kSf * (1 + kBTiles);
-  static constexpr int kMaxStages = (232448 - 1024 - 512) / kStageBytes;
+  static constexpr int kOutBytes = kSwap ? 0 : 4 * 2048;   // wide: 32 rows x 32 columns of output per epilogue warp
+  static constexpr int kMaxStages = (232448 - 1024 - 512 - kOutBytes) / kStageBytes;
   static constexpr int kStages = kMaxStages > 10 ? 10 : kMaxStages;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 512;
-  static constexpr int kAccs = BN > 128 ? 1 : 2;
-  // TMEM: accumulators, then kSfBufs buffers of scales (kGroups * 4 columns per 128 rows)
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024 + 512;
+  // TMEM: two accumulators, then kSfBufs buffers of scales (kGroups * 4 columns
+  // per 128 rows).  The wide form's accumulators share kOverlap columns, which
+  // are drained first: the next tile begins when they are free.
   static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * (1 + kBTiles);
   static constexpr int kSfBufs = BN > 128 ? 2 : 4;
-  static constexpr int kAccCols = BN > 128 ? 256 : 2 * BN;
+  static constexpr int kOverlap = BN > 128 ? 96 : 0;
+  static constexpr int kAccCols = 2 * BN - kOverlap;
   static_assert(kAccCols + kSfBufs * kSfCols <= 512, "TMEM columns");
 };
 
 // Block-scaled MMA, E2M1 x E2M1 -> fp32, K = 64, scales of A and B in TMEM:
 // one E4M3 scale per 16 values (NVFP4) or one power of two per 32 (MXFP4).
+// a, b: low words of the operands' descriptors (address / 16, K-major rows of
+// 128 swizzled bytes, 8-row groups 1024 bytes apart).
+constexpr uint32_t kDescRows = 1u << 16, kDescRowsHi = (1024u >> 4) | 1u << 14 | 2u << 29;
 template <int BS>
-__device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+__device__ __forceinline__ void umma_fp4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                          uint32_t accumulate) {
   if constexpr (BS == 16)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %7};\n mov.b64 y, {%2, %7};\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], x, y, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "r"(a | kDescRows), "r"(b | kDescRows), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "n"(kDescRowsHi)
         : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %7};\n mov.b64 y, {%2, %7};\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "r"(a | kDescRows), "r"(b | kDescRows), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "n"(kDescRowsHi)
         : "memory");
 }
 
@@ -236,13 +300,34 @@ __host__ __device__ constexpr uint32_t idesc_fp4(int N, uint32_t sf_id) {
          ((uint32_t)(128 >> 4) << 24) | (sf_id << 29);
 }
 
-// 32 rows of 16 bytes (512 contiguous bytes) -> 4 TMEM columns, spread to all
-// four 32-lane quarters.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
-  // no swizzle; 8-row groups 128 bytes apart
-  const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 |
-                        (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// 32 rows of 16 bytes (512 contiguous bytes at 16 * lo, no swizzle, 8-row groups
+// 128 bytes apart) -> 4 TMEM columns, spread to all four 32-lane quarters.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t lo) {
+  asm volatile(
+      "{\n .reg .b64 x;\n mov.b64 x, {%1, %2};\n tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], x;\n}\n" ::"r"(taddr),
+      "r"(lo | (128u >> 4) << 16), "n"((128u >> 4) | 1u << 14)
+      : "memory");
+}
+
+// 32 lanes x 32 bits, C consecutive columns per thread.
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[C]) {
+  if constexpr (C == 16) {
+    tmem_ld16(taddr, v);
+  } else {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  }
 }
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
@@ -263,48 +348,83 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   else static_cast<uint16_t*>(p)[i] = (uint16_t)(pack16(v, 0.0f, dtype) & 0xffffu);
 }
 
-struct LinUnit {
-  int64_t a, b, tile;
-  int split, s0, s1;
+// One CTA's work: its whole tiles, then its run of the shared stages, which may
+// begin and end inside a tile.
+template <bool SWAP>
+struct LinWork {
+  const LinearParams& p;
+  int64_t a, b;        // tile coordinates
+  int s0, s1;          // stages [s0, s1) of it
+  int64_t shared;      // index among the shared tiles, -1 for a whole tile
+  bool first;          // the run begins with this segment
+  int64_t tile, pos, end;
+
+  __device__ __forceinline__ explicit LinWork(const LinearParams& q) : p(q), tile(blockIdx.x) {
+    pos = end = 0;
+    if ((int)blockIdx.x < p.sharers) {
+      pos = (int64_t)blockIdx.x * p.shared_steps / p.sharers;
+      end = (int64_t)(blockIdx.x + 1) * p.shared_steps / p.sharers;
+    }
+    first = true;
+    shared = -1;
+  }
+  __device__ __forceinline__ void coords(int64_t i) {
+    if (SWAP) {
+      a = i % p.tiles_a;
+      b = i / p.tiles_a;
+    } else {
+      // bands of 16 token tiles: the ~148 tiles in flight are about as many
+      // token rows as weight rows and share both through L2
+      const int64_t per = 16 * p.tiles_b, band = i / per, r = i % per;
+      const int64_t left = p.tiles_a - band * 16, rows = left < 16 ? left : 16;
+      b = r / rows;
+      a = band * 16 + r % rows;
+    }
+  }
+  __device__ __forceinline__ bool next() {
+    if (tile < p.whole) {
+      coords(tile);
+      s0 = 0;
+      s1 = p.n_steps;
+      tile += gridDim.x;
+      return true;
+    }
+    if (pos >= end) return false;
+    if (shared >= 0) first = false;
+    shared = pos / p.n_steps;
+    coords(p.whole + shared);
+    s0 = (int)(pos % p.n_steps);
+    s1 = end - pos < p.n_steps - s0 ? s0 + (int)(end - pos) : p.n_steps;
+    pos += s1 - s0;
+    return true;
+  }
+  // the sharer that has stage `at` of the shared list
+  __device__ __forceinline__ int owner(int64_t at) const {
+    return (int)(((at + 1) * p.sharers - 1) / p.shared_steps);
+  }
 };
 
-// Units: the splits of one tile side by side; wide tiles in bands of 16 token
-// tiles, so that the ~148 tiles in flight are about as many token rows as
-// weight rows and share both through L2.
-template <bool SWAP>
-__device__ __forceinline__ LinUnit lin_unit(const LinearParams& p, int64_t t) {
-  LinUnit u;
-  u.split = (int)(t % p.splits);
-  u.tile = t / p.splits;
-  if (SWAP) {
-    u.a = u.tile % p.tiles_a;
-    u.b = u.tile / p.tiles_a;
-  } else {
-    const int64_t per = 16 * p.tiles_b, band = u.tile / per, r = u.tile % per;
-    const int64_t left = p.tiles_a - band * 16, rows = left < 16 ? left : 16;
-    u.b = r / rows;
-    u.a = band * 16 + r % rows;
-  }
-  u.s0 = (int)((int64_t)u.split * p.n_steps / p.splits);
-  u.s1 = (int)((int64_t)(u.split + 1) * p.n_steps / p.splits);
-  return u;
-}
+constexpr int kLinThreads = 224;
 
 template <int BN, int BS>
-__global__ void __launch_bounds__(192, 1)
-    linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, LinearParams p) {
+__global__ void __launch_bounds__(kLinThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LinearParams p) {
   using G = LinGeo<BN, BS>;
   constexpr bool SWAP = G::kSwap;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // operands first (1024-byte swizzle atoms), then the scales of all stages, then barriers
-  unsigned char* smem_sf = smem + G::kStages * (G::kABytes + G::kBBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes);
+  // operands (1024-byte swizzle atoms), output staging, the scales of all stages, barriers
+  unsigned char* smem_out = smem + G::kStages * (G::kABytes + G::kBBytes);
+  unsigned char* smem_sf = smem_out + G::kOutBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes + G::kOutBytes);
   uint64_t* empty = full + G::kStages;
   uint64_t* tfull = empty + G::kStages;
   uint64_t* tempty = tfull + 2;
-  uint64_t* mma_done = tempty + 2;
-  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* sf_full = tempty + 2;
+  uint64_t* mma_done = sf_full + G::kSfBufs;
+  uint64_t* sf_done = mma_done + 1;
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(sf_done + 1);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
   volatile int* last_s = abort_s + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -312,7 +432,9 @@ __global__ void __launch_bounds__(192, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull + a, 1); mbar_init(tempty + a, 128); }
+    for (int b = 0; b < G::kSfBufs; ++b) mbar_init(sf_full + b, 1);
     mbar_init(mma_done, 1);
+    mbar_init(sf_done, 1);
     *abort_s = 0;
     fence_barrier_init();
   }
@@ -339,21 +461,45 @@ __global__ void __launch_bounds__(192, 1)
   if (warp == 0) {
     // ---------------- producer ----------------
     if (lane == 0) {
-      uint32_t it = 0;
-      for (int64_t t = blockIdx.x; t < p.n_units; t += gridDim.x) {
-        const LinUnit u = lin_unit<SWAP>(p, t);
-        for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
-          const int s = it % G::kStages;
-          if (!wait(empty + s, ((it / G::kStages) & 1) ^ 1, kDevErrLoadTimeout)) goto producer_done;
-          unsigned char* sa = smem + s * (G::kABytes + G::kBBytes);
-          unsigned char* sf = smem_sf + s * G::kSf * (1 + G::kBTiles);
-          mbar_arrive_expect_tx(full + s, G::kStageBytes);
+      auto load_w = [&](const LinWork<SWAP>& u, int ks, int s) {
+        unsigned char* sa = smem + s * (G::kABytes + G::kBBytes);
+        unsigned char* sf = smem_sf + s * G::kSf * (1 + G::kBTiles);
+        mbar_arrive_expect_tx(full + s, G::kStageBytes);
+        if (SWAP) {
           tma_load_2d(sa, &map_a, ks * 128, (int)(u.a * 128), full + s);
-          tma_load_2d(sa + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
           bulk_load(sf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+        } else {
+          tma_load_2d(sa + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
 #pragma unroll
           for (int h = 0; h < G::kBTiles; ++h)
             bulk_load(sf + (1 + h) * G::kSf, p.sf_b + ((u.b * G::kBTiles + h) * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+        }
+      };
+      auto load_x = [&](const LinWork<SWAP>& u, int ks, int s) {
+        unsigned char* sa = smem + s * (G::kABytes + G::kBBytes);
+        unsigned char* sf = smem_sf + s * G::kSf * (1 + G::kBTiles);
+        if (SWAP) {
+          tma_load_2d(sa + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
+          bulk_load(sf + G::kSf, p.sf_b + (u.b * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+        } else {
+          tma_load_2d(sa, &map_a, ks * 128, (int)(u.a * 128), full + s);
+          bulk_load(sf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+        }
+      };
+      // the first ring of weights does not wait for the quantization launch
+      uint32_t ahead = 0;
+      for (LinWork<SWAP> u(p); ahead < (uint32_t)G::kStages && u.next();)
+        for (int ks = u.s0; ks < u.s1 && ahead < (uint32_t)G::kStages; ++ks, ++ahead) load_w(u, ks, ahead);
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      uint32_t it = 0;
+      for (LinWork<SWAP> u(p); u.next();) {
+        for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
+          const int s = it % G::kStages;
+          if (it >= ahead) {
+            if (!wait(empty + s, ((it / G::kStages) & 1) ^ 1, kDevErrLoadTimeout)) goto producer_done;
+            load_w(u, ks, s);
+          }
+          load_x(u, ks, s);
         }
       }
     producer_done:
@@ -362,146 +508,224 @@ __global__ void __launch_bounds__(192, 1)
         mbar_wait_bounded(full + (k % G::kStages), (k / G::kStages) & 1, kDevErrLoadTimeout);
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      uint32_t it = 0, lt = 0;
-      for (int64_t t = blockIdx.x; t < p.n_units; t += gridDim.x, ++lt) {
-        const LinUnit u = lin_unit<SWAP>(p, t);
-        const uint32_t acc = G::kAccs == 2 ? (lt & 1) : 0u;
-        const uint32_t phase = G::kAccs == 2 ? ((lt >> 1) & 1) : (lt & 1);
-        if (!wait(tempty + acc, phase ^ 1, kDevErrMmaTimeout)) break;
+    // ---------------- MMA issuer (the warp waits together, one lane issues) ----------------
+    // low words of the descriptors of stage 0; a stage further is an addition
+    const uint32_t lo_a = smem_u32(smem) >> 4, lo_b = lo_a + (G::kABytes >> 4);
+    uint32_t lt = 0, s = 0, ph = 0, sb = 0, sph = 0;  // stage, scale buffer, their phases
+    for (LinWork<SWAP> u(p); u.next(); ++lt) {
+      const uint32_t acc = lt & 1;
+      // narrow: this accumulator is drained; wide: the columns shared with the previous tile's are
+      bool ok = SWAP ? wait(tempty + acc, (lt >> 1 & 1) ^ 1, kDevErrMmaTimeout)
+                     : lt == 0 || wait(tempty, (lt - 1) & 1, kDevErrMmaTimeout);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + acc * (BN - G::kOverlap);
+      for (int ks = u.s0; ks < u.s1; ++ks) {
+        ok = wait(full + s, ph, kDevErrMmaTimeout) && wait(sf_full + sb, sph, kDevErrMmaTimeout);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        bool ok = true;
-        for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
-          const int s = it % G::kStages;
-          if (!wait(full + s, (it / G::kStages) & 1, kDevErrMmaTimeout)) { ok = false; break; }
-          // this scale buffer was last read by the MMAs kSfBufs stages ago
-          if (it >= (uint32_t)G::kSfBufs) {
-            const uint32_t j = it - G::kSfBufs;
-            if (!wait(empty + j % G::kStages, (j / G::kStages) & 1, kDevErrMmaTimeout)) { ok = false; break; }
-          }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * (G::kABytes + G::kBBytes)), sb = sa + G::kABytes;
-          const uint32_t sf = smem_u32(smem_sf + s * G::kSf * (1 + G::kBTiles));
-          const uint32_t t_sfa = tmem_base + G::kAccCols + (it % G::kSfBufs) * G::kSfCols;
-          const uint32_t t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
-#pragma unroll
-          for (int q = 0; q < Fmt<BS>::kGroups; ++q) {
-            tmem_cp_scales(t_sfa + 4 * q, sf + q * kGroupBytes);
-#pragma unroll
-            for (int h = 0; h < G::kBTiles; ++h)
-              tmem_cp_scales(t_sfb + (q * G::kBTiles + h) * 4, sf + (1 + h) * G::kSf + q * kGroupBytes);
-          }
+        const uint32_t da = lo_a + s * ((G::kABytes + G::kBBytes) >> 4), db = lo_b + s * ((G::kABytes + G::kBBytes) >> 4);
+        const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
+        const uint32_t first = ks > u.s0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const int q = BS == 16 ? kk : kk / 2;
-            umma_fp4<BS>(d_tmem, smem_desc(sa + kk * 32, 16, 1024), smem_desc(sb + kk * 32, 16, 1024),
-                         idesc_fp4<BS>(BN, BS == 16 ? 0u : (kk & 1) * 2u), t_sfa + 4 * q, t_sfb + 4 * q * G::kBTiles,
-                         (ks > u.s0 || kk > 0) ? 1u : 0u);
+            umma_fp4<BS>(d_tmem, da + 2 * kk, db + 2 * kk, idesc_fp4<BS>(BN, BS == 16 ? 0u : (kk & 1) * 2u), t_sfa + 4 * q,
+                         t_sfb + 4 * q * G::kBTiles, kk > 0 ? 1u : first);
           }
           umma_commit(empty + s);
+          if (ks + 1 == u.s1) umma_commit(tfull + acc);
         }
-        if (!ok) break;
-        umma_commit(tfull + acc);
+        __syncwarp();
+        if (++sb == (uint32_t)G::kSfBufs) { sb = 0; sph ^= 1; }
+        if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
       }
-      // the MMAs issued must retire before TMEM is freed (also after an abort)
-      umma_commit(mma_done);
-      mbar_wait_bounded(mma_done, 0u, kDevErrMmaTimeout);
+      if (!ok) break;
     }
+    // the MMAs issued must retire before TMEM is freed (also after an abort)
+    __syncwarp();
+    if (elect_one()) umma_commit(mma_done);
+    __syncwarp();
+    mbar_wait_bounded(mma_done, 0u, kDevErrMmaTimeout);
+  } else if (warp == 6) {
+    // ---------------- scales to TMEM ----------------
+    const uint32_t lo_sf = smem_u32(smem_sf) >> 4;
+    uint32_t s = 0, ph = 0, sb = 0, warm = 0;  // warm: scale buffers used so far, up to kSfBufs
+    bool ok = true;
+    for (LinWork<SWAP> u(p); ok && u.next();) {
+      for (int ks = u.s0; ks < u.s1; ++ks) {
+        ok = wait(full + s, ph, kDevErrMmaTimeout);
+        // this scale buffer was last read by the MMAs kSfBufs stages ago
+        if (warm == (uint32_t)G::kSfBufs) {
+          const bool wrap = s < (uint32_t)G::kSfBufs;
+          ok = ok && wait(empty + (wrap ? s + G::kStages - G::kSfBufs : s - G::kSfBufs), wrap ? ph ^ 1 : ph, kDevErrMmaTimeout);
+        } else {
+          ++warm;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ds = lo_sf + s * (G::kSf * (1 + G::kBTiles) >> 4);
+        const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
+        if (elect_one()) {
+#pragma unroll
+          for (int q = 0; q < Fmt<BS>::kGroups; ++q) {
+            tmem_cp_scales(t_sfa + 4 * q, ds + q * (kGroupBytes >> 4));
+#pragma unroll
+            for (int h = 0; h < G::kBTiles; ++h)
+              tmem_cp_scales(t_sfb + (q * G::kBTiles + h) * 4, ds + (((1 + h) * G::kSf + q * kGroupBytes) >> 4));
+          }
+          umma_commit(sf_full + sb);
+        }
+        __syncwarp();
+        if (++sb == (uint32_t)G::kSfBufs) sb = 0;
+        if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
+      }
+    }
+    // the copies issued must have ended before TMEM is freed (also after an abort)
+    __syncwarp();
+    if (elect_one()) umma_commit(sf_done);
+    __syncwarp();
+    mbar_wait_bounded(sf_done, 0u, kDevErrMmaTimeout);
   } else {
     // ---------------- epilogue (warps 2-5) ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales and counters are the quantization launch's
+    constexpr int C = BN < 32 ? BN : 32;     // columns drained at a time
     const int row = (warp & 3) * 32 + lane;  // accumulator row of this thread
+    unsigned char* stage_out = smem_out + (warp & 3) * 2048;
     uint32_t lt = 0;
-    for (int64_t t = blockIdx.x; t < p.n_units; t += gridDim.x, ++lt) {
-      const LinUnit u = lin_unit<SWAP>(p, t);
-      const uint32_t acc = G::kAccs == 2 ? (lt & 1) : 0u;
-      const uint32_t phase = G::kAccs == 2 ? ((lt >> 1) & 1) : (lt & 1);
+    for (LinWork<SWAP> u(p); u.next(); ++lt) {
+      const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
+      const int64_t ra = u.a * 128 + row;       // swapped: output feature; wide: token
+      const int64_t cb = u.b * BN;              // swapped: first token; wide: first output feature
+      const int64_t cols_left = (SWAP ? p.T : p.N) - cb;
+      const int cols = cols_left < BN ? (int)cols_left : BN;
+      const bool in = ra < (SWAP ? p.N : p.T);
+      // what belongs to this thread's row: the scale of its token, or the bias of its feature
+      const float mine = !in ? 0.0f : SWAP ? (p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f) : __ldg(p.row_scale + ra) * p.w_scale;
+      // sharers of this tile
+      int c0 = 0, c1 = 0;
+      if (u.shared >= 0) {
+        c0 = u.owner(u.shared * p.n_steps);
+        c1 = u.owner((u.shared + 1) * p.n_steps - 1);
+      }
+      const bool split = c0 != c1;
       uint32_t go = wait(tfull + acc, phase, kDevErrEpilogueTimeout) ? 1u : 0u;
-      if (p.splits > 1)  // all epilogue threads go on or all stop: the barriers below count on it
+      if (split)  // all epilogue threads go on or all stop: the barriers below count on it
         asm volatile(
             "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, 1, 128, a;\n selp.u32 %0, 1, 0, b;\n}\n"
             : "+r"(go)::"memory");
       if (!go) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * BN;
-      const int64_t ra = u.a * 128 + row;       // swapped: output feature; wide: token
-      const int64_t cb = u.b * BN;              // swapped: first token; wide: first output feature
-      const int64_t cols_left = (SWAP ? p.T : p.N) - cb;
-      const int cols = cols_left < BN ? (int)cols_left : BN;
-      // finish 16 columns: scale, bias, round once, store
-      auto finish = [&](int c, const float(&v)[16]) {
-        if (ra >= (SWAP ? p.N : p.T)) return;
+      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * (BN - G::kOverlap);
+      // the order in which columns are drained: the wide form's shared ones (the
+      // last of accumulator 0, the first of accumulator 1) come first
+      const int c_first = !SWAP && acc == 0 ? BN - G::kOverlap : 0;
+      auto drained = [&](int i) {  // after the i-th group of C columns
+        if (SWAP ? i + 1 == BN / C : i + 1 == G::kOverlap / C) {
+          tc_fence_before();
+          mbar_arrive(SWAP ? tempty + acc : tempty);
+        }
+      };
+      // the column's share: lane q has the token scale, or the bias, of column c + q
+      auto column = [&](int c) -> float {
+        if (c + lane >= cols || lane >= C) return 0.0f;
+        if (SWAP) return __ldg(p.row_scale + cb + c + lane) * p.w_scale;
+        return p.bias ? load_any(p.bias, p.bias_dtype, cb + c + lane) : 0.0f;
+      };
+      // finish C columns: scale, bias, round once, store
+      auto finish = [&](int c, float(&v)[C], float col) {
         if constexpr (SWAP) {
-          const float bias = p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f;
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (c + q < cols) {
-              const int64_t tok = cb + c + q;
-              store_any(p.out, p.out_dtype, tok * p.ldo + ra, __fmaf_rn(v[q], p.row_scale[tok] * p.w_scale, bias));
-            }
+          for (int q = 0; q < C; ++q) {
+            const float f = __fmaf_rn(v[q], __shfl_sync(0xffffffffu, col, q), mine);
+            if (in && c + q < cols) store_any(p.out, p.out_dtype, (cb + c + q) * p.ldo + ra, f);
+          }
         } else {
-          const float sc = p.row_scale[ra] * p.w_scale;
-          float o[16];
+          if (p.bias) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            o[q] = __fmaf_rn(v[q], sc, p.bias && c + q < cols ? load_any(p.bias, p.bias_dtype, cb + c + q) : 0.0f);
-          const int64_t at = ra * p.ldo + cb + c;
-          if (p.vec && c + 16 <= cols) {
-            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
-            d[0] = make_uint4(pack16(o[0], o[1], p.out_dtype), pack16(o[2], o[3], p.out_dtype),
-                              pack16(o[4], o[5], p.out_dtype), pack16(o[6], o[7], p.out_dtype));
-            d[1] = make_uint4(pack16(o[8], o[9], p.out_dtype), pack16(o[10], o[11], p.out_dtype),
-                              pack16(o[12], o[13], p.out_dtype), pack16(o[14], o[15], p.out_dtype));
+            for (int q = 0; q < C; ++q) v[q] = __fmaf_rn(v[q], mine, __shfl_sync(0xffffffffu, col, q));
           } else {
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-              if (c + q < cols) store_any(p.out, p.out_dtype, at + q, o[q]);
+            for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], mine);
+          }
+          if (p.tma_out) {
+            // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+                  make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
+                             pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
+                           "r"((int)cb + c), "r"((int)(u.a * 128) + (warp & 3) * 32), "r"(smem_u32(stage_out))
+                           : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else if (in) {
+#pragma unroll
+            for (int q = 0; q < C; ++q)
+              if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
           }
         }
       };
-      if (p.splits == 1) {
+      if (!split) {
+        float col = column(c_first);
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 16) {
-          float v[16];
-          tmem_ld16(taddr + c, v);
-          finish(c, v);
+        for (int i = 0; i < BN / C; ++i) {
+          const int c = (c_first + i * C) % BN;
+          const float now = col;
+          col = column((c + C) % BN);
+          float v[C];
+          if (c < cols) tmem_ld<C>(taddr + c, v);
+          drained(i);
+          if (c < cols) finish(c, v, now);
         }
-        tc_fence_before();
-        mbar_arrive(tempty + acc);
         continue;
       }
-      float* part = p.partial + (u.tile * p.splits + u.split) * (int64_t)(BN * 128) + row;
+      float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u.first ? 0 : 1)) * (BN * 128) + row;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 16) {
-        float v[16];
-        tmem_ld16(taddr + c, v);
+      for (int i = 0; i < BN / C; ++i) {
+        const int c = (c_first + i * C) % BN;
+        float v[C];
+        if (c < cols) tmem_ld<C>(taddr + c, v);
+        drained(i);
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (c + q < cols) part[(c + q) * 128] = v[q];
+        for (int q = 0; q < C; ++q)
+          if (c + q < cols) __stcg(part + (c + q) * 128, v[q]);
       }
-      tc_fence_before();
-      mbar_arrive(tempty + acc);
       __threadfence();
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x == 64) *last_s = atomicAdd(p.counters + u.tile, 1) == p.splits - 1;
+      if (threadIdx.x == 64) *last_s = atomicAdd(p.counters + u.shared, 1) == c1 - c0;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       const bool last = *last_s != 0;
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // last_s is read before the next unit writes it
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // last_s is read before the next segment writes it
       if (!last) continue;
       __threadfence();
-      const float* all = p.partial + u.tile * p.splits * (int64_t)(BN * 128) + row;
+      // c0 may have begun with an earlier tile; the others begin with this one
+      const int begin = (int64_t)c0 * p.shared_steps / p.sharers >= u.shared * p.n_steps ? 0 : 1;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 16) {
-        float v[16] = {};
-        for (int sp = 0; sp < p.splits; ++sp) {
+      for (int c = 0; c < cols; c += C) {
+        float v[C] = {};
+        const float col = column(c);
+#pragma unroll 1
+        for (int w = c0; w <= c1; ++w) {
+          const float* from = p.partial + ((int64_t)w * 2 + (w == c0 ? begin : 0)) * (BN * 128) + row;
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (c + q < cols) v[q] += __ldcg(all + sp * (int64_t)(BN * 128) + (c + q) * 128);
+          for (int q = 0; q < C; ++q)
+            if (c + q < cols) v[q] += __ldcg(from + (c + q) * 128);
         }
-        finish(c, v);
+        finish(c, v, col);
       }
     }
+    // staged output has been written (the staging area goes away with the CTA)
+    if (!SWAP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -536,15 +760,31 @@ static int code_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t r
   return QZ_OK;
 }
 
-// Tile form and K splits of one call, and its workspace.
+// 16-bit output (T, N), written in boxes of 32 x 32.
+static int out_map(CUtensorMap* m, void* base, uint64_t N, uint64_t T, uint64_t ldo) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(QZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {N, T};
+  cuuint64_t strides[1] = {ldo * 2};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QZ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return QZ_OK;
+}
+
+// Tile form and sharing of one call, and its workspace.
 struct LinPlan {
-  int bn, splits, n_steps;
-  int64_t tiles_a, tiles_b, ldp;
+  int bn, sharers, n_steps;
+  int64_t tiles_a, tiles_b, whole, ldp;
   int64_t off_sf, off_scale, off_counter, off_partial, bytes;
 };
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// Chooses the form by an estimate in SM clocks: a stage costs its MMAs or its
+// bytes, a tile its epilogue, a shared tile the partials written and added.
 static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   LinPlan best{};
   double best_cost = -1.0;
@@ -554,17 +794,20 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     const bool swap = bn < 256;
     const int64_t ta = swap ? (N + 127) / 128 : (T + 127) / 128;
     const int64_t tb = swap ? (T + bn - 1) / bn : (N + 255) / 256;
-    const double stage = 128.0 * 128 + 128.0 * bn + 128.0 * 256 / bs * (1 + (bn > 128 ? 2 : 1));
-    for (int sp = 1; sp <= n_steps && sp <= 32; ++sp) {
-      const int64_t units = ta * tb * sp;
-      if (sp > 1 && units > 4 * sms) break;
-      const double waves = (double)((units + sms - 1) / sms);
-      // clocks: a stage's bytes at about 40 per clock and SM, or its MMAs; a unit's fill and epilogue
-      const double step = stage / 40.0 > 2.0 * bn ? stage / 40.0 : 2.0 * bn;
-      const double cost = waves * ((n_steps + sp - 1) / sp * step + 1200.0 + 6.0 * bn) + (sp > 1 ? 1500.0 + 4.0 * sp * (T < bn ? T : bn) : 0.0);
+    const double bytes = 128.0 * 128 + 128.0 * bn + 128.0 * 256 / bs * (1 + (bn > 128 ? 2 : 1));
+    const double step = bytes / 40.0 > 2.0 * bn ? bytes / 40.0 : 2.0 * bn;
+    const double epilogue = 600.0 + 12.0 * bn, add = 600.0 + (T < bn ? T : bn) * 128 * 4 / 60.0;
+    const int64_t tiles = ta * tb, whole = tiles / sms * sms, rest = tiles - whole;
+    for (int sp = 1; sp <= n_steps && sp <= 32; ++sp) {  // CTAs per shared tile, on average
+      if (rest == 0 && sp > 1) break;
+      int64_t sharers = rest * sp < sms ? rest * sp : sms;
+      if (sp > 1 && rest * (sp - 1) >= sms) break;
+      const double parts = rest ? (double)sharers / rest : 1.0;
+      const double cost = (double)(whole / sms) * (n_steps * step + epilogue) +
+                          (rest ? n_steps * step / parts + epilogue + (parts > 1.0 ? 1500.0 + (1.0 + parts) * add : 0.0) : 0.0);
       if (best_cost < 0 || cost < best_cost) {
         best_cost = cost;
-        best.bn = bn; best.splits = sp; best.tiles_a = ta; best.tiles_b = tb;
+        best.bn = bn; best.sharers = (int)sharers; best.tiles_a = ta; best.tiles_b = tb; best.whole = whole;
       }
     }
   }
@@ -572,33 +815,48 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   best.ldp = up(K, 32) / 2;
   const int gran = best.bn < 128 ? best.bn : 128;
   const int64_t sf_tiles = (T + gran - 1) / gran;
+  const int64_t rest = best.tiles_a * best.tiles_b - best.whole;
   best.off_sf = up(T * best.ldp, 256);
   best.off_scale = best.off_sf + up(sf_tiles * n_steps * (int64_t)(kStepK / bs / 4 * kGroupBytes), 256);
   best.off_counter = best.off_scale + up(T * 4, 256);
-  const int64_t tiles = best.tiles_a * best.tiles_b;
-  best.off_partial = best.off_counter + (best.splits > 1 ? up(tiles * 4, 256) : 0);
-  best.bytes = best.off_partial + (best.splits > 1 ? tiles * best.splits * best.bn * 128 * 4 : 0);
+  best.off_partial = best.off_counter + up(rest * 4, 256);
+  best.bytes = best.off_partial + (best.sharers > rest ? (int64_t)best.sharers * 2 * best.bn * 128 * 4 : 0);
   return best;
 }
 
-template <int BS>
-static cudaError_t launch_quantize_rows(const void* x, int dt, int64_t ldx, int64_t T, int64_t K, uint8_t* packed,
-                                        int64_t ldp, uint8_t* sf, int gran, int64_t n_steps, float* row_scale,
-                                        int* counters, int n_counters, cudaStream_t st) {
-  const int64_t nb = n_steps * Fmt<BS>::kBlocks;
-  const int nt = nb >= 512 ? 512 : (nb < 64 ? 64 : (int)up(nb, 32));
-  const unsigned grid = (unsigned)T;
-  if (dt == kDtBF16)
-    quantize_rows_kernel<BS, kDtBF16><<<grid, nt, 0, st>>>(x, ldx, K, packed, ldp, sf, gran, n_steps, row_scale, counters, n_counters);
-  else if (dt == kDtF16)
-    quantize_rows_kernel<BS, kDtF16><<<grid, nt, 0, st>>>(x, ldx, K, packed, ldp, sf, gran, n_steps, row_scale, counters, n_counters);
-  else
-    quantize_rows_kernel<BS, kDtF32><<<grid, nt, 0, st>>>(x, ldx, K, packed, ldp, sf, gran, n_steps, row_scale, counters, n_counters);
+struct QuantizeRows {
+  const void* x;
+  int dtype;
+  int64_t ldx, T, K;
+  uint8_t* packed;
+  int64_t ldp;
+  uint8_t* sf;
+  int gran;
+  int64_t n_steps;
+  float* row_scale;
+  int* counters;
+  int n_counters;
+};
+
+template <int BS, int R>
+static cudaError_t launch_quantize_rows(const QuantizeRows& q, cudaStream_t st) {
+  const int64_t threads = (q.n_steps * Fmt<BS>::kBlocks + R - 1) / R;
+  const int64_t most = R == 1 ? 512 : 256;
+  const int nt = threads >= most ? (int)most : (threads < 64 ? 64 : (int)up(threads, 32));
+  const unsigned grid = (unsigned)q.T;
+#define QZ_ROWS(DT)                                                                                                     \
+  quantize_rows_kernel<BS, DT, R><<<grid, nt, 0, st>>>(q.x, q.ldx, q.K, q.packed, q.ldp, q.sf, q.gran, q.n_steps,       \
+                                                       q.row_scale, q.counters, q.n_counters)
+  if (q.dtype == kDtBF16) QZ_ROWS(kDtBF16);
+  else if (q.dtype == kDtF16) QZ_ROWS(kDtF16);
+  else QZ_ROWS(kDtF32);
+#undef QZ_ROWS
   return cudaGetLastError();
 }
 
 template <int BN, int BS>
-static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p, int sms, cudaStream_t st) {
+static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
+                         cudaStream_t st) {
   using G = LinGeo<BN, BS>;
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
@@ -609,19 +867,28 @@ static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const Linea
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const int64_t grid = p.n_units < sms ? p.n_units : sms;
-  linear_kernel<BN, BS><<<(unsigned)grid, 192, G::kSmem, st>>>(a, b, p);
-  return cuda_status(cudaGetLastError(), "linear launch");
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.whole > 0 ? sms : p.sharers));
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS>, a, b, o, p), "linear launch");
 }
 
 template <int BS>
-static int run_linear(int bn, const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p, int sms, cudaStream_t st) {
+static int run_linear(int bn, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
+                      cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_linear<16, BS>(a, b, p, sms, st);
-    case 32: return launch_linear<32, BS>(a, b, p, sms, st);
-    case 64: return launch_linear<64, BS>(a, b, p, sms, st);
-    case 128: return launch_linear<128, BS>(a, b, p, sms, st);
-    default: return launch_linear<256, BS>(a, b, p, sms, st);
+    case 16: return launch_linear<16, BS>(a, b, o, p, sms, st);
+    case 32: return launch_linear<32, BS>(a, b, o, p, sms, st);
+    case 64: return launch_linear<64, BS>(a, b, o, p, sms, st);
+    case 128: return launch_linear<128, BS>(a, b, o, p, sms, st);
+    default: return launch_linear<256, BS>(a, b, o, p, sms, st);
   }
 }
 
@@ -705,8 +972,11 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   LinearParams p{};
   p.T = T; p.N = N;
   p.tiles_a = pl.tiles_a; p.tiles_b = pl.tiles_b;
-  p.splits = pl.splits; p.n_steps = pl.n_steps;
-  p.n_units = pl.tiles_a * pl.tiles_b * pl.splits;
+  p.whole = pl.whole;
+  const int64_t rest = pl.tiles_a * pl.tiles_b - pl.whole;
+  p.shared_steps = rest * pl.n_steps;
+  p.sharers = pl.sharers;
+  p.n_steps = pl.n_steps;
   p.sf_a = swap ? scales : ws + pl.off_sf;
   p.sf_b = swap ? ws + pl.off_sf : scales;
   p.row_scale = reinterpret_cast<float*>(ws + pl.off_scale);
@@ -715,16 +985,16 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   p.w_scale = tensor_scale;
   p.bias = bias; p.bias_dtype = bias_dtype;
   p.out = out; p.out_dtype = out_dtype; p.ldo = ldo;
-  p.vec = out_dtype != QZ_DTYPE_F32 && ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const int n_counters = pl.splits > 1 ? (int)(pl.tiles_a * pl.tiles_b) : 0;
-  const int gran = pl.bn < 128 ? pl.bn : 128;
-  float* rs = reinterpret_cast<float*>(ws + pl.off_scale);
-  s = cuda_status(bs == 16 ? launch_quantize_rows<16>(x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, gran, pl.n_steps,
-                                                      rs, p.counters, n_counters, st)
-                           : launch_quantize_rows<32>(x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, gran, pl.n_steps,
-                                                      rs, p.counters, n_counters, st),
+  p.tma_out = !swap && out_dtype != QZ_DTYPE_F32 && ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  CUtensorMap mo = mx;
+  if (p.tma_out && (s = out_map(&mo, out, (uint64_t)N, (uint64_t)T, (uint64_t)ldo)) != QZ_OK) return s;
+  const QuantizeRows q{x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, pl.bn < 128 ? pl.bn : 128, pl.n_steps,
+                       reinterpret_cast<float*>(ws + pl.off_scale), p.counters, pl.sharers > rest ? (int)rest : 0};
+  const bool few = T < 4 * sms;
+  s = cuda_status(bs == 16 ? (few ? launch_quantize_rows<16, 1>(q, st) : launch_quantize_rows<16, 4>(q, st))
+                           : (few ? launch_quantize_rows<32, 1>(q, st) : launch_quantize_rows<32, 2>(q, st)),
                   "quantize rows launch");
   if (s != QZ_OK) return s;
   const CUtensorMap &ma = swap ? mw : mx, &mb = swap ? mx : mw;
-  return bs == 16 ? run_linear<16>(pl.bn, ma, mb, p, sms, st) : run_linear<32>(pl.bn, ma, mb, p, sms, st);
+  return bs == 16 ? run_linear<16>(pl.bn, ma, mb, mo, p, sms, st) : run_linear<32>(pl.bn, ma, mb, mo, p, sms, st);
 }
