@@ -22,12 +22,11 @@
 // stage) could not keep up with the MMAs (543).  The wide form (BN = 256) has 128 token rows as A and 256 rows
 // of W as B.  The narrow forms (BN = 16 .. 128) swap the operands: 128 rows of
 // W are A and BN tokens are B, so that a decode step multiplies few padded
-// rows, and W streams through the ring once.  Tiles that do not fill a wave of
-// the SMs (all of a decode step's, the last ones of a prompt's) are cut along K:
-// their stages form one list that a number of CTAs share evenly; the last CTA
-// to finish a tile adds the CTAs' fp32 partials in order (the order of arrival
-// changes nothing).  The second launch starts before the first has ended and
-// fetches its first stages of W meanwhile.
+// rows, and W streams through the ring once.  Where the tiles leave SMs idle, a
+// cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
+// through distributed shared memory, each CTA finishing its share of the columns.
+// The second launch starts before the first has ended and fetches its first
+// stages of W meanwhile.
 //
 // Scales in memory, for both operands: row tiles of 128 rows (x, narrow form:
 // BN rows), groups of 4 blocks of K; a group is 512 bytes, row r at
@@ -101,8 +100,7 @@ __device__ __forceinline__ void unpack(const uint4 (&w)[VEC], float (&v)[BS]) {
 template <int BS, int DT, int R>
 __global__ void __launch_bounds__(R == 1 ? 512 : 256)
     quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t K, uint8_t* __restrict__ packed, int64_t ldp,
-                         uint8_t* __restrict__ sf, int gran, int64_t n_steps, float* __restrict__ row_scale,
-                         int* __restrict__ counters, int n_counters) {
+                         uint8_t* __restrict__ sf, int gran, int64_t n_steps, float* __restrict__ row_scale) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ uint32_t s_max[16];
   constexpr int kVec = BS * Elem<DT>::kSize / 16;  // 16-byte loads per block
@@ -110,8 +108,6 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
   const uint4* base = reinterpret_cast<const uint4*>(static_cast<const char*>(x) + row * ldx * Elem<DT>::kSize);
   const int64_t nb = K / BS, nb_pad = n_steps * Fmt<BS>::kBlocks, nb_packed = ldp * 2 / BS;
   const int tid = threadIdx.x, nt = blockDim.x;
-  if (row == 0)
-    for (int i = tid; i < n_counters; i += nt) counters[i] = 0;
   uint4 raw[R][kVec];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -231,13 +227,9 @@ __global__ void scale_layout_kernel(const uint8_t* __restrict__ codes, int64_t N
 struct LinearParams {
   int64_t T, N;                       // tokens, output features
   int64_t tiles_a, tiles_b;           // 128-row A tiles, BN-row B tiles
-  int64_t whole;                      // tiles run whole, tile i by CTA i % grid
-  int64_t shared_steps;               // stages of the tiles after them, in tile order,
-  int sharers;                        // which the CTAs below `sharers` take in equal runs
+  int split;                          // CTAs of a cluster that share a tile (1: no cluster)
   int n_steps;                        // stages over the whole of K
   const uint8_t *sf_a, *sf_b;         // scales: tile-major, n_steps * kSfBytes each
-  float* partial;                     // (sharer, 2, column, 128) fp32
-  int* counters;                      // arrivals per shared tile, zeroed by the quantization launch
   const float* row_scale;             // p_t
   float w_scale;
   const void* bias;
@@ -348,59 +340,121 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   else static_cast<uint16_t*>(p)[i] = (uint16_t)(pack16(v, 0.0f, dtype) & 0xffffu);
 }
 
-// One CTA's work: its whole tiles, then its run of the shared stages, which may
-// begin and end inside a tile.
+// One CTA's work: every gridDim-th tile, or its cluster's tile and its share of
+// the stages.
 template <bool SWAP>
 struct LinWork {
   const LinearParams& p;
-  int64_t a, b;        // tile coordinates
-  int s0, s1;          // stages [s0, s1) of it
-  int64_t shared;      // index among the shared tiles, -1 for a whole tile
-  bool first;          // the run begins with this segment
-  int64_t tile, pos, end;
+  int64_t a, b;  // tile coordinates
+  int s0, s1;    // stages [s0, s1) of it
+  int64_t tile;
 
-  __device__ __forceinline__ explicit LinWork(const LinearParams& q) : p(q), tile(blockIdx.x) {
-    pos = end = 0;
-    if ((int)blockIdx.x < p.sharers) {
-      pos = (int64_t)blockIdx.x * p.shared_steps / p.sharers;
-      end = (int64_t)(blockIdx.x + 1) * p.shared_steps / p.sharers;
-    }
-    first = true;
-    shared = -1;
+  __device__ __forceinline__ explicit LinWork(const LinearParams& q) : p(q), tile(blockIdx.x / q.split) {
+    const int rank = blockIdx.x % p.split;
+    s0 = rank * p.n_steps / p.split;
+    s1 = (rank + 1) * p.n_steps / p.split;
   }
-  __device__ __forceinline__ void coords(int64_t i) {
+  __device__ __forceinline__ bool next() {
+    if (tile >= p.tiles_a * p.tiles_b) return false;
     if (SWAP) {
-      a = i % p.tiles_a;
-      b = i / p.tiles_a;
+      a = tile % p.tiles_a;
+      b = tile / p.tiles_a;
     } else {
       // bands of 16 token tiles: the ~148 tiles in flight are about as many
       // token rows as weight rows and share both through L2
-      const int64_t per = 16 * p.tiles_b, band = i / per, r = i % per;
+      const int64_t per = 16 * p.tiles_b, band = tile / per, r = tile % per;
       const int64_t left = p.tiles_a - band * 16, rows = left < 16 ? left : 16;
       b = r / rows;
       a = band * 16 + r % rows;
     }
-  }
-  __device__ __forceinline__ bool next() {
-    if (tile < p.whole) {
-      coords(tile);
-      s0 = 0;
-      s1 = p.n_steps;
-      tile += gridDim.x;
-      return true;
-    }
-    if (pos >= end) return false;
-    if (shared >= 0) first = false;
-    shared = pos / p.n_steps;
-    coords(p.whole + shared);
-    s0 = (int)(pos % p.n_steps);
-    s1 = end - pos < p.n_steps - s0 ? s0 + (int)(end - pos) : p.n_steps;
-    pos += s1 - s0;
+    tile += gridDim.x / p.split;
     return true;
   }
-  // the sharer that has stage `at` of the shared list
-  __device__ __forceinline__ int owner(int64_t at) const {
-    return (int)(((at + 1) * p.sharers - 1) / p.shared_steps);
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float load_peer(uint32_t saddr, int rank) {
+  uint32_t at;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
+// Where one tile's sums go: this thread's accumulator row, and what belongs to it.
+template <int BN, bool SWAP>
+struct LinOut {
+  static constexpr int C = BN < 32 ? BN : 32;  // columns drained at a time
+  const LinearParams& p;
+  int row, lane, cols;     // accumulator row; columns of the tile that exist
+  int64_t ra, ra0, cb;     // swapped: output feature, first token; wide: token, first output feature
+  bool in;
+  float mine;              // swapped: the bias of this feature; wide: the scale of this token
+
+  __device__ __forceinline__ LinOut(const LinearParams& q, const LinWork<SWAP>& u) : p(q) {
+    lane = threadIdx.x & 31;
+    row = (threadIdx.x >> 5 & 3) * 32 + lane;
+    ra0 = u.a * 128;
+    ra = ra0 + row;
+    cb = u.b * BN;
+    const int64_t left = (SWAP ? p.T : p.N) - cb;
+    cols = left < BN ? (int)left : BN;
+    in = ra < (SWAP ? p.N : p.T);
+    mine = !in ? 0.0f : SWAP ? (p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f) : __ldg(p.row_scale + ra) * p.w_scale;
+  }
+  // lane q: the token scale (swapped) or the bias of column c + q
+  __device__ __forceinline__ float column(int c) const {
+    if (c + lane >= cols || lane >= C) return 0.0f;
+    if (SWAP) return __ldg(p.row_scale + cb + c + lane) * p.w_scale;
+    return p.bias ? load_any(p.bias, p.bias_dtype, cb + c + lane) : 0.0f;
+  }
+  // swapped: one column
+  __device__ __forceinline__ void store(int c, float v, float scale) const {
+    if (in) store_any(p.out, p.out_dtype, (cb + c) * p.ldo + ra, __fmaf_rn(v, scale, mine));
+  }
+  // C columns from c: scale, bias, round once, store
+  __device__ __forceinline__ void finish(int c, float (&v)[C], float col, const CUtensorMap& map_out, unsigned char* smem_out) const {
+    if constexpr (SWAP) {
+#pragma unroll
+      for (int q = 0; q < C; ++q) {
+        const float scale = __shfl_sync(0xffffffffu, col, q);
+        if (c + q < cols) store(c + q, v[q], scale);
+      }
+    } else {
+      if (p.bias) {
+#pragma unroll
+        for (int q = 0; q < C; ++q) v[q] = __fmaf_rn(v[q], mine, __shfl_sync(0xffffffffu, col, q));
+      } else {
+#pragma unroll
+        for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], mine);
+      }
+      if (p.tma_out) {
+        // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
+        unsigned char* stage = smem_out + (row >> 5) * 2048;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+              make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
+                         pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
+                       "r"((int)cb + c), "r"((int)ra0 + (row & ~31)), "r"(smem_u32(stage))
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else if (in) {
+#pragma unroll
+        for (int q = 0; q < C; ++q)
+          if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
+      }
+    }
   }
 };
 
@@ -426,7 +480,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   uint64_t* sf_done = mma_done + 1;
   uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(sf_done + 1);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
-  volatile int* last_s = abort_s + 1;
+  constexpr int C = LinOut<BN, SWAP>::C;
+  float* part = reinterpret_cast<float*>(smem);  // (BN, 128) fp32, over the ring's first stages
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -591,141 +646,75 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     mbar_wait_bounded(sf_done, 0u, kDevErrMmaTimeout);
   } else {
     // ---------------- epilogue (warps 2-5) ----------------
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales and counters are the quantization launch's
-    constexpr int C = BN < 32 ? BN : 32;     // columns drained at a time
-    const int row = (warp & 3) * 32 + lane;  // accumulator row of this thread
-    unsigned char* stage_out = smem_out + (warp & 3) * 2048;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales are the quantization launch's
     uint32_t lt = 0;
     for (LinWork<SWAP> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
-      const int64_t ra = u.a * 128 + row;       // swapped: output feature; wide: token
-      const int64_t cb = u.b * BN;              // swapped: first token; wide: first output feature
-      const int64_t cols_left = (SWAP ? p.T : p.N) - cb;
-      const int cols = cols_left < BN ? (int)cols_left : BN;
-      const bool in = ra < (SWAP ? p.N : p.T);
-      // what belongs to this thread's row: the scale of its token, or the bias of its feature
-      const float mine = !in ? 0.0f : SWAP ? (p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f) : __ldg(p.row_scale + ra) * p.w_scale;
-      // sharers of this tile
-      int c0 = 0, c1 = 0;
-      if (u.shared >= 0) {
-        c0 = u.owner(u.shared * p.n_steps);
-        c1 = u.owner((u.shared + 1) * p.n_steps - 1);
-      }
-      const bool split = c0 != c1;
-      uint32_t go = wait(tfull + acc, phase, kDevErrEpilogueTimeout) ? 1u : 0u;
-      if (split)  // all epilogue threads go on or all stop: the barriers below count on it
-        asm volatile(
-            "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, 1, 128, a;\n selp.u32 %0, 1, 0, b;\n}\n"
-            : "+r"(go)::"memory");
-      if (!go) break;
+      LinOut<BN, SWAP> out(p, u);
+      if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * (BN - G::kOverlap);
       // the order in which columns are drained: the wide form's shared ones (the
       // last of accumulator 0, the first of accumulator 1) come first
       const int c_first = !SWAP && acc == 0 ? BN - G::kOverlap : 0;
-      auto drained = [&](int i) {  // after the i-th group of C columns
+      float col = out.column(c_first);
+#pragma unroll 1
+      for (int i = 0; i < BN / C; ++i) {
+        const int c = (c_first + i * C) % BN;
+        const float now = col;
+        col = out.column((c + C) % BN);
+        float v[C];
+        if (c < out.cols) tmem_ld<C>(taddr + c, v);
         if (SWAP ? i + 1 == BN / C : i + 1 == G::kOverlap / C) {
           tc_fence_before();
           mbar_arrive(SWAP ? tempty + acc : tempty);
         }
-      };
-      // the column's share: lane q has the token scale, or the bias, of column c + q
-      auto column = [&](int c) -> float {
-        if (c + lane >= cols || lane >= C) return 0.0f;
-        if (SWAP) return __ldg(p.row_scale + cb + c + lane) * p.w_scale;
-        return p.bias ? load_any(p.bias, p.bias_dtype, cb + c + lane) : 0.0f;
-      };
-      // finish C columns: scale, bias, round once, store
-      auto finish = [&](int c, float(&v)[C], float col) {
-        if constexpr (SWAP) {
+        if (c >= out.cols) continue;
+        if (SWAP && p.split > 1) {  // this CTA's part, to be added below (the ring is idle: all its MMAs are done)
 #pragma unroll
-          for (int q = 0; q < C; ++q) {
-            const float f = __fmaf_rn(v[q], __shfl_sync(0xffffffffu, col, q), mine);
-            if (in && c + q < cols) store_any(p.out, p.out_dtype, (cb + c + q) * p.ldo + ra, f);
-          }
+          for (int q = 0; q < C; ++q) part[(c + q) * 128 + out.row] = v[q];
         } else {
-          if (p.bias) {
-#pragma unroll
-            for (int q = 0; q < C; ++q) v[q] = __fmaf_rn(v[q], mine, __shfl_sync(0xffffffffu, col, q));
-          } else {
-#pragma unroll
-            for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], mine);
-          }
-          if (p.tma_out) {
-            // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
-                  make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
-                             pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
-                           "r"((int)cb + c), "r"((int)(u.a * 128) + (warp & 3) * 32), "r"(smem_u32(stage_out))
-                           : "memory");
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else if (in) {
-#pragma unroll
-            for (int q = 0; q < C; ++q)
-              if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
-          }
+          out.finish(c, v, now, map_out, smem_out);
         }
-      };
-      if (!split) {
-        float col = column(c_first);
-#pragma unroll 1
-        for (int i = 0; i < BN / C; ++i) {
-          const int c = (c_first + i * C) % BN;
-          const float now = col;
-          col = column((c + C) % BN);
-          float v[C];
-          if (c < cols) tmem_ld<C>(taddr + c, v);
-          drained(i);
-          if (c < cols) finish(c, v, now);
-        }
-        continue;
-      }
-      float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u.first ? 0 : 1)) * (BN * 128) + row;
-#pragma unroll 1
-      for (int i = 0; i < BN / C; ++i) {
-        const int c = (c_first + i * C) % BN;
-        float v[C];
-        if (c < cols) tmem_ld<C>(taddr + c, v);
-        drained(i);
-#pragma unroll
-        for (int q = 0; q < C; ++q)
-          if (c + q < cols) __stcg(part + (c + q) * 128, v[q]);
-      }
-      __threadfence();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x == 64) *last_s = atomicAdd(p.counters + u.shared, 1) == c1 - c0;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const bool last = *last_s != 0;
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // last_s is read before the next segment writes it
-      if (!last) continue;
-      __threadfence();
-      // c0 may have begun with an earlier tile; the others begin with this one
-      const int begin = (int64_t)c0 * p.shared_steps / p.sharers >= u.shared * p.n_steps ? 0 : 1;
-#pragma unroll 1
-      for (int c = 0; c < cols; c += C) {
-        float v[C] = {};
-        const float col = column(c);
-#pragma unroll 1
-        for (int w = c0; w <= c1; ++w) {
-          const float* from = p.partial + ((int64_t)w * 2 + (w == c0 ? begin : 0)) * (BN * 128) + row;
-#pragma unroll
-          for (int q = 0; q < C; ++q)
-            if (c + q < cols) v[q] += __ldcg(from + (c + q) * 128);
-        }
-        finish(c, v, col);
       }
     }
     // staged output has been written (the staging area goes away with the CTA)
     if (!SWAP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  if constexpr (SWAP) {
+    if (p.split > 1) {
+      __syncwarp();
+      cluster_sync();
+      if (warp >= 2 && warp < 6) {
+        LinWork<SWAP> u(p);
+        if (u.next()) {
+          // rank r finishes columns [r, r + 1) * BN / split
+          LinOut<BN, SWAP> out(p, u);
+          const int rank = blockIdx.x % p.split, per = BN / p.split;
+          const float col = out.column(rank * per / C * C);
+          const uint32_t at = smem_u32(part) + out.row * 4;
+          const int c_end = (rank + 1) * per < out.cols ? (rank + 1) * per : out.cols;
+          for (int c0 = rank * per; c0 < c_end; c0 += 4) {
+            float x[4][8];  // all loads of four columns before the first sum
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) x[q][w] = w < p.split && c0 + q < c_end ? load_peer(at + (c0 + q) * 512, w) : 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v = x[q][0];
+#pragma unroll
+              for (int w = 1; w < 8; ++w) v += x[q][w];
+              const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
+                                           : (c0 + q < c_end ? __ldg(p.row_scale + u.b * BN + c0 + q) * p.w_scale : 0.0f);
+              if (c0 + q < c_end) out.store(c0 + q, v, scale);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();  // the parts have been read
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -774,17 +763,18 @@ static int out_map(CUtensorMap* m, void* base, uint64_t N, uint64_t T, uint64_t 
   return QZ_OK;
 }
 
-// Tile form and sharing of one call, and its workspace.
+// Tile form and cluster size of one call, and its workspace.
 struct LinPlan {
-  int bn, sharers, n_steps;
-  int64_t tiles_a, tiles_b, whole, ldp;
-  int64_t off_sf, off_scale, off_counter, off_partial, bytes;
+  int bn, split, n_steps;
+  int64_t tiles_a, tiles_b, ldp;
+  int64_t off_sf, off_scale, bytes;
 };
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Chooses the form by an estimate in SM clocks: a stage costs its MMAs or its
-// bytes, a tile its epilogue, a shared tile the partials written and added.
+// Chooses the form by an estimate in SM clocks: a stage costs its MMAs (2.1 clocks
+// per column) or its bytes (64 per clock and SM from L2), a tile its epilogue,
+// a cluster its exchange.
 static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   LinPlan best{};
   double best_cost = -1.0;
@@ -795,19 +785,16 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     const int64_t ta = swap ? (N + 127) / 128 : (T + 127) / 128;
     const int64_t tb = swap ? (T + bn - 1) / bn : (N + 255) / 256;
     const double bytes = 128.0 * 128 + 128.0 * bn + 128.0 * 256 / bs * (1 + (bn > 128 ? 2 : 1));
-    const double step = bytes / 40.0 > 2.0 * bn ? bytes / 40.0 : 2.0 * bn;
-    const double epilogue = 600.0 + 12.0 * bn, add = 600.0 + (T < bn ? T : bn) * 128 * 4 / 60.0;
-    const int64_t tiles = ta * tb, whole = tiles / sms * sms, rest = tiles - whole;
-    for (int sp = 1; sp <= n_steps && sp <= 32; ++sp) {  // CTAs per shared tile, on average
-      if (rest == 0 && sp > 1) break;
-      int64_t sharers = rest * sp < sms ? rest * sp : sms;
-      if (sp > 1 && rest * (sp - 1) >= sms) break;
-      const double parts = rest ? (double)sharers / rest : 1.0;
-      const double cost = (double)(whole / sms) * (n_steps * step + epilogue) +
-                          (rest ? n_steps * step / parts + epilogue + (parts > 1.0 ? 1500.0 + (1.0 + parts) * add : 0.0) : 0.0);
+    double step = bytes / 60.0 > 2.1 * bn ? bytes / 60.0 : 2.1 * bn;
+    if (step < 400.0) step = 400.0;  // the waits and issues of one stage
+    for (int split : {1, 2, 4, 8}) {
+      if (split > 1 && (!swap || split > n_steps || ta * tb * split > sms)) break;
+      const double waves = (double)((ta * tb * split + sms - 1) / sms);
+      const double cost = waves * ((n_steps + split - 1) / split * step) + (swap ? waves : 1.0) * (500.0 + 10.0 * bn) +
+                          (split > 1 ? 1000.0 + 4.0 * bn : 0.0);
       if (best_cost < 0 || cost < best_cost) {
         best_cost = cost;
-        best.bn = bn; best.sharers = (int)sharers; best.tiles_a = ta; best.tiles_b = tb; best.whole = whole;
+        best.bn = bn; best.split = split; best.tiles_a = ta; best.tiles_b = tb;
       }
     }
   }
@@ -815,12 +802,9 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   best.ldp = up(K, 32) / 2;
   const int gran = best.bn < 128 ? best.bn : 128;
   const int64_t sf_tiles = (T + gran - 1) / gran;
-  const int64_t rest = best.tiles_a * best.tiles_b - best.whole;
   best.off_sf = up(T * best.ldp, 256);
   best.off_scale = best.off_sf + up(sf_tiles * n_steps * (int64_t)(kStepK / bs / 4 * kGroupBytes), 256);
-  best.off_counter = best.off_scale + up(T * 4, 256);
-  best.off_partial = best.off_counter + up(rest * 4, 256);
-  best.bytes = best.off_partial + (best.sharers > rest ? (int64_t)best.sharers * 2 * best.bn * 128 * 4 : 0);
+  best.bytes = best.off_scale + up(T * 4, 256);
   return best;
 }
 
@@ -834,8 +818,6 @@ struct QuantizeRows {
   int gran;
   int64_t n_steps;
   float* row_scale;
-  int* counters;
-  int n_counters;
 };
 
 template <int BS, int R>
@@ -846,7 +828,7 @@ static cudaError_t launch_quantize_rows(const QuantizeRows& q, cudaStream_t st) 
   const unsigned grid = (unsigned)q.T;
 #define QZ_ROWS(DT)                                                                                                     \
   quantize_rows_kernel<BS, DT, R><<<grid, nt, 0, st>>>(q.x, q.ldx, q.K, q.packed, q.ldp, q.sf, q.gran, q.n_steps,       \
-                                                       q.row_scale, q.counters, q.n_counters)
+                                                       q.row_scale)
   if (q.dtype == kDtBF16) QZ_ROWS(kDtBF16);
   else if (q.dtype == kDtF16) QZ_ROWS(kDtF16);
   else QZ_ROWS(kDtF32);
@@ -867,16 +849,19 @@ static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const CUten
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)p.split, 1, 1};
+  const int64_t ctas = p.tiles_a * p.tiles_b * p.split;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.whole > 0 ? sms : p.sharers));
+  cfg.gridDim = dim3((unsigned)(ctas < sms ? ctas : sms));
   cfg.blockDim = dim3(kLinThreads);
   cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS>, a, b, o, p), "linear launch");
 }
 
@@ -972,16 +957,11 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   LinearParams p{};
   p.T = T; p.N = N;
   p.tiles_a = pl.tiles_a; p.tiles_b = pl.tiles_b;
-  p.whole = pl.whole;
-  const int64_t rest = pl.tiles_a * pl.tiles_b - pl.whole;
-  p.shared_steps = rest * pl.n_steps;
-  p.sharers = pl.sharers;
+  p.split = pl.split;
   p.n_steps = pl.n_steps;
   p.sf_a = swap ? scales : ws + pl.off_sf;
   p.sf_b = swap ? ws + pl.off_sf : scales;
   p.row_scale = reinterpret_cast<float*>(ws + pl.off_scale);
-  p.counters = reinterpret_cast<int*>(ws + pl.off_counter);
-  p.partial = reinterpret_cast<float*>(ws + pl.off_partial);
   p.w_scale = tensor_scale;
   p.bias = bias; p.bias_dtype = bias_dtype;
   p.out = out; p.out_dtype = out_dtype; p.ldo = ldo;
@@ -989,7 +969,7 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   CUtensorMap mo = mx;
   if (p.tma_out && (s = out_map(&mo, out, (uint64_t)N, (uint64_t)T, (uint64_t)ldo)) != QZ_OK) return s;
   const QuantizeRows q{x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, pl.bn < 128 ? pl.bn : 128, pl.n_steps,
-                       reinterpret_cast<float*>(ws + pl.off_scale), p.counters, pl.sharers > rest ? (int)rest : 0};
+                       reinterpret_cast<float*>(ws + pl.off_scale)};
   const bool few = T < 4 * sms;
   s = cuda_status(bs == 16 ? (few ? launch_quantize_rows<16, 1>(q, st) : launch_quantize_rows<16, 4>(q, st))
                            : (few ? launch_quantize_rows<32, 1>(q, st) : launch_quantize_rows<32, 2>(q, st)),
