@@ -311,10 +311,12 @@ QZ_API int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T, int
  * codes (E, rows, K / bs) and nibbles (E, rows, K / 2), in the order qz_moe reads
  * (once per weight; rows and K multiples of 32).  gate_up != 0: rows are the
  * gate rows, then as many up rows.  codes_out: E * rows * up(K, 64) / 2 bytes,
- * scales_out: E * rows * up(K, 64) / bs bytes, both 16-byte aligned.
+ * scales_out: E * rows * up(K, 64) / bs bytes, both 16-byte aligned.  norms_out
+ * (gate_up only): (E, 2) fp32, the largest norms of a gate and of an up row.
  */
 QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int64_t E, int64_t rows, int64_t K,
-                         int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, void* stream);
+                         int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, float* norms_out,
+                         void* stream);
 
 /*
  * qz_moe -- a mixture-of-experts layer for at most 64 tokens: router logits
@@ -323,7 +325,7 @@ QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int6
  * out = sum c * D_e (silu(G_e x) * (U_e x)), fp32 sums, one rounding to x's type.
  *   x        (T, H) bf16 or fp16, rows ldx elements apart, 16-byte aligned
  *   router   (E, H) fp32, bf16 or fp16;  E <= 512, top_k <= 16
- *   *_codes, *_scales, *_tensor_scale: from qz_moe_layout; gate / up (2 I, H) and
+ *   *_codes, *_scales, up_norms, *_tensor_scale: from qz_moe_layout; gate / up (2 I, H) and
  *            down (H, I), I and H multiples of 32
  *   out      (T, H) of x's type;  ids (T, top_k) and weights (T, top_k): the
  *            routing, descending logits (NULL: not written)
@@ -334,7 +336,7 @@ QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int6
 QZ_API int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k, int64_t* bytes);
 QZ_API int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k,
                   int renormalize, const void* router, int router_dtype, int format, const uint8_t* up_codes,
-                  const uint8_t* up_scales, float up_tensor_scale, const uint8_t* down_codes,
+                  const uint8_t* up_scales, const float* up_norms, float up_tensor_scale, const uint8_t* down_codes,
                   const uint8_t* down_scales, float down_tensor_scale, void* out, int* ids, float* weights,
                   void* workspace, int64_t workspace_bytes, void* stream);
 

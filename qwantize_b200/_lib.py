@@ -80,10 +80,10 @@ def load():
     L.qz_fp4_linear.argtypes = [vp, i32, i64, i64, i64, i64, i32, vp, i64, vp, ctypes.c_float, vp, i32, vp, i32, i64,
                                 vp, i64, vp]
     f32 = ctypes.c_float
-    L.qz_moe_layout.argtypes = [vp, vp, i64, i64, i64, i32, i32, vp, vp, vp]
+    L.qz_moe_layout.argtypes = [vp, vp, i64, i64, i64, i32, i32, vp, vp, vp, vp]
     L.qz_moe_workspace.argtypes = [i64, i64, i64, i64, i64, vp]
-    L.qz_moe.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, i32, i32, vp, vp, f32, vp, vp, f32, vp, vp,
-                         vp, vp, i64, vp]
+    L.qz_moe.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, i32, i32, vp, vp, vp, f32, vp, vp, f32, vp,
+                         vp, vp, vp, i64, vp]
     L.qz_kv_append.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, vp, i64, i64, vp,
                                vp, i64, i64, vp]
     L.qz_kv_read.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp, vp, i32, vp]

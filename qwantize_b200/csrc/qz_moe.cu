@@ -10,31 +10,40 @@
 // stay in 16 bits (quantizing them would save nothing).
 //
 // Two launches.  moe_router_kernel: the logits, and x as fp16 in the order of
-// the matrix instructions' B fragments.  moe_experts_kernel, cooperative, every
-// CTA resident: each CTA derives the routing from the logits for itself (they
-// are a few KB), then the CTAs share the (expert, row tile) units of the
-// gate / up product; a grid barrier; the units of the down product; a grid
-// barrier; the weighted sum over each token's experts in a fixed order.
+// the matrix instructions' B fragments.  moe_experts_kernel, cooperative, one
+// CTA of 12 warps per SM: each CTA derives the routing from the logits for itself
+// (they are a few KB), then the CTAs share the units of the gate / up product; a
+// grid barrier; the units of the down product; a grid barrier; the weighted sum
+// over each token's experts in a fixed order.
 //
-// A unit is 16 weight rows; a CTA's 8 warps split K and add up through shared
-// memory.  Weights are laid out once in the order of the A fragments of
-// mma.m16n8k16 (fp16, fp32 accumulation): a lane's 16 bytes hold its 4 mma
-// steps of one 64-column chunk.  One mma step covers one NVFP4 scale block (two
-// an MXFP4 block), so the block scale multiplies the fp32 partial product and
-// the codes convert exactly to fp16 by hardware.  A gate / up tile interleaves 8
-// gate rows with the 8 up rows of the same outputs, so the activation function
-// needs no second pass.  tcgen05 would need 128 weight rows per instruction and
-// 16-bit operands in shared memory; with 1 to 32 tokens per expert the
-// fragments go straight from HBM to registers instead.
+// A unit is 32 weight rows of one expert times up to 32 of its tokens.  A CTA has
+// a run of neighbouring units, so its warps share an expert's tokens in L1; a
+// warp takes a unit alone and streams its weights through its own ring of bulk
+// copies, never waiting for another warp.  Where units are few, 2 or 4 warps cut a
+// unit's K and add up through shared memory.
+//
+// Weights are laid out once in the order of the A fragments of mma.m16n8k16
+// (fp16, fp32 accumulation): a lane's 16 bytes hold its 4 steps of one 16-row
+// tile and 64-column chunk.  The codes convert exactly to fp16 by hardware; an
+// NVFP4 scale (one per step) is multiplied in there, exactly (6 significant
+// bits, 2^-10 .. 2688), an MXFP4 scale (one per two steps, any power of two)
+// multiplies the fp32 partial product.  A gate / up tile interleaves 8 gate rows
+// with the 8 up rows of the same outputs, so a lane holds both and the
+// activation function needs no exchange.  tcgen05 would need 128 weight rows per
+// instruction and 16-bit operands in shared memory; with 1 to 32 tokens per expert
+// the matrix work is a tenth of what mma.sync can do while HBM delivers the codes.
 //
 // fp16 operands: a bf16 token is scaled by the power of two that puts its
-// largest magnitude in [2^14, 2^15), exact for values within 2^-28 of it
-// (smaller ones lose bits below 2^-39 of it); an activation row likewise, one
-// rounding to 11 bits, a quarter of the step of the 16-bit result's.
+// largest magnitude in [2^14, 2^15), exact for values within 2^-28 of it.  An
+// activation row is scaled by a power of two from the bound |silu(g) u| <= |g| |u|
+// <= |x|^2 max|G row| max|U row| (row norms kept with the weights), so it cannot
+// overflow whatever the data, and rounded to 11 bits; for fp16 outputs, whose
+// own rounding is no coarser, the remainder is kept as a second fp16 operand.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/qwantize_b200.h"
 #include "qz_common.cuh"
@@ -48,8 +57,11 @@ int cuda_status(cudaError_t e, const char* what);
 int current_sms(int* sms);
 
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTop = 16;
-constexpr int kMoeWarps = 8, kMoeThreads = kMoeWarps * 32;
+constexpr int kMoeWarps = 12, kMoeThreads = kMoeWarps * 32;
 constexpr int kMoeMaxSlots = kMoeMaxTokens * kMoeMaxTop;
+constexpr int kMoeGroup = 32;                                                  // tokens of a unit
+constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxSlots / kMoeGroup;
+constexpr int kMoePiece = 4, kMoeStages = 2;                                   // chunks per bulk copy, copies in flight per warp
 
 struct MoeParams {
   int T, H, I, E, top;
@@ -57,15 +69,14 @@ struct MoeParams {
   int renorm;
   int dtype;                        // of x and out
   const float* logits;              // (T, E)
-  const uint4* up_codes;            // (E, I / 8 tiles, hc chunks, 32 lanes) 16 bytes
-  const uint32_t* up_scales;        // (E, I / 8 tiles, hc chunks, 8 row pairs): words of scales
-  const uint4* down_codes;          // (E, H / 16 tiles, ic chunks, 32 lanes)
-  const uint32_t* down_scales;
+  const uint8_t *up_codes, *up_scales;      // (E, I / 16 units, hc chunks, 2 tiles) 512 and 8 * 2 * 64 / bs bytes
+  const uint8_t *down_codes, *down_scales;  // (E, H / 32 units, ic chunks, 2 tiles)
+  const float* norms;               // (E, 2): largest row norm of gate and of up, without the tensor scale
   float up_scale, down_scale;       // tensor scales
-  const uint4* xh;                  // (T, hc, 64) fp16 in fragment order
-  const float* xs;                  // (T) power of two of each token
-  float* act;                       // (T * top, I)
-  unsigned* act_max;                // (T * top) bits of the largest |act|
+  const __half* xh;                 // (T, hc, 64) in fragment order
+  const int2* xp;                   // (T): power of two of the token, exponent bound of its scaled squared norm
+  __half* act;                      // (parts, T * top, ic, 64) in fragment order: the rounded row, then the remainder
+  int64_t act_part;                 // elements of one part
   float* y;                         // (T * top, H)
   int* barrier;
   void* out;                        // (T, H)
@@ -79,7 +90,8 @@ struct MoeParams {
 // Lane (g, t) of a 16-row tile and 64-column chunk: word j (one mma step, 16
 // columns) holds columns 16j + 4t .. + 3 of row g (low half) and row g + 8 (high
 // half).  gate_up: rows 0-7 of tile i are gate rows 8i .., rows 8-15 the up rows
-// rows / 2 + 8i ...  Scales: the words of row g and row g + 8 side by side.
+// rows / 2 + 8i ...  Scales: those of row g and row g + 8 side by side.  A chunk's
+// two tiles of a unit are neighbours.
 template <int BS>
 __global__ void moe_layout_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales, int64_t E,
                                   int64_t rows, int64_t K, int gate_up, uint32_t* __restrict__ codes_out,
@@ -89,7 +101,8 @@ __global__ void moe_layout_kernel(const uint8_t* __restrict__ packed, const uint
   constexpr int kSc = 64 / BS;                     // scales per row and chunk
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int j = i & 3, lane = (int)(i >> 2) & 31, g = lane >> 2, t = lane & 3;
-    const int64_t chunk = i / 128 % chunks, tile = i / 128 / chunks % tiles, e = i / 128 / chunks / tiles;
+    const int64_t chunk = i / 256 % chunks, unit = i / 256 / chunks % (tiles / 2), e = i / 256 / chunks / (tiles / 2);
+    const int64_t tile = unit * 2 + (i / 128 & 1);
     const int64_t col = chunk * 64 + 16 * j + 4 * t;
     uint32_t w = 0;
     for (int h = 0; h < 2; ++h) {
@@ -98,7 +111,7 @@ __global__ void moe_layout_kernel(const uint8_t* __restrict__ packed, const uint
       if (col < K) w |= ((uint32_t)p[0] | (uint32_t)p[1] << 8) << (16 * h);
       if (j == 0 && t < kSc) {  // lane t < kSc of the quad writes scale t of both rows
         const int64_t b = chunk * kSc + t;
-        scales_out[((((e * tiles + tile) * chunks + chunk) * 8 + g) * 2 + h) * kSc + t] =
+        scales_out[((i / 128 * 8 + g) * 2 + h) * kSc + t] =
             b < K / BS ? scales[(e * rows + row) * (K / BS) + b] : 0;
       }
     }
@@ -106,11 +119,39 @@ __global__ void moe_layout_kernel(const uint8_t* __restrict__ packed, const uint
   }
 }
 
+// Largest row norms of the gate and of the up rows, one warp per row.
+template <int BS>
+__global__ void moe_norm_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales, int64_t E,
+                                int64_t rows, int64_t K, float* __restrict__ norms) {
+  const int lane = threadIdx.x & 31;
+  const int64_t n_warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < E * rows; r += n_warps) {
+    float sum = 0.0f;
+    for (int64_t b = lane; b < K / BS; b += 32) {
+      const uint32_t c = scales[r * (K / BS) + b];
+      const float s = BS == 32 ? (c == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(c == 0 ? 0x00400000u : c << 23))
+                    : c == 127 ? __uint_as_float(0x7fffffffu) : e4m3_value((int)c);
+      float q2 = 0.0f;
+      for (int k = 0; k < BS / 2; ++k) {
+        const float2 v = e2m1x2_to_float2(packed[r * (K / 2) + b * (BS / 2) + k]);
+        q2 += v.x * v.x + v.y * v.y;
+      }
+      sum += q2 * s * s;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0)  // non-negative floats order like their bits, NaN above all
+      atomicMax(reinterpret_cast<unsigned*>(norms) + r / rows * 2 + (r % rows >= rows / 2), __float_as_uint(sqrtf(sum)) & 0x7fffffffu);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // router logits, fp16 tokens
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void load8(const void* p, int dtype, int64_t i, float (&v)[8]) {
-  if (dtype == kDtF32) {
+// 8 consecutive elements as fp32.
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+  if (DT == kDtF32) {
     const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
     const float4 a = __ldg(q), b = __ldg(q + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -120,12 +161,12 @@ __device__ __forceinline__ void load8(const void* p, int dtype, int64_t i, float
   const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    v[2 * k] = dtype == kDtBF16 ? bf16_bits_to_float(ww[k] & 0xffffu) : f16_bits_to_float(ww[k] & 0xffffu);
-    v[2 * k + 1] = dtype == kDtBF16 ? bf16_bits_to_float(ww[k] >> 16) : f16_bits_to_float(ww[k] >> 16);
+    v[2 * k] = DT == kDtBF16 ? bf16_bits_to_float(ww[k] & 0xffffu) : f16_bits_to_float(ww[k] & 0xffffu);
+    v[2 * k + 1] = DT == kDtBF16 ? bf16_bits_to_float(ww[k] >> 16) : f16_bits_to_float(ww[k] >> 16);
   }
 }
 
-// 2^e with x * 2^-e in [2^14, 2^15) for the largest magnitude (its bits m); 1
+// e with x * 2^-e in [2^14, 2^15) for the largest magnitude (its bits m); 0
 // for 0, inf and NaN
 __device__ __forceinline__ int f16_power(uint32_t m) {
   if (m == 0 || m >= 0x7f800000u) return 0;
@@ -133,13 +174,19 @@ __device__ __forceinline__ int f16_power(uint32_t m) {
   return e < -112 ? -112 : e;
 }
 
+// Smallest e with |v| < 2^e for a finite v > 0 (a bound of its exponent); 0 else
+__device__ __forceinline__ int exponent_bound(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return v > 0.0f && u < 0x7f800000u ? (int)(u >> 23) - 126 : 0;
+}
+
 // Blocks [0, E * ceil(T / 8)): one expert and 8 tokens, the 4 warps splitting H.
-// The T blocks after them: one token to fp16, and the counters' zeroing.
+// The T blocks after them: one token to fp16; the first also zeroes the barriers.
 constexpr int kRouterThreads = 128;
+template <int DT, int RDT>
 __global__ void __launch_bounds__(kRouterThreads)
-    moe_router_kernel(const void* __restrict__ x, int64_t ldx, int dtype, const void* __restrict__ router, int rdtype,
-                      int T, int H, int E, float* __restrict__ logits, __half* __restrict__ xh, float* __restrict__ xs,
-                      unsigned* __restrict__ act_max, int n_slots, int* __restrict__ barrier) {
+    moe_router_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ router, int T, int H, int E,
+                      float* __restrict__ logits, uint4* __restrict__ xh, int2* __restrict__ xp, int* __restrict__ barrier) {
   __shared__ float s_part[4][8];
   __shared__ uint32_t s_max[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -149,16 +196,14 @@ __global__ void __launch_bounds__(kRouterThreads)
     const int nt = T - t0 < 8 ? T - t0 : 8;
     float acc[8] = {};
     for (int h = tid * 8; h < H; h += kRouterThreads * 8) {
-      float r[8];
-      load8(router, rdtype, (int64_t)e * H + h, r);
+      float r[8], v[8][8];
+      load8<RDT>(router, (int64_t)e * H + h, r);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (n >= nt) break;
-        float v[8];
-        load8(x, dtype, (t0 + n) * ldx + h, v);
+      for (int n = 0; n < 8; ++n) load8<DT>(x, (t0 + (n < nt ? n : 0)) * ldx + h, v[n]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[n] = fmaf(v[k], r[k], acc[n]);
-      }
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[n] = fmaf(v[n][k], r[k], acc[n]);
     }
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
@@ -171,45 +216,48 @@ __global__ void __launch_bounds__(kRouterThreads)
     return;
   }
   const int t = blockIdx.x - E * groups;
-  if (t == 0) {
-    for (int i = tid; i < n_slots; i += kRouterThreads) act_max[i] = 0u;
-    if (tid < 2) barrier[tid] = 0;
-  }
-  float p = 1.0f, inv = 1.0f;
-  if (dtype == kDtBF16) {
+  if (t == 0 && tid < 2) barrier[tid] = 0;
+  int e = 0;
+  if (DT == kDtBF16) {
     uint32_t m = 0;
     for (int h = tid * 8; h < H; h += kRouterThreads * 8) {
       float v[8];
-      load8(x, dtype, t * ldx + h, v);
+      load8<DT>(x, t * ldx + h, v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) s_max[warp] = m;
     __syncthreads();
-    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
-    const int e = f16_power(m);
-    p = pow2f(e);
-    inv = pow2f(-e);
+    e = f16_power(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
   }
-  if (tid == 0) xs[t] = p;
+  const float inv = pow2f(-e);
+  // thread: 32 columns (half a chunk); lane t' of the fragment takes columns 4t' .. + 3 of each 16
   const int hc = (H + 63) / 64;
-  // thread: 8 halves = (half, t) of a chunk: columns 16 (2 half + i / 4) + 4 t + i % 4
-  for (int i = tid; i < hc * 8; i += kRouterThreads) {
-    const int chunk = i >> 3, half = (i >> 2) & 1, q = i & 3;
-    __half v[8];
+  float norm2 = 0.0f;
+  for (int i = tid; i < hc * 2; i += kRouterThreads) {
+    uint32_t w[16];  // 32 halves
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int col = chunk * 64 + 16 * (2 * half + k / 4) + 4 * q + k % 4;
-      float f = 0.0f;
-      if (col < H) {
-        const uint32_t b = static_cast<const uint16_t*>(x)[t * ldx + col];
-        f = (dtype == kDtBF16 ? bf16_bits_to_float(b) : f16_bits_to_float(b)) * inv;
+    for (int q = 0; q < 4; ++q) {
+      float v[8] = {};
+      if (i * 32 < H) load8<DT>(x, t * ldx + i * 32 + q * 8, v);  // H is a multiple of 32
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a = v[2 * k] * inv, b = v[2 * k + 1] * inv;
+        norm2 = fmaf(a, a, fmaf(b, b, norm2));
+        const __half2 h = __floats2half2_rn(a, b);
+        w[4 * q + k] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      v[k] = __float2half_rn(f);
     }
-    *reinterpret_cast<uint4*>(xh + ((int64_t)t * hc + chunk) * 64 + half * 32 + q * 8) = *reinterpret_cast<uint4*>(v);
+    uint4* out = xh + ((int64_t)t * hc * 2 + i) * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) out[q] = make_uint4(w[2 * q], w[2 * q + 1], w[8 + 2 * q], w[8 + 2 * q + 1]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) norm2 += __shfl_xor_sync(0xffffffffu, norm2, o);
+  if (lane == 0) s_part[0][warp] = norm2;
+  __syncthreads();
+  if (tid == 0) xp[t] = make_int2(e, exponent_bound((s_part[0][0] + s_part[0][1]) + (s_part[0][2] + s_part[0][3])));
 }
 
 // ---------------------------------------------------------------------------
@@ -218,11 +266,14 @@ __global__ void __launch_bounds__(kRouterThreads)
 struct MoeShared {
   float weight[kMoeMaxSlots];
   uint16_t id[kMoeMaxSlots];
-  uint16_t list[kMoeMaxSlots];       // slots (token * top + k) grouped by expert, tokens ascending
-  uint16_t start[kMoeMaxExperts + 1];
-  uint16_t active[kMoeMaxExperts];   // experts with tokens, ascending
-  int n_active, ok;
-  float part[kMoeWarps * 16 * 32];   // per warp: 16 rows x up to 32 tokens
+  uint16_t list[kMoeMaxSlots];            // slots (token * top + k) grouped by expert, tokens ascending
+  uint16_t count[kMoeMaxExperts];
+  uint16_t start[kMoeMaxExperts];
+  // groups: up to kMoeGroup tokens of one expert, experts ascending
+  uint16_t g_expert[kMoeMaxGroups], g_begin[kMoeMaxGroups], g_count[kMoeMaxGroups];
+  int n_groups, ok;
+  uint64_t full[kMoeWarps * kMoeStages];  // the warps' rings
+  float part[kMoeWarps][32 * 32];         // sums of warps that share a unit: (value, lane)
 };
 
 // All CTAs arrive, then wait for each other (they are all resident: cooperative
@@ -261,12 +312,14 @@ __device__ __forceinline__ uint32_t order_bits(float f) {
 __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int t = warp; t < p.T; t += kMoeWarps) {
-    uint32_t key[kMoeMaxExperts / 32];
+    constexpr int W = kMoeMaxExperts / 32;
+    const int ne = (p.E + 31) / 32;  // words in use
+    uint32_t key[W];
+    float val[W];
     float top0 = 0.0f, sum = 0.0f;
     uint32_t taken_key = 0, mine = 0;
-    float val[kMoeMaxExperts / 32];
 #pragma unroll
-    for (int i = 0; i < kMoeMaxExperts / 32; ++i) {
+    for (int i = 0; i < W; ++i) {
       const int e = i * 32 + lane;
       val[i] = e < p.E ? __ldcg(p.logits + (int64_t)t * p.E + e) : 0.0f;
       key[i] = e < p.E ? max(order_bits(val[i]), 1u) : 0u;  // 0: not there, or taken
@@ -275,17 +328,18 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     for (int k = 0; k < p.top; ++k) {
       taken_key = 0;
 #pragma unroll
-      for (int i = 0; i < kMoeMaxExperts / 32; ++i) taken_key = max(taken_key, key[i]);
+      for (int i = 0; i < W; ++i)
+        if (i < ne) taken_key = max(taken_key, key[i]);
       taken_key = __reduce_max_sync(0xffffffffu, taken_key);
       uint32_t e = 0xffffffffu;
       float v = 0.0f;
 #pragma unroll
-      for (int i = kMoeMaxExperts / 32 - 1; i >= 0; --i)
-        if (key[i] == taken_key) e = i * 32 + lane;
+      for (int i = W - 1; i >= 0; --i)
+        if (i < ne && key[i] == taken_key) e = i * 32 + lane;
       e = __reduce_min_sync(0xffffffffu, e);
 #pragma unroll
-      for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-        if (e == (uint32_t)(i * 32 + lane)) { v = val[i]; key[i] = 0; }
+      for (int i = 0; i < W; ++i)
+        if (i < ne && e == (uint32_t)(i * 32 + lane)) { v = val[i]; key[i] = 0; }
       v = __shfl_sync(0xffffffffu, v, e & 31);
       if (k == 0) top0 = v;
       if (lane == k) { chosen = v; mine = e; }
@@ -294,7 +348,7 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
       sum = lane < p.top ? expf(chosen - top0) : 0.0f;
     } else {
 #pragma unroll
-      for (int i = 0; i < kMoeMaxExperts / 32; ++i)
+      for (int i = 0; i < W; ++i)
         if (i * 32 + lane < p.E) sum += expf(val[i] - top0);
     }
 #pragma unroll
@@ -310,31 +364,46 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     }
   }
   __syncthreads();
-  // counts, starts and lists per expert
+  // counts per expert, starts and groups, lists: a warp compares 32 slots at a time
   const int n = p.T * p.top;
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
+  for (int e = warp; e < p.E; e += kMoeWarps) {
     int c = 0;
-    for (int i = 0; i < n; ++i) c += s.id[i] == e;
-    s.start[e + 1] = (uint16_t)c;
+    for (int i = 0; i < n; i += 32) c += __popc(__ballot_sync(0xffffffffu, i + lane < n && s.id[i + lane] == e));
+    if (lane == 0) s.count[e] = (uint16_t)c;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int a = 0, at = 0;
-    for (int e = 0; e < p.E; ++e) {
-      const int c = s.start[e + 1];
-      s.start[e] = (uint16_t)at;
-      if (c) s.active[a++] = (uint16_t)e;
-      at += c;
+  if (warp == 0) {
+    int at = 0, groups = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int c = e0 + lane < p.E ? s.count[e0 + lane] : 0, m = (c + kMoeGroup - 1) / kMoeGroup;
+      int a = c, b = m;  // inclusive prefix sums
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) { a += x; b += y; }
+      }
+      if (e0 + lane < p.E) s.start[e0 + lane] = (uint16_t)(at + a - c);
+      for (int k = 0; k < m; ++k) {
+        const int g = groups + b - m + k;
+        s.g_expert[g] = (uint16_t)(e0 + lane);
+        s.g_begin[g] = (uint16_t)(at + a - c + k * kMoeGroup);
+        s.g_count[g] = (uint16_t)(c - k * kMoeGroup < kMoeGroup ? c - k * kMoeGroup : kMoeGroup);
+      }
+      at += __shfl_sync(0xffffffffu, a, 31);
+      groups += __shfl_sync(0xffffffffu, b, 31);
     }
-    s.start[p.E] = (uint16_t)at;
-    s.n_active = a;
+    if (lane == 0) s.n_groups = groups;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
+  for (int e = warp; e < p.E; e += kMoeWarps) {
+    if (s.count[e] == 0) continue;
     int at = s.start[e];
-    if (at == s.start[e + 1]) continue;
-    for (int i = 0; i < n; ++i)
-      if (s.id[i] == e) s.list[at++] = (uint16_t)i;
+    for (int i = 0; i < n; i += 32) {
+      const bool mine = i + lane < n && s.id[i + lane] == e;
+      const unsigned m = __ballot_sync(0xffffffffu, mine);
+      if (mine) s.list[at + __popc(m & ((1u << lane) - 1u))] = (uint16_t)(i + lane);
+      at += __popc(m);
+    }
   }
   __syncthreads();
 }
@@ -353,220 +422,324 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Four E4M3 scales of a word, or two power-of-two ones of a half word.
-__device__ __forceinline__ void scales_nv(uint32_t w, float (&s)[4]) {
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Four E4M3 scales of a word as fp16 pairs (s, s).
+__device__ __forceinline__ void scales_nv(uint32_t w, uint32_t (&s)[4]) {
   uint32_t h0, h1;
   asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
       : "=r"(h0), "=r"(h1)
       : "r"(w));
-  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h0)), b = __half22float2(*reinterpret_cast<__half2*>(&h1));
-  s[0] = a.x; s[1] = a.y; s[2] = b.x; s[3] = b.y;
+  s[0] = __byte_perm(h0, 0, 0x1010);
+  s[1] = __byte_perm(h0, 0, 0x3232);
+  s[2] = __byte_perm(h1, 0, 0x1010);
+  s[3] = __byte_perm(h1, 0, 0x3232);
 }
 __device__ __forceinline__ float scale_mx(uint32_t c) {
   return __uint_as_float(c == 0 ? 0x00400000u : c == 255 ? 0x7fffffffu : c << 23);
 }
 
-// One 16-row tile times up to 8 NT tokens: this warp's chunks (warp, warp + 8,
-// ...) of K.  load_b(chunk, n, b): the 8 B words of n-tile n and this lane.
-template <int NT, int BS, typename LoadB>
-__device__ __forceinline__ void tile_product(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales,
-                                             int chunks, float (&acc)[NT][4], LoadB&& load_b) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
-  constexpr int kBatch = 4;
-  for (int c0 = warp; c0 < chunks; c0 += kMoeWarps * kBatch) {
-    uint4 w[kBatch];
-    uint2 sc[kBatch];
+// One chunk (64 columns) of a unit: two 16-row tiles of weights in shared memory
+// (a lane's 16 bytes of each, its rows' scales) times NT tiles of 8 tokens, whose
+// B words come in `PARTS` addends.
+template <int NT, int BS, int PARTS>
+__device__ __forceinline__ void chunk_product(const uint8_t* codes, const uint8_t* scales, const uint32_t (&b)[PARTS][NT][8],
+                                              float (&acc)[2][NT][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int c = c0 + i * kMoeWarps;
-      if (c < chunks) {
-        w[i] = __ldcs(codes + c * 32 + lane);
-        if constexpr (BS == 16) sc[i] = __ldcs(reinterpret_cast<const uint2*>(scales) + c * 8 + g);
-        else sc[i].x = __ldcs(scales + c * 8 + g);
+  for (int r = 0; r < 2; ++r) {
+    const uint4 w4 = *reinterpret_cast<const uint4*>(codes + r * 512 + lane * 16);
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    if constexpr (BS == 16) {
+      const uint2 sc = *reinterpret_cast<const uint2*>(scales + r * 64 + g * 8);
+      uint32_t s0[4], s1[4];
+      scales_nv(sc.x, s0);
+      scales_nv(sc.y, s1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a[4];  // row g, columns 0-1 and 2-3; row g + 8
+        e2m1x8_to_f16(w[j], a);
+        a[0] = mul_f16x2(a[0], s0[j]);
+        a[1] = mul_f16x2(a[1], s0[j]);
+        a[2] = mul_f16x2(a[2], s1[j]);
+        a[3] = mul_f16x2(a[3], s1[j]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) mma_f16(acc[r][n], a[0], a[2], a[1], a[3], b[q][n][2 * j], b[q][n][2 * j + 1]);
       }
-    }
+    } else {
+      const uint32_t sc = *reinterpret_cast<const uint32_t*>(scales + r * 32 + g * 4);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int c = c0 + i * kMoeWarps;
-      if (c >= chunks) break;
-      float s0[4], s1[4];
-      if constexpr (BS == 16) {
-        scales_nv(sc[i].x, s0);
-        scales_nv(sc[i].y, s1);
-      } else {
-        s0[0] = s0[1] = scale_mx(sc[i].x & 255u);
-        s0[2] = s0[3] = scale_mx(sc[i].x >> 8 & 255u);
-        s1[0] = s1[1] = scale_mx(sc[i].x >> 16 & 255u);
-        s1[2] = s1[3] = scale_mx(sc[i].x >> 24);
-      }
-      const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-      uint32_t b[NT][8];
+      for (int j = 0; j < 4; j += 2) {
+        const float s0 = scale_mx(sc >> (4 * j) & 255u), s1 = scale_mx(sc >> (16 + 4 * j) & 255u);
+        float d[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) load_b(c, n, b[n]);
+        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; j += BS / 16) {
-        float d[NT][4] = {};
-#pragma unroll
-        for (int q = 0; q < BS / 16; ++q) {
+        for (int k = j; k < j + 2; ++k) {
           uint32_t a[4];
-          e2m1x8_to_f16(ww[j + q], a);
+          e2m1x8_to_f16(w[k], a);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(d[n], a[0], a[2], a[1], a[3], b[n][2 * (j + q)], b[n][2 * (j + q) + 1]);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) mma_f16(d[n], a[0], a[2], a[1], a[3], b[q][n][2 * k], b[q][n][2 * k + 1]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(d[n][0], s0[j], acc[n][0]);
-          acc[n][1] = fmaf(d[n][1], s0[j], acc[n][1]);
-          acc[n][2] = fmaf(d[n][2], s1[j], acc[n][2]);
-          acc[n][3] = fmaf(d[n][3], s1[j], acc[n][3]);
+          acc[r][n][0] = fmaf(d[n][0], s0, acc[r][n][0]);
+          acc[r][n][1] = fmaf(d[n][1], s0, acc[r][n][1]);
+          acc[r][n][2] = fmaf(d[n][2], s1, acc[r][n][2]);
+          acc[r][n][3] = fmaf(d[n][3], s1, acc[r][n][3]);
         }
       }
     }
   }
 }
 
-// Partial sums of the 8 warps, added in warp order: row r, token n of the tile.
-template <int NT>
-__device__ __forceinline__ void put_partials(MoeShared& s, const float (&acc)[NT][4]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float* part = s.part + warp * (16 * NT * 8);
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    part[(n * 8 + 2 * t) * 16 + g] = acc[n][0];
-    part[(n * 8 + 2 * t + 1) * 16 + g] = acc[n][1];
-    part[(n * 8 + 2 * t) * 16 + g + 8] = acc[n][2];
-    part[(n * 8 + 2 * t + 1) * 16 + g + 8] = acc[n][3];
-  }
-}
-template <int NT>
-__device__ __forceinline__ float sum_partials(const MoeShared& s, int n, int r) {
-  float v = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kMoeWarps; ++w) v += s.part[w * (16 * NT * 8) + n * 16 + r];
-  return v;
-}
-
-// slots: the tokens of this unit (count <= 8 NT), in the expert's list
-template <int NT, int BS>
-__device__ __forceinline__ void up_unit(const MoeParams& p, MoeShared& s, int e, int tile, const uint16_t* slots, int count) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t at = ((int64_t)e * (p.I / 8) + tile) * p.hc;
-  const uint4* xrow[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int i = n * 8 + g;
-    xrow[n] = p.xh + (int64_t)(slots[i < count ? i : count - 1] / p.top) * p.hc * 8 + t;
-  }
-  float acc[NT][4] = {};
-  tile_product<NT, BS>(p.up_codes + at * 32, p.up_scales + at * 8 * (BS == 16 ? 2 : 1), p.hc, acc,
-                       [&](int c, int n, uint32_t(&b)[8]) {
-                         const uint4 lo = __ldg(xrow[n] + c * 8), hi = __ldg(xrow[n] + c * 8 + 4);
-                         b[0] = lo.x; b[1] = lo.y; b[2] = lo.z; b[3] = lo.w;
-                         b[4] = hi.x; b[5] = hi.y; b[6] = hi.z; b[7] = hi.w;
-                       });
-  put_partials<NT>(s, acc);
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 64; i += kMoeThreads) {
-    const int n = i >> 3, r = i & 7;
-    const bool there = n < count;
-    float a = 0.0f;
-    const int slot = slots[there ? n : 0];
-    if (there) {
-      const float f = p.xs[slot / p.top] * p.up_scale;
-      const float gate = sum_partials<NT>(s, n, r) * f, up = sum_partials<NT>(s, n, r + 8) * f;
-      a = __fdiv_rn(gate, 1.0f + expf(-gate)) * up;  // gate far below 0: expf overflows and the quotient is -0
-      p.act[(int64_t)slot * p.I + tile * 8 + r] = a;
-    }
-    uint32_t m = __float_as_uint(a) & 0x7fffffffu;
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-    if (there && r == 0) atomicMax(p.act_max + slot, m);  // a maximum: order changes nothing
-  }
-  __syncthreads();
-}
-
-template <int NT, int BS>
-__device__ __forceinline__ void down_unit(const MoeParams& p, MoeShared& s, int e, int tile, const uint16_t* slots, int count) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t at = ((int64_t)e * (p.H / 16) + tile) * p.ic;
-  const float* arow[NT];
-  float inv[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int i = n * 8 + g;
-    const int slot = slots[i < count ? i : count - 1];
-    arow[n] = p.act + (int64_t)slot * p.I + 4 * t;
-    inv[n] = pow2f(-f16_power(__ldcg(p.act_max + slot)));
-  }
-  float acc[NT][4] = {};
-  tile_product<NT, BS>(p.down_codes + at * 32, p.down_scales + at * 8 * (BS == 16 ? 2 : 1), p.ic, acc,
-                       [&](int c, int n, uint32_t(&b)[8]) {
-#pragma unroll
-                         for (int j = 0; j < 4; ++j) {
-                           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                           if (c * 64 + j * 16 < p.I) v = __ldcg(reinterpret_cast<const float4*>(arow[n] + c * 64 + j * 16));
-                           const __half2 lo = __floats2half2_rn(v.x * inv[n], v.y * inv[n]);
-                           const __half2 hi = __floats2half2_rn(v.z * inv[n], v.w * inv[n]);
-                           b[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
-                           b[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-                         }
-                       });
-  put_partials<NT>(s, acc);
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 128; i += kMoeThreads) {
-    const int n = i >> 4, r = i & 15;
-    if (n >= count) continue;
-    const int slot = slots[n];
-    const float f = pow2f(f16_power(__ldcg(p.act_max + slot))) * p.down_scale * s.weight[slot];
-    p.y[(int64_t)slot * p.H + tile * 16 + r] = sum_partials<NT>(s, n, r) * f;
-  }
-  __syncthreads();
-}
-
-// Runs f(expert, tile, slots, count) for this CTA's units: every active expert,
-// its tokens in groups of at most 32, its tiles.
-template <typename F>
-__device__ __forceinline__ void for_units(const MoeShared& s, int tiles, F&& f) {
-  int first = 0;  // index of the group's first unit
-  for (int a = 0; a < s.n_active; ++a) {
-    const int e = s.active[a], begin = s.start[e], end = s.start[e + 1];
-    for (int b = begin; b < end; b += 32) {
-      // units first .. first + tiles - 1 belong to CTA (unit % grid)
-      int u = (int)((blockIdx.x + gridDim.x - first % gridDim.x) % gridDim.x);
-      for (; u < tiles; u += gridDim.x) f(e, u, s.list + b, end - b < 32 ? end - b : 32);
-      first += tiles;
-    }
-  }
-}
-
+// The ring of one warp: pieces of up to kMoePiece chunks.
 template <int BS>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const __grid_constant__ MoeParams p) {
-  __shared__ MoeShared s;
-  route(p, s);
-  for_units(s, p.I / 8, [&](int e, int tile, const uint16_t* slots, int count) {
-    if (count <= 8) up_unit<1, BS>(p, s, e, tile, slots, count);
-    else if (count <= 16) up_unit<2, BS>(p, s, e, tile, slots, count);
-    else up_unit<4, BS>(p, s, e, tile, slots, count);
-  });
-  if (!grid_barrier(p.barrier, s)) return;
-  for_units(s, p.H / 16, [&](int e, int tile, const uint16_t* slots, int count) {
-    if (count <= 8) down_unit<1, BS>(p, s, e, tile, slots, count);
-    else if (count <= 16) down_unit<2, BS>(p, s, e, tile, slots, count);
-    else down_unit<4, BS>(p, s, e, tile, slots, count);
-  });
-  if (!grid_barrier(p.barrier + 1, s)) return;
-  for (int i = blockIdx.x * kMoeThreads + threadIdx.x; i < p.T * p.H; i += gridDim.x * kMoeThreads) {
-    const int t = i / p.H, h = i % p.H;
-    float v = 0.0f;
-    for (int k = 0; k < p.top; ++k) v += __ldcg(p.y + (int64_t)(t * p.top + k) * p.H + h);
-    if (p.dtype == kDtBF16) {
-      uint16_t r;
-      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
-      static_cast<uint16_t*>(p.out)[i] = r;
-    } else {
-      static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+struct MoeRing {
+  static constexpr int kCodes = 1024, kScales = 1024 * 2 / BS;  // bytes per chunk
+  static constexpr int kStage = kMoePiece * (kCodes + kScales);
+  static constexpr int kBytes = kMoeWarps * kMoeStages * kStage;
+};
+
+// This warp's part of a phase: units `unit`, unit + stride, ... below `end`, chunks
+// [c0, c1) of each.
+struct MoeWalk {
+  int unit, end, stride, c0, c1, chunks, units;  // units per group
+  int c;
+  __device__ __forceinline__ bool done() const { return unit >= end; }
+  __device__ __forceinline__ int piece() const { return c1 - c < kMoePiece ? c1 - c : kMoePiece; }
+  __device__ __forceinline__ void advance() {
+    c += kMoePiece;
+    if (c >= c1) { c = c0; unit += stride; }
+  }
+};
+
+// A phase: every group times `units` units of `chunks` chunks.  begin_unit(group,
+// unit) is called for a new unit, load_b(chunk, b) gives the B words, finish(group,
+// unit, acc) takes the sums (in every lane of the unit's first warp).
+template <int BS, bool UP, int PARTS>
+__device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint8_t* ring, uint32_t& it) {
+  using R = MoeRing<BS>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
+  const uint8_t* codes = UP ? p.up_codes : p.down_codes;
+  const uint8_t* scales = UP ? p.up_scales : p.down_scales;
+  const int64_t total = (int64_t)s.n_groups * units;
+  const int most = (int)((total + gridDim.x - 1) / gridDim.x);  // units of the busiest CTA
+  // warps per unit: the cut of K with the fewest rounds of work
+  int share = 1;
+  for (int c = 2; c <= 4; c *= 2)
+    if (c <= chunks && (most * c + kMoeWarps - 1) / kMoeWarps * share < (most * share + kMoeWarps - 1) / kMoeWarps * c) share = c;
+  const int part = warp % share;
+  MoeWalk w;
+  w.unit = (int)((int64_t)blockIdx.x * total / gridDim.x) + warp / share;
+  w.end = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
+  w.stride = kMoeWarps / share;
+  w.chunks = chunks;
+  w.units = units;
+  w.c0 = part * chunks / share;
+  w.c1 = (part + 1) * chunks / share;
+  w.c = w.c0;
+  MoeWalk ahead = w;
+  uint8_t* mine = ring + warp * kMoeStages * R::kStage;
+  uint64_t* full = s.full + warp * kMoeStages;
+  auto issue = [&](uint32_t at) {  // lane 0: the piece at `ahead` into stage at % kMoeStages
+    const int st = at % kMoeStages, n = ahead.piece();
+    const int64_t chunk = ((int64_t)s.g_expert[ahead.unit / units] * units + ahead.unit % units) * chunks + ahead.c;
+    mbar_arrive_expect_tx(full + st, n * (R::kCodes + R::kScales));
+    bulk_load(mine + st * R::kStage, codes + chunk * R::kCodes, n * R::kCodes, full + st);
+    bulk_load(mine + st * R::kStage + kMoePiece * R::kCodes, scales + chunk * R::kScales, n * R::kScales, full + st);
+  };
+  uint32_t issued = it;
+  for (int k = 0; k < kMoeStages && !ahead.done(); ++k, ++issued) {
+    if (lane == 0) issue(issued);
+    ahead.advance();
+  }
+  bool ok = true;
+  auto unit_of = [&](auto nt_tag) {
+    constexpr int NT = decltype(nt_tag)::value;
+    const int group = w.unit / units, u = w.unit % units, e = s.g_expert[group], count = s.g_count[group];
+    const uint16_t* slots = s.list + s.g_begin[group];
+    // this lane's B rows: token g of each tile of 8 (rows beyond the count repeat the last)
+    const uint4* row[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int i = n * 8 + g, slot = slots[i < count ? i : count - 1];
+      row[n] = reinterpret_cast<const uint4*>(UP ? p.xh + (int64_t)(slot / p.top) * p.hc * 64 : p.act + (int64_t)slot * p.ic * 64) + t;
     }
+    float acc[2][NT][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][n][c] = 0.0f;
+    const int unit = w.unit;
+    while (w.unit == unit) {
+      const int st = it % kMoeStages, pieces = w.piece();
+      if (!mbar_wait_bounded(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
+      const uint8_t* at = mine + st * R::kStage;
+#pragma unroll
+      for (int k = 0; k < kMoePiece; ++k) {
+        if (k >= pieces) break;
+        uint32_t b[PARTS][NT][8];
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4* from = row[n] + (UP ? 0 : q * (p.act_part / 8)) + (w.c + k) * 8;
+            const uint4 lo = UP ? __ldg(from) : *from, hi = UP ? __ldg(from + 4) : from[4];
+            b[q][n][0] = lo.x; b[q][n][1] = lo.y; b[q][n][2] = lo.z; b[q][n][3] = lo.w;
+            b[q][n][4] = hi.x; b[q][n][5] = hi.y; b[q][n][6] = hi.z; b[q][n][7] = hi.w;
+          }
+        chunk_product<NT, BS, PARTS>(at + k * R::kCodes, at + kMoePiece * R::kCodes + k * R::kScales, b, acc);
+      }
+      __syncwarp();  // every lane has read the stage
+      if (!ahead.done()) {
+        if (lane == 0) issue(issued);
+        ahead.advance();
+        ++issued;
+      }
+      ++it;
+      w.advance();
+    }
+    if (share > 1) {
+      // the unit's warps meet twice: sums written, sums read
+      float* mem = s.part[warp];
+      if (part > 0) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mem[((r * NT + n) * 4 + c) * 32 + lane] = acc[r][n][c];
+      }
+      // (a warp whose copy did not come takes the others with it)
+      uint32_t go = __all_sync(0xffffffffu, ok) ? 1u : 0u;
+      asm volatile(
+          "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, %1, %2, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+          : "+r"(go)
+          : "r"(1 + warp / share), "r"(share * 32)
+          : "memory");
+      ok = go != 0;
+      if (!ok) return;
+      if (part == 0) {
+        for (int q = 1; q < share; ++q)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[r][n][c] += s.part[warp + q][((r * NT + n) * 4 + c) * 32 + lane];
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / share), "r"(share * 32) : "memory");
+      if (part > 0) return;
+    }
+    if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
+    if constexpr (UP) {
+      const int en = exponent_bound(__ldg(p.norms + 2 * e)) + exponent_bound(__ldg(p.norms + 2 * e + 1));
+      const int ets = 2 * exponent_bound(fabsf(p.up_scale));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int i = n * 8 + 2 * t + c;
+          if (i >= count) continue;
+          const int slot = slots[i];
+          const int2 xp = __ldg(p.xp + slot / p.top);
+          const float f = pow2f(xp.x) * p.up_scale;
+          const int ea = xp.y + 2 * xp.x + en + ets - 15;  // |act| < 2^(ea + 15)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float gate = acc[r][n][c] * f, up = acc[r][n][c + 2] * f;
+            const float a = __fdiv_rn(gate, 1.0f + expf(-gate)) * up;  // gate far below 0: expf overflows and the quotient is -0
+            const float v = scalbnf(a, -ea);
+            // column 16 u + 8 r + g: block j = u % 4 of its chunk, lane (8 r + g) / 4 of the fragment
+            const int j = u & 3, at = (j >> 1) * 32 + ((8 * r + g) >> 2) * 8 + (j & 1) * 4 + (g & 3);
+            __half* to = p.act + ((int64_t)slot * p.ic + (u >> 2)) * 64 + at;
+            const __half hi = __float2half_rn(v);
+            *to = hi;
+            if (p.dtype == kDtF16) to[p.act_part] = __float2half_rn(v - __half2float(hi));
+            if (u + 1 == units && (units & 3))  // the other half of the last chunk is padding
+              for (int q = 0; q < 2; ++q) {
+                __half* pad = to + 32 - (j & 1) * 4 + q * 4;
+                *pad = __float2half_rn(0.0f);
+                if (p.dtype == kDtF16) pad[p.act_part] = __float2half_rn(0.0f);
+              }
+          }
+        }
+    } else {
+      const int en = exponent_bound(__ldg(p.norms + 2 * e)) + exponent_bound(__ldg(p.norms + 2 * e + 1));
+      const int ets = 2 * exponent_bound(fabsf(p.up_scale));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int i = n * 8 + 2 * t + c;
+          if (i >= count) continue;
+          const int slot = slots[i];
+          const int2 xp = __ldg(p.xp + slot / p.top);
+          const int ea = xp.y + 2 * xp.x + en + ets - 15;
+          const float f = p.down_scale * s.weight[slot];
+          float* to = p.y + (int64_t)slot * p.H + u * 32 + g;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            to[r * 16] = scalbnf(acc[r][n][c], ea) * f;
+            to[r * 16 + 8] = scalbnf(acc[r][n][c + 2], ea) * f;
+          }
+        }
+    }
+  };
+  while (ok && !w.done()) {
+    const int count = s.g_count[w.unit / units];
+    if (count <= 8) unit_of(std::integral_constant<int, 1>());
+    else if (count <= 16) unit_of(std::integral_constant<int, 2>());
+    else unit_of(std::integral_constant<int, 4>());
+  }
+  if (!ok)  // copies in flight must land before the CTA exits (bounded)
+    for (; it < issued; ++it) mbar_wait_bounded(full + it % kMoeStages, it / kMoeStages & 1, kDevErrLoadTimeout);
+  return ok;
+}
+
+template <int BS, int PARTS>
+__global__ void __launch_bounds__(kMoeThreads, 1) moe_experts_kernel(const __grid_constant__ MoeParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  MoeShared& s = *reinterpret_cast<MoeShared*>(ring + MoeRing<BS>::kBytes);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMoeWarps * kMoeStages; ++i) mbar_init(s.full + i, 1);
+    fence_barrier_init();
+  }
+  route(p, s);
+  uint32_t it = 0;  // pieces this warp has consumed
+  run_phase<BS, true, 1>(p, s, ring, it);
+  if (!grid_barrier(p.barrier, s)) return;
+  run_phase<BS, false, PARTS>(p, s, ring, it);
+  if (!grid_barrier(p.barrier + 1, s)) return;
+  const int h4 = p.H / 4;
+  for (int i = blockIdx.x * kMoeThreads + threadIdx.x; i < p.T * h4; i += gridDim.x * kMoeThreads) {
+    const int t = i / h4, h = i % h4;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < p.top; ++k) {
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.y + (int64_t)(t * p.top + k) * p.H) + h);
+      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+    }
+    uint32_t lo, hi;
+    if (p.dtype == kDtBF16) {
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
+    } else {
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
+    }
+    reinterpret_cast<uint2*>(p.out)[i] = make_uint2(lo, hi);
   }
 }
 
@@ -583,17 +756,16 @@ cudaError_t read_device_error_moe(unsigned* out, bool clear) {
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct MoeWorkspace {
-  int64_t logits, xh, xs, act, act_max, y, barrier, bytes;
+  int64_t logits, xh, xp, act, y, barrier, bytes;
 };
 
 static MoeWorkspace moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top) {
   MoeWorkspace w;
   w.logits = 0;
   w.xh = up256(T * E * 4);
-  w.xs = w.xh + up256(T * ((H + 63) / 64) * 128);
-  w.act = w.xs + up256(T * 4);
-  w.act_max = w.act + up256(T * top * I * 4);
-  w.y = w.act_max + up256(T * top * 4);
+  w.xp = w.xh + up256(T * ((H + 63) / 64) * 128);
+  w.act = w.xp + up256(T * 8);
+  w.y = w.act + 2 * up256(T * top * ((I + 63) / 64) * 128);
   w.barrier = w.y + up256(T * top * H * 4);
   w.bytes = w.barrier + 256;
   return w;
@@ -616,25 +788,28 @@ static int check_moe(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top, in
 using namespace qz;
 
 extern "C" int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int64_t E, int64_t rows, int64_t K,
-                             int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, void* stream) {
+                             int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, float* norms_out,
+                             void* stream) {
   if (format != QZ_FMT_NVFP4 && format != QZ_FMT_MXFP4)
     return fail(QZ_ERR_INVALID, "the experts are NVFP4 (blocks of 16) or MXFP4 (blocks of 32), got format %d", format);
   if (E < 1 || E > kMoeMaxExperts || rows <= 0 || rows % 32 || K <= 0 || K % 32)
     return fail(QZ_ERR_INVALID, "need 1 to %d experts, rows and K positive multiples of 32", kMoeMaxExperts);
-  if (!scale_codes || !packed || !codes_out || !scales_out) return fail(QZ_ERR_INVALID, "NULL pointer");
+  if (!scale_codes || !packed || !codes_out || !scales_out || (gate_up && !norms_out)) return fail(QZ_ERR_INVALID, "NULL pointer");
   if ((reinterpret_cast<uintptr_t>(codes_out) | reinterpret_cast<uintptr_t>(scales_out)) % 16)
     return fail(QZ_ERR_INVALID, "codes_out and scales_out must be 16-byte aligned");
   int sms = 0;
   const int s = current_sms(&sms);
   if (s != QZ_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (format == QZ_FMT_NVFP4)
-    moe_layout_kernel<16><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, gate_up,
-                                                   reinterpret_cast<uint32_t*>(codes_out), scales_out);
-  else
-    moe_layout_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, gate_up,
-                                                   reinterpret_cast<uint32_t*>(codes_out), scales_out);
-  return cuda_status(cudaGetLastError(), "moe layout launch");
+  uint32_t* co = reinterpret_cast<uint32_t*>(codes_out);
+  if (format == QZ_FMT_NVFP4) moe_layout_kernel<16><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, gate_up, co, scales_out);
+  else moe_layout_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, gate_up, co, scales_out);
+  int r = cuda_status(cudaGetLastError(), "moe layout launch");
+  if (r != QZ_OK || !gate_up) return r;
+  if ((r = cuda_status(cudaMemsetAsync(norms_out, 0, (size_t)E * 8, st), "cudaMemsetAsync")) != QZ_OK) return r;
+  if (format == QZ_FMT_NVFP4) moe_norm_kernel<16><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms_out);
+  else moe_norm_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms_out);
+  return cuda_status(cudaGetLastError(), "moe norm launch");
 }
 
 extern "C" int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k, int64_t* bytes) {
@@ -647,7 +822,7 @@ extern "C" int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int6
 
 extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k,
                       int renormalize, const void* router, int router_dtype, int format, const uint8_t* up_codes,
-                      const uint8_t* up_scales, float up_tensor_scale, const uint8_t* down_codes,
+                      const uint8_t* up_scales, const float* up_norms, float up_tensor_scale, const uint8_t* down_codes,
                       const uint8_t* down_scales, float down_tensor_scale, void* out, int* ids, float* weights,
                       void* workspace, int64_t workspace_bytes, void* stream) {
   int s = check_moe(T, H, I, E, top_k, format);
@@ -656,7 +831,7 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   if (router_dtype != QZ_DTYPE_F32 && router_dtype != QZ_DTYPE_BF16 && router_dtype != QZ_DTYPE_F16)
     return fail(QZ_ERR_INVALID, "unknown dtype %d", router_dtype);
   if (T == 0) return QZ_OK;
-  if (!x || !router || !up_codes || !up_scales || !down_codes || !down_scales || !out || !workspace)
+  if (!x || !router || !up_codes || !up_scales || !up_norms || !down_codes || !down_scales || !out || !workspace)
     return fail(QZ_ERR_INVALID, "NULL pointer");
   if (ldx < H || ldx % 8) return fail(QZ_ERR_INVALID, "rows of x must be at least H apart and 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(up_codes) |
@@ -675,33 +850,45 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   p.hc = (int)((H + 63) / 64); p.ic = (int)((I + 63) / 64);
   p.renorm = renormalize; p.dtype = dtype;
   p.logits = reinterpret_cast<float*>(ws + w.logits);
-  p.up_codes = reinterpret_cast<const uint4*>(up_codes); p.up_scales = reinterpret_cast<const uint32_t*>(up_scales);
-  p.down_codes = reinterpret_cast<const uint4*>(down_codes); p.down_scales = reinterpret_cast<const uint32_t*>(down_scales);
+  p.up_codes = up_codes; p.up_scales = up_scales; p.norms = up_norms;
+  p.down_codes = down_codes; p.down_scales = down_scales;
   p.up_scale = up_tensor_scale; p.down_scale = down_tensor_scale;
-  p.xh = reinterpret_cast<const uint4*>(ws + w.xh);
-  p.xs = reinterpret_cast<float*>(ws + w.xs);
-  p.act = reinterpret_cast<float*>(ws + w.act);
-  p.act_max = reinterpret_cast<unsigned*>(ws + w.act_max);
+  p.xh = reinterpret_cast<const __half*>(ws + w.xh);
+  p.xp = reinterpret_cast<const int2*>(ws + w.xp);
+  p.act = reinterpret_cast<__half*>(ws + w.act);
+  p.act_part = up256(T * top_k * p.ic * 128) / 2;
   p.y = reinterpret_cast<float*>(ws + w.y);
   p.barrier = reinterpret_cast<int*>(ws + w.barrier);
   p.out = out; p.ids = ids; p.weights = weights;
-  const int groups = (int)((T + 7) / 8);
-  moe_router_kernel<<<(unsigned)(E * groups + T), kRouterThreads, 0, st>>>(
-      x, ldx, dtype, router, router_dtype, p.T, p.H, p.E, reinterpret_cast<float*>(ws + w.logits),
-      reinterpret_cast<__half*>(ws + w.xh), reinterpret_cast<float*>(ws + w.xs), p.act_max, (int)(T * top_k), p.barrier);
+  const unsigned grid = (unsigned)(E * ((T + 7) / 8) + T);
+#define QZ_ROUTER(DT, RDT)                                                                                              \
+  moe_router_kernel<DT, RDT><<<grid, kRouterThreads, 0, st>>>(x, ldx, router, p.T, p.H, p.E,                            \
+                                                              reinterpret_cast<float*>(ws + w.logits),                  \
+                                                              reinterpret_cast<uint4*>(ws + w.xh),                      \
+                                                              reinterpret_cast<int2*>(ws + w.xp), p.barrier)
+#define QZ_ROUTER_OF(DT)                                                                                                \
+  if (router_dtype == QZ_DTYPE_F32) QZ_ROUTER(DT, kDtF32);                                                              \
+  else if (router_dtype == QZ_DTYPE_BF16) QZ_ROUTER(DT, kDtBF16);                                                       \
+  else QZ_ROUTER(DT, kDtF16)
+  if (dtype == QZ_DTYPE_BF16) { QZ_ROUTER_OF(kDtBF16); }
+  else { QZ_ROUTER_OF(kDtF16); }
+#undef QZ_ROUTER_OF
+#undef QZ_ROUTER
   if ((s = cuda_status(cudaGetLastError(), "moe router launch")) != QZ_OK) return s;
-  void* args[] = {&p};
-  const void* fn = format == QZ_FMT_NVFP4 ? reinterpret_cast<const void*>(&moe_experts_kernel<16>)
-                                          : reinterpret_cast<const void*>(&moe_experts_kernel<32>);
-  static int per_sm[2] = {0, 0};  // resident CTAs per SM (a benign race: every thread computes the same value)
-  int& occ = per_sm[format == QZ_FMT_NVFP4 ? 0 : 1];
-  if (!occ) {
-    int n = 0;
-    s = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kMoeThreads, 0), "moe occupancy");
+  const bool nv = format == QZ_FMT_NVFP4, two = dtype == QZ_DTYPE_F16;
+  const void* fn = nv ? (two ? reinterpret_cast<const void*>(&moe_experts_kernel<16, 2>) : reinterpret_cast<const void*>(&moe_experts_kernel<16, 1>))
+                      : (two ? reinterpret_cast<const void*>(&moe_experts_kernel<32, 2>) : reinterpret_cast<const void*>(&moe_experts_kernel<32, 1>));
+  const int smem = (nv ? MoeRing<16>::kBytes : MoeRing<32>::kBytes) + (int)sizeof(MoeShared);
+  static bool attr_set[4][64] = {};  // per kernel and device (a benign race: every thread sets the same value)
+  int dev = 0;
+  if ((s = cuda_status(cudaGetDevice(&dev), "cudaGetDevice")) != QZ_OK) return s;
+  bool* done = dev >= 0 && dev < 64 ? &attr_set[(nv ? 0 : 2) + (two ? 1 : 0)][dev] : nullptr;
+  if (!done || !*done) {
+    s = cuda_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
     if (s != QZ_OK) return s;
-    if (n < 1) return fail(QZ_ERR_CUDA, "moe kernel does not fit an SM");
-    occ = n > 2 ? 2 : n;
+    if (done) *done = true;
   }
-  return cuda_status(cudaLaunchCooperativeKernel(fn, dim3((unsigned)(sms * occ)), dim3(kMoeThreads), args, 0, st),
+  void* args[] = {&p};
+  return cuda_status(cudaLaunchCooperativeKernel(fn, dim3((unsigned)sms), dim3(kMoeThreads), args, (size_t)smem, st),
                      "moe experts launch");
 }

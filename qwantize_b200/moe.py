@@ -26,10 +26,11 @@ def _lay_out(codes, packed, fmt, gate_up, dev):
     Kp = (K + 63) // 64 * 64
     c = torch.empty(E * rows * Kp // 2, dtype=torch.uint8, device=dev)
     s = torch.empty(E * rows * Kp // bs, dtype=torch.uint8, device=dev)
+    norms = torch.empty(E, 2, dtype=torch.float32, device=dev) if gate_up else None
     with torch.cuda.device(dev):
         L.check(L.load().qz_moe_layout(L.ptr(codes), L.ptr(packed), E, rows, K, _FMT[fmt], int(gate_up), L.ptr(c),
-                                       L.ptr(s), L.stream_ptr(dev)), "qz_moe_layout")
-    return c, s, E, rows, K
+                                       L.ptr(s), L.ptr(norms), L.stream_ptr(dev)), "qz_moe_layout")
+    return c, s, norms, E, rows, K
 
 
 class FP4Experts:
@@ -42,8 +43,8 @@ class FP4Experts:
 
     def __init__(self, gate_up, down, fmt="nvfp4", tensor_scales=(1.0, 1.0)):
         self.device = dev = cuda_device(gate_up[0])
-        self.up_codes, self.up_scales, self.E, rows, self.H = _lay_out(*gate_up, fmt, True, dev)
-        self.down_codes, self.down_scales, E, H, self.I = _lay_out(*down, fmt, False, dev)
+        self.up_codes, self.up_scales, self.up_norms, self.E, rows, self.H = _lay_out(*gate_up, fmt, True, dev)
+        self.down_codes, self.down_scales, _, E, H, self.I = _lay_out(*down, fmt, False, dev)
         assert (E, H, 2 * self.I) == (self.E, self.H, rows), (
             f"gate_up ({self.E}, {rows}, {self.H}) and down ({E}, {H}, {self.I}) do not belong together")
         assert self.E <= 512, f"{self.E} experts, expected at most 512"
@@ -115,7 +116,7 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
             L.check(L.load().qz_moe(
                 xd.data_ptr(), L.dtype_code(xd.dtype), ldx, T, H, experts.I, E, top_k, int(bool(renormalize)),
                 r.data_ptr(), L.dtype_code(r.dtype), _FMT[experts.fmt], experts.up_codes.data_ptr(),
-                experts.up_scales.data_ptr(), experts.tensor_scales[0], experts.down_codes.data_ptr(),
+                experts.up_scales.data_ptr(), experts.up_norms.data_ptr(), experts.tensor_scales[0], experts.down_codes.data_ptr(),
                 experts.down_scales.data_ptr(), experts.tensor_scales[1], y.data_ptr(),
                 ids.data_ptr() if return_routing else None, weights.data_ptr() if return_routing else None,
                 ws.data_ptr(), n, L.stream_ptr(dev)), "qz_moe")
