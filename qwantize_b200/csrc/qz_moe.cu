@@ -11,16 +11,18 @@
 //
 // Two launches.  moe_router_kernel: the logits, and x as fp16 in the order of
 // the matrix instructions' B fragments.  moe_experts_kernel, cooperative, one
-// CTA of 12 warps per SM: each CTA derives the routing from the logits for itself
+// CTA of 16 warps per SM: each CTA derives the routing from the logits for itself
 // (they are a few KB), then the CTAs share the units of the gate / up product; a
 // grid barrier; the units of the down product; a grid barrier; the weighted sum
 // over each token's experts in a fixed order.
 //
-// A unit is 32 weight rows of one expert times up to 32 of its tokens.  A CTA has
-// a run of neighbouring units, so its warps share an expert's tokens in L1; a
-// warp takes a unit alone and streams its weights through its own ring of bulk
-// copies, never waiting for another warp.  Where units are few, 2 or 4 warps cut a
-// unit's K and add up through shared memory.
+// A unit is 32 weight rows of one expert times up to 16 of its tokens (more would
+// be bound by the matrix instructions and gain nothing).  A CTA has a run of
+// neighbouring units, so its warps share an expert's tokens in L1; a warp takes
+// a unit alone and streams its weights through its own ring of bulk copies,
+// never waiting for another warp.  The units that are left when every warp has had
+// its share are cut along K by 2, 4 or 8 warps each, which add up through shared
+// memory.
 //
 // Weights are laid out once in the order of the A fragments of mma.m16n8k16
 // (fp16, fp32 accumulation): a lane's 16 bytes hold its 4 steps of one 16-row
@@ -57,9 +59,9 @@ int cuda_status(cudaError_t e, const char* what);
 int current_sms(int* sms);
 
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTop = 16;
-constexpr int kMoeWarps = 12, kMoeThreads = kMoeWarps * 32;
+constexpr int kMoeWarps = 16, kMoeThreads = kMoeWarps * 32;
 constexpr int kMoeMaxSlots = kMoeMaxTokens * kMoeMaxTop;
-constexpr int kMoeGroup = 32;                                                  // tokens of a unit
+constexpr int kMoeGroup = 16;                                                  // tokens of a unit
 constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxSlots / kMoeGroup;
 constexpr int kMoePiece = 4, kMoeStages = 2;                                   // chunks per bulk copy, copies in flight per warp
 
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kRouterThreads)
 // ---------------------------------------------------------------------------
 struct MoeShared {
   float weight[kMoeMaxSlots];
-  uint16_t id[kMoeMaxSlots];
+  uint16_t id[kMoeMaxSlots], rank[kMoeMaxSlots];  // a slot's expert, its place among the expert's slots
   uint16_t list[kMoeMaxSlots];            // slots (token * top + k) grouped by expert, tokens ascending
   uint16_t count[kMoeMaxExperts];
   uint16_t start[kMoeMaxExperts];
@@ -273,7 +275,9 @@ struct MoeShared {
   uint16_t g_expert[kMoeMaxGroups], g_begin[kMoeMaxGroups], g_count[kMoeMaxGroups];
   int n_groups, ok;
   uint64_t full[kMoeWarps * kMoeStages];  // the warps' rings
-  float part[kMoeWarps][32 * 32];         // sums of warps that share a unit: (value, lane)
+  float x_scale[kMoeMaxTokens];           // power of two of a token times the tensor scale
+  int16_t act_exp[kMoeMaxSlots];          // e: |activation| of the slot < 2^(e + 15)
+  float part[kMoeWarps][16 * 32];         // sums of warps that share a unit: (value, lane)
 };
 
 // All CTAs arrive, then wait for each other (they are all resident: cooperative
@@ -309,70 +313,113 @@ __device__ __forceinline__ uint32_t order_bits(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int t = warp; t < p.T; t += kMoeWarps) {
-    constexpr int W = kMoeMaxExperts / 32;
-    const int ne = (p.E + 31) / 32;  // words in use
-    uint32_t key[W];
-    float val[W];
-    float top0 = 0.0f, sum = 0.0f;
-    uint32_t taken_key = 0, mine = 0;
+// The choices of N tokens t0, t0 + kMoeWarps, ... by one warp, side by side (one
+// choice is a chain of warp-wide operations): lane l holds experts W l .. W l + W -
+// 1, so the lowest index among equal logits is in the lowest lane.
+template <int W, int N>
+__device__ __forceinline__ void choose(const MoeParams& p, MoeShared& s, int t0) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[N][W], chosen[N];
+  uint16_t mine[N];  // lane k keeps choice k
+  float all[N];
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const int e = i * 32 + lane;
-      val[i] = e < p.E ? __ldcg(p.logits + (int64_t)t * p.E + e) : 0.0f;
-      key[i] = e < p.E ? max(order_bits(val[i]), 1u) : 0u;  // 0: not there, or taken
-    }
-    float chosen = 0.0f;  // lane k keeps the logit of choice k
-    for (int k = 0; k < p.top; ++k) {
-      taken_key = 0;
+  for (int n = 0; n < N; ++n) {
+    const int t = t0 + n * kMoeWarps;
+    all[n] = 0.0f;
+    chosen[n] = 0;
+    mine[n] = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      key[n][i] = t < p.T && lane * W + i < p.E ? order_bits(__ldcg(p.logits + (int64_t)t * p.E + lane * W + i)) : 0u;  // 0: not there, or taken
+  }
+  uint32_t top[N];
+  auto logit = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); };
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max(m, key[n][i]);
+    top[n] = __reduce_max_sync(0xffffffffu, m);
+    if (!p.renorm)
 #pragma unroll
       for (int i = 0; i < W; ++i)
-        if (i < ne) taken_key = max(taken_key, key[i]);
-      taken_key = __reduce_max_sync(0xffffffffu, taken_key);
-      uint32_t e = 0xffffffffu;
-      float v = 0.0f;
+        if (key[n][i]) all[n] += expf(logit(key[n][i]) - logit(top[n]));
+  }
+  for (int k = 0; k < p.top; ++k) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) m = max(m, key[n][i]);
+      const uint32_t best = __reduce_max_sync(0xffffffffu, m);
+      const int src = __ffs(__ballot_sync(0xffffffffu, m == best)) - 1;
+      int at = 0;
 #pragma unroll
       for (int i = W - 1; i >= 0; --i)
-        if (i < ne && key[i] == taken_key) e = i * 32 + lane;
-      e = __reduce_min_sync(0xffffffffu, e);
+        if (key[n][i] == best) at = i;
+      if (lane == src) {
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (i < ne && e == (uint32_t)(i * 32 + lane)) { v = val[i]; key[i] = 0; }
-      v = __shfl_sync(0xffffffffu, v, e & 31);
-      if (k == 0) top0 = v;
-      if (lane == k) { chosen = v; mine = e; }
+        for (int i = 0; i < W; ++i)
+          if (i == at) key[n][i] = 0;
+      }
+      at = __shfl_sync(0xffffffffu, at, src);
+      if (lane == k) { chosen[n] = best; mine[n] = (uint16_t)(src * W + at); }
     }
-    if (p.renorm) {
-      sum = lane < p.top ? expf(chosen - top0) : 0.0f;
-    } else {
+  }
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (i * 32 + lane < p.E) sum += expf(val[i] - top0);
-    }
+  for (int n = 0; n < N; ++n) {
+    const int t = t0 + n * kMoeWarps;
+    const float e = lane < p.top ? expf(logit(chosen[n]) - logit(top[n])) : 0.0f;
+    float sum = p.renorm ? e : all[n];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < p.top) {
-      const float w = __fdiv_rn(expf(chosen - top0), sum);
-      s.id[t * p.top + lane] = (uint16_t)mine;
+    if (t < p.T && lane < p.top) {
+      const float w = __fdiv_rn(e, sum);
+      s.id[t * p.top + lane] = mine[n];
       s.weight[t * p.top + lane] = w;
       if (blockIdx.x == 0) {
-        if (p.ids) p.ids[t * p.top + lane] = (int)mine;
+        if (p.ids) p.ids[t * p.top + lane] = (int)mine[n];
         if (p.weights) p.weights[t * p.top + lane] = w;
       }
     }
   }
-  __syncthreads();
-  // counts per expert, starts and groups, lists: a warp compares 32 slots at a time
-  const int n = p.T * p.top;
-  for (int e = warp; e < p.E; e += kMoeWarps) {
-    int c = 0;
-    for (int i = 0; i < n; i += 32) c += __popc(__ballot_sync(0xffffffffu, i + lane < n && s.id[i + lane] == e));
-    if (lane == 0) s.count[e] = (uint16_t)c;
+}
+
+template <int W, int N>
+__device__ __forceinline__ void choose_all(const MoeParams& p, MoeShared& s) {
+  const int warp = threadIdx.x >> 5;
+  if (p.T <= kMoeWarps) {
+    if (warp < p.T) choose<W, 1>(p, s, warp);
+  } else {
+    for (int t0 = warp; t0 < p.T; t0 += N * kMoeWarps) choose<W, N>(p, s, t0);
   }
+}
+
+__device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) s.count[e] = 0;
+  if (p.E <= 32) choose_all<1, 4>(p, s);
+  else if (p.E <= 64) choose_all<2, 4>(p, s);
+  else if (p.E <= 128) choose_all<4, 4>(p, s);
+  else if (p.E <= 256) choose_all<8, 2>(p, s);
+  else choose_all<16, 1>(p, s);
   __syncthreads();
+  // one warp numbers each expert's slots in ascending order, 32 slots at a time,
+  // then lays out the groups
+  const int n = p.T * p.top;
   if (warp == 0) {
+    for (int i = lane; i < (n + 31) / 32 * 32; i += 32) {
+      const unsigned there = __ballot_sync(0xffffffffu, i < n);
+      if (i < n) {
+        const int e = s.id[i];
+        const unsigned same = __match_any_sync(there, e);
+        const int before = s.count[e], rank = __popc(same & ((1u << lane) - 1u));
+        s.rank[i] = (uint16_t)(before + rank);
+        __syncwarp(there);
+        if (rank == 0) s.count[e] = (uint16_t)(before + __popc(same));
+      }
+      __syncwarp();
+    }
     int at = 0, groups = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int c = e0 + lane < p.E ? s.count[e0 + lane] : 0, m = (c + kMoeGroup - 1) / kMoeGroup;
@@ -395,15 +442,14 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     if (lane == 0) s.n_groups = groups;
   }
   __syncthreads();
-  for (int e = warp; e < p.E; e += kMoeWarps) {
-    if (s.count[e] == 0) continue;
-    int at = s.start[e];
-    for (int i = 0; i < n; i += 32) {
-      const bool mine = i + lane < n && s.id[i + lane] == e;
-      const unsigned m = __ballot_sync(0xffffffffu, mine);
-      if (mine) s.list[at + __popc(m & ((1u << lane) - 1u))] = (uint16_t)(i + lane);
-      at += __popc(m);
-    }
+  for (int i = threadIdx.x; i < n; i += kMoeThreads) {
+    const int e = s.id[i];
+    s.list[s.start[e] + s.rank[i]] = (uint16_t)i;
+    const int2 xp = __ldg(p.xp + i / p.top);
+    const float2 norm = __ldg(reinterpret_cast<const float2*>(p.norms) + e);
+    const int bound = xp.y + 2 * xp.x + exponent_bound(norm.x) + exponent_bound(norm.y) + 2 * exponent_bound(fabsf(p.up_scale)) - 15;
+    s.act_exp[i] = (int16_t)min(max(bound, -140), 113);  // an fp32 activation is below 2^128; below 2^-125 nothing is left
+    if (i % p.top == 0) s.x_scale[i / p.top] = pow2f(xp.x) * p.up_scale;
   }
   __syncthreads();
 }
@@ -422,21 +468,22 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Four E4M3 scales of a word as fp16 pairs (s, s).
-__device__ __forceinline__ void scales_nv(uint32_t w, uint32_t (&s)[4]) {
+// Four E4M3 scales of a word as fp16 pairs (s, s) (the multiplication reads one half twice).
+__device__ __forceinline__ void scales_nv(uint32_t w, __half2 (&s)[4]) {
   uint32_t h0, h1;
   asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
       : "=r"(h0), "=r"(h1)
       : "r"(w));
-  s[0] = __byte_perm(h0, 0, 0x1010);
-  s[1] = __byte_perm(h0, 0, 0x3232);
-  s[2] = __byte_perm(h1, 0, 0x1010);
-  s[3] = __byte_perm(h1, 0, 0x3232);
+  const __half2 x = *reinterpret_cast<const __half2*>(&h0), y = *reinterpret_cast<const __half2*>(&h1);
+  s[0] = __low2half2(x);
+  s[1] = __high2half2(x);
+  s[2] = __low2half2(y);
+  s[3] = __high2half2(y);
 }
 __device__ __forceinline__ float scale_mx(uint32_t c) {
   return __uint_as_float(c == 0 ? 0x00400000u : c == 255 ? 0x7fffffffu : c << 23);
@@ -455,7 +502,7 @@ __device__ __forceinline__ void chunk_product(const uint8_t* codes, const uint8_
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
     if constexpr (BS == 16) {
       const uint2 sc = *reinterpret_cast<const uint2*>(scales + r * 64 + g * 8);
-      uint32_t s0[4], s1[4];
+      __half2 s0[4], s1[4];
       scales_nv(sc.x, s0);
       scales_nv(sc.y, s1);
 #pragma unroll
@@ -508,65 +555,95 @@ struct MoeRing {
   static constexpr int kBytes = kMoeWarps * kMoeStages * kStage;
 };
 
-// This warp's part of a phase: units `unit`, unit + stride, ... below `end`, chunks
-// [c0, c1) of each.
+// This warp's part of a phase: `whole` units of its own, kMoeWarps apart, then
+// perhaps a share of one more.
 struct MoeWalk {
-  int unit, end, stride, c0, c1, chunks, units;  // units per group
-  int c;
-  __device__ __forceinline__ bool done() const { return unit >= end; }
+  int group, unit;             // current group and unit in it
+  int units, chunks;           // per group; per unit
+  int left;                    // units after the current one
+  int c, c0, c1;               // current chunk; this warp's chunks of the current unit
+  int share, part;             // warps that share the last unit, this warp's place among them; 0: no last unit
+  int last_group, last_unit;
+  bool whole;                  // the current unit is this warp's alone
+
+  __device__ __forceinline__ MoeWalk(int64_t total, int units_, int chunks_) : units(units_), chunks(chunks_) {
+    const int warp = threadIdx.x >> 5;
+    const int begin = (int)((int64_t)blockIdx.x * total / gridDim.x), end = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
+    const int rounds = (end - begin) / kMoeWarps, rest = (end - begin) % kMoeWarps;
+    share = 1;
+    while (share < 8 && rest * share * 2 <= kMoeWarps && share * 2 <= chunks) share *= 2;
+    const int last = begin + rounds * kMoeWarps + warp / share;
+    if (last < end) {
+      part = warp % share;
+      last_group = last / units;
+      last_unit = last % units;
+    } else {
+      share = 0;
+    }
+    left = rounds + (share ? 1 : 0);
+    whole = true;
+    c0 = 0;
+    c1 = chunks;
+    group = (begin + warp) / units;
+    unit = (begin + warp) % units;
+    enter();
+  }
+  __device__ __forceinline__ bool done() const { return left < 0; }
+  __device__ __forceinline__ void enter() {  // the next unit's first chunk
+    if (--left == 0 && share) {
+      whole = share == 1;
+      group = last_group;
+      unit = last_unit;
+      c0 = part * chunks / share;
+      c1 = (part + 1) * chunks / share;
+    }
+    c = c0;
+  }
   __device__ __forceinline__ int piece() const { return c1 - c < kMoePiece ? c1 - c : kMoePiece; }
-  __device__ __forceinline__ void advance() {
+  __device__ __forceinline__ bool advance() {  // true: a new unit
     c += kMoePiece;
-    if (c >= c1) { c = c0; unit += stride; }
+    if (c < c1) return false;
+    unit += kMoeWarps;
+    while (unit >= units) { unit -= units; ++group; }
+    enter();
+    return true;
   }
 };
 
-// A phase: every group times `units` units of `chunks` chunks.  begin_unit(group,
-// unit) is called for a new unit, load_b(chunk, b) gives the B words, finish(group,
-// unit, acc) takes the sums (in every lane of the unit's first warp).
+// One phase: every group times its units.  UP: gate / up and the activation from
+// x; else: down from the activations (in PARTS addends), weighted.
 template <int BS, bool UP, int PARTS>
 __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint8_t* ring, uint32_t& it) {
   using R = MoeRing<BS>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
   const uint8_t* codes = UP ? p.up_codes : p.down_codes;
   const uint8_t* scales = UP ? p.up_scales : p.down_scales;
-  const int64_t total = (int64_t)s.n_groups * units;
-  const int most = (int)((total + gridDim.x - 1) / gridDim.x);  // units of the busiest CTA
-  // warps per unit: the cut of K with the fewest rounds of work
-  int share = 1;
-  for (int c = 2; c <= 4; c *= 2)
-    if (c <= chunks && (most * c + kMoeWarps - 1) / kMoeWarps * share < (most * share + kMoeWarps - 1) / kMoeWarps * c) share = c;
-  const int part = warp % share;
-  MoeWalk w;
-  w.unit = (int)((int64_t)blockIdx.x * total / gridDim.x) + warp / share;
-  w.end = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
-  w.stride = kMoeWarps / share;
-  w.chunks = chunks;
-  w.units = units;
-  w.c0 = part * chunks / share;
-  w.c1 = (part + 1) * chunks / share;
-  w.c = w.c0;
-  MoeWalk ahead = w;
+  const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
+  MoeWalk w((int64_t)s.n_groups * units, units, chunks), ahead = w;
   uint8_t* mine = ring + warp * kMoeStages * R::kStage;
   uint64_t* full = s.full + warp * kMoeStages;
-  auto issue = [&](uint32_t at) {  // lane 0: the piece at `ahead` into stage at % kMoeStages
-    const int st = at % kMoeStages, n = ahead.piece();
-    const int64_t chunk = ((int64_t)s.g_expert[ahead.unit / units] * units + ahead.unit % units) * chunks + ahead.c;
+  int64_t at_unit = 0;  // first chunk of the unit that is loaded
+  auto locate = [&]() {
+    if (!ahead.done()) at_unit = ((int64_t)s.g_expert[ahead.group] * units + ahead.unit) * chunks;
+  };
+  auto issue = [&](uint32_t i) {  // lane 0: the piece at `ahead` into stage i % kMoeStages
+    const int st = i % kMoeStages, n = ahead.piece();
+    const int64_t chunk = at_unit + ahead.c;
     mbar_arrive_expect_tx(full + st, n * (R::kCodes + R::kScales));
     bulk_load(mine + st * R::kStage, codes + chunk * R::kCodes, n * R::kCodes, full + st);
     bulk_load(mine + st * R::kStage + kMoePiece * R::kCodes, scales + chunk * R::kScales, n * R::kScales, full + st);
   };
+  locate();
   uint32_t issued = it;
   for (int k = 0; k < kMoeStages && !ahead.done(); ++k, ++issued) {
     if (lane == 0) issue(issued);
-    ahead.advance();
+    if (ahead.advance()) locate();
   }
   bool ok = true;
   auto unit_of = [&](auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
-    const int group = w.unit / units, u = w.unit % units, e = s.g_expert[group], count = s.g_count[group];
-    const uint16_t* slots = s.list + s.g_begin[group];
+    const int u = w.unit, count = s.g_count[w.group], share = w.whole ? 1 : w.share, part = w.part;
+    const uint16_t* slots = s.list + s.g_begin[w.group];
     // this lane's B rows: token g of each tile of 8 (rows beyond the count repeat the last)
     const uint4* row[NT];
 #pragma unroll
@@ -581,14 +658,13 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][n][c] = 0.0f;
-    const int unit = w.unit;
-    while (w.unit == unit) {
+    bool more = true;
+    while (more) {
       const int st = it % kMoeStages, pieces = w.piece();
       if (!mbar_wait_bounded(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
       const uint8_t* at = mine + st * R::kStage;
-#pragma unroll
-      for (int k = 0; k < kMoePiece; ++k) {
-        if (k >= pieces) break;
+#pragma unroll 1
+      for (int k = 0; k < pieces; ++k) {
         uint32_t b[PARTS][NT][8];
 #pragma unroll
         for (int q = 0; q < PARTS; ++q)
@@ -604,14 +680,15 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
       __syncwarp();  // every lane has read the stage
       if (!ahead.done()) {
         if (lane == 0) issue(issued);
-        ahead.advance();
+        if (ahead.advance()) locate();
         ++issued;
       }
       ++it;
-      w.advance();
+      more = !w.advance();
     }
     if (share > 1) {
-      // the unit's warps meet twice: sums written, sums read
+      // the unit's warps meet twice: sums written, sums read (a warp whose copy did
+      // not come takes the others with it)
       float* mem = s.part[warp];
       if (part > 0) {
 #pragma unroll
@@ -621,7 +698,6 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
 #pragma unroll
             for (int c = 0; c < 4; ++c) mem[((r * NT + n) * 4 + c) * 32 + lane] = acc[r][n][c];
       }
-      // (a warp whose copy did not come takes the others with it)
       uint32_t go = __all_sync(0xffffffffu, ok) ? 1u : 0u;
       asm volatile(
           "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, %1, %2, a;\n selp.u32 %0, 1, 0, b;\n}\n"
@@ -642,66 +718,49 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
       asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / share), "r"(share * 32) : "memory");
       if (part > 0) return;
     }
-    if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
-    if constexpr (UP) {
-      const int en = exponent_bound(__ldg(p.norms + 2 * e)) + exponent_bound(__ldg(p.norms + 2 * e + 1));
-      const int ets = 2 * exponent_bound(fabsf(p.up_scale));
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int i = n * 8 + 2 * t + c;
-          if (i >= count) continue;
-          const int slot = slots[i];
-          const int2 xp = __ldg(p.xp + slot / p.top);
-          const float f = pow2f(xp.x) * p.up_scale;
-          const int ea = xp.y + 2 * xp.x + en + ets - 15;  // |act| < 2^(ea + 15)
+      for (int c = 0; c < 2; ++c) {
+        const int i = n * 8 + 2 * t + c;
+        if (i >= count) continue;
+        const int slot = slots[i], e = s.act_exp[slot], e1 = e / 2;
+        if constexpr (UP) {
+          const float f = s.x_scale[slot / p.top], q1 = pow2f(-e1), q2 = pow2f(e1 - e);  // 2^-e in two factors
+          // column 16 u + 8 r + g: block j = u % 4 of its chunk, lane (8 r + g) / 4 of the fragment
+          const int j = u & 3;
+          __half* to = p.act + ((int64_t)slot * p.ic + (u >> 2)) * 64 + (j >> 1) * 32 + (g >> 2) * 8 + (j & 1) * 4 + (g & 3);
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float gate = acc[r][n][c] * f, up = acc[r][n][c + 2] * f;
-            const float a = __fdiv_rn(gate, 1.0f + expf(-gate)) * up;  // gate far below 0: expf overflows and the quotient is -0
-            const float v = scalbnf(a, -ea);
-            // column 16 u + 8 r + g: block j = u % 4 of its chunk, lane (8 r + g) / 4 of the fragment
-            const int j = u & 3, at = (j >> 1) * 32 + ((8 * r + g) >> 2) * 8 + (j & 1) * 4 + (g & 3);
-            __half* to = p.act + ((int64_t)slot * p.ic + (u >> 2)) * 64 + at;
+            // gate far below 0: the exponential overflows and the quotient is -0
+            const float v = __fdividef(gate, 1.0f + __expf(-gate)) * up * q1 * q2;
             const __half hi = __float2half_rn(v);
-            *to = hi;
-            if (p.dtype == kDtF16) to[p.act_part] = __float2half_rn(v - __half2float(hi));
+            to[r * 16] = hi;
+            if (p.dtype == kDtF16) to[r * 16 + p.act_part] = __float2half_rn(v - __half2float(hi));
             if (u + 1 == units && (units & 3))  // the other half of the last chunk is padding
               for (int q = 0; q < 2; ++q) {
-                __half* pad = to + 32 - (j & 1) * 4 + q * 4;
+                __half* pad = to + r * 16 + 32 - (j & 1) * 4 + q * 4;
                 *pad = __float2half_rn(0.0f);
                 if (p.dtype == kDtF16) pad[p.act_part] = __float2half_rn(0.0f);
               }
           }
-        }
-    } else {
-      const int en = exponent_bound(__ldg(p.norms + 2 * e)) + exponent_bound(__ldg(p.norms + 2 * e + 1));
-      const int ets = 2 * exponent_bound(fabsf(p.up_scale));
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int i = n * 8 + 2 * t + c;
-          if (i >= count) continue;
-          const int slot = slots[i];
-          const int2 xp = __ldg(p.xp + slot / p.top);
-          const int ea = xp.y + 2 * xp.x + en + ets - 15;
-          const float f = p.down_scale * s.weight[slot];
+        } else {
+          const float f = p.down_scale * s.weight[slot], q1 = pow2f(e1), q2 = pow2f(e - e1);
           float* to = p.y + (int64_t)slot * p.H + u * 32 + g;
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            to[r * 16] = scalbnf(acc[r][n][c], ea) * f;
-            to[r * 16 + 8] = scalbnf(acc[r][n][c + 2], ea) * f;
+            to[r * 16] = acc[r][n][c] * q1 * q2 * f;
+            to[r * 16 + 8] = acc[r][n][c + 2] * q1 * q2 * f;
           }
         }
-    }
+      }
   };
   while (ok && !w.done()) {
-    const int count = s.g_count[w.unit / units];
-    if (count <= 8) unit_of(std::integral_constant<int, 1>());
-    else if (count <= 16) unit_of(std::integral_constant<int, 2>());
-    else unit_of(std::integral_constant<int, 4>());
+    if (s.g_count[w.group] <= 8) unit_of(std::integral_constant<int, 1>());
+    else unit_of(std::integral_constant<int, 2>());
   }
   if (!ok)  // copies in flight must land before the CTA exits (bounded)
     for (; it < issued; ++it) mbar_wait_bounded(full + it % kMoeStages, it / kMoeStages & 1, kDevErrLoadTimeout);
