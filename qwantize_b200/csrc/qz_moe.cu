@@ -9,19 +9,21 @@
 // are read once, and the floor is their bytes over the HBM rate.  Activations
 // stay in 16 bits (quantizing them would save nothing).
 //
-// Two launches.  moe_router_kernel: the logits, and x as fp16 in the order of
-// the matrix instructions' B fragments.  moe_experts_kernel, cooperative, one
-// CTA of 16 warps per SM: each CTA derives the routing from the logits for itself
-// (they are a few KB), then the CTAs share the units of the gate / up product; a
-// grid barrier; the units of the down product; a grid barrier; the weighted sum
-// over each token's experts in a fixed order.
+// Two launches.  moe_router_kernel, a cluster of 8 CTAs per 4 tokens: the CTAs
+// share the experts' logits, send them to the CTA of their token through
+// distributed shared memory, and that one chooses; it also writes the token
+// as fp16 in the order of the matrix instructions' B fragments.
+// moe_experts_kernel, cooperative, one CTA of 16 warps per SM: each CTA groups the
+// choices by expert, then the CTAs share the units of the gate / up product; a grid
+// barrier; the units of the down product; a grid barrier; the weighted sum over
+// each token's experts in a fixed order.
 //
 // A unit is 32 weight rows of one expert times up to 16 of its tokens (more would
 // be bound by the matrix instructions and gain nothing).  A CTA has a run of
 // neighbouring units, so its warps share an expert's tokens in L1; a warp takes
 // a unit alone and streams its weights through its own ring of bulk copies,
 // never waiting for another warp.  The units that are left when every warp has had
-// its share are cut along K by 2, 4 or 8 warps each, which add up through shared
+// its share are cut along K by up to 8 warps each, which add up through shared
 // memory.
 //
 // Weights are laid out once in the order of the A fragments of mma.m16n8k16
@@ -70,7 +72,8 @@ struct MoeParams {
   int hc, ic;                       // 64-column chunks of H and I
   int renorm;
   int dtype;                        // of x and out
-  const float* logits;              // (T, E)
+  const int* choice;                // (T, top) experts
+  const float* choice_weight;       // (T, top)
   const uint8_t *up_codes, *up_scales;      // (E, I / 16 units, hc chunks, 2 tiles) 512 and 8 * 2 * 64 / bs bytes
   const uint8_t *down_codes, *down_scales;  // (E, H / 32 units, ic chunks, 2 tiles)
   const float* norms;               // (E, 2): largest row norm of gate and of up, without the tensor scale
@@ -82,8 +85,6 @@ struct MoeParams {
   float* y;                         // (T * top, H)
   int* barrier;
   void* out;                        // (T, H)
-  int* ids;                         // (T, top) or NULL
-  float* weights;                   // (T, top) or NULL
 };
 
 // ---------------------------------------------------------------------------
@@ -182,45 +183,134 @@ __device__ __forceinline__ int exponent_bound(float v) {
   return v > 0.0f && u < 0x7f800000u ? (int)(u >> 23) - 126 : 0;
 }
 
-// Blocks [0, E * ceil(T / 8)): one expert and 8 tokens, the 4 warps splitting H.
-// The T blocks after them: one token to fp16; the first also zeroes the barriers.
-constexpr int kRouterThreads = 128;
-template <int DT, int RDT>
-__global__ void __launch_bounds__(kRouterThreads)
-    moe_router_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ router, int T, int H, int E,
-                      float* __restrict__ logits, uint4* __restrict__ xh, int2* __restrict__ xp, int* __restrict__ barrier) {
-  __shared__ float s_part[4][8];
-  __shared__ uint32_t s_max[4];
+// Ascending order of the bits is ascending order of the floats, NaN on top;
+// never 0.
+__device__ __forceinline__ uint32_t order_bits(float f) {
+  const uint32_t u = __float_as_uint(f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The top_k largest of a token's logits, by one warp: lane l holds experts W l .. W
+// l + W - 1, so the lowest index among equal logits is in the lowest lane.
+template <int W>
+__device__ __forceinline__ void choose(const float* logits, int E, int top, int renorm, int* ids, float* weights) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[W];  // 0: not there, or taken
+  auto logit = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); };
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    key[i] = lane * W + i < E ? order_bits(logits[lane * W + i]) : 0u;
+    m = max(m, key[i]);
+  }
+  const float best = logit(__reduce_max_sync(0xffffffffu, m));
+  float sum = 0.0f;
+  if (!renorm)
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (key[i]) sum += expf(logit(key[i]) - best);
+  uint32_t chosen = 0;  // lane k keeps choice k
+  int mine = 0;
+#pragma unroll 1
+  for (int k = 0; k < top; ++k) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max(m, key[i]);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, m);
+    const int src = __ffs(__ballot_sync(0xffffffffu, m == most)) - 1;
+    int at = 0;
+#pragma unroll
+    for (int i = W - 1; i >= 0; --i)
+      if (key[i] == most) at = i;
+    if (lane == src) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i == at) key[i] = 0;
+    }
+    at = __shfl_sync(0xffffffffu, at, src);
+    if (lane == k) { chosen = most; mine = src * W + at; }
+  }
+  const float e = lane < top ? expf(logit(chosen) - best) : 0.0f;
+  if (renorm) sum = e;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane < top) {
+    ids[lane] = mine;
+    weights[lane] = __fdiv_rn(e, sum);
+  }
+}
+
+// A cluster of kRouterCtas CTAs has up to kRouterTokens tokens: CTA r computes the
+// logits of every kRouterCtas-th expert for all of them and owns token r.
+constexpr int kRouterCtas = 8, kRouterTokens = 4, kRouterThreads = 512;
+template <int DT, int RDT, int NTK>  // NTK: tokens of a cluster
+__global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThreads)
+    moe_router_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ router, int T, int H, int E, int top,
+                      int renorm, int* __restrict__ ids, float* __restrict__ weights, uint4* __restrict__ xh,
+                      int2* __restrict__ xp, int* __restrict__ barrier) {
+  constexpr int kWarps = kRouterThreads / 32;
+  __shared__ float s_logits[kMoeMaxExperts];
+  __shared__ float s_part[kWarps][NTK];
+  __shared__ float s_norm[kRouterThreads / 32];
+  __shared__ uint32_t s_max[kRouterThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int groups = (T + 7) / 8;
-  if ((int)blockIdx.x < E * groups) {
-    const int e = blockIdx.x % E, t0 = blockIdx.x / E * 8;
-    const int nt = T - t0 < 8 ? T - t0 : 8;
-    float acc[8] = {};
-    for (int h = tid * 8; h < H; h += kRouterThreads * 8) {
-      float r[8], v[8][8];
-      load8<RDT>(router, (int64_t)e * H + h, r);
+  const int rank = blockIdx.x % kRouterCtas, t0 = blockIdx.x / kRouterCtas * NTK;
+  const int nt = T - t0 < NTK ? T - t0 : NTK, t = rank < nt ? t0 + rank : T;  // T: no token
+  if (blockIdx.x == 0 && tid < 2) barrier[tid] = 0;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // every CTA has begun before another writes to it
+  // warps per expert of this CTA, so that all are busy: they split H
+  const int mine = (E - rank + kRouterCtas - 1) / kRouterCtas;
+  int cut = 1;
+  while (cut < kWarps && mine * cut * 2 <= kWarps) cut *= 2;
+  for (int i0 = 0; i0 < mine; i0 += kWarps / cut) {
+    const int i = i0 + warp / cut, e = rank + i * kRouterCtas;
+    float acc[NTK] = {};
+    if (i < mine) {
+#pragma unroll(NTK == 1 ? 8 : 2)
+      for (int h = (warp % cut * 32 + lane) * 8; h < H; h += cut * 256) {
+        float r[8];
+        uint4 raw[NTK];  // all loads before the first product
+        load8<RDT>(router, (int64_t)e * H + h, r);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) load8<DT>(x, (t0 + (n < nt ? n : 0)) * ldx + h, v[n]);
+        for (int n = 0; n < NTK; ++n)
+          raw[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + (t0 + (n < nt ? n : 0)) * ldx + h));
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < NTK; ++n) {
+          const uint32_t ww[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[n] = fmaf(v[n][k], r[k], acc[n]);
+          for (int k = 0; k < 4; ++k) {
+            acc[n] = fmaf(DT == kDtBF16 ? bf16_bits_to_float(ww[k] & 0xffffu) : f16_bits_to_float(ww[k] & 0xffffu), r[2 * k], acc[n]);
+            acc[n] = fmaf(DT == kDtBF16 ? bf16_bits_to_float(ww[k] >> 16) : f16_bits_to_float(ww[k] >> 16), r[2 * k + 1], acc[n]);
+          }
+        }
+      }
     }
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
+    for (int n = 0; n < NTK; ++n) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc[n] += __shfl_xor_sync(0xffffffffu, acc[n], o);
       if (lane == 0) s_part[warp][n] = acc[n];
     }
     __syncthreads();
-    if (tid < nt) logits[(int64_t)(t0 + tid) * E + e] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
-    return;
+    if (i0 == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    // thread (expert, token): the parts in order, to the token's CTA
+    if (tid < kWarps / cut * NTK) {
+      const int j = tid / NTK, n = tid % NTK;
+      if (i0 + j < mine && n < nt) {
+        float v = 0.0f;
+        for (int q = 0; q < cut; ++q) v += s_part[j * cut + q][n];
+        uint32_t at;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(s_logits + rank + (i0 + j) * kRouterCtas)), "r"(n));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+      }
+    }
+    __syncthreads();
   }
-  const int t = blockIdx.x - E * groups;
-  if (t == 0 && tid < 2) barrier[tid] = 0;
+  if (mine <= 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  // this CTA's token as fp16
   int e = 0;
-  if (DT == kDtBF16) {
+  if (DT == kDtBF16 && t < T) {
     uint32_t m = 0;
     for (int h = tid * 8; h < H; h += kRouterThreads * 8) {
       float v[8];
@@ -231,35 +321,53 @@ __global__ void __launch_bounds__(kRouterThreads)
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) s_max[warp] = m;
     __syncthreads();
-    e = f16_power(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+    m = s_max[lane % (kRouterThreads / 32)];
+    e = f16_power(__reduce_max_sync(0xffffffffu, m));
   }
   const float inv = pow2f(-e);
-  // thread: 32 columns (half a chunk); lane t' of the fragment takes columns 4t' .. + 3 of each 16
   const int hc = (H + 63) / 64;
   float norm2 = 0.0f;
-  for (int i = tid; i < hc * 2; i += kRouterThreads) {
-    uint32_t w[16];  // 32 halves
+  if (t < T) {
+    // thread: 8 halves; lane t' of the fragment takes columns 4t' .. + 3 of two blocks of 16
+    for (int i = tid; i < hc * 8; i += kRouterThreads) {
+      const int col = (i >> 2) * 32 + (i & 3) * 4;  // and 16 further
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (col < H) {  // H is a multiple of 32
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float v[8] = {};
-      if (i * 32 < H) load8<DT>(x, t * ldx + i * 32 + q * 8, v);  // H is a multiple of 32
+        for (int k = 0; k < 2; ++k) {
+          const uint2 raw = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(x) + t * ldx + col + 16 * k));
+          const uint32_t rr[2] = {raw.x, raw.y};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float a = v[2 * k] * inv, b = v[2 * k + 1] * inv;
-        norm2 = fmaf(a, a, fmaf(b, b, norm2));
-        const __half2 h = __floats2half2_rn(a, b);
-        w[4 * q + k] = *reinterpret_cast<const uint32_t*>(&h);
+          for (int q = 0; q < 2; ++q) {
+            const float a = (DT == kDtBF16 ? bf16_bits_to_float(rr[q] & 0xffffu) : f16_bits_to_float(rr[q] & 0xffffu)) * inv;
+            const float b = (DT == kDtBF16 ? bf16_bits_to_float(rr[q] >> 16) : f16_bits_to_float(rr[q] >> 16)) * inv;
+            norm2 = fmaf(a, a, fmaf(b, b, norm2));
+            const __half2 h = __floats2half2_rn(a, b);
+            w[2 * k + q] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
       }
+      xh[(int64_t)t * hc * 8 + i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    uint4* out = xh + ((int64_t)t * hc * 2 + i) * 4;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) out[q] = make_uint4(w[2 * q], w[2 * q + 1], w[8 + 2 * q], w[8 + 2 * q + 1]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) norm2 += __shfl_xor_sync(0xffffffffu, norm2, o);
-  if (lane == 0) s_part[0][warp] = norm2;
-  __syncthreads();
-  if (tid == 0) xp[t] = make_int2(e, exponent_bound((s_part[0][0] + s_part[0][1]) + (s_part[0][2] + s_part[0][3])));
+  if (lane == 0) s_norm[warp] = norm2;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (t >= T) return;
+  if (warp == 0) {
+    int* id = ids + (int64_t)t * top;
+    float* w = weights + (int64_t)t * top;
+    if (E <= 32) choose<1>(s_logits, E, top, renorm, id, w);
+    else if (E <= 64) choose<2>(s_logits, E, top, renorm, id, w);
+    else if (E <= 128) choose<4>(s_logits, E, top, renorm, id, w);
+    else choose<kMoeMaxExperts / 32>(s_logits, E, top, renorm, id, w);
+  } else if (tid == 32) {
+    float sum = 0.0f;
+    for (int i = 0; i < kRouterThreads / 32; ++i) sum += s_norm[i];
+    xp[t] = make_int2(e, exponent_bound(sum));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -273,6 +381,7 @@ struct MoeShared {
   uint16_t start[kMoeMaxExperts];
   // groups: up to kMoeGroup tokens of one expert, experts ascending
   uint16_t g_expert[kMoeMaxGroups], g_begin[kMoeMaxGroups], g_count[kMoeMaxGroups];
+  uint16_t g_cost[kMoeMaxGroups + 1];     // cost of one unit of each group before this one
   int n_groups, ok;
   uint64_t full[kMoeWarps * kMoeStages];  // the warps' rings
   float x_scale[kMoeMaxTokens];           // power of two of a token times the tensor scale
@@ -306,128 +415,47 @@ __device__ __forceinline__ bool grid_barrier(int* counter, MoeShared& s) {
   return s.ok != 0;
 }
 
-// Ascending order of the bits is ascending order of the floats, NaN on top.
-__device__ __forceinline__ uint32_t order_bits(float f) {
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-// The choices of N tokens t0, t0 + kMoeWarps, ... by one warp, side by side (one
-// choice is a chain of warp-wide operations): lane l holds experts W l .. W l + W -
-// 1, so the lowest index among equal logits is in the lowest lane.
-template <int W, int N>
-__device__ __forceinline__ void choose(const MoeParams& p, MoeShared& s, int t0) {
-  const int lane = threadIdx.x & 31;
-  uint32_t key[N][W], chosen[N];
-  uint16_t mine[N];  // lane k keeps choice k
-  float all[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int t = t0 + n * kMoeWarps;
-    all[n] = 0.0f;
-    chosen[n] = 0;
-    mine[n] = 0;
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      key[n][i] = t < p.T && lane * W + i < p.E ? order_bits(__ldcg(p.logits + (int64_t)t * p.E + lane * W + i)) : 0u;  // 0: not there, or taken
-  }
-  uint32_t top[N];
-  auto logit = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); };
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) m = max(m, key[n][i]);
-    top[n] = __reduce_max_sync(0xffffffffu, m);
-    if (!p.renorm)
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (key[n][i]) all[n] += expf(logit(key[n][i]) - logit(top[n]));
-  }
-  for (int k = 0; k < p.top; ++k) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) m = max(m, key[n][i]);
-      const uint32_t best = __reduce_max_sync(0xffffffffu, m);
-      const int src = __ffs(__ballot_sync(0xffffffffu, m == best)) - 1;
-      int at = 0;
-#pragma unroll
-      for (int i = W - 1; i >= 0; --i)
-        if (key[n][i] == best) at = i;
-      if (lane == src) {
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-          if (i == at) key[n][i] = 0;
-      }
-      at = __shfl_sync(0xffffffffu, at, src);
-      if (lane == k) { chosen[n] = best; mine[n] = (uint16_t)(src * W + at); }
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int t = t0 + n * kMoeWarps;
-    const float e = lane < p.top ? expf(logit(chosen[n]) - logit(top[n])) : 0.0f;
-    float sum = p.renorm ? e : all[n];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (t < p.T && lane < p.top) {
-      const float w = __fdiv_rn(e, sum);
-      s.id[t * p.top + lane] = mine[n];
-      s.weight[t * p.top + lane] = w;
-      if (blockIdx.x == 0) {
-        if (p.ids) p.ids[t * p.top + lane] = (int)mine[n];
-        if (p.weights) p.weights[t * p.top + lane] = w;
-      }
-    }
-  }
-}
-
-template <int W, int N>
-__device__ __forceinline__ void choose_all(const MoeParams& p, MoeShared& s) {
-  const int warp = threadIdx.x >> 5;
-  if (p.T <= kMoeWarps) {
-    if (warp < p.T) choose<W, 1>(p, s, warp);
-  } else {
-    for (int t0 = warp; t0 < p.T; t0 += N * kMoeWarps) choose<W, N>(p, s, t0);
-  }
-}
+// Relative time of a unit with one or two tiles of 8 tokens.
+__device__ __forceinline__ int unit_cost(int tokens) { return tokens <= 8 ? 4 : 5; }
 
 __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) s.count[e] = 0;
-  if (p.E <= 32) choose_all<1, 4>(p, s);
-  else if (p.E <= 64) choose_all<2, 4>(p, s);
-  else if (p.E <= 128) choose_all<4, 4>(p, s);
-  else if (p.E <= 256) choose_all<8, 2>(p, s);
-  else choose_all<16, 1>(p, s);
-  __syncthreads();
-  // one warp numbers each expert's slots in ascending order, 32 slots at a time,
-  // then lays out the groups
   const int n = p.T * p.top;
-  if (warp == 0) {
-    for (int i = lane; i < (n + 31) / 32 * 32; i += 32) {
-      const unsigned there = __ballot_sync(0xffffffffu, i < n);
-      if (i < n) {
-        const int e = s.id[i];
-        const unsigned same = __match_any_sync(there, e);
-        const int before = s.count[e], rank = __popc(same & ((1u << lane) - 1u));
-        s.rank[i] = (uint16_t)(before + rank);
-        __syncwarp(there);
-        if (rank == 0) s.count[e] = (uint16_t)(before + __popc(same));
+  for (int i = threadIdx.x; i < n; i += kMoeThreads) {
+    s.id[i] = (uint16_t)__ldg(p.choice + i);
+    s.weight[i] = __ldg(p.choice_weight + i);
+  }
+  __syncthreads();
+  // a warp numbers the slots of every kMoeWarps-th expert in ascending order
+  {
+    uint16_t ids[kMoeMaxSlots / 32];
+#pragma unroll
+    for (int i = 0; i < kMoeMaxSlots / 32; ++i) ids[i] = i * 32 + lane < n ? s.id[i * 32 + lane] : (uint16_t)0xffffu;
+#pragma unroll 1
+    for (int e = warp; e < p.E; e += kMoeWarps) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < kMoeMaxSlots / 32; ++i) {
+        if (i * 32 >= n) break;
+        const unsigned same = __ballot_sync(0xffffffffu, ids[i] == e);
+        if (ids[i] == e) s.rank[i * 32 + lane] = (uint16_t)(c + __popc(same & ((1u << lane) - 1u)));
+        c += __popc(same);
       }
-      __syncwarp();
+      if (lane == 0) s.count[e] = (uint16_t)c;
     }
-    int at = 0, groups = 0;
+  }
+  __syncthreads();
+  // one warp lays out the groups
+  if (warp == 0) {
+    int at = 0, groups = 0, cost = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int c = e0 + lane < p.E ? s.count[e0 + lane] : 0, m = (c + kMoeGroup - 1) / kMoeGroup;
-      int a = c, b = m;  // inclusive prefix sums
+      const int z = m == 0 ? 0 : (m - 1) * unit_cost(kMoeGroup) + unit_cost(c - (m - 1) * kMoeGroup);
+      int a = c, b = m, d = z;  // inclusive prefix sums
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-        if (lane >= o) { a += x; b += y; }
+        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o), v = __shfl_up_sync(0xffffffffu, d, o);
+        if (lane >= o) { a += x; b += y; d += v; }
       }
       if (e0 + lane < p.E) s.start[e0 + lane] = (uint16_t)(at + a - c);
       for (int k = 0; k < m; ++k) {
@@ -435,11 +463,16 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
         s.g_expert[g] = (uint16_t)(e0 + lane);
         s.g_begin[g] = (uint16_t)(at + a - c + k * kMoeGroup);
         s.g_count[g] = (uint16_t)(c - k * kMoeGroup < kMoeGroup ? c - k * kMoeGroup : kMoeGroup);
+        s.g_cost[g] = (uint16_t)(cost + d - z + k * unit_cost(kMoeGroup));
       }
       at += __shfl_sync(0xffffffffu, a, 31);
       groups += __shfl_sync(0xffffffffu, b, 31);
+      cost += __shfl_sync(0xffffffffu, d, 31);
     }
-    if (lane == 0) s.n_groups = groups;
+    if (lane == 0) {
+      s.n_groups = groups;
+      s.g_cost[groups] = (uint16_t)cost;
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kMoeThreads) {
@@ -496,51 +529,72 @@ template <int NT, int BS, int PARTS>
 __device__ __forceinline__ void chunk_product(const uint8_t* codes, const uint8_t* scales, const uint32_t (&b)[PARTS][NT][8],
                                               float (&acc)[2][NT][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
+  uint32_t w[2][4];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const uint4 w4 = *reinterpret_cast<const uint4*>(codes + r * 512 + lane * 16);
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-    if constexpr (BS == 16) {
-      const uint2 sc = *reinterpret_cast<const uint2*>(scales + r * 64 + g * 8);
-      __half2 s0[4], s1[4];
-      scales_nv(sc.x, s0);
-      scales_nv(sc.y, s1);
+    w[r][0] = w4.x; w[r][1] = w4.y; w[r][2] = w4.z; w[r][3] = w4.w;
+  }
+  // the two tiles side by side: their chains of conversions and products are independent
+  if constexpr (BS == 16) {
+    __half2 s0[2][4], s1[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a[4];  // row g, columns 0-1 and 2-3; row g + 8
-        e2m1x8_to_f16(w[j], a);
-        a[0] = mul_f16x2(a[0], s0[j]);
-        a[1] = mul_f16x2(a[1], s0[j]);
-        a[2] = mul_f16x2(a[2], s1[j]);
-        a[3] = mul_f16x2(a[3], s1[j]);
+    for (int r = 0; r < 2; ++r) {
+      const uint2 sc = *reinterpret_cast<const uint2*>(scales + r * 64 + g * 8);
+      scales_nv(sc.x, s0[r]);
+      scales_nv(sc.y, s1[r]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a[2][4];  // row g, columns 0-1 and 2-3; row g + 8
+#pragma unroll
+      for (int r = 0; r < 2; ++r) e2m1x8_to_f16(w[r][j], a[r]);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        a[r][0] = mul_f16x2(a[r][0], s0[r][j]);
+        a[r][1] = mul_f16x2(a[r][1], s0[r][j]);
+        a[r][2] = mul_f16x2(a[r][2], s1[r][j]);
+        a[r][3] = mul_f16x2(a[r][3], s1[r][j]);
+      }
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) mma_f16(acc[r][n], a[0], a[2], a[1], a[3], b[q][n][2 * j], b[q][n][2 * j + 1]);
-      }
-    } else {
-      const uint32_t sc = *reinterpret_cast<const uint32_t*>(scales + r * 32 + g * 4);
+          for (int r = 0; r < 2; ++r) mma_f16(acc[r][n], a[r][0], a[r][2], a[r][1], a[r][3], b[q][n][2 * j], b[q][n][2 * j + 1]);
+    }
+  } else {
+    uint32_t sc[2];
 #pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const float s0 = scale_mx(sc >> (4 * j) & 255u), s1 = scale_mx(sc >> (16 + 4 * j) & 255u);
-        float d[NT][4];
+    for (int r = 0; r < 2; ++r) sc[r] = *reinterpret_cast<const uint32_t*>(scales + r * 32 + g * 4);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+    for (int j = 0; j < 4; j += 2) {
+      float d[2][NT][4];
 #pragma unroll
-        for (int k = j; k < j + 2; ++k) {
-          uint32_t a[4];
-          e2m1x8_to_f16(w[k], a);
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) d[r][n][0] = d[r][n][1] = d[r][n][2] = d[r][n][3] = 0.0f;
+#pragma unroll
+      for (int k = j; k < j + 2; ++k) {
+        uint32_t a[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) e2m1x8_to_f16(w[r][k], a[r]);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) mma_f16(d[n], a[0], a[2], a[1], a[3], b[q][n][2 * k], b[q][n][2 * k + 1]);
-        }
+            for (int r = 0; r < 2; ++r) mma_f16(d[r][n], a[r][0], a[r][2], a[r][1], a[r][3], b[q][n][2 * k], b[q][n][2 * k + 1]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float s0 = scale_mx(sc[r] >> (4 * j) & 255u), s1 = scale_mx(sc[r] >> (16 + 4 * j) & 255u);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          acc[r][n][0] = fmaf(d[n][0], s0, acc[r][n][0]);
-          acc[r][n][1] = fmaf(d[n][1], s0, acc[r][n][1]);
-          acc[r][n][2] = fmaf(d[n][2], s1, acc[r][n][2]);
-          acc[r][n][3] = fmaf(d[n][3], s1, acc[r][n][3]);
+          acc[r][n][0] = fmaf(d[r][n][0], s0, acc[r][n][0]);
+          acc[r][n][1] = fmaf(d[r][n][1], s0, acc[r][n][1]);
+          acc[r][n][2] = fmaf(d[r][n][2], s1, acc[r][n][2]);
+          acc[r][n][3] = fmaf(d[r][n][3], s1, acc[r][n][3]);
         }
       }
     }
@@ -566,12 +620,24 @@ struct MoeWalk {
   int last_group, last_unit;
   bool whole;                  // the current unit is this warp's alone
 
-  __device__ __forceinline__ MoeWalk(int64_t total, int units_, int chunks_) : units(units_), chunks(chunks_) {
+  // the first unit at or behind share i / gridDim of the phase's cost
+  __device__ __forceinline__ int boundary(const MoeShared& s, int i) const {
+    const int64_t at = (int64_t)s.g_cost[s.n_groups] * units * i / gridDim.x;
+    int lo = 0, hi = s.n_groups;  // last group that begins at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)s.g_cost[mid] * units <= at) lo = mid; else hi = mid;
+    }
+    const int cost = s.g_cost[lo + 1] - s.g_cost[lo];
+    return lo * units + ((int)(at - (int64_t)s.g_cost[lo] * units) + cost - 1) / cost;
+  }
+  __device__ __forceinline__ MoeWalk(const MoeShared& s, int units_, int chunks_) : units(units_), chunks(chunks_) {
     const int warp = threadIdx.x >> 5;
-    const int begin = (int)((int64_t)blockIdx.x * total / gridDim.x), end = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
+    const int begin = boundary(s, blockIdx.x), end = boundary(s, blockIdx.x + 1);
     const int rounds = (end - begin) / kMoeWarps, rest = (end - begin) % kMoeWarps;
-    share = 1;
-    while (share < 8 && rest * share * 2 <= kMoeWarps && share * 2 <= chunks) share *= 2;
+    share = rest ? kMoeWarps / rest : 1;
+    share = share < 8 ? share : 8;
+    share = share < chunks ? share : chunks;
     const int last = begin + rounds * kMoeWarps + warp / share;
     if (last < end) {
       part = warp % share;
@@ -619,7 +685,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
   const uint8_t* codes = UP ? p.up_codes : p.down_codes;
   const uint8_t* scales = UP ? p.up_scales : p.down_scales;
   const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
-  MoeWalk w((int64_t)s.n_groups * units, units, chunks), ahead = w;
+  MoeWalk w(s, units, chunks), ahead = w;
   uint8_t* mine = ring + warp * kMoeStages * R::kStage;
   uint64_t* full = s.full + warp * kMoeStages;
   int64_t at_unit = 0;  // first chunk of the unit that is loaded
@@ -658,24 +724,42 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][n][c] = 0.0f;
+    // the B words of chunk c
+    auto load_b = [&](uint32_t(&b)[PARTS][NT][8], int c) {
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4* from = row[n] + (UP ? 0 : q * (p.act_part / 8)) + c * 8;
+          const uint4 lo = UP ? __ldg(from) : *from, hi = UP ? __ldg(from + 4) : from[4];
+          b[q][n][0] = lo.x; b[q][n][1] = lo.y; b[q][n][2] = lo.z; b[q][n][3] = lo.w;
+          b[q][n][4] = hi.x; b[q][n][5] = hi.y; b[q][n][6] = hi.z; b[q][n][7] = hi.w;
+        }
+    };
+    constexpr bool kAhead = NT * PARTS <= 2;  // one chunk ahead of its product while registers allow
+    uint32_t b0[PARTS][NT][8], b1[PARTS][NT][8];
+    if (kAhead) load_b(b0, w.c);
     bool more = true;
     while (more) {
       const int st = it % kMoeStages, pieces = w.piece();
       if (!mbar_wait_bounded(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
       const uint8_t* at = mine + st * R::kStage;
 #pragma unroll 1
-      for (int k = 0; k < pieces; ++k) {
-        uint32_t b[PARTS][NT][8];
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4* from = row[n] + (UP ? 0 : q * (p.act_part / 8)) + (w.c + k) * 8;
-            const uint4 lo = UP ? __ldg(from) : *from, hi = UP ? __ldg(from + 4) : from[4];
-            b[q][n][0] = lo.x; b[q][n][1] = lo.y; b[q][n][2] = lo.z; b[q][n][3] = lo.w;
-            b[q][n][4] = hi.x; b[q][n][5] = hi.y; b[q][n][6] = hi.z; b[q][n][7] = hi.w;
+      for (int k = 0; k < pieces; k += 2) {
+        const uint8_t *codes0 = at + k * R::kCodes, *scales0 = at + kMoePiece * R::kCodes + k * R::kScales;
+        if constexpr (kAhead) {
+          if (k + 1 < pieces) load_b(b1, w.c + k + 1);
+          chunk_product<NT, BS, PARTS>(codes0, scales0, b0, acc);
+          if (w.c + k + 2 < w.c1) load_b(b0, w.c + k + 2);
+          if (k + 1 < pieces) chunk_product<NT, BS, PARTS>(codes0 + R::kCodes, scales0 + R::kScales, b1, acc);
+        } else {
+          load_b(b0, w.c + k);
+          chunk_product<NT, BS, PARTS>(codes0, scales0, b0, acc);
+          if (k + 1 < pieces) {
+            load_b(b0, w.c + k + 1);
+            chunk_product<NT, BS, PARTS>(codes0 + R::kCodes, scales0 + R::kScales, b0, acc);
           }
-        chunk_product<NT, BS, PARTS>(at + k * R::kCodes, at + kMoePiece * R::kCodes + k * R::kScales, b, acc);
+        }
       }
       __syncwarp();  // every lane has read the stage
       if (!ahead.done()) {
@@ -815,13 +899,14 @@ cudaError_t read_device_error_moe(unsigned* out, bool clear) {
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct MoeWorkspace {
-  int64_t logits, xh, xp, act, y, barrier, bytes;
+  int64_t choice, weight, xh, xp, act, y, barrier, bytes;
 };
 
-static MoeWorkspace moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top) {
+static MoeWorkspace moe_workspace(int64_t T, int64_t H, int64_t I, int64_t top) {
   MoeWorkspace w;
-  w.logits = 0;
-  w.xh = up256(T * E * 4);
+  w.choice = 0;
+  w.weight = up256(T * top * 4);
+  w.xh = 2 * w.weight;
   w.xp = w.xh + up256(T * ((H + 63) / 64) * 128);
   w.act = w.xp + up256(T * 8);
   w.y = w.act + 2 * up256(T * top * ((I + 63) / 64) * 128);
@@ -875,7 +960,7 @@ extern "C" int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int6
   const int s = check_moe(T, H, I, E, top_k, QZ_FMT_NVFP4);
   if (s != QZ_OK) return s;
   if (!bytes) return fail(QZ_ERR_INVALID, "NULL pointer");
-  *bytes = moe_workspace(T, H, I, E, top_k).bytes;
+  *bytes = moe_workspace(T, H, I, top_k).bytes;
   return QZ_OK;
 }
 
@@ -897,7 +982,7 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
        reinterpret_cast<uintptr_t>(up_scales) | reinterpret_cast<uintptr_t>(down_codes) |
        reinterpret_cast<uintptr_t>(down_scales)) % 16 || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(QZ_ERR_INVALID, "inputs must be 16-byte aligned, workspace 256-byte");
-  const MoeWorkspace w = moe_workspace(T, H, I, E, top_k);
+  const MoeWorkspace w = moe_workspace(T, H, I, top_k);
   if (workspace_bytes < w.bytes)
     return fail(QZ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.bytes);
   int sms = 0;
@@ -908,7 +993,9 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   p.T = (int)T; p.H = (int)H; p.I = (int)I; p.E = (int)E; p.top = (int)top_k;
   p.hc = (int)((H + 63) / 64); p.ic = (int)((I + 63) / 64);
   p.renorm = renormalize; p.dtype = dtype;
-  p.logits = reinterpret_cast<float*>(ws + w.logits);
+  if (!ids) ids = reinterpret_cast<int*>(ws + w.choice);
+  if (!weights) weights = reinterpret_cast<float*>(ws + w.weight);
+  p.choice = ids; p.choice_weight = weights;
   p.up_codes = up_codes; p.up_scales = up_scales; p.norms = up_norms;
   p.down_codes = down_codes; p.down_scales = down_scales;
   p.up_scale = up_tensor_scale; p.down_scale = down_tensor_scale;
@@ -918,21 +1005,24 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   p.act_part = up256(T * top_k * p.ic * 128) / 2;
   p.y = reinterpret_cast<float*>(ws + w.y);
   p.barrier = reinterpret_cast<int*>(ws + w.barrier);
-  p.out = out; p.ids = ids; p.weights = weights;
-  const unsigned grid = (unsigned)(E * ((T + 7) / 8) + T);
+  p.out = out;
+  const unsigned grid = (unsigned)((T + kRouterTokens - 1) / kRouterTokens * kRouterCtas);
+#define QZ_ROUTER_N(DT, RDT, NTK)                                                                                       \
+  moe_router_kernel<DT, RDT, NTK><<<grid, kRouterThreads, 0, st>>>(x, ldx, router, p.T, p.H, p.E, p.top, renormalize,     \
+                                                                   ids, weights, reinterpret_cast<uint4*>(ws + w.xh),   \
+                                                                   reinterpret_cast<int2*>(ws + w.xp), p.barrier)
 #define QZ_ROUTER(DT, RDT)                                                                                              \
-  moe_router_kernel<DT, RDT><<<grid, kRouterThreads, 0, st>>>(x, ldx, router, p.T, p.H, p.E,                            \
-                                                              reinterpret_cast<float*>(ws + w.logits),                  \
-                                                              reinterpret_cast<uint4*>(ws + w.xh),                      \
-                                                              reinterpret_cast<int2*>(ws + w.xp), p.barrier)
+  if (T == 1) QZ_ROUTER_N(DT, RDT, 1);                                                                                  \
+  else QZ_ROUTER_N(DT, RDT, kRouterTokens)
 #define QZ_ROUTER_OF(DT)                                                                                                \
-  if (router_dtype == QZ_DTYPE_F32) QZ_ROUTER(DT, kDtF32);                                                              \
-  else if (router_dtype == QZ_DTYPE_BF16) QZ_ROUTER(DT, kDtBF16);                                                       \
-  else QZ_ROUTER(DT, kDtF16)
-  if (dtype == QZ_DTYPE_BF16) { QZ_ROUTER_OF(kDtBF16); }
-  else { QZ_ROUTER_OF(kDtF16); }
+  if (router_dtype == QZ_DTYPE_F32) { QZ_ROUTER(DT, kDtF32); }                                                          \
+  else if (router_dtype == QZ_DTYPE_BF16) { QZ_ROUTER(DT, kDtBF16); }                                                   \
+  else { QZ_ROUTER(DT, kDtF16); }
+  if (dtype == QZ_DTYPE_BF16) { QZ_ROUTER_OF(kDtBF16) }
+  else { QZ_ROUTER_OF(kDtF16) }
 #undef QZ_ROUTER_OF
 #undef QZ_ROUTER
+#undef QZ_ROUTER_N
   if ((s = cuda_status(cudaGetLastError(), "moe router launch")) != QZ_OK) return s;
   const bool nv = format == QZ_FMT_NVFP4, two = dtype == QZ_DTYPE_F16;
   const void* fn = nv ? (two ? reinterpret_cast<const void*>(&moe_experts_kernel<16, 2>) : reinterpret_cast<const void*>(&moe_experts_kernel<16, 1>))
