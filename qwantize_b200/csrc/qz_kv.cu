@@ -70,10 +70,6 @@ __device__ __forceinline__ uint32_t encode8(float y) {
   return r & 255u;
 }
 
-__device__ __forceinline__ float load16(const uint16_t* p, int dtype, int64_t i) {
-  return dtype == kDtBF16 ? bf16_bits_to_float(p[i]) : f16_bits_to_float(p[i]);
-}
-
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
@@ -81,7 +77,7 @@ struct AppendParams {
   uint8_t *k, *v;
   float *ks, *vs;
   int64_t num_pages;
-  int Hkv, D, dtype;
+  int Hkv;
   const uint16_t *nk, *nv;      // new tokens: (token, head, D), strides in elements
   int64_t k_tok, k_head, v_tok, v_head, N;
   const int* table;             // (B, max_pages)
@@ -92,14 +88,76 @@ struct AppendParams {
   int64_t max_new;
 };
 
-// One CTA per (page a sequence touches, head, sequence); keys, then values.  The
-// page's block is rebuilt in shared memory and written whole.  Memory-bound for
-// prompts, one round trip for a decode step.
+// Codes of y = x / s, the quotient correctly rounded, four to a word.  The product
+// with r = 1 / s is within three units of the last place of it, so the code
+// can differ only where y lies that close to a tie of its rounding: `near` is set
+// there, and the caller divides.
 template <int KV>
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float r, bool& near) {
+  uint32_t w;
+  if constexpr (KV == kKvInt8) {
+    const float magic = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the rounded product
+    uint32_t t[4];
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = __fmaf_rn(x[i], r, magic);
+      t[i] = __float_as_uint(v);
+      far = fmaxf(far, fabsf(__fmaf_rn(x[i], r, -(v - magic))));
+    }
+    near |= far >= 0.5f - 0x1p-14f;
+    w = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+  } else {
+    uint16_t lo, hi;
+    float y[4], least = 1.0f;
+    uint32_t tie = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // ties: the middle of the 20 dropped bits
+      y[i] = __fmul_rn(x[i], r);
+      tie = min(tie, (__float_as_uint(y[i]) - 0x7fff8u) & 0xfffffu);
+      least = fminf(least, fabsf(y[i]));
+    }
+    near |= tie <= 16u;
+    if (least < 0.015625f) {  // below 2^-6: odd multiples of 2^-10
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float t = __fmul_rn(y[i], 512.0f);
+        near |= fabsf(t) < 8.0f && fabsf(t - (__fadd_rn(t, 12582912.0f) - 12582912.0f)) >= 0.5f - 0x1p-12f;
+      }
+    }
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
+    w = (uint32_t)lo | (uint32_t)hi << 16;
+  }
+  return w;
+}
+template <int KV>
+__device__ __noinline__ uint32_t encode4_div(float a, float b, float c, float d, float s) {
+  return encode8<KV>(__fdiv_rn(a, s)) | encode8<KV>(__fdiv_rn(b, s)) << 8 | encode8<KV>(__fdiv_rn(c, s)) << 16 |
+         encode8<KV>(__fdiv_rn(d, s)) << 24;
+}
+
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int i) {
+  const uint32_t h = i ? w >> 16 : w & 0xffffu;
+  return DT == kDtBF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
+}
+// The larger magnitude of two 16-bit values, as 16 bits that order like it.
+__device__ __forceinline__ uint32_t abs_max16(uint32_t w) { return max(w >> 16 & 0x7fffu, w & 0x7fffu); }
+
+// One CTA per (page a sequence touches, head, keys or values, sequence).  All
+// it reads -- the new values, the page's block and scale -- is asked for at once and
+// kept in registers; the block is rebuilt in shared memory and written whole.  A
+// decode step is one such round trip.  Threads own 8 values of a token (keys) or
+// two values of 4 neighbouring slots (values), so that a word of the block has one
+// owner.
+template <int KV, int D, int DT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ __align__(16) uint8_t s_block[];  // 64 D bytes
+  constexpr int kStride = 68;  // bytes between value rows in shared memory: words of neighbouring rows in different banks
+  constexpr int kVecs = kPage * D / 16 / 256, kNew = kPage * D / 8 / 256;  // 16-byte vectors of codes, of new values per thread
+  __shared__ __align__(16) uint8_t s_block[D * kStride];
   __shared__ uint32_t s_max[8];
-  const int tid = threadIdx.x, D = p.D, head = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, which = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
   int64_t first = b, end = b + 1;
   if (p.cu) { first = p.cu[b]; end = p.cu[b + 1]; }
   const int64_t old = p.lengths[b];
@@ -113,132 +171,195 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
   if (t0 >= t1) return;
   const int64_t page = p.table[b * p.ld_table + blk];
   if (page < 0 || page >= p.num_pages) return;
-  const int off = (int)(t0 - blk * kPage), count = (int)(t1 - t0);
-  const int64_t src = first + (t0 - old), at = page * p.Hkv + head;
+  const int off = (int)(t0 - blk * kPage), fill = (int)(t1 - blk * kPage);  // new tokens take slots [off, fill)
+  const int64_t at = page * p.Hkv + head;
+  const int64_t tok = which ? p.v_tok : p.k_tok;
+  const uint16_t* x = (which ? p.nv + head * p.v_head : p.nk + head * p.k_head) + (first + (t0 - old) - off) * tok;  // slot 0's row
+  float* scale_p = (which ? p.vs : p.ks) + at;
+  uint8_t* block = (which ? p.v : p.k) + at * (int64_t)(kPage * D);
   const float per_top = KV == kKvInt8 ? 1.0f / 127.0f : 1.0f / 448.0f;  // rounded once, a constant
-  const int vecs = count * (D / 8);  // 8 values each
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const uint16_t* x = which ? p.nv + src * p.v_tok + head * p.v_head : p.nk + src * p.k_tok + head * p.k_head;
-    const int64_t tok = which ? p.v_tok : p.k_tok;
-    float* scale_p = (which ? p.vs : p.ks) + at;
-    uint8_t* block = (which ? p.v : p.k) + at * (int64_t)(kPage * D);
-    uint32_t m = 0;
-    for (int i = tid; i < vecs; i += 256) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + i / (D / 8) * tok + i % (D / 8) * 8));
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+
+  // new values: keys 8 of a slot; values two (d, d + 1) of 4 slots in x, y, z, w
+  uint4 raw[kNew];
+  uint32_t m = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float lo = p.dtype == kDtBF16 ? bf16_bits_to_float(ww[q] & 0xffffu) : f16_bits_to_float(ww[q] & 0xffffu);
-        const float hi = p.dtype == kDtBF16 ? bf16_bits_to_float(ww[q] >> 16) : f16_bits_to_float(ww[q] >> 16);
-        m = max(m, max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu));
-      }
+  for (int i = 0; i < kNew; ++i) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (which == 0) {
+      const int n = (tid + i * 256) / (D / 8), d = (tid + i * 256) % (D / 8) * 8;
+      if (n >= off && n < fill) raw[i] = __ldg(reinterpret_cast<const uint4*>(x + n * tok + d));
+    } else {
+      const int n = (tid + i * 256) / (D / 2) * 4, d = (tid + i * 256) % (D / 2) * 2;
+      const uint16_t* from = x + n * tok + d;
+      if (n >= off && n < fill) raw[i].x = __ldg(reinterpret_cast<const uint32_t*>(from));
+      if (n + 1 >= off && n + 1 < fill) raw[i].y = __ldg(reinterpret_cast<const uint32_t*>(from + tok));
+      if (n + 2 >= off && n + 2 < fill) raw[i].z = __ldg(reinterpret_cast<const uint32_t*>(from + 2 * tok));
+      if (n + 3 >= off && n + 3 < fill) raw[i].w = __ldg(reinterpret_cast<const uint32_t*>(from + 3 * tok));
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    const float before = off > 0 ? *scale_p : 0.0f;
-    __syncthreads();  // the previous half's block has been written out
-    if ((tid & 31) == 0) s_max[tid >> 5] = m;
-    __syncthreads();
-    m = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, s_max[w]);
-    const float need = __fmul_rn(__uint_as_float(m), per_top);
-    float s = before > need ? before : need;
-    // a value that is not finite, now or earlier, leaves the page's scale NaN and its codes 0
-    const bool fine = m < 0x7f800000u && before <= 3.0e38f;
-    if (!fine) s = __uint_as_float(0x7fc00000u);
-    const float ratio = s > 0.0f ? __fdiv_rn(before, s) : 0.0f;
-    // older tokens (slots below off), zeros elsewhere
-    for (int i = tid * 16; i < kPage * D; i += 256 * 16) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (off > 0 && fine && before > 0.0f) {
-        w = *reinterpret_cast<const uint4*>(block + i);
-        uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-        const int kt = key_token(i, D);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r = 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int n = which ? (i + 4 * q + c) % 64 : kt;
-            uint32_t code = ww[q] >> (8 * c) & 255u;
-            if (ratio != 1.0f) code = encode8<KV>(__fmul_rn(decode8<KV>(code), ratio));
-            if (n < off) r |= code << (8 * c);
-          }
-          ww[q] = r;
-        }
-        w = make_uint4(ww[0], ww[1], ww[2], ww[3]);
-      }
-      *reinterpret_cast<uint4*>(s_block + i) = w;
-    }
-    __syncthreads();
-    if (fine && s > 0.0f) {
-      for (int i = tid; i < vecs; i += 256) {
-        const int n = i / (D / 8), d0 = i % (D / 8) * 8;
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + n * tok + d0));
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const uint32_t h = ww[q / 2] >> (16 * (q & 1)) & 0xffffu;
-          const float f = p.dtype == kDtBF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
-          s_block[which ? value_at(off + n, d0 + q) : key_at(off + n, d0 + q, D)] = (uint8_t)encode8<KV>(__fdiv_rn(f, s));
-        }
-      }
-    }
-    __syncthreads();
-    for (int i = tid * 16; i < kPage * D; i += 256 * 16)
-      *reinterpret_cast<uint4*>(block + i) = *reinterpret_cast<const uint4*>(s_block + i);
-    if (tid == 0) *scale_p = s;
   }
+  uint4 have[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+    have[i] = off > 0 ? *reinterpret_cast<const uint4*>(block + (tid + i * 256) * 16) : make_uint4(0, 0, 0, 0);
+  const float before = off > 0 ? *scale_p : 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNew; ++i)
+    m = max(max(m, max(abs_max16(raw[i].x), abs_max16(raw[i].y))), max(abs_max16(raw[i].z), abs_max16(raw[i].w)));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((tid & 31) == 0) s_max[tid >> 5] = m;
+  __syncthreads();
+  m = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = max(m, s_max[w]);
+  m = __float_as_uint(half_of<DT>(m, 0));
+  const float need = __fmul_rn(__uint_as_float(m), per_top);
+  float s = before > need ? before : need;
+  // a value that is not finite, now or earlier, leaves the page's scale NaN and its codes 0
+  const bool fine = m < 0x7f800000u && before <= 3.0e38f;
+  if (!fine) s = __uint_as_float(0x7fc00000u);
+  const float ratio = s > 0.0f ? __fdiv_rn(before, s) : 0.0f;
+  // older tokens (slots below off), zeros elsewhere
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = (tid + i * 256) * 16, kt = key_token(v, D);
+    uint32_t ww[4] = {have[i].x, have[i].y, have[i].z, have[i].w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // bytes of slots below off
+      const int left = which ? off - (v % 64 + 4 * q) : (kt < off ? 4 : 0);
+      ww[q] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      if (!fine) ww[q] = 0;
+      if (ratio != 1.0f && ww[q]) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r |= encode8<KV>(__fmul_rn(decode8<KV>(ww[q] >> (8 * c) & 255u), ratio)) << (8 * c);
+        ww[q] = r;
+      }
+      *reinterpret_cast<uint32_t*>(s_block + (which ? v / 64 * kStride + v % 64 : v) + 4 * q) = ww[q];
+    }
+  }
+  __syncthreads();
+  if (fine && s > 0.0f) {
+    const float r = __frcp_rn(s);
+    const bool slow = s < 0x1p-100f;  // the reciprocal or its products may leave fp32's normal range
+#pragma unroll
+    for (int i = 0; i < kNew; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      const int n = which ? (tid + i * 256) / (D / 2) * 4 : (tid + i * 256) / (D / 8);
+      if (which ? n + 3 < off || n >= fill : n < off || n >= fill) continue;
+      float f[2][4];  // keys: values 0-3, 4-7; values: row d, row d + 1
+      bool near = slow;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[h][c] = which ? half_of<DT>(w[c], h) : half_of<DT>(w[2 * h + c / 2], c & 1);
+      uint32_t code[2] = {encode4<KV>(f[0], r, near), encode4<KV>(f[1], r, near)};
+      if (near) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) code[h] = encode4_div<KV>(f[h][0], f[h][1], f[h][2], f[h][3], s);
+      }
+      if (which == 0) {
+        *reinterpret_cast<uint2*>(s_block + key_at(n, (tid + i * 256) % (D / 8) * 8, D)) = make_uint2(code[0], code[1]);
+      } else {
+        // slots without a new token have code 0 here, and their old code in the block
+        const int d = (tid + i * 256) % (D / 2) * 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t*>(s_block + (d + h) * kStride + n) |= code[h];
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = (tid + i * 256) * 16;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(s_block + (which ? v / 64 * kStride + v % 64 : v));
+    *reinterpret_cast<uint4*>(block + v) = make_uint4(from[0], from[1], from[2], from[3]);
+  }
+  if (tid == 0) *scale_p = s;
 }
 
 // ---------------------------------------------------------------------------
 // read back
 // ---------------------------------------------------------------------------
-// One CTA per (page of the list, head): codes times scale, (n, Hkv, 64, D).
 template <int KV>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (KV == kKvInt8) {
+    // 0x6400 | (code + 128) is 1024 + code + 128 in fp16
+    w ^= 0x80808080u;
+    lo = __byte_perm(w, 0x64646464u, 0x4140);
+    hi = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), c), b = __hsub2(*reinterpret_cast<__half2*>(&hi), c);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+  } else {
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store16or32(void* out, int64_t i, float v) {
+  if (DT == kDtF32) static_cast<float*>(out)[i] = v;
+  else if (DT == kDtF16) static_cast<__half*>(out)[i] = __float2half_rn(v);
+  else {
+    uint16_t r;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+    static_cast<uint16_t*>(out)[i] = r;
+  }
+}
+
+// One CTA per (page of the list, head, keys or values): codes times scale, (n,
+// Hkv, 64, D).  Bound by the writes: four times the codes' bytes for fp32.
+template <int KV, int D, int DT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
                                                       const float* __restrict__ ks, const float* __restrict__ vs,
-                                                      int64_t num_pages, int Hkv, int D, const int* __restrict__ pages,
-                                                      void* __restrict__ ok, void* __restrict__ ov, int dtype) {
-  extern __shared__ __align__(16) uint8_t s_block[];  // 68 D bytes
-  const int tid = threadIdx.x, head = blockIdx.x;
-  const int64_t n = blockIdx.y, page = pages[n];
+                                                      int64_t num_pages, int Hkv, const int* __restrict__ pages,
+                                                      void* __restrict__ ok, void* __restrict__ ov) {
+  constexpr int kStride = 68, kVecs = kPage * D / 16 / 256;
+  __shared__ __align__(16) uint8_t s_block[D * kStride];
+  const int tid = threadIdx.x, which = blockIdx.x & 1, head = blockIdx.x >> 1;
+  void* out = which ? ov : ok;
+  if (!out) return;
+  const int64_t n = blockIdx.y, page = pages[n], at = page * Hkv + head;
   const bool there = page >= 0 && page < num_pages;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    void* out = which ? ov : ok;
-    if (!out) continue;
-    const int64_t at = page * Hkv + head;
-    const uint8_t* block = (which ? v : k) + at * (int64_t)(kPage * D);
-    const float s = there ? (which ? vs : ks)[at] : __uint_as_float(0x7fc00000u);
-    __syncthreads();
-    for (int i = tid * 16; i < kPage * D; i += 256 * 16) {
-      const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(block + i)) : make_uint4(0, 0, 0, 0);
-      uint32_t* d = reinterpret_cast<uint32_t*>(s_block + (which ? i / 64 * 68 + i % 64 : i));
-      d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
-    }
-    __syncthreads();
-    const int64_t o0 = (n * Hkv + head) * kPage * D;
-    for (int i = tid * 4; i < kPage * D; i += 256 * 4) {
-      const int tkn = i / D, d = i % D;
-      float f[4];
+  const uint8_t* block = (which ? v : k) + at * (int64_t)(kPage * D);
+  const float s = there ? __ldg((which ? vs : ks) + at) : __uint_as_float(0x7fc00000u);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        f[q] = __fmul_rn(decode8<KV>(s_block[which ? (d + q) * 68 + tkn : key_at(tkn, d + q, D)]), s);
-      if (dtype == kDtF32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(out) + o0 + i) = make_float4(f[0], f[1], f[2], f[3]);
+  for (int i = 0; i < kVecs; ++i) {
+    const int b = (tid + i * 256) * 16;
+    const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(block + b)) : make_uint4(0, 0, 0, 0);
+    uint32_t* d = reinterpret_cast<uint32_t*>(s_block + (which ? b / 64 * kStride + b % 64 : b));
+    d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
+  }
+  __syncthreads();
+  const int64_t o0 = (n * Hkv + head) * kPage * D;
+#pragma unroll 4
+  for (int i = tid; i < kPage * D / 4; i += 256) {
+    // keys: four values of a token; values: four tokens of a value, neighbouring lanes' stores side by side
+    const int tkn = which ? i / D * 4 : i / (D / 4), d = which ? i % D : i % (D / 4) * 4;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(s_block + (which ? d * kStride + tkn : key_at(tkn, d, D)));
+    uint32_t lo, hi;
+    codes_to_f16<KV>(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    const float f[4] = {__fmul_rn(a.x, s), __fmul_rn(a.y, s), __fmul_rn(b.x, s), __fmul_rn(b.y, s)};
+    const int64_t o = o0 + tkn * D + d;
+    if (which) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) store16or32<DT>(out, o + q * D, f[q]);
+    } else if constexpr (DT == kDtF32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(out) + o) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+      uint32_t x, y;
+      if (DT == kDtBF16) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(f[1]), "f"(f[0]));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(f[3]), "f"(f[2]));
       } else {
-        uint32_t a, c;
-        if (dtype == kDtBF16) {
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(f[1]), "f"(f[0]));
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(c) : "f"(f[3]), "f"(f[2]));
-        } else {
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(a) : "f"(f[1]), "f"(f[0]));
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(c) : "f"(f[3]), "f"(f[2]));
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o0 + i) = make_uint2(a, c);
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(f[1]), "f"(f[0]));
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(f[3]), "f"(f[2]));
       }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o) = make_uint2(x, y);
     }
   }
 }
@@ -290,24 +411,6 @@ __device__ __forceinline__ void page_prefix(const AttnParams& p, int* prefix) {
     if (threadIdx.x == 0) prefix[0] = 0;
   }
   __syncthreads();
-}
-
-template <int KV>
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (KV == kKvInt8) {
-    // 0x6400 | (code + 128) is 1024 + code + 128 in fp16
-    w ^= 0x80808080u;
-    lo = __byte_perm(w, 0x64646464u, 0x4140);
-    hi = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), c), b = __hsub2(*reinterpret_cast<__half2*>(&hi), c);
-    lo = *reinterpret_cast<uint32_t*>(&a);
-    hi = *reinterpret_cast<uint32_t*>(&b);
-  } else {
-    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-  }
 }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -797,13 +900,19 @@ extern "C" int qz_kv_append(uint8_t* k, float* k_scale, uint8_t* v, float* v_sca
   // a run of max_new tokens touches at most this many pages, wherever it starts
   int64_t touched = (max_new + kPage - 2) / kPage + 1;
   if (touched > max_pages) touched = max_pages;
-  AppendParams p{k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, dtype, static_cast<const uint16_t*>(new_k),
+  AppendParams p{k, v, k_scale, v_scale, num_pages, (int)Hkv, static_cast<const uint16_t*>(new_k),
                  static_cast<const uint16_t*>(new_v), k_tok, k_head, v_tok, v_head, N, table, ld_table, (int)max_pages,
                  lengths, cu_new, max_new};
-  const dim3 grid((unsigned)touched, (unsigned)Hkv, (unsigned)B);
+  const dim3 grid((unsigned)touched, (unsigned)(Hkv * 2), (unsigned)B);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (kv_dtype == QZ_KV_INT8) kv_append_kernel<kKvInt8><<<grid, 256, kPage * D, st>>>(p);
-  else kv_append_kernel<kKvE4M3><<<grid, 256, kPage * D, st>>>(p);
+#define QZ_APPEND(KV, DIM)                                                                     \
+  if (dtype == QZ_DTYPE_BF16) kv_append_kernel<KV, DIM, kDtBF16><<<grid, 256, 0, st>>>(p);     \
+  else kv_append_kernel<KV, DIM, kDtF16><<<grid, 256, 0, st>>>(p)
+  if (kv_dtype == QZ_KV_INT8 && D == 128) { QZ_APPEND(kKvInt8, 128); }
+  else if (kv_dtype == QZ_KV_INT8) { QZ_APPEND(kKvInt8, 64); }
+  else if (D == 128) { QZ_APPEND(kKvE4M3, 128); }
+  else { QZ_APPEND(kKvE4M3, 64); }
+#undef QZ_APPEND
   return cuda_status(cudaGetLastError(), "kv append launch");
 }
 
@@ -825,11 +934,19 @@ extern "C" int qz_kv_read(const uint8_t* k, const float* k_scale, const uint8_t*
   for (int64_t n0 = 0; n0 < n; n0 += 65535) {  // the grid's y dimension
     const unsigned ny = (unsigned)(n - n0 < 65535 ? n - n0 : 65535);
     uint8_t *ok = out_k ? static_cast<uint8_t*>(out_k) + n0 * out_page : nullptr, *ov = out_v ? static_cast<uint8_t*>(out_v) + n0 * out_page : nullptr;
-    const dim3 grid((unsigned)Hkv, ny);
-    if (kv_dtype == QZ_KV_INT8)
-      kv_read_kernel<kKvInt8><<<grid, 256, 68 * D, st>>>(k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, pages + n0, ok, ov, out_dtype);
-    else
-      kv_read_kernel<kKvE4M3><<<grid, 256, 68 * D, st>>>(k, v, k_scale, v_scale, num_pages, (int)Hkv, (int)D, pages + n0, ok, ov, out_dtype);
+    const dim3 grid((unsigned)(Hkv * 2), ny);
+#define QZ_READ(KV, DIM, DT) \
+  kv_read_kernel<KV, DIM, DT><<<grid, 256, 0, st>>>(k, v, k_scale, v_scale, num_pages, (int)Hkv, pages + n0, ok, ov)
+#define QZ_READ_OF(KV, DIM)                                     \
+  if (out_dtype == QZ_DTYPE_F32) QZ_READ(KV, DIM, kDtF32);      \
+  else if (out_dtype == QZ_DTYPE_BF16) QZ_READ(KV, DIM, kDtBF16); \
+  else QZ_READ(KV, DIM, kDtF16)
+    if (kv_dtype == QZ_KV_INT8 && D == 128) { QZ_READ_OF(kKvInt8, 128); }
+    else if (kv_dtype == QZ_KV_INT8) { QZ_READ_OF(kKvInt8, 64); }
+    else if (D == 128) { QZ_READ_OF(kKvE4M3, 128); }
+    else { QZ_READ_OF(kKvE4M3, 64); }
+#undef QZ_READ_OF
+#undef QZ_READ
     s = cuda_status(cudaGetLastError(), "kv read launch");
     if (s != QZ_OK) return s;
   }
