@@ -114,6 +114,29 @@ def stream_ptr(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class on_device:
+    """``with on_device(dev) as stream``: dev is the current device inside, and
+    stream the handle of its current stream (a decode step's calls are short enough
+    that the general context manager and stream object would show)."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.previous = torch._C._cuda_exchangeDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.previous != self.index:
+            torch._C._cuda_exchangeDevice(self.previous)
+        return False
+
+
+DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return DTYPE_BF16

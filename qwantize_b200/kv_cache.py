@@ -39,6 +39,10 @@ class KVCache8:
         self.k_scale = torch.zeros(num_pages, kv_heads, dtype=torch.float32, device=device)
         self.v_scale = torch.zeros_like(self.k_scale)
         self.device = self.k.device
+        self.lib = L.load()
+        # the pointers and sizes that every call passes on
+        self.args = (self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), _KV[dtype],
+                     num_pages, kv_heads, head_dim)
 
     def load_codes(self, k, k_scale, v, v_scale):
         """Set the whole cache from codes (num_pages, kv_heads, 64, head_dim) of its
@@ -63,32 +67,37 @@ class KVCache8:
 
 
 def _index(t, name, dev, ndim):
-    assert t.ndim == ndim and t.dtype in (torch.int32, torch.int64), f"{name} must be a {ndim}-d int32 tensor"
+    assert t.ndim == ndim and (t.dtype == torch.int32 or t.dtype == torch.int64), f"{name} must be a {ndim}-d int32 tensor"
     assert t.device == dev, f"{name} is on {t.device}, the cache on {dev}"
-    t = t if t.dtype == torch.int32 else t.to(torch.int32)
-    return t if ndim == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _table(block_table, lengths, cache):
     assert isinstance(cache, KVCache8), "cache must be a KVCache8"
     table = _index(block_table, "block_table", cache.device, 2)
     lengths = _index(lengths, "lengths", cache.device, 1)
-    assert lengths.shape[0] == table.shape[0], f"{lengths.shape[0]} lengths for {table.shape[0]} rows of block_table"
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
-        table = table.contiguous()
-    return table, lengths, table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    B, pages = table.shape
+    assert lengths.shape[0] == B, f"{lengths.shape[0]} lengths for {B} rows of block_table"
+    ld = table.stride(0) if B > 1 else pages
+    if ld < pages:
+        table, ld = table.contiguous(), pages
+    return table, lengths, B, pages, ld
 
 
 def _rows16(x, name, shape_tail, dev):
     """x (n, heads, D) of 16 bits with contiguous, 16-byte aligned rows, and its strides."""
-    assert x.ndim == 3 and tuple(x.shape[1:]) == shape_tail, f"{name} is {tuple(x.shape)}, expected (n, {shape_tail[0]}, {shape_tail[1]})"
-    assert x.dtype in (torch.bfloat16, torch.float16), f"unsupported dtype {x.dtype}, expected bfloat16 or float16"
+    assert x.ndim == 3 and x.shape[1:] == shape_tail, f"{name} is {tuple(x.shape)}, expected (n, {shape_tail[0]}, {shape_tail[1]})"
+    assert x.dtype == torch.bfloat16 or x.dtype == torch.float16, f"unsupported dtype {x.dtype}, expected bfloat16 or float16"
     assert x.device == dev, f"{name} is on {x.device}, the cache on {dev}"
-    if x.stride(2) != 1 or x.stride(1) % 8 or x.stride(0) % 8 or x.data_ptr() % 16:
+    s0, s1, s2 = x.stride()
+    if s2 != 1 or s1 % 8 or s0 % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x, x.stride(0), x.stride(1)
+        s0, s1, _ = x.stride()
+    return x, s0, s1
 
 
 def kv_cache_append(cache, k, v, block_table, lengths, cu_new=None, max_new=None):
@@ -101,12 +110,13 @@ def kv_cache_append(cache, k, v, block_table, lengths, cu_new=None, max_new=None
     page's scale grows to what its new tokens need, its older codes being taken
     over to the larger scale, and slots behind the last token become zero.  A
     page must belong to one of the sequences only.  ``lengths`` stays as it is."""
-    table, lengths, ld = _table(block_table, lengths, cache)
+    table, lengths, B, pages, ld = _table(block_table, lengths, cache)
     tail = (cache.kv_heads, cache.head_dim)
     k, k0, k1 = _rows16(k, "k", tail, cache.device)
     v, v0, v1 = _rows16(v, "v", tail, cache.device)
-    N, B = k.shape[0], table.shape[0]
+    N = k.shape[0]
     assert v.shape[0] == N and v.dtype == k.dtype, "k and v must have the same number of tokens and type"
+    cu = None
     if cu_new is None:
         assert N == B, f"without cu_new there is one new token per sequence: {N} tokens, {B} sequences"
         max_new = 1
@@ -114,12 +124,12 @@ def kv_cache_append(cache, k, v, block_table, lengths, cu_new=None, max_new=None
         cu_new = _index(cu_new, "cu_new", cache.device, 1)
         assert cu_new.shape[0] == B + 1, f"cu_new has {cu_new.shape[0]} entries, expected {B + 1}"
         max_new = N if max_new is None else int(max_new)
-    with torch.cuda.device(cache.device):
-        L.check(L.load().qz_kv_append(
-            cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), _KV[cache.dtype],
-            cache.num_pages, cache.kv_heads, cache.head_dim, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
-            L.dtype_code(k.dtype), N, table.data_ptr(), ld, table.shape[1], lengths.data_ptr(),
-            None if cu_new is None else cu_new.data_ptr(), max_new, B, L.stream_ptr(cache.device)), "qz_kv_append")
+        cu = cu_new.data_ptr()
+    with L.on_device(cache.device) as stream:
+        st = cache.lib.qz_kv_append(*cache.args, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, L.DTYPE_CODES[k.dtype], N,
+                                    table.data_ptr(), ld, pages, lengths.data_ptr(), cu, max_new, B, stream)
+    if st:
+        L.check(st, "qz_kv_append")
 
 
 def kv_cache_read(cache, pages, dtype=torch.float32):
@@ -128,14 +138,15 @@ def kv_cache_read(cache, pages, dtype=torch.float32):
     cache does not have."""
     assert isinstance(cache, KVCache8), "cache must be a KVCache8"
     pages = _index(pages, "pages", cache.device, 1)
-    assert dtype in (torch.float32, torch.bfloat16, torch.float16), f"unsupported dtype {dtype}"
-    shape = (pages.shape[0], cache.kv_heads, PAGE, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
-    with torch.cuda.device(cache.device):
-        L.check(L.load().qz_kv_read(
-            cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), _KV[cache.dtype],
-            cache.num_pages, cache.kv_heads, cache.head_dim, pages.data_ptr(), pages.shape[0], k.data_ptr(), v.data_ptr(),
-            L.dtype_code(dtype), L.stream_ptr(cache.device)), "qz_kv_read")
+    assert dtype in L.DTYPE_CODES, f"unsupported dtype {dtype}"
+    n = pages.shape[0]
+    shape = (n, cache.kv_heads, PAGE, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=cache.device)
+    v = torch.empty(shape, dtype=dtype, device=cache.device)
+    with L.on_device(cache.device) as stream:
+        st = cache.lib.qz_kv_read(*cache.args, pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), L.DTYPE_CODES[dtype], stream)
+    if st:
+        L.check(st, "qz_kv_read")
     return k, v
 
 
@@ -147,28 +158,28 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     behind block_table[b] are attended to (an empty sequence gives zeros); scale
     defaults to 1 / sqrt(head_dim).  Products of 16-bit operands (codes fit fp16
     exactly), softmax and sums in fp32, rounded once to q's type."""
-    table, lengths, ld = _table(block_table, lengths, cache)
-    B, D, dev = table.shape[0], cache.head_dim, cache.device
+    table, lengths, B, pages, ld = _table(block_table, lengths, cache)
+    D, dev = cache.head_dim, cache.device
     assert q.ndim == 3 and q.shape[0] == B, f"q is {tuple(q.shape)}, expected ({B}, heads, {D})"
     Hq = q.shape[1]
     assert Hq >= 1 and Hq % cache.kv_heads == 0, f"{Hq} query heads are not a multiple of {cache.kv_heads} cache heads"
     q, q0, q1 = _rows16(q, "q", (Hq, D), dev)
     assert B <= 4096, f"{B} sequences, expected at most 4096"
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=dev)
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
     else:
         assert tuple(out.shape) == (B, Hq, D) and out.dtype == q.dtype and out.device == dev and out.is_contiguous(), (
             f"out must be a contiguous {q.dtype} tensor of shape {(B, Hq, D)} on {dev}")
-    with torch.cuda.device(dev):
+    with L.on_device(dev) as stream:
         n = _workspace.get((dev, D))
         if n is None:
             b = ctypes.c_int64(0)
-            L.check(L.load().qz_kv_attention_workspace(D, ctypes.byref(b)), "qz_kv_attention_workspace")
+            L.check(cache.lib.qz_kv_attention_workspace(D, ctypes.byref(b)), "qz_kv_attention_workspace")
             n = _workspace[dev, D] = b.value
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        L.check(L.load().qz_kv_attention(
-            cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), _KV[cache.dtype],
-            cache.num_pages, cache.kv_heads, D, q.data_ptr(), q0, q1, L.dtype_code(q.dtype), B, Hq, table.data_ptr(), ld,
-            table.shape[1], lengths.data_ptr(), D**-0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(),
-            n, L.stream_ptr(dev)), "qz_kv_attention")
+        st = cache.lib.qz_kv_attention(*cache.args, q.data_ptr(), q0, q1, L.DTYPE_CODES[q.dtype], B, Hq, table.data_ptr(), ld,
+                                       pages, lengths.data_ptr(), D**-0.5 if scale is None else float(scale),
+                                       out.data_ptr(), ws.data_ptr(), n, stream)
+    if st:
+        L.check(st, "qz_kv_attention")
     return out

@@ -91,6 +91,8 @@ class FP4Weight:
             self.scales = torch.empty(n.value, dtype=torch.uint8, device=dev)
             L.check(L.load().qz_fp4_scale_layout(L.ptr(self.scale_codes), self.N, self.K, _FMT[fmt], L.ptr(self.scales),
                                                  L.stream_ptr(dev)), "qz_fp4_scale_layout")
+        self.lib, self.fmt_code = L.load(), _FMT[fmt]
+        self.packed_ptr, self.scales_ptr = self.packed.data_ptr(), self.scales.data_ptr()
         self._workspace = {}  # tokens -> bytes
 
     @classmethod
@@ -128,41 +130,47 @@ def fp4_linear(x, weight, bias=None, out_dtype=None, out=None):
     once to out_dtype (default: x's).  ``out`` may supply the result's buffer, a
     contiguous (..., N) tensor."""
     assert isinstance(weight, FP4Weight), "weight must be an FP4Weight"
-    assert x.dtype in _DTYPES, f"unsupported dtype {x.dtype}, expected one of {_DTYPES}"
+    dtype, codes = x.dtype, L.DTYPE_CODES
+    assert dtype in codes, f"unsupported dtype {dtype}, expected one of {_DTYPES}"
     K, N, dev = weight.K, weight.N, weight.device
     assert x.ndim >= 1 and x.shape[-1] == K, f"x has {x.shape[-1] if x.ndim else 0} columns, the weight {K}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the weight on {dev}"
-    out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-    assert out_dtype in _DTYPES, f"unsupported dtype {out_dtype}, expected one of {_DTYPES}"
+    if out_dtype is None:
+        out_dtype = dtype if out is None else out.dtype
+    assert out_dtype in codes, f"unsupported dtype {out_dtype}, expected one of {_DTYPES}"
     shape = (*x.shape[:-1], N)
     xd = x if x.is_cuda else to_device(x, dev)
     if xd.ndim != 2:
         xd = xd.reshape(-1, K)
-    size = 4 if xd.dtype == torch.float32 else 2
     T = xd.shape[0]
-    ldx = xd.stride(0) if T > 1 else K
-    if (K > 1 and xd.stride(1) != 1) or ldx < K or ldx * size % 16 or xd.data_ptr() % 16:
+    ldx, step = xd.stride()
+    if T == 1:
+        ldx = K
+    if step != 1 or ldx < K or ldx * xd.element_size() % 16 or xd.data_ptr() % 16:
         xd, ldx = xd.contiguous(), K
         if xd.data_ptr() % 16:
             xd = xd.clone()
+    bias_ptr, bias_code = None, 0
     if bias is not None:
-        assert tuple(bias.shape) == (N,) and bias.dtype in _DTYPES, f"bias must be ({N},) in one of {_DTYPES}"
+        assert tuple(bias.shape) == (N,) and bias.dtype in codes, f"bias must be ({N},) in one of {_DTYPES}"
         bias = bias.to(dev).contiguous()
-    if out is not None:
-        assert tuple(out.shape) == shape and out.dtype == out_dtype and out.device == dev and out.is_contiguous(), (
-            f"out must be a contiguous {out_dtype} tensor of shape {shape} on {dev}")
-        y = out
-    else:
+        bias_ptr, bias_code = bias.data_ptr(), codes[bias.dtype]
+    if out is None:
         y = torch.empty(shape, dtype=out_dtype, device=dev)
+    else:
+        y = out
+        assert tuple(y.shape) == shape and y.dtype == out_dtype and y.device == dev and y.is_contiguous(), (
+            f"out must be a contiguous {out_dtype} tensor of shape {shape} on {dev}")
     if T:
-        with torch.cuda.device(dev):
+        with L.on_device(dev) as stream:
             n = weight.workspace_bytes(T)
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            L.check(L.load().qz_fp4_linear(
-                xd.data_ptr(), L.dtype_code(xd.dtype), ldx, T, K, N, _FMT[weight.fmt], weight.packed.data_ptr(),
-                weight.ldp, weight.scales.data_ptr(), weight.tensor_scale, None if bias is None else bias.data_ptr(),
-                0 if bias is None else L.dtype_code(bias.dtype), y.data_ptr(), L.dtype_code(out_dtype), N,
-                ws.data_ptr(), n, L.stream_ptr(dev)), "qz_fp4_linear")
+            st = weight.lib.qz_fp4_linear(
+                xd.data_ptr(), codes[dtype], ldx, T, K, N, weight.fmt_code, weight.packed_ptr, weight.ldp,
+                weight.scales_ptr, weight.tensor_scale, bias_ptr, bias_code, y.data_ptr(), codes[out_dtype], N,
+                ws.data_ptr(), n, stream)
+        if st:
+            L.check(st, "qz_fp4_linear")
     if x.is_cuda or out is not None:
         return y
     return to_host_like((y,), x.device, dev)[0]

@@ -50,6 +50,10 @@ class FP4Experts:
         assert self.E <= 512, f"{self.E} experts, expected at most 512"
         self.fmt = fmt
         self.tensor_scales = float(tensor_scales[0]), float(tensor_scales[1])
+        self.lib = L.load()
+        self.weight_args = (_FMT[fmt], self.up_codes.data_ptr(), self.up_scales.data_ptr(), self.up_norms.data_ptr(),
+                            self.tensor_scales[0], self.down_codes.data_ptr(), self.down_scales.data_ptr(),
+                            self.tensor_scales[1])
         self._workspace = {}
 
     @classmethod
@@ -79,11 +83,13 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     type.  With return_routing: (out, ids int32 (..., top_k), weights fp32)."""
     assert isinstance(experts, FP4Experts), "experts must be an FP4Experts"
     dev, H, E = experts.device, experts.H, experts.E
-    assert x.dtype in (torch.bfloat16, torch.float16), f"unsupported dtype {x.dtype}, expected bfloat16 or float16"
+    dtype, codes = x.dtype, L.DTYPE_CODES
+    assert dtype == torch.bfloat16 or dtype == torch.float16, f"unsupported dtype {dtype}, expected bfloat16 or float16"
     assert x.ndim >= 1 and x.shape[-1] == H, f"x has {x.shape[-1] if x.ndim else 0} columns, the experts {H}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the experts on {dev}"
-    assert tuple(router_weight.shape) == (E, H), f"router_weight {tuple(router_weight.shape)}, expected {(E, H)}"
-    assert router_weight.dtype in (torch.bfloat16, torch.float16, torch.float32), f"unsupported dtype {router_weight.dtype}"
+    r = router_weight
+    assert tuple(r.shape) == (E, H), f"router_weight {tuple(r.shape)}, expected {(E, H)}"
+    assert r.dtype in codes, f"unsupported dtype {r.dtype}"
     top_k = int(top_k)
     assert 1 <= top_k <= min(16, E), f"top_k={top_k}, expected 1 to {min(16, E)}"
     xd = x if x.is_cuda else to_device(x, dev)
@@ -91,35 +97,37 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
         xd = xd.reshape(-1, H)
     T = xd.shape[0]
     assert T <= MAX_TOKENS, f"{T} tokens, expected at most {MAX_TOKENS}"
-    ldx = xd.stride(0) if T > 1 else H
-    if xd.stride(1) != 1 or ldx < H or ldx % 8 or xd.data_ptr() % 16:
+    ldx, step = xd.stride()
+    if T == 1:
+        ldx = H
+    if step != 1 or ldx < H or ldx % 8 or xd.data_ptr() % 16:
         xd, ldx = xd.contiguous(), H
         if xd.data_ptr() % 16:
             xd = xd.clone()
-    r = router_weight.to(dev).contiguous()
+    if r.device != dev or not r.is_contiguous():
+        r = r.to(dev).contiguous()
     if r.data_ptr() % 16:
         r = r.clone()
-    if out is not None:
-        assert out.shape == x.shape and out.dtype == x.dtype and out.device == dev and out.is_contiguous(), (
-            f"out must be a contiguous {x.dtype} tensor of shape {tuple(x.shape)} on {dev}")
-        y = out
+    if out is None:
+        y = torch.empty(x.shape, dtype=dtype, device=dev)
     else:
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = out
+        assert y.shape == x.shape and y.dtype == dtype and y.device == dev and y.is_contiguous(), (
+            f"out must be a contiguous {dtype} tensor of shape {tuple(x.shape)} on {dev}")
     ids = weights = None
     if return_routing:
-        ids = torch.empty(*x.shape[:-1], top_k, dtype=torch.int32, device=dev)
-        weights = torch.empty(*x.shape[:-1], top_k, dtype=torch.float32, device=dev)
+        ids = torch.empty((*x.shape[:-1], top_k), dtype=torch.int32, device=dev)
+        weights = torch.empty((*x.shape[:-1], top_k), dtype=torch.float32, device=dev)
     if T:
         n = experts.workspace_bytes(T, top_k)
-        with torch.cuda.device(dev):
+        with L.on_device(dev) as stream:
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            L.check(L.load().qz_moe(
-                xd.data_ptr(), L.dtype_code(xd.dtype), ldx, T, H, experts.I, E, top_k, int(bool(renormalize)),
-                r.data_ptr(), L.dtype_code(r.dtype), _FMT[experts.fmt], experts.up_codes.data_ptr(),
-                experts.up_scales.data_ptr(), experts.up_norms.data_ptr(), experts.tensor_scales[0], experts.down_codes.data_ptr(),
-                experts.down_scales.data_ptr(), experts.tensor_scales[1], y.data_ptr(),
-                ids.data_ptr() if return_routing else None, weights.data_ptr() if return_routing else None,
-                ws.data_ptr(), n, L.stream_ptr(dev)), "qz_moe")
+            st = experts.lib.qz_moe(
+                xd.data_ptr(), codes[dtype], ldx, T, H, experts.I, E, top_k, 1 if renormalize else 0, r.data_ptr(),
+                codes[r.dtype], *experts.weight_args, y.data_ptr(), ids.data_ptr() if return_routing else None,
+                weights.data_ptr() if return_routing else None, ws.data_ptr(), n, stream)
+        if st:
+            L.check(st, "qz_moe")
     res = (y, ids, weights) if return_routing else (y,)
     if not x.is_cuda and out is None:
         res = to_host_like(res, x.device, dev)
