@@ -134,6 +134,12 @@ class on_device:
         return False
 
 
+# Scratch memory of one call from torch's caching allocator, on the call's stream:
+# released right after the launches, it is reused only by later work of that stream.
+# (A tensor would do the same at three times the host time.)
+take_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
+give_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
+
 DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
 

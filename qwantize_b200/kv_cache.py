@@ -176,10 +176,13 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
             b = ctypes.c_int64(0)
             L.check(cache.lib.qz_kv_attention_workspace(D, ctypes.byref(b)), "qz_kv_attention_workspace")
             n = _workspace[dev, D] = b.value
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        st = cache.lib.qz_kv_attention(*cache.args, q.data_ptr(), q0, q1, L.DTYPE_CODES[q.dtype], B, Hq, table.data_ptr(), ld,
-                                       pages, lengths.data_ptr(), D**-0.5 if scale is None else float(scale),
-                                       out.data_ptr(), ws.data_ptr(), n, stream)
+        ws = L.take_scratch(n, stream)
+        try:
+            st = cache.lib.qz_kv_attention(*cache.args, q.data_ptr(), q0, q1, L.DTYPE_CODES[q.dtype], B, Hq, table.data_ptr(), ld,
+                                           pages, lengths.data_ptr(), D**-0.5 if scale is None else float(scale),
+                                           out.data_ptr(), ws, n, stream)
+        finally:
+            L.give_scratch(ws)
     if st:
         L.check(st, "qz_kv_attention")
     return out

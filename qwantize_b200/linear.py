@@ -164,11 +164,14 @@ def fp4_linear(x, weight, bias=None, out_dtype=None, out=None):
     if T:
         with L.on_device(dev) as stream:
             n = weight.workspace_bytes(T)
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            st = weight.lib.qz_fp4_linear(
-                xd.data_ptr(), codes[dtype], ldx, T, K, N, weight.fmt_code, weight.packed_ptr, weight.ldp,
-                weight.scales_ptr, weight.tensor_scale, bias_ptr, bias_code, y.data_ptr(), codes[out_dtype], N,
-                ws.data_ptr(), n, stream)
+            ws = L.take_scratch(n, stream)
+            try:
+                st = weight.lib.qz_fp4_linear(
+                    xd.data_ptr(), codes[dtype], ldx, T, K, N, weight.fmt_code, weight.packed_ptr, weight.ldp,
+                    weight.scales_ptr, weight.tensor_scale, bias_ptr, bias_code, y.data_ptr(), codes[out_dtype], N,
+                    ws, n, stream)
+            finally:
+                L.give_scratch(ws)
         if st:
             L.check(st, "qz_fp4_linear")
     if x.is_cuda or out is not None:

@@ -121,11 +121,14 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     if T:
         n = experts.workspace_bytes(T, top_k)
         with L.on_device(dev) as stream:
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            st = experts.lib.qz_moe(
-                xd.data_ptr(), codes[dtype], ldx, T, H, experts.I, E, top_k, 1 if renormalize else 0, r.data_ptr(),
-                codes[r.dtype], *experts.weight_args, y.data_ptr(), ids.data_ptr() if return_routing else None,
-                weights.data_ptr() if return_routing else None, ws.data_ptr(), n, stream)
+            ws = L.take_scratch(n, stream)
+            try:
+                st = experts.lib.qz_moe(
+                    xd.data_ptr(), codes[dtype], ldx, T, H, experts.I, E, top_k, 1 if renormalize else 0, r.data_ptr(),
+                    codes[r.dtype], *experts.weight_args, y.data_ptr(), ids.data_ptr() if return_routing else None,
+                    weights.data_ptr() if return_routing else None, ws, n, stream)
+            finally:
+                L.give_scratch(ws)
         if st:
             L.check(st, "qz_moe")
     res = (y, ids, weights) if return_routing else (y,)
