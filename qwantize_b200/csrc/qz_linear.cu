@@ -61,19 +61,24 @@ struct Fmt {
 // ---------------------------------------------------------------------------
 // activations to FP4
 // ---------------------------------------------------------------------------
-// The largest magnitude of 16 bytes of elements, as bits that order like it:
-// fp32 bits (bf16 and fp32 input) or fp16 bits.
+// The largest magnitude of 16 bytes of elements: fp32 bits for fp32, else two
+// 16-bit patterns side by side that order like the magnitudes (NaN above inf).
 template <int DT>
-__device__ __forceinline__ uint32_t abs_max(const uint4& w) {
+__device__ __forceinline__ uint32_t abs_max(uint32_t m, const uint4& w) {
   const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-  uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (DT == kDtF32) m = max(m, ww[k] & 0x7fffffffu);
-    else if (DT == kDtBF16) m = max(m, max(ww[k] & 0x7fff0000u, ww[k] << 16 & 0x7fff0000u));
-    else m = max(m, max(ww[k] >> 16 & 0x7fffu, ww[k] & 0x7fffu));
+    else m = __vmaxu2(m, ww[k] & 0x7fff7fffu);
   }
   return m;
+}
+// ... as fp32 bits
+template <int DT>
+__device__ __forceinline__ uint32_t abs_bits(uint32_t m) {
+  if (DT == kDtF32) return m;
+  m = max(m >> 16, m & 0xffffu);
+  return DT == kDtBF16 ? m << 16 : __float_as_uint(f16_bits_to_float(m));
 }
 
 template <int DT, int VEC, int BS>
@@ -117,21 +122,29 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
       raw[r][v] = b < nb ? __ldg(base + b * kVec + v) : make_uint4(0, 0, 0, 0);
     }
   float inv = 1.0f, p = 1.0f;
+  uint32_t am[R];  // the blocks' largest magnitudes
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) m = abs_max<DT>(m, raw[r][v]);
+    am[r] = abs_bits<DT>(m);
+  }
   if (BS == 16) {
     uint32_t m = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) m = max(m, am[r]);
+    for (int64_t b = tid + (int64_t)R * nt; b < nb; b += nt) {
+      uint32_t o = 0;
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) m = max(m, abs_max<DT>(raw[r][v]));
-    for (int64_t b = tid + (int64_t)R * nt; b < nb; b += nt)
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) m = max(m, abs_max<DT>(__ldg(base + b * kVec + v)));
+      for (int v = 0; v < kVec; ++v) o = abs_max<DT>(o, __ldg(base + b * kVec + v));
+      m = max(m, abs_bits<DT>(o));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
     m = 0;
     for (int w = 0; w < (nt >> 5); ++w) m = max(m, s_max[w]);
-    if (DT == kDtF16) m = __float_as_uint(f16_bits_to_float(m));
     // smallest e with max <= 1.3125 * 2^(11 + e); 0 for an all-zero row and for inf / NaN
     int e = 0;
     if (m != 0 && m < 0x7f800000u) {
@@ -143,39 +156,38 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
   }
   if (tid == 0) row_scale[row] = p;
   uint8_t* sf_row = sf + (row / gran) * n_steps * Fmt<BS>::kSfBytes + (row % gran % 32) * 16 + (row % gran / 32) * 4;
-  auto block = [&](int64_t b, const uint4 (&w)[kVec]) {
+  auto block = [&](int64_t b, const uint4 (&w)[kVec], uint32_t largest) {
     uint32_t code = 0;
     uint32_t words[BS / 8] = {};
     if (b < nb) {
-      float v[BS];
-      unpack<DT, kVec>(w, v);
-      uint32_t am = 0;
-#pragma unroll
-      for (int i = 0; i < BS; ++i) {
-        v[i] = __fmul_rn(v[i], inv);
-        am = max(am, __float_as_uint(v[i]) & 0x7fffffffu);
-      }
+      // the block of x / p: a power of two moves no bit of a 16-bit value
+      const uint32_t y = __float_as_uint(__fmul_rn(__uint_as_float(largest), inv));
       float s;
       if (BS == 16) {
-        s = e4m3_snap_nonneg(__fdiv_rn(__uint_as_float(am), 6.0f));
+        s = e4m3_snap_nonneg(__fdiv_rn(__uint_as_float(y), 6.0f));
         code = e4m3_code(s);
       } else {
-        code = is_nan_bits(am) ? 255u : (uint32_t)ue8m0_naive_exp(am);
+        code = is_nan_bits(y) ? 255u : (uint32_t)ue8m0_naive_exp(y);
         s = code == 255u ? __uint_as_float(kMxNanBits) : pow2f((int)code - 127);
       }
       if (s > 0.0f) {  // a zero (or NaN) scale keeps codes 0
+        float v[BS];
+        unpack<DT, kVec>(w, v);
         if (DT != kDtF32) {
+          // the conversion rounds the magnitude and keeps the sign
           const float c = __fmul_rn(__frcp_rn(s), kBiasDown);
+          const bool in_range = inv >= 0x1p-60f && inv <= 0x1p60f;  // inv * c is exact: one product per value
+          const float ci = in_range ? __fmul_rn(c, inv) : c;
 #pragma unroll
           for (int i = 0; i < BS; i += 2) {
-            const uint32_t lo = __float_as_uint(v[i]) >> 31, hi = __float_as_uint(v[i + 1]) >> 31;
-            words[i / 8] |= (e2m1x2_rn(__fmul_rn(fabsf(v[i]), c), __fmul_rn(fabsf(v[i + 1]), c)) | lo << 3 | hi << 7)
-                            << (4 * (i % 8));
+            float lo = v[i], hi = v[i + 1];
+            if (!in_range) { lo = __fmul_rn(lo, inv); hi = __fmul_rn(hi, inv); }
+            words[i / 8] |= e2m1x2_rn(__fmul_rn(lo, ci), __fmul_rn(hi, ci)) << (4 * (i % 8));
           }
         } else {
 #pragma unroll
           for (int i = 0; i < BS; ++i) {
-            const float q = __fdiv_rn(fabsf(v[i]), s);
+            const float q = __fdiv_rn(fabsf(__fmul_rn(v[i], inv)), s);
             uint32_t n = __float_as_uint(v[i]) >> 31 << 3;
 #pragma unroll
             for (int k = 0; k < 7; ++k) n += q > bnd(k) ? 1u : 0u;
@@ -195,12 +207,16 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
   };
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if ((int64_t)r * nt < nb_pad) block(tid + (int64_t)r * nt, raw[r]);
+    if ((int64_t)r * nt < nb_pad) block(tid + (int64_t)r * nt, raw[r], am[r]);
   for (int64_t b0 = (int64_t)R * nt; b0 < nb_pad; b0 += nt) {
     uint4 w[kVec];
+    uint32_t m = 0;
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) w[v] = b0 + tid < nb ? __ldg(base + (b0 + tid) * kVec + v) : make_uint4(0, 0, 0, 0);
-    block(b0 + tid, w);
+    for (int v = 0; v < kVec; ++v) {
+      w[v] = b0 + tid < nb ? __ldg(base + (b0 + tid) * kVec + v) : make_uint4(0, 0, 0, 0);
+      m = abs_max<DT>(m, w[v]);
+    }
+    block(b0 + tid, w, abs_bits<DT>(m));
   }
 }
 
