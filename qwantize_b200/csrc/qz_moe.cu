@@ -383,6 +383,7 @@ struct MoeShared {
   uint16_t g_expert[kMoeMaxGroups], g_begin[kMoeMaxGroups], g_count[kMoeMaxGroups];
   uint16_t g_cost[kMoeMaxGroups + 1];     // cost of one unit of each group before this one
   int n_groups, ok;
+  int bound[4];                           // this CTA's first unit and the one behind its last: gate / up, down
   uint64_t full[kMoeWarps * kMoeStages];  // the warps' rings
   float x_scale[kMoeMaxTokens];           // power of two of a token times the tensor scale
   int16_t act_exp[kMoeMaxSlots];          // e: |activation| of the slot < 2^(e + 15)
@@ -472,6 +473,19 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     if (lane == 0) {
       s.n_groups = groups;
       s.g_cost[groups] = (uint16_t)cost;
+    }
+    __syncwarp();
+    if (lane < 4) {
+      // the first unit at or behind this CTA's (the next one's) share of the phase's cost
+      const int units = lane < 2 ? p.I / 16 : p.H / 32;
+      const int64_t at = (int64_t)cost * units * (blockIdx.x + (lane & 1)) / gridDim.x;
+      int lo = 0, hi = groups;  // last group that begins at or before it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)s.g_cost[mid] * units <= at) lo = mid; else hi = mid;
+      }
+      const int one = s.g_cost[lo + 1] - s.g_cost[lo];
+      s.bound[lane] = lo * units + ((int)(at - (int64_t)s.g_cost[lo] * units) + one - 1) / one;
     }
   }
   __syncthreads();
@@ -620,20 +634,9 @@ struct MoeWalk {
   int last_group, last_unit;
   bool whole;                  // the current unit is this warp's alone
 
-  // the first unit at or behind share i / gridDim of the phase's cost
-  __device__ __forceinline__ int boundary(const MoeShared& s, int i) const {
-    const int64_t at = (int64_t)s.g_cost[s.n_groups] * units * i / gridDim.x;
-    int lo = 0, hi = s.n_groups;  // last group that begins at or before it
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)s.g_cost[mid] * units <= at) lo = mid; else hi = mid;
-    }
-    const int cost = s.g_cost[lo + 1] - s.g_cost[lo];
-    return lo * units + ((int)(at - (int64_t)s.g_cost[lo] * units) + cost - 1) / cost;
-  }
-  __device__ __forceinline__ MoeWalk(const MoeShared& s, int units_, int chunks_) : units(units_), chunks(chunks_) {
+  __device__ __forceinline__ MoeWalk(const int* bound, int units_, int chunks_) : units(units_), chunks(chunks_) {
     const int warp = threadIdx.x >> 5;
-    const int begin = boundary(s, blockIdx.x), end = boundary(s, blockIdx.x + 1);
+    const int begin = bound[0], end = bound[1];
     const int rounds = (end - begin) / kMoeWarps, rest = (end - begin) % kMoeWarps;
     share = rest ? kMoeWarps / rest : 1;
     share = share < 8 ? share : 8;
@@ -685,7 +688,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
   const uint8_t* codes = UP ? p.up_codes : p.down_codes;
   const uint8_t* scales = UP ? p.up_scales : p.down_scales;
   const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
-  MoeWalk w(s, units, chunks), ahead = w;
+  MoeWalk w(s.bound + (UP ? 0 : 2), units, chunks), ahead = w;
   uint8_t* mine = ring + warp * kMoeStages * R::kStage;
   uint64_t* full = s.full + warp * kMoeStages;
   int64_t at_unit = 0;  // first chunk of the unit that is loaded
