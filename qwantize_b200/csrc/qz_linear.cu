@@ -11,22 +11,23 @@
 // is exact, so 16-bit inputs keep their 11 significant bits and the rounding
 // shortcut of qz_common.cuh holds.  w is the weight's tensor scale.
 //
-// Two launches: quantize_rows_kernel (one CTA per row), then linear_kernel.
+// Two launches: quantize_rows_kernel (one CTA per row), then the product, in one
+// of two forms; both walk K in stages of 256 values (128-byte swizzled rows of A
+// and B by TMA, their scales by bulk copies) with a ring of stages per CTA:
 //
-// linear_kernel, one persistent CTA per SM, 224 threads: warp 0 feeds a ring of
-// stages (256 values of K: 128-byte swizzled rows of A and B by TMA, their
-// scales by bulk copies), warp 6 copies a stage's scales to TMEM (tcgen05.cp),
-// warp 1 issues its four block-scaled MMAs of K = 64, warps 2-5 drain the
-// accumulator.  A stage of the wide form is 12 copies and 4 MMAs, and issuing an
-// instruction takes about 30 clocks, so one warp issuing both (700 clocks a
-// stage) could not keep up with the MMAs (543).  The wide form (BN = 256) has 128 token rows as A and 256 rows
-// of W as B.  The narrow forms (BN = 16 .. 128) swap the operands: 128 rows of
-// W are A and BN tokens are B, so that a decode step multiplies few padded
-// rows, and W streams through the ring once.  Where the tiles leave SMs idle, a
-// cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
-// through distributed shared memory, each CTA finishing its share of the columns.
+//   linear_kernel (few tokens; BN = 16, 32 or 64): 128 rows of W are A and BN tokens
+//   are B, so that a decode step multiplies few padded rows, and W streams through
+//   the ring once: the bytes of W bound it.  Where the tiles leave SMs idle, a
+//   cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
+//   through distributed shared memory, each CTA finishing its share of the columns.
+//
+//   linear_pair_kernel (prompts): a pair of CTAs on 256 tokens x 256 features; the
+//   tensor cores bound it.
+//
 // The second launch starts before the first has ended and fetches its first
-// stages of W meanwhile.
+// stages of W meanwhile.  Issuing a copy or an MMA takes about 30 clocks from an
+// elected lane of a converged warp and about 60 from a branch on the lane, so
+// each role has a warp of its own and stays converged.
 //
 // Scales in memory, for both operands: row tiles of 128 rows (x, narrow form:
 // BN rows), groups of 4 blocks of K; a group is 512 bytes, row r at
@@ -101,7 +102,9 @@ __device__ __forceinline__ void unpack(const uint4 (&w)[VEC], float (&v)[BS]) {
 // One CTA per row.  A thread keeps its first R blocks of BS values in registers
 // between the row's maximum and the rounding (later ones of very long rows
 // are read again, from L2): R = 1 for few rows, where the latency of one row
-// counts, R = 4 for many, where loads in flight do.
+// counts, R = 4 (NVFP4) or 2 (MXFP4) for many, where loads in flight do.  With the
+// product, 64 rows of 8192: 16.9 us with R = 1, 18.0 with 4; 256 rows: 18.8 with
+// both; 1024: 27.1 and 25.9; 8192: 90.8 and 72.1.
 template <int BS, int DT, int R>
 __global__ void __launch_bounds__(R == 1 ? 512 : 256)
     quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t K, uint8_t* __restrict__ packed, int64_t ldp,
@@ -253,27 +256,22 @@ struct LinearParams {
   void* out;
   int out_dtype;
   int64_t ldo;
-  int tma_out;                        // map_out is valid (wide form, 16-bit output, 16-byte rows)
+  int tma_out;                        // map_out is valid (pair form, 16-bit output, 16-byte rows)
 };
 
+// The form of few tokens: A = weight rows, B = tokens.
 template <int BN, int BS>
 struct LinGeo {
-  static constexpr bool kSwap = BN < 256;  // A = weight rows, B = tokens
   static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
-  static constexpr int kBTiles = BN > 128 ? BN / 128 : 1;  // 128-row scale tiles of B
   static constexpr int kSf = Fmt<BS>::kSfBytes;
-  static constexpr int kStageBytes = kABytes + kBBytes + kSf * (1 + kBTiles);
-  static constexpr int kOutBytes = kSwap ? 0 : 4 * 2048;   // wide: 32 rows x 32 columns of output per epilogue warp
-  static constexpr int kMaxStages = (232448 - 1024 - 512 - kOutBytes) / kStageBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kSf;
+  static constexpr int kMaxStages = (232448 - 1024 - 512) / kStageBytes;
   static constexpr int kStages = kMaxStages > 10 ? 10 : kMaxStages;
-  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024 + 512;
-  // TMEM: two accumulators, then kSfBufs buffers of scales (kGroups * 4 columns
-  // per 128 rows).  The wide form's accumulators share kOverlap columns, which
-  // are drained first: the next tile begins when they are free.
-  static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * (1 + kBTiles);
-  static constexpr int kSfBufs = BN > 128 ? 2 : 4;
-  static constexpr int kOverlap = BN > 128 ? 96 : 0;
-  static constexpr int kAccCols = 2 * BN - kOverlap;
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 512;
+  // TMEM columns: two accumulators, then kSfBufs buffers of scales (kGroups * 4 of A, as many of B)
+  static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * 2;
+  static constexpr int kSfBufs = 4;
+  static constexpr int kAccCols = 2 * BN;
   static_assert(kAccCols + kSfBufs * kSfCols <= 512, "TMEM columns");
 };
 
@@ -365,10 +363,10 @@ struct LinWork {
   int s0, s1;    // stages [s0, s1) of it
   int64_t tile;
 
-  __device__ __forceinline__ explicit LinWork(const LinearParams& q) : p(q), tile(blockIdx.x / q.split) {
-    const int rank = blockIdx.x % p.split;
-    s0 = rank * p.n_steps / p.split;
-    s1 = (rank + 1) * p.n_steps / p.split;
+  __device__ __forceinline__ explicit LinWork(const LinearParams& q) : p(q), tile(blockIdx.x / (SWAP ? q.split : 2)) {
+    const int rank = SWAP ? blockIdx.x % p.split : 0, parts = SWAP ? p.split : 1;
+    s0 = rank * p.n_steps / parts;
+    s1 = (rank + 1) * p.n_steps / parts;
   }
   __device__ __forceinline__ bool next() {
     if (tile >= p.tiles_a * p.tiles_b) return false;
@@ -376,14 +374,14 @@ struct LinWork {
       a = tile % p.tiles_a;
       b = tile / p.tiles_a;
     } else {
-      // bands of 16 token tiles: the ~148 tiles in flight are about as many
+      // bands of 8 tiles of tokens: the ~74 tiles in flight are about as many
       // token rows as weight rows and share both through L2
-      const int64_t per = 16 * p.tiles_b, band = tile / per, r = tile % per;
-      const int64_t left = p.tiles_a - band * 16, rows = left < 16 ? left : 16;
+      const int64_t per = 8 * p.tiles_b, band = tile / per, r = tile % per;
+      const int64_t left = p.tiles_a - band * 8, rows = left < 8 ? left : 8;
       b = r / rows;
-      a = band * 16 + r % rows;
+      a = band * 8 + r % rows;
     }
-    tile += gridDim.x / p.split;
+    tile += gridDim.x / (SWAP ? p.split : 2);
     return true;
   }
 };
@@ -400,76 +398,102 @@ __device__ __forceinline__ float load_peer(uint32_t saddr, int rank) {
   return v;
 }
 
-// Where one tile's sums go: this thread's accumulator row, and what belongs to it.
-template <int BN, bool SWAP>
-struct LinOut {
+// Where a tile's sums go (few tokens): this thread's accumulator row is an output feature, columns are tokens.
+template <int BN>
+struct LinOutTokens {
   static constexpr int C = BN < 32 ? BN : 32;  // columns drained at a time
   const LinearParams& p;
-  int row, lane, cols;     // accumulator row; columns of the tile that exist
-  int64_t ra, ra0, cb;     // swapped: output feature, first token; wide: token, first output feature
+  int row, lane, cols;  // accumulator row; tokens of the tile that exist
+  int64_t ra, cb;       // output feature, first token
   bool in;
-  float mine;              // swapped: the bias of this feature; wide: the scale of this token
+  float bias;
 
-  __device__ __forceinline__ LinOut(const LinearParams& q, const LinWork<SWAP>& u) : p(q) {
+  __device__ __forceinline__ LinOutTokens(const LinearParams& q, const LinWork<true>& u) : p(q) {
+    lane = threadIdx.x & 31;
+    row = (threadIdx.x >> 5 & 3) * 32 + lane;
+    ra = u.a * 128 + row;
+    cb = u.b * BN;
+    cols = p.T - cb < BN ? (int)(p.T - cb) : BN;
+    in = ra < p.N;
+    bias = in && p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f;
+  }
+  // lane q: the scale of token c + q
+  __device__ __forceinline__ float column(int c) const {
+    return c + lane < cols && lane < C ? __ldg(p.row_scale + cb + c + lane) * p.w_scale : 0.0f;
+  }
+  __device__ __forceinline__ void store(int c, float v, float scale) const {
+    if (in) store_any(p.out, p.out_dtype, (cb + c) * p.ldo + ra, __fmaf_rn(v, scale, bias));
+  }
+  // C columns from c: scale, bias, round once, store.  The output type is asked for once: with a branch on it in every
+  // column their conversions and stores do not overlap.
+  template <int DT>
+  __device__ __forceinline__ void finish_as(int c, float (&v)[C], float col) const {
+    const int64_t at = (cb + c) * p.ldo + ra;
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      const float y = __fmaf_rn(v[q], __shfl_sync(0xffffffffu, col, q), bias);
+      if (in && c + q < cols) store_any(p.out, DT, at + q * p.ldo, y);
+    }
+  }
+  __device__ __forceinline__ void finish(int c, float (&v)[C], float col) const {
+    if (p.out_dtype == kDtBF16) finish_as<kDtBF16>(c, v, col);
+    else if (p.out_dtype == kDtF16) finish_as<kDtF16>(c, v, col);
+    else finish_as<kDtF32>(c, v, col);
+  }
+};
+
+// The same for a tile of a prompt: rows are tokens, columns are output features.
+struct LinOutRows {
+  static constexpr int BN = 256, C = 32;
+  const LinearParams& p;
+  int row, lane, cols;   // accumulator row; features of the tile that exist
+  int64_t ra, ra0, cb;   // token, first token, first feature
+  bool in;
+  float scale;           // of this token
+
+  __device__ __forceinline__ LinOutRows(const LinearParams& q, const LinWork<false>& u) : p(q) {
     lane = threadIdx.x & 31;
     row = (threadIdx.x >> 5 & 3) * 32 + lane;
     ra0 = u.a * 128;
     ra = ra0 + row;
     cb = u.b * BN;
-    const int64_t left = (SWAP ? p.T : p.N) - cb;
-    cols = left < BN ? (int)left : BN;
-    in = ra < (SWAP ? p.N : p.T);
-    mine = !in ? 0.0f : SWAP ? (p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f) : __ldg(p.row_scale + ra) * p.w_scale;
-  }
-  // lane q: the token scale (swapped) or the bias of column c + q
-  __device__ __forceinline__ float column(int c) const {
-    if (c + lane >= cols || lane >= C) return 0.0f;
-    if (SWAP) return __ldg(p.row_scale + cb + c + lane) * p.w_scale;
-    return p.bias ? load_any(p.bias, p.bias_dtype, cb + c + lane) : 0.0f;
-  }
-  // swapped: one column
-  __device__ __forceinline__ void store(int c, float v, float scale) const {
-    if (in) store_any(p.out, p.out_dtype, (cb + c) * p.ldo + ra, __fmaf_rn(v, scale, mine));
+    cols = p.N - cb < BN ? (int)(p.N - cb) : BN;
+    in = ra < p.T;
+    scale = in ? __ldg(p.row_scale + ra) * p.w_scale : 0.0f;
   }
   // C columns from c: scale, bias, round once, store
-  __device__ __forceinline__ void finish(int c, float (&v)[C], float col, const CUtensorMap& map_out, unsigned char* smem_out) const {
-    if constexpr (SWAP) {
+  __device__ __forceinline__ void finish(int c, float (&v)[C], const CUtensorMap& map_out, unsigned char* smem_out) const {
+    if (p.bias) {
+      const float b = c + lane < cols ? load_any(p.bias, p.bias_dtype, cb + c + lane) : 0.0f;
 #pragma unroll
-      for (int q = 0; q < C; ++q) {
-        const float scale = __shfl_sync(0xffffffffu, col, q);
-        if (c + q < cols) store(c + q, v[q], scale);
-      }
+      for (int q = 0; q < C; ++q) v[q] = __fmaf_rn(v[q], scale, __shfl_sync(0xffffffffu, b, q));
     } else {
-      if (p.bias) {
 #pragma unroll
-        for (int q = 0; q < C; ++q) v[q] = __fmaf_rn(v[q], mine, __shfl_sync(0xffffffffu, col, q));
-      } else {
+      for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], scale);
+    }
+    if (p.tma_out) {
+      if (ra0 + (row & ~31) >= p.T) return;
+      // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
+      unsigned char* stage = smem_out + (row >> 5) * 2048;
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
 #pragma unroll
-        for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], mine);
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+            make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
+                       pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
+                     "r"((int)cb + c), "r"((int)ra0 + (row & ~31)), "r"(smem_u32(stage))
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
-      if (p.tma_out) {
-        // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
-        unsigned char* stage = smem_out + (row >> 5) * 2048;
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
+    } else if (in) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
-              make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
-                         pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
-                       "r"((int)cb + c), "r"((int)ra0 + (row & ~31)), "r"(smem_u32(stage))
-                       : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-      } else if (in) {
-#pragma unroll
-        for (int q = 0; q < C; ++q)
-          if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
-      }
+      for (int q = 0; q < C; ++q)
+        if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
     }
   }
 };
@@ -479,15 +503,15 @@ constexpr int kLinThreads = 224;
 template <int BN, int BS>
 __global__ void __launch_bounds__(kLinThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LinearParams p) {
+                  const __grid_constant__ LinearParams p) {
+  // 224 threads: warp 0 feeds the ring, warp 6 copies a stage's scales to TMEM (tcgen05.cp), warp 1 issues its four
+  // block-scaled MMAs of K = 64, warps 2-5 drain the accumulator
   using G = LinGeo<BN, BS>;
-  constexpr bool SWAP = G::kSwap;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // operands (1024-byte swizzle atoms), output staging, the scales of all stages, barriers
-  unsigned char* smem_out = smem + G::kStages * (G::kABytes + G::kBBytes);
-  unsigned char* smem_sf = smem_out + G::kOutBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes + G::kOutBytes);
+  // operands (1024-byte swizzle atoms), the scales of all stages, barriers
+  unsigned char* smem_sf = smem + G::kStages * (G::kABytes + G::kBBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes);
   uint64_t* empty = full + G::kStages;
   uint64_t* tfull = empty + G::kStages;
   uint64_t* tempty = tfull + 2;
@@ -496,9 +520,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   uint64_t* sf_done = mma_done + 1;
   uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(sf_done + 1);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
-  constexpr int C = LinOut<BN, SWAP>::C;
+  constexpr int C = LinOutTokens<BN>::C;
   float* part = reinterpret_cast<float*>(smem);  // (BN, 128) fp32, over the ring's first stages
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
@@ -530,67 +554,54 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   };
 
   if (warp == 0) {
-    // ---------------- producer ----------------
-    if (lane == 0) {
-      auto load_w = [&](const LinWork<SWAP>& u, int ks, int s) {
-        unsigned char* sa = smem + s * (G::kABytes + G::kBBytes);
-        unsigned char* sf = smem_sf + s * G::kSf * (1 + G::kBTiles);
-        mbar_arrive_expect_tx(full + s, G::kStageBytes);
-        if (SWAP) {
-          tma_load_2d(sa, &map_a, ks * 128, (int)(u.a * 128), full + s);
-          bulk_load(sf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
-        } else {
-          tma_load_2d(sa + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
-#pragma unroll
-          for (int h = 0; h < G::kBTiles; ++h)
-            bulk_load(sf + (1 + h) * G::kSf, p.sf_b + ((u.b * G::kBTiles + h) * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+    // ---------------- producer (the warp stays converged: one elected lane issues) ----------------
+    auto load_w = [&](const LinWork<true>& u, int ks, int s) {
+      mbar_arrive_expect_tx(full + s, G::kStageBytes);
+      tma_load_2d(smem + s * (G::kABytes + G::kBBytes), &map_a, ks * 128, (int)(u.a * 128), full + s);
+      bulk_load(smem_sf + s * 2 * G::kSf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+    };
+    auto load_x = [&](const LinWork<true>& u, int ks, int s) {
+      tma_load_2d(smem + s * (G::kABytes + G::kBBytes) + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
+      bulk_load(smem_sf + (s * 2 + 1) * G::kSf, p.sf_b + (u.b * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+    };
+    // the first ring of weights does not wait for the quantization launch
+    uint32_t ahead = 0;
+    for (LinWork<true> u(p); ahead < (uint32_t)G::kStages && u.next();)
+      for (int ks = u.s0; ks < u.s1 && ahead < (uint32_t)G::kStages; ++ks, ++ahead) {
+        if (elect_one()) load_w(u, ks, ahead);
+        __syncwarp();
+      }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    uint32_t it = 0, s = 0, ph = 1;
+    bool ok = true;
+    for (LinWork<true> u(p); ok && u.next();) {
+      for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
+        if (it >= ahead) {
+          ok = __all_sync(0xffffffffu, wait(empty + s, ph, kDevErrLoadTimeout));
+          if (!ok) break;
         }
-      };
-      auto load_x = [&](const LinWork<SWAP>& u, int ks, int s) {
-        unsigned char* sa = smem + s * (G::kABytes + G::kBBytes);
-        unsigned char* sf = smem_sf + s * G::kSf * (1 + G::kBTiles);
-        if (SWAP) {
-          tma_load_2d(sa + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
-          bulk_load(sf + G::kSf, p.sf_b + (u.b * p.n_steps + ks) * G::kSf, G::kSf, full + s);
-        } else {
-          tma_load_2d(sa, &map_a, ks * 128, (int)(u.a * 128), full + s);
-          bulk_load(sf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
-        }
-      };
-      // the first ring of weights does not wait for the quantization launch
-      uint32_t ahead = 0;
-      for (LinWork<SWAP> u(p); ahead < (uint32_t)G::kStages && u.next();)
-        for (int ks = u.s0; ks < u.s1 && ahead < (uint32_t)G::kStages; ++ks, ++ahead) load_w(u, ks, ahead);
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      uint32_t it = 0;
-      for (LinWork<SWAP> u(p); u.next();) {
-        for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
-          const int s = it % G::kStages;
-          if (it >= ahead) {
-            if (!wait(empty + s, ((it / G::kStages) & 1) ^ 1, kDevErrLoadTimeout)) goto producer_done;
-            load_w(u, ks, s);
-          }
+        if (elect_one()) {
+          if (it >= ahead) load_w(u, ks, s);
           load_x(u, ks, s);
         }
+        __syncwarp();
+        if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
       }
-    producer_done:
-      // every load issued must have landed before the CTA can exit (bounded)
-      for (uint32_t k = it > (uint32_t)G::kStages ? it - G::kStages : 0u; k < it; ++k)
-        mbar_wait_bounded(full + (k % G::kStages), (k / G::kStages) & 1, kDevErrLoadTimeout);
     }
+    // every load issued must have landed before the CTA can exit (bounded)
+    for (uint32_t k = it > (uint32_t)G::kStages ? it - G::kStages : 0u; k < it; ++k)
+      mbar_wait_bounded(full + (k % G::kStages), (k / G::kStages) & 1, kDevErrLoadTimeout);
   } else if (warp == 1) {
     // ---------------- MMA issuer (the warp waits together, one lane issues) ----------------
     // low words of the descriptors of stage 0; a stage further is an addition
     const uint32_t lo_a = smem_u32(smem) >> 4, lo_b = lo_a + (G::kABytes >> 4);
     uint32_t lt = 0, s = 0, ph = 0, sb = 0, sph = 0;  // stage, scale buffer, their phases
-    for (LinWork<SWAP> u(p); u.next(); ++lt) {
+    for (LinWork<true> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1;
-      // narrow: this accumulator is drained; wide: the columns shared with the previous tile's are
-      bool ok = SWAP ? wait(tempty + acc, (lt >> 1 & 1) ^ 1, kDevErrMmaTimeout)
-                     : lt == 0 || wait(tempty, (lt - 1) & 1, kDevErrMmaTimeout);
+      bool ok = wait(tempty + acc, (lt >> 1 & 1) ^ 1, kDevErrMmaTimeout);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t d_tmem = tmem_base + acc * (BN - G::kOverlap);
+      const uint32_t d_tmem = tmem_base + acc * BN;
       for (int ks = u.s0; ks < u.s1; ++ks) {
         ok = wait(full + s, ph, kDevErrMmaTimeout) && wait(sf_full + sb, sph, kDevErrMmaTimeout);
         ok = __all_sync(0xffffffffu, ok);
@@ -604,7 +615,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           for (int kk = 0; kk < 4; ++kk) {
             const int q = BS == 16 ? kk : kk / 2;
             umma_fp4<BS>(d_tmem, da + 2 * kk, db + 2 * kk, idesc_fp4<BS>(BN, BS == 16 ? 0u : (kk & 1) * 2u), t_sfa + 4 * q,
-                         t_sfb + 4 * q * G::kBTiles, kk > 0 ? 1u : first);
+                         t_sfb + 4 * q, kk > 0 ? 1u : first);
           }
           umma_commit(empty + s);
           if (ks + 1 == u.s1) umma_commit(tfull + acc);
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     const uint32_t lo_sf = smem_u32(smem_sf) >> 4;
     uint32_t s = 0, ph = 0, sb = 0, warm = 0;  // warm: scale buffers used so far, up to kSfBufs
     bool ok = true;
-    for (LinWork<SWAP> u(p); ok && u.next();) {
+    for (LinWork<true> u(p); ok && u.next();) {
       for (int ks = u.s0; ks < u.s1; ++ks) {
         ok = wait(full + s, ph, kDevErrMmaTimeout);
         // this scale buffer was last read by the MMAs kSfBufs stages ago
@@ -638,15 +649,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ds = lo_sf + s * (G::kSf * (1 + G::kBTiles) >> 4);
+        const uint32_t ds = lo_sf + s * (2 * G::kSf >> 4);
         const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
         if (elect_one()) {
 #pragma unroll
           for (int q = 0; q < Fmt<BS>::kGroups; ++q) {
             tmem_cp_scales(t_sfa + 4 * q, ds + q * (kGroupBytes >> 4));
-#pragma unroll
-            for (int h = 0; h < G::kBTiles; ++h)
-              tmem_cp_scales(t_sfb + (q * G::kBTiles + h) * 4, ds + (((1 + h) * G::kSf + q * kGroupBytes) >> 4));
+            tmem_cp_scales(t_sfb + 4 * q, ds + ((G::kSf + q * kGroupBytes) >> 4));
           }
           umma_commit(sf_full + sb);
         }
@@ -664,73 +673,65 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     // ---------------- epilogue (warps 2-5) ----------------
     asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales are the quantization launch's
     uint32_t lt = 0;
-    for (LinWork<SWAP> u(p); u.next(); ++lt) {
+    for (LinWork<true> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
-      LinOut<BN, SWAP> out(p, u);
+      LinOutTokens<BN> out(p, u);
       if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * (BN - G::kOverlap);
-      // the order in which columns are drained: the wide form's shared ones (the
-      // last of accumulator 0, the first of accumulator 1) come first
-      const int c_first = !SWAP && acc == 0 ? BN - G::kOverlap : 0;
-      float col = out.column(c_first);
+      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * BN;
+      float col = out.column(0);
 #pragma unroll 1
-      for (int i = 0; i < BN / C; ++i) {
-        const int c = (c_first + i * C) % BN;
+      for (int c = 0; c < BN; c += C) {
         const float now = col;
         col = out.column((c + C) % BN);
         float v[C];
         if (c < out.cols) tmem_ld<C>(taddr + c, v);
-        if (SWAP ? i + 1 == BN / C : i + 1 == G::kOverlap / C) {
+        if (c + C == BN) {
           tc_fence_before();
-          mbar_arrive(SWAP ? tempty + acc : tempty);
+          mbar_arrive(tempty + acc);
         }
         if (c >= out.cols) continue;
-        if (SWAP && p.split > 1) {  // this CTA's part, to be added below (the ring is idle: all its MMAs are done)
+        if (p.split > 1) {  // this CTA's part, to be added below (the ring is idle: all its MMAs are done)
 #pragma unroll
           for (int q = 0; q < C; ++q) part[(c + q) * 128 + out.row] = v[q];
         } else {
-          out.finish(c, v, now, map_out, smem_out);
+          out.finish(c, v, now);
         }
       }
     }
-    // staged output has been written (the staging area goes away with the CTA)
-    if (!SWAP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
-  if constexpr (SWAP) {
-    if (p.split > 1) {
-      __syncwarp();
-      cluster_sync();
-      if (warp >= 2 && warp < 6) {
-        LinWork<SWAP> u(p);
-        if (u.next()) {
-          // rank r finishes columns [r, r + 1) * BN / split
-          LinOut<BN, SWAP> out(p, u);
-          const int rank = blockIdx.x % p.split, per = BN / p.split;
-          const float col = out.column(rank * per / C * C);
-          const uint32_t at = smem_u32(part) + out.row * 4;
-          const int c_end = (rank + 1) * per < out.cols ? (rank + 1) * per : out.cols;
-          for (int c0 = rank * per; c0 < c_end; c0 += 4) {
-            float x[4][8];  // all loads of four columns before the first sum
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2 && warp < 6) {
+      LinWork<true> u(p);
+      if (u.next()) {
+        // rank r finishes columns [r, r + 1) * BN / split
+        LinOutTokens<BN> out(p, u);
+        const int rank = blockIdx.x % p.split, per = BN / p.split;
+        const float col = out.column(rank * per / C * C);
+        const uint32_t at = smem_u32(part) + out.row * 4;
+        const int c_end = (rank + 1) * per < out.cols ? (rank + 1) * per : out.cols;
+        for (int c0 = rank * per; c0 < c_end; c0 += 4) {
+          float x[4][8];  // all loads of four columns before the first sum
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
+          for (int w = 0; w < 8; ++w)
 #pragma unroll
-              for (int q = 0; q < 4; ++q) x[q][w] = w < p.split && c0 + q < c_end ? load_peer(at + (c0 + q) * 512, w) : 0.0f;
+            for (int q = 0; q < 4; ++q) x[q][w] = w < p.split && c0 + q < c_end ? load_peer(at + (c0 + q) * 512, w) : 0.0f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v = x[q][0];
+          for (int q = 0; q < 4; ++q) {
+            float v = x[q][0];
 #pragma unroll
-              for (int w = 1; w < 8; ++w) v += x[q][w];
-              const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
-                                           : (c0 + q < c_end ? __ldg(p.row_scale + u.b * BN + c0 + q) * p.w_scale : 0.0f);
-              if (c0 + q < c_end) out.store(c0 + q, v, scale);
-            }
+            for (int w = 1; w < 8; ++w) v += x[q][w];
+            const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
+                                         : (c0 + q < c_end ? __ldg(p.row_scale + u.b * BN + c0 + q) * p.w_scale : 0.0f);
+            if (c0 + q < c_end) out.store(c0 + q, v, scale);
           }
         }
       }
-      __syncwarp();
-      cluster_sync();  // the parts have been read
     }
+    __syncwarp();
+    cluster_sync();  // the parts have been read
   }
   tc_fence_before();
   __syncthreads();
@@ -738,6 +739,357 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+}
+
+// ---------------------------------------------------------------------------
+// the product of a prompt: two CTAs on one tile
+// ---------------------------------------------------------------------------
+// 256 tokens x 256 output features by a cluster of two CTAs (cta_group::2): each
+// has 128 token rows of A, 128 of the tile's 256 rows of W, and the sums of its
+// own tokens; the tensor cores of both read both halves of B.  A stage is then
+// 38 KB per SM for 512 clocks of MMAs, where one CTA on 128 x 256 needs 55 KB: the
+// SMs take about 64 bytes per clock from L2, and that bounded a form of one CTA
+// per tile (945 clocks a stage, 829 us for 8192 x 8192 x 28672; this one 610).
+//
+// 320 threads: warp 0 feeds this CTA's ring; its tiles signal the leader (rank 0),
+// its scales this CTA.  Warps 6-9 put a stage's scales in this CTA's TMEM (its
+// tokens', and those of all 256 features) and tell the leader, whose warp 1 issues
+// the MMAs of the pair; commits free a stage and publish the sums in both CTAs;
+// warps 2-5 drain.  TMEM holds two accumulators that share 96 columns, so that two
+// buffers of scales fit beside them; the epilogue takes the shared columns into
+// registers first, and the next tile begins once it has (with 160 shared columns
+// and three buffers: 695 clocks a stage).  Everything another CTA reads or signals
+// lies between the cluster barriers at both ends.
+template <int BS>
+struct PairGeo {
+  static constexpr int BN = LinOutRows::BN;
+  static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
+  static constexpr int kSf = Fmt<BS>::kSfBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes + 3 * kSf;
+  static constexpr int kOutBytes = 4 * 2048;
+  static constexpr int kMaxStages = (232448 - 1024 - 512 - kOutBytes) / kStageBytes;
+  static constexpr int kStages = kMaxStages > 6 ? 6 : kMaxStages;
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024 + 512;
+  // TMEM columns: two accumulators that share kOverlap columns, then kSfBufs buffers of scales
+  static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * 3;
+  static constexpr int kOverlap = 96;
+  static constexpr int kAccCols = 2 * BN - kOverlap;
+  static constexpr int kSfBufs = (512 - kAccCols) / kSfCols;
+  static_assert(kSfBufs >= 2 && kStages > kSfBufs && kOverlap % LinOutRows::C == 0, "TMEM columns");
+};
+constexpr int kPairThreads = 320;
+
+template <int BS>
+__device__ __forceinline__ void umma_fp4_pair(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                              uint32_t accumulate) {
+  if constexpr (BS == 16)
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %7};\n mov.b64 y, {%2, %7};\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], x, y, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "r"(a | kDescRows), "r"(b | kDescRows), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "n"(kDescRowsHi)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %7};\n mov.b64 y, {%2, %7};\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "r"(a | kDescRows), "r"(b | kDescRows), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "n"(kDescRowsHi)
+        : "memory");
+}
+
+// Arrive on the barrier at this offset in both CTAs once the pair's MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b16 m;\n mov.b16 m, 3;\n"
+      " tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// Arrivals at the leader's barrier and waits for the pair's. They are relaxed: what they order is in TMEM (the
+// tcgen05 fences beside them do that) or was loaded into registers that have been used; the operands themselves signal
+// the leader's barrier directly. With release.cluster an arrival took about 1300 clocks, and every stage waits for one.
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b32 at;\n mapa.shared::cluster.u32 at, %0, 0;\n"
+      " mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [at];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// A tile into this CTA's memory that signals the leader's barrier at this offset.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b32 at;\n mapa.shared::cluster.u32 at, %4, 0;\n"
+      " cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[at];\n}\n" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// C columns of 32 bits from registers to TMEM, one row per lane.
+template <int C>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* r) {
+  if constexpr (C == 32)
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+        "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+  else if constexpr (C == 16)
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+  else
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+template <int BS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ LinearParams p) {
+  using G = PairGeo<BS>;
+  constexpr int BN = G::BN;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* smem_out = smem + G::kStages * (G::kABytes + G::kBBytes);
+  unsigned char* smem_sf = smem_out + G::kOutBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes + G::kOutBytes);  // the leader's: operands
+  uint64_t* sf_in = full + G::kStages;       // this CTA's scales of a stage are in shared memory
+  uint64_t* empty = sf_in + G::kStages;
+  uint64_t* tfull = empty + G::kStages;
+  uint64_t* tempty = tfull + 2;              // the leader's: both CTAs' shared columns are drained
+  uint64_t* sf_full = tempty + 1;            // the leader's: both CTAs' scales are in TMEM
+  uint64_t* mma_done = sf_full + G::kSfBufs;
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < G::kStages; ++s) { mbar_init(full + s, 1); mbar_init(sf_in + s, 1); mbar_init(empty + s, 1); }
+    for (int a = 0; a < 2; ++a) mbar_init(tfull + a, 1);
+    mbar_init(tempty, 2 * 128);
+    for (int b = 0; b < G::kSfBufs; ++b) mbar_init(sf_full + b, 2 * 4);
+    mbar_init(mma_done, 1);
+    *abort_s = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_base_s)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers and TMEM exist
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_s;
+
+  // data: the wait is for loads that this CTA's threads or the tensor core read from shared memory
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned err, bool data = false) -> bool {
+    if (data ? mbar_try_wait(bar, parity) : mbar_try_wait_cluster(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!(data ? mbar_try_wait(bar, parity) : mbar_try_wait_cluster(bar, parity))) {
+      if (*abort_s) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        atomicOr(&qz_device_error, err);
+        *abort_s = 1;
+        return false;
+      }
+    }
+    return true;
+  };
+
+  if (warp == 0) {
+    // ---------------- producer (the warp stays converged: one elected lane issues) ----------------
+    auto load_w = [&](const LinWork<false>& u, int ks, int s) {
+      unsigned char* sb = smem + s * (G::kABytes + G::kBBytes) + G::kABytes;
+      unsigned char* sf = smem_sf + s * 3 * G::kSf;
+      if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * (G::kABytes + G::kBBytes));
+      mbar_arrive_expect_tx(sf_in + s, 3 * G::kSf);
+      tma_load_2d_pair(sb, &map_b, ks * 128, (int)(u.b * BN) + rank * 128, full + s);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        bulk_load(sf + (1 + h) * G::kSf, p.sf_b + ((u.b * 2 + h) * p.n_steps + ks) * G::kSf, G::kSf, sf_in + s);
+    };
+    auto load_x = [&](const LinWork<false>& u, int ks, int s) {
+      const int64_t a = u.a * 2 + rank;
+      tma_load_2d_pair(smem + s * (G::kABytes + G::kBBytes), &map_a, ks * 128, (int)(a * 128), full + s);
+      bulk_load(smem_sf + s * 3 * G::kSf, p.sf_a + (a * p.n_steps + ks) * G::kSf, G::kSf, sf_in + s);
+    };
+    // the first ring of weights does not wait for the quantization launch
+    uint32_t ahead = 0;
+    for (LinWork<false> u(p); ahead < (uint32_t)G::kStages && u.next();)
+      for (int ks = u.s0; ks < u.s1 && ahead < (uint32_t)G::kStages; ++ks, ++ahead) {
+        if (elect_one()) load_w(u, ks, ahead);
+        __syncwarp();
+      }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    uint32_t it = 0, s = 0, ph = 1;
+    bool ok = true;
+    for (LinWork<false> u(p); ok && u.next();) {
+      for (int ks = u.s0; ks < u.s1; ++ks, ++it) {
+        if (it >= ahead) {
+          ok = __all_sync(0xffffffffu, wait(empty + s, ph, kDevErrLoadTimeout));
+          if (!ok) break;
+        }
+        if (elect_one()) {
+          if (it >= ahead) load_w(u, ks, s);
+          load_x(u, ks, s);
+        }
+        __syncwarp();
+        if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
+      }
+    }
+    // every load issued must have landed before the CTA can exit (bounded)
+    for (uint32_t k = it > (uint32_t)G::kStages ? it - G::kStages : 0u; k < it; ++k) {
+      mbar_wait_bounded(sf_in + (k % G::kStages), (k / G::kStages) & 1, kDevErrLoadTimeout);
+      if (rank == 0) mbar_wait_bounded(full + (k % G::kStages), (k / G::kStages) & 1, kDevErrLoadTimeout);
+    }
+    // after an abort the leader may not have waited for this CTA's last operands
+    if (rank == 1 && *abort_s)
+      for (int k = 0; k < 100; ++k) __nanosleep(1000);
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (the leader's) ----------------
+    if (rank == 0) {
+      const uint32_t lo_a = smem_u32(smem) >> 4, lo_b = lo_a + (G::kABytes >> 4);
+      uint32_t lt = 0, s = 0, ph = 0, sb = 0, sph = 0;
+      for (LinWork<false> u(p); u.next(); ++lt) {
+        const uint32_t acc = lt & 1;
+        bool ok = lt == 0 || wait(tempty, (lt - 1) & 1, kDevErrMmaTimeout);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * (BN - G::kOverlap);
+        for (int ks = u.s0; ks < u.s1; ++ks) {
+          ok = wait(full + s, ph, kDevErrMmaTimeout, true);
+          ok = __all_sync(0xffffffffu, ok && wait(sf_full + sb, sph, kDevErrMmaTimeout));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t da = lo_a + s * ((G::kABytes + G::kBBytes) >> 4), db = lo_b + s * ((G::kABytes + G::kBBytes) >> 4);
+          const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
+          const uint32_t first = ks > u.s0 ? 1u : 0u;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const int q = BS == 16 ? kk : kk / 2;
+              // M = 256: the descriptor's field counts 16 rows, as for 128
+              constexpr uint32_t m256 = (uint32_t)(256 >> 4) << 24, m128 = (uint32_t)(128 >> 4) << 24;
+              umma_fp4_pair<BS>(d_tmem, da + 2 * kk, db + 2 * kk, idesc_fp4<BS>(BN, BS == 16 ? 0u : (kk & 1) * 2u) - m128 + m256,
+                                t_sfa + 4 * q, t_sfb + 8 * q, kk > 0 ? 1u : first);
+            }
+            umma_commit_pair(empty + s);
+            if (ks + 1 == u.s1) umma_commit_pair(tfull + acc);
+          }
+          __syncwarp();
+          if (++sb == (uint32_t)G::kSfBufs) { sb = 0; sph ^= 1; }
+          if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+      }
+      // the MMAs issued must retire before either CTA's TMEM is freed (also after an abort)
+      __syncwarp();
+      if (elect_one()) umma_commit_pair(mma_done);
+      __syncwarp();
+      mbar_wait_bounded(mma_done, 0u, kDevErrMmaTimeout);
+    }
+  } else if (warp >= 6) {
+    // ---------------- scales to TMEM (warps 6-9, one quarter of the lanes each) ----------------
+    const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t s = 0, ph = 0, sb = 0, warm = 0;  // warm: scale buffers used so far, up to kSfBufs
+    bool ok = true;
+    for (LinWork<false> u(p); ok && u.next();) {
+      for (int ks = u.s0; ks < u.s1; ++ks) {
+        ok = wait(sf_in + s, ph, kDevErrMmaTimeout, true);
+        uint32_t r[G::kSfCols];
+        const unsigned char* sf = smem_sf + s * 3 * G::kSf + lane * 16;
+#pragma unroll
+        for (int q = 0; q < Fmt<BS>::kGroups; ++q) {
+          *reinterpret_cast<uint4*>(r + 4 * q) = *reinterpret_cast<const uint4*>(sf + q * kGroupBytes);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<uint4*>(r + (Fmt<BS>::kGroups + 2 * q + h) * 4) =
+                *reinterpret_cast<const uint4*>(sf + (1 + h) * G::kSf + q * kGroupBytes);
+        }
+        // this scale buffer was last read by the MMAs kSfBufs stages ago
+        if (warm == (uint32_t)G::kSfBufs) {
+          const bool wrap = s < (uint32_t)G::kSfBufs;
+          ok = ok && wait(empty + (wrap ? s + G::kStages - G::kSfBufs : s - G::kSfBufs), wrap ? ph ^ 1 : ph, kDevErrMmaTimeout);
+        } else {
+          ++warm;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t t_sf = tmem_base + quarter + G::kAccCols + sb * G::kSfCols;
+        constexpr int kLow = G::kSfCols == 48 ? 32 : 16;
+        tmem_st<kLow>(t_sf, r);
+        tmem_st<G::kSfCols - kLow>(t_sf + kLow, r + kLow);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(sf_full + sb);
+        if (++sb == (uint32_t)G::kSfBufs) sb = 0;
+        if (++s == (uint32_t)G::kStages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else {
+    // ---------------- epilogue (warps 2-5) ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales are the quantization launch's
+    constexpr int C = LinOutRows::C, kShared = G::kOverlap / C;
+    uint32_t lt = 0;
+    for (LinWork<false> u(p); u.next(); ++lt) {
+      const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
+      u.a = u.a * 2 + rank;  // this CTA's 128 rows
+      LinOutRows out(p, u);
+      if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * (BN - G::kOverlap);
+      // the columns shared with the next tile's accumulator come first
+      const int c_first = acc == 0 ? BN - G::kOverlap : 0;
+      float v[kShared][C];
+#pragma unroll
+      for (int i = 0; i < kShared; ++i)
+        if (c_first + i * C < out.cols) tmem_ld<C>(taddr + c_first + i * C, v[i]);
+      tc_fence_before();
+      mbar_arrive_leader(tempty);
+#pragma unroll
+      for (int i = 0; i < kShared; ++i) {
+        const int c = c_first + i * C;
+        if (c < out.cols) out.finish(c, v[i], map_out, smem_out);
+      }
+#pragma unroll 1
+      for (int i = kShared; i < BN / C; ++i) {
+        const int c = (c_first + i * C) % BN;
+        if (c >= out.cols) continue;
+        tmem_ld<C>(taddr + c, v[0]);
+        out.finish(c, v[0], map_out, smem_out);
+      }
+    }
+    // staged output has been written (the staging area goes away with the CTA)
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA's memory is read or signalled any more
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+  }
+  __syncwarp();
+  cluster_sync();  // both CTAs take part in freeing the pair's TMEM
 }
 
 // ---------------------------------------------------------------------------
@@ -782,42 +1134,53 @@ static int out_map(CUtensorMap* m, void* base, uint64_t N, uint64_t T, uint64_t 
 // Tile form and cluster size of one call, and its workspace.
 struct LinPlan {
   int bn, split, n_steps;
+  int gran;  // rows of a tile of x's scales
   int64_t tiles_a, tiles_b, ldp;
   int64_t off_sf, off_scale, bytes;
 };
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Chooses the form by an estimate in SM clocks: a stage costs its MMAs (2.1 clocks
-// per column) or its bytes (64 per clock and SM from L2), a tile its epilogue,
-// a cluster its exchange.
+// Chooses the form by an estimate in microseconds: waves of tiles x stages x time
+// of a stage, what follows the last stage, and a cluster's exchange of sums.
+// The times were fitted to measurements of every form at 1 .. 2048 tokens and
+// (K, N) = (1024, 1024), (2560, 9728), (9728, 2560), (4096, 4096) and
+// (8192, 28672); the choice is the fastest or within 10% of it in all.  Some, in
+// microseconds with the quantization: 2560 x 9728, 64 tokens: 64 columns 13.4, 32
+// (two waves) 14.7, pair 14.5; 128 tokens: 16.8, 18.6, pair 14.8; 2048 tokens: 128
+// columns 84.4, pair 36.2.  9728 x 2560, 1 token: clusters of 4, 2, 1: 12.7, 14.8,
+// 18.9; 64 tokens: 64 columns and clusters of 4 16.8, 16 columns alone 20.9.
+// 128 columns were never the fastest by more than 8% and are not built.
+struct LinForm {
+  int bn;               // tokens of a tile (256: the pair form)
+  double stage, last, join;
+};
+constexpr LinForm kForms[] = {{16, 0.27, 0.0, 1.0}, {32, 0.32, 0.0, 1.8}, {64, 0.40, 1.2, 2.4}, {256, 0.36, 4.0, 0.0}};
+
 static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   LinPlan best{};
   double best_cost = -1.0;
   const int n_steps = (int)((K + kStepK - 1) / kStepK);
-  for (int bn : {16, 32, 64, 128, 256}) {
-    if (bn < 128 && T > 4 * bn) continue;
-    const bool swap = bn < 256;
-    const int64_t ta = swap ? (N + 127) / 128 : (T + 127) / 128;
-    const int64_t tb = swap ? (T + bn - 1) / bn : (N + 255) / 256;
-    const double bytes = 128.0 * 128 + 128.0 * bn + 128.0 * 256 / bs * (1 + (bn > 128 ? 2 : 1));
-    double step = bytes / 60.0 > 2.1 * bn ? bytes / 60.0 : 2.1 * bn;
-    if (step < 400.0) step = 400.0;  // the waits and issues of one stage
+  for (const LinForm& f : kForms) {
+    const bool pair = f.bn == 256;
+    if (!pair && T > 8 * f.bn) continue;  // W would pass through L2 more than eight times
+    const int64_t ta = pair ? (T + 255) / 256 : (N + 127) / 128;
+    const int64_t tb = pair ? (N + 255) / 256 : (T + f.bn - 1) / f.bn;
+    const int64_t slots = pair ? sms / 2 : sms;
     for (int split : {1, 2, 4, 8}) {
-      if (split > 1 && (!swap || split > n_steps || ta * tb * split > sms)) break;
-      const double waves = (double)((ta * tb * split + sms - 1) / sms);
-      const double cost = waves * ((n_steps + split - 1) / split * step) + (swap ? waves : 1.0) * (500.0 + 10.0 * bn) +
-                          (split > 1 ? 1000.0 + 4.0 * bn : 0.0);
+      if (split > 1 && (pair || split > n_steps || ta * tb * split > sms)) break;
+      const double waves = (double)((ta * tb * split + slots - 1) / slots);
+      const double cost = waves * ((n_steps + split - 1) / split) * f.stage + f.last + (split > 1 ? f.join : 0.0);
       if (best_cost < 0 || cost < best_cost) {
         best_cost = cost;
-        best.bn = bn; best.split = split; best.tiles_a = ta; best.tiles_b = tb;
+        best.bn = f.bn; best.split = split; best.tiles_a = ta; best.tiles_b = tb;
       }
     }
   }
   best.n_steps = n_steps;
   best.ldp = up(K, 32) / 2;
-  const int gran = best.bn < 128 ? best.bn : 128;
-  const int64_t sf_tiles = (T + gran - 1) / gran;
+  best.gran = best.bn < 128 ? best.bn : 128;
+  const int64_t sf_tiles = best.bn == 256 ? best.tiles_a * 2 : best.tiles_b;
   best.off_sf = up(T * best.ldp, 256);
   best.off_scale = best.off_sf + up(sf_tiles * n_steps * (int64_t)(kStepK / bs / 4 * kGroupBytes), 256);
   best.bytes = best.off_scale + up(T * 4, 256);
@@ -853,8 +1216,7 @@ static cudaError_t launch_quantize_rows(const QuantizeRows& q, cudaStream_t st) 
 }
 
 template <int BN, int BS>
-static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
-                         cudaStream_t st) {
+static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p, int sms, cudaStream_t st) {
   using G = LinGeo<BN, BS>;
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
@@ -878,18 +1240,44 @@ static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const CUten
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS>, a, b, o, p), "linear launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS>, a, b, p), "linear launch");
+}
+
+template <int BS>
+static int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
+                       cudaStream_t st) {
+  using G = PairGeo<BS>;
+  static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(linear_pair_kernel<BS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  const int64_t pairs = p.tiles_a * p.tiles_b;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * (pairs < sms / 2 ? pairs : sms / 2)));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, linear_pair_kernel<BS>, a, b, o, p), "linear launch");
 }
 
 template <int BS>
 static int run_linear(int bn, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
                       cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_linear<16, BS>(a, b, o, p, sms, st);
-    case 32: return launch_linear<32, BS>(a, b, o, p, sms, st);
-    case 64: return launch_linear<64, BS>(a, b, o, p, sms, st);
-    case 128: return launch_linear<128, BS>(a, b, o, p, sms, st);
-    default: return launch_linear<256, BS>(a, b, o, p, sms, st);
+    case 16: return launch_linear<16, BS>(a, b, p, sms, st);
+    case 32: return launch_linear<32, BS>(a, b, p, sms, st);
+    case 64: return launch_linear<64, BS>(a, b, p, sms, st);
+    default: return launch_pair<BS>(a, b, o, p, sms, st);
   }
 }
 
@@ -968,7 +1356,7 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   const bool swap = pl.bn < 256;
   CUtensorMap mx, mw;
   s = code_map(&mx, ws, (uint64_t)pl.ldp, (uint64_t)T, (uint64_t)pl.ldp, swap ? pl.bn : 128);
-  if (s == QZ_OK) s = code_map(&mw, packed, (uint64_t)pl.ldp, (uint64_t)N, (uint64_t)ldp, swap ? 128 : 256);
+  if (s == QZ_OK) s = code_map(&mw, packed, (uint64_t)pl.ldp, (uint64_t)N, (uint64_t)ldp, 128);
   if (s != QZ_OK) return s;
   LinearParams p{};
   p.T = T; p.N = N;
@@ -984,9 +1372,9 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   p.tma_out = !swap && out_dtype != QZ_DTYPE_F32 && ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   CUtensorMap mo = mx;
   if (p.tma_out && (s = out_map(&mo, out, (uint64_t)N, (uint64_t)T, (uint64_t)ldo)) != QZ_OK) return s;
-  const QuantizeRows q{x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, pl.bn < 128 ? pl.bn : 128, pl.n_steps,
+  const QuantizeRows q{x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, pl.gran, pl.n_steps,
                        reinterpret_cast<float*>(ws + pl.off_scale)};
-  const bool few = T < 4 * sms;
+  const bool few = T < 2 * sms;
   s = cuda_status(bs == 16 ? (few ? launch_quantize_rows<16, 1>(q, st) : launch_quantize_rows<16, 4>(q, st))
                            : (few ? launch_quantize_rows<32, 1>(q, st) : launch_quantize_rows<32, 2>(q, st)),
                   "quantize rows launch");
