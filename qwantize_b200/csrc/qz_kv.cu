@@ -88,48 +88,54 @@ struct AppendParams {
   int64_t max_new;
 };
 
-// Codes of y = x / s, the quotient correctly rounded, four to a word.  The product
-// with r = 1 / s is within three units of the last place of it, so the code
-// can differ only where y lies that close to a tie of its rounding: `near` is set
-// there, and the caller divides.
-template <int KV>
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float r, bool& near) {
+// Codes of y = x / s, the quotient correctly rounded, four to a word.  lo and hi
+// are the reciprocal of s, 2^-21 down and up: their products enclose the quotient
+// (each of reciprocal, its scaling and product is off by 2^-24 at most), and
+// rounding is monotonic, so where both give the same code it is the quotient's.
+// `near` is set where they do not, and the caller divides.
+struct Reciprocal {
+  float2 lo, hi;
+};
+__device__ __forceinline__ Reciprocal reciprocal(float s) {
+  const float r = __frcp_rn(s), a = __fmul_rn(r, 1.0f - 0x1p-21f), b = __fmul_rn(r, 1.0f + 0x1p-21f);
+  return {make_float2(a, a), make_float2(b, b)};
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) {
   uint32_t w;
-  if constexpr (KV == kKvInt8) {
-    const float magic = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the rounded product
-    uint32_t t[4];
-    float far = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = __fmaf_rn(x[i], r, magic);
-      t[i] = __float_as_uint(v);
-      far = fmaxf(far, fabsf(__fmaf_rn(x[i], r, -(v - magic))));
-    }
-    near |= far >= 0.5f - 0x1p-14f;
-    w = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
-  } else {
-    uint16_t lo, hi;
-    float y[4], least = 1.0f;
-    uint32_t tie = 0xffffffffu;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // ties: the middle of the 20 dropped bits
-      y[i] = __fmul_rn(x[i], r);
-      tie = min(tie, (__float_as_uint(y[i]) - 0x7fff8u) & 0xfffffu);
-      least = fminf(least, fabsf(y[i]));
-    }
-    near |= tie <= 16u;
-    if (least < 0.015625f) {  // below 2^-6: odd multiples of 2^-10
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float t = __fmul_rn(y[i], 512.0f);
-        near |= fabsf(t) < 8.0f && fabsf(t - (__fadd_rn(t, 12582912.0f) - 12582912.0f)) >= 0.5f - 0x1p-12f;
-      }
-    }
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
-    w = (uint32_t)lo | (uint32_t)hi << 16;
-  }
+  asm("{\n .reg .b16 x, y;\n cvt.rn.satfinite.e4m3x2.f32 x, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 y, %4, %3;\n mov.b32 %0, {x, y};\n}\n"
+      : "=r"(w)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return w;
+}
+template <int KV>
+__device__ __forceinline__ uint32_t encode4(float2 a, float2 b, const Reciprocal& r, bool& near) {
+  if constexpr (KV == kKvInt8) {
+    const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low byte is the rounded product
+    const float2 l0 = fma2(a, r.lo, magic), l1 = fma2(b, r.lo, magic), h0 = fma2(a, r.hi, magic), h1 = fma2(b, r.hi, magic);
+    near |= ((__float_as_uint(l0.x) ^ __float_as_uint(h0.x)) | (__float_as_uint(l0.y) ^ __float_as_uint(h0.y)) |
+             (__float_as_uint(l1.x) ^ __float_as_uint(h1.x)) | (__float_as_uint(l1.y) ^ __float_as_uint(h1.y))) != 0;
+    return __byte_perm(__byte_perm(__float_as_uint(h0.x), __float_as_uint(h0.y), 0x0040),
+                       __byte_perm(__float_as_uint(h1.x), __float_as_uint(h1.y), 0x0040), 0x5410);
+  } else {
+    const uint32_t w = e4m3x4(mul2(a, r.hi), mul2(b, r.hi));
+    near |= w != e4m3x4(mul2(a, r.lo), mul2(b, r.lo));
+    return w;
+  }
 }
 template <int KV>
 __device__ __noinline__ uint32_t encode4_div(float a, float b, float c, float d, float s) {
@@ -142,8 +148,12 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {
   const uint32_t h = i ? w >> 16 : w & 0xffffu;
   return DT == kDtBF16 ? bf16_bits_to_float(h) : f16_bits_to_float(h);
 }
-// The larger magnitude of two 16-bit values, as 16 bits that order like it.
-__device__ __forceinline__ uint32_t abs_max16(uint32_t w) { return max(w >> 16 & 0x7fffu, w & 0x7fffu); }
+// The larger magnitudes of two pairs of 16-bit values, as 16 bits that order like them (NaN above all).
+__device__ __forceinline__ uint32_t abs_max16(uint32_t m, uint32_t w) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(w & 0x7fff7fffu));
+  return r;
+}
 
 // One CTA per (page a sequence touches, head, keys or values, sequence).  All
 // it reads -- the new values, the page's block and scale -- is asked for at once and
@@ -203,9 +213,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     have[i] = off > 0 ? *reinterpret_cast<const uint4*>(block + (tid + i * 256) * 16) : make_uint4(0, 0, 0, 0);
   const float before = off > 0 ? *scale_p : 0.0f;
 #pragma unroll
-  for (int i = 0; i < kNew; ++i)
-    m = max(max(m, max(abs_max16(raw[i].x), abs_max16(raw[i].y))), max(abs_max16(raw[i].z), abs_max16(raw[i].w)));
-  m = __reduce_max_sync(0xffffffffu, m);
+  for (int i = 0; i < kNew; ++i) m = abs_max16(abs_max16(abs_max16(abs_max16(m, raw[i].x), raw[i].y), raw[i].z), raw[i].w);
+  m = __reduce_max_sync(0xffffffffu, max(m >> 16, m & 0xffffu));
   if ((tid & 31) == 0) s_max[tid >> 5] = m;
   __syncthreads();
   m = 0;
@@ -218,45 +227,50 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
   const bool fine = m < 0x7f800000u && before <= 3.0e38f;
   if (!fine) s = __uint_as_float(0x7fc00000u);
   const float ratio = s > 0.0f ? __fdiv_rn(before, s) : 0.0f;
-  // older tokens (slots below off), zeros elsewhere
+  // older tokens (slots below off), zeros elsewhere; a page that new tokens fill has neither
+  const bool whole = off == 0 && fill == kPage && fine && s > 0.0f;
+  if (!whole) {
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int v = (tid + i * 256) * 16, kt = key_token(v, D);
-    uint32_t ww[4] = {have[i].x, have[i].y, have[i].z, have[i].w};
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = (tid + i * 256) * 16, kt = key_token(v, D);
+      uint32_t ww[4] = {have[i].x, have[i].y, have[i].z, have[i].w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      // bytes of slots below off
-      const int left = which ? off - (v % 64 + 4 * q) : (kt < off ? 4 : 0);
-      ww[q] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-      if (!fine) ww[q] = 0;
-      if (ratio != 1.0f && ww[q]) {
-        uint32_t r = 0;
+      for (int q = 0; q < 4; ++q) {
+        // bytes of slots below off
+        const int left = which ? off - (v % 64 + 4 * q) : (kt < off ? 4 : 0);
+        ww[q] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        if (!fine) ww[q] = 0;
+        if (ratio != 1.0f && ww[q]) {
+          uint32_t r = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) r |= encode8<KV>(__fmul_rn(decode8<KV>(ww[q] >> (8 * c) & 255u), ratio)) << (8 * c);
-        ww[q] = r;
+          for (int c = 0; c < 4; ++c) r |= encode8<KV>(__fmul_rn(decode8<KV>(ww[q] >> (8 * c) & 255u), ratio)) << (8 * c);
+          ww[q] = r;
+        }
+        *reinterpret_cast<uint32_t*>(s_block + (which ? v / 64 * kStride + v % 64 : v) + 4 * q) = ww[q];
       }
-      *reinterpret_cast<uint32_t*>(s_block + (which ? v / 64 * kStride + v % 64 : v) + 4 * q) = ww[q];
     }
+    __syncthreads();
   }
-  __syncthreads();
   if (fine && s > 0.0f) {
-    const float r = __frcp_rn(s);
+    const Reciprocal r = reciprocal(s);
     const bool slow = s < 0x1p-100f;  // the reciprocal or its products may leave fp32's normal range
 #pragma unroll
     for (int i = 0; i < kNew; ++i) {
       const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
       const int n = which ? (tid + i * 256) / (D / 2) * 4 : (tid + i * 256) / (D / 8);
       if (which ? n + 3 < off || n >= fill : n < off || n >= fill) continue;
-      float f[2][4];  // keys: values 0-3, 4-7; values: row d, row d + 1
+      float2 f[2][2];  // keys: values 0-3, 4-7; values: row d, row d + 1
       bool near = slow;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) f[h][c] = which ? half_of<DT>(w[c], h) : half_of<DT>(w[2 * h + c / 2], c & 1);
-      uint32_t code[2] = {encode4<KV>(f[0], r, near), encode4<KV>(f[1], r, near)};
+        for (int c = 0; c < 2; ++c)
+          f[h][c] = which ? make_float2(half_of<DT>(w[2 * c], h), half_of<DT>(w[2 * c + 1], h))
+                          : make_float2(half_of<DT>(w[2 * h + c], 0), half_of<DT>(w[2 * h + c], 1));
+      uint32_t code[2] = {encode4<KV>(f[0][0], f[0][1], r, near), encode4<KV>(f[1][0], f[1][1], r, near)};
       if (near) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) code[h] = encode4_div<KV>(f[h][0], f[h][1], f[h][2], f[h][3], s);
+        for (int h = 0; h < 2; ++h) code[h] = encode4_div<KV>(f[h][0].x, f[h][0].y, f[h][1].x, f[h][1].y, s);
       }
       if (which == 0) {
         *reinterpret_cast<uint2*>(s_block + key_at(n, (tid + i * 256) % (D / 8) * 8, D)) = make_uint2(code[0], code[1]);
@@ -264,7 +278,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
         // slots without a new token have code 0 here, and their old code in the block
         const int d = (tid + i * 256) % (D / 2) * 2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t*>(s_block + (d + h) * kStride + n) |= code[h];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t* to = reinterpret_cast<uint32_t*>(s_block + (d + h) * kStride + n);
+          *to = whole ? code[h] : *to | code[h];
+        }
       }
     }
   }
