@@ -53,6 +53,7 @@
 #include "qz_common.cuh"
 #include "qz_kernels.h"
 #include "qz_ptx.cuh"
+#include "qz_tc.cuh"
 
 namespace qz {
 
@@ -393,11 +394,10 @@ struct MoeShared {
 // All CTAs arrive, then wait for each other (they are all resident: cooperative
 // launch).  Bounded: on timeout the error flag is set and the kernel ends.
 __device__ __forceinline__ bool grid_barrier(int* counter, MoeShared& s) {
-  __threadfence();
-  __syncthreads();
+  __syncthreads();  // one thread's release and acquire stand for the CTA's
   if (threadIdx.x == 0) {
     int ok = 1;
-    atomicAdd(counter, 1);
+    asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(counter) : "memory");
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
       int v;
@@ -412,7 +412,6 @@ __device__ __forceinline__ bool grid_barrier(int* counter, MoeShared& s) {
     s.ok = ok;
   }
   __syncthreads();
-  __threadfence();
   return s.ok != 0;
 }
 
@@ -427,6 +426,18 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     s.weight[i] = __ldg(p.choice_weight + i);
   }
   __syncthreads();
+  // asked for here, used at the end
+  constexpr int kPer = kMoeMaxSlots / kMoeThreads;
+  int2 xp[kPer];
+  float2 norm[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int i = k * kMoeThreads + threadIdx.x;
+    if (i < n) {
+      xp[k] = __ldg(p.xp + i / p.top);
+      norm[k] = __ldg(reinterpret_cast<const float2*>(p.norms) + s.id[i]);
+    }
+  }
   // a warp numbers the slots of every kMoeWarps-th expert in ascending order
   {
     uint16_t ids[kMoeMaxSlots / 32];
@@ -452,12 +463,15 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int c = e0 + lane < p.E ? s.count[e0 + lane] : 0, m = (c + kMoeGroup - 1) / kMoeGroup;
       const int z = m == 0 ? 0 : (m - 1) * unit_cost(kMoeGroup) + unit_cost(c - (m - 1) * kMoeGroup);
-      int a = c, b = m, d = z;  // inclusive prefix sums
+      // inclusive prefix sums of the three in one word: slots <= 1024, groups <= 128, cost <= 640
+      static_assert(kMoeMaxSlots <= 1024 && kMoeMaxTokens <= 4 * kMoeGroup, "fields of the word");
+      unsigned sums = (unsigned)c | (unsigned)m << 11 | (unsigned)z << 20;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o), v = __shfl_up_sync(0xffffffffu, d, o);
-        if (lane >= o) { a += x; b += y; d += v; }
+        const unsigned x = __shfl_up_sync(0xffffffffu, sums, o);
+        if (lane >= o) sums += x;
       }
+      const int a = sums & 2047, b = sums >> 11 & 511, d = sums >> 20;
       if (e0 + lane < p.E) s.start[e0 + lane] = (uint16_t)(at + a - c);
       for (int k = 0; k < m; ++k) {
         const int g = groups + b - m + k;
@@ -466,9 +480,10 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
         s.g_count[g] = (uint16_t)(c - k * kMoeGroup < kMoeGroup ? c - k * kMoeGroup : kMoeGroup);
         s.g_cost[g] = (uint16_t)(cost + d - z + k * unit_cost(kMoeGroup));
       }
-      at += __shfl_sync(0xffffffffu, a, 31);
-      groups += __shfl_sync(0xffffffffu, b, 31);
-      cost += __shfl_sync(0xffffffffu, d, 31);
+      sums = __shfl_sync(0xffffffffu, sums, 31);
+      at += sums & 2047;
+      groups += sums >> 11 & 511;
+      cost += sums >> 20;
     }
     if (lane == 0) {
       s.n_groups = groups;
@@ -489,14 +504,14 @@ __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kMoeThreads) {
-    const int e = s.id[i];
-    s.list[s.start[e] + s.rank[i]] = (uint16_t)i;
-    const int2 xp = __ldg(p.xp + i / p.top);
-    const float2 norm = __ldg(reinterpret_cast<const float2*>(p.norms) + e);
-    const int bound = xp.y + 2 * xp.x + exponent_bound(norm.x) + exponent_bound(norm.y) + 2 * exponent_bound(fabsf(p.up_scale)) - 15;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int i = k * kMoeThreads + threadIdx.x;
+    if (i >= n) break;
+    s.list[s.start[s.id[i]] + s.rank[i]] = (uint16_t)i;
+    const int bound = xp[k].y + 2 * xp[k].x + exponent_bound(norm[k].x) + exponent_bound(norm[k].y) + 2 * exponent_bound(fabsf(p.up_scale)) - 15;
     s.act_exp[i] = (int16_t)min(max(bound, -140), 113);  // an fp32 activation is below 2^128; below 2^-125 nothing is left
-    if (i % p.top == 0) s.x_scale[i / p.top] = pow2f(xp.x) * p.up_scale;
+    if (i % p.top == 0) s.x_scale[i / p.top] = pow2f(xp[k].x) * p.up_scale;
   }
   __syncthreads();
 }
@@ -695,7 +710,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
   auto locate = [&]() {
     if (!ahead.done()) at_unit = ((int64_t)s.g_expert[ahead.group] * units + ahead.unit) * chunks;
   };
-  auto issue = [&](uint32_t i) {  // lane 0: the piece at `ahead` into stage i % kMoeStages
+  auto issue = [&](uint32_t i) {  // one lane: the piece at `ahead` into stage i % kMoeStages
     const int st = i % kMoeStages, n = ahead.piece();
     const int64_t chunk = at_unit + ahead.c;
     mbar_arrive_expect_tx(full + st, n * (R::kCodes + R::kScales));
@@ -705,7 +720,8 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
   locate();
   uint32_t issued = it;
   for (int k = 0; k < kMoeStages && !ahead.done(); ++k, ++issued) {
-    if (lane == 0) issue(issued);
+    if (elect_one()) issue(issued);
+    __syncwarp();
     if (ahead.advance()) locate();
   }
   bool ok = true;
@@ -739,34 +755,32 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
           b[q][n][4] = hi.x; b[q][n][5] = hi.y; b[q][n][6] = hi.z; b[q][n][7] = hi.w;
         }
     };
-    constexpr bool kAhead = NT * PARTS <= 2;  // one chunk ahead of its product while registers allow
-    uint32_t b0[PARTS][NT][8], b1[PARTS][NT][8];
-    if (kAhead) load_b(b0, w.c);
+    // the B words are asked for kAhead chunks before their product, as far as registers allow (0: at once)
+    constexpr int kAhead = NT * PARTS == 1 ? 2 : NT * PARTS == 2 ? 1 : 0, kBuffers = kAhead ? kAhead : 1;
+    static_assert(kMoePiece % kBuffers == 0, "a piece begins with the first buffer");
+    uint32_t b[kBuffers][PARTS][NT][8];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+      if (w.c + d < w.c1) load_b(b[d], w.c + d);
     bool more = true;
     while (more) {
       const int st = it % kMoeStages, pieces = w.piece();
       if (!mbar_wait_bounded(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
       const uint8_t* at = mine + st * R::kStage;
 #pragma unroll 1
-      for (int k = 0; k < pieces; k += 2) {
-        const uint8_t *codes0 = at + k * R::kCodes, *scales0 = at + kMoePiece * R::kCodes + k * R::kScales;
-        if constexpr (kAhead) {
-          if (k + 1 < pieces) load_b(b1, w.c + k + 1);
-          chunk_product<NT, BS, PARTS>(codes0, scales0, b0, acc);
-          if (w.c + k + 2 < w.c1) load_b(b0, w.c + k + 2);
-          if (k + 1 < pieces) chunk_product<NT, BS, PARTS>(codes0 + R::kCodes, scales0 + R::kScales, b1, acc);
-        } else {
-          load_b(b0, w.c + k);
-          chunk_product<NT, BS, PARTS>(codes0, scales0, b0, acc);
-          if (k + 1 < pieces) {
-            load_b(b0, w.c + k + 1);
-            chunk_product<NT, BS, PARTS>(codes0 + R::kCodes, scales0 + R::kScales, b0, acc);
-          }
+      for (int k = 0; k < pieces; k += kBuffers) {
+#pragma unroll
+        for (int d = 0; d < kBuffers; ++d) {
+          if (k + d >= pieces) break;
+          if (kAhead == 0) load_b(b[d], w.c + k + d);
+          chunk_product<NT, BS, PARTS>(at + (k + d) * R::kCodes, at + kMoePiece * R::kCodes + (k + d) * R::kScales, b[d], acc);
+          if (kAhead != 0 && w.c + k + d + kAhead < w.c1) load_b(b[d], w.c + k + d + kAhead);
         }
       }
       __syncwarp();  // every lane has read the stage
       if (!ahead.done()) {
-        if (lane == 0) issue(issued);
+        if (elect_one()) issue(issued);
+        __syncwarp();
         if (ahead.advance()) locate();
         ++issued;
       }
