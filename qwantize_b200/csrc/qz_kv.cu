@@ -22,7 +22,8 @@
 // there); a warp streams its run through its own ring of bulk copies with a
 // running maximum and sum, and never waits for another warp.  A pair that one warp
 // covers is written at once; of the others each warp leaves a partial result and
-// a second kernel joins them in order.
+// a second kernel joins them in order.  Few short sequences go without the second
+// launch: a CTA per pair, joined through shared memory.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -450,6 +451,33 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 units of the last pl
   return r;
 }
 
+// Four values of a result, joined from partial sums in order.
+struct Joined {
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -INFINITY, l = 0.0f;
+
+  __device__ __forceinline__ void take(const float2 ml, const float4 o) {
+    const float n = fmaxf(m, ml.x), z = n == -INFINITY ? 0.0f : n;
+    const float c = exp2_fast(m - z), cw = exp2_fast(ml.x - z);
+    v = make_float4(v.x * c + o.x * cw, v.y * c + o.y * cw, v.z * c + o.z * cw, v.w * c + o.w * cw);
+    l = l * c + ml.y * cw;
+    m = n;
+  }
+  // divided by the sum (0 where nothing was attended to) and rounded once
+  __device__ __forceinline__ void store(const AttnParams& p, int64_t at) const {
+    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    uint32_t x, y;
+    if (p.dtype == kDtBF16) {
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y * inv), "f"(v.x * inv));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w * inv), "f"(v.z * inv));
+    } else {
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y * inv), "f"(v.x * inv));
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w * inv), "f"(v.z * inv));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(x, y);
+  }
+};
+
 // NH tiles of 8 query heads share the warp's pass over a page.  Warps per SM:
 // what the registers allow (D = 128: 12 of at most 168 with one tile; two tiles
 // keep twice the sums: 8) and the ring, one page of keys and values per warp.
@@ -467,7 +495,10 @@ constexpr int kAttnMaxWarps = 16;
 // and a page costs 4 D/16 + 4 D/16 matrix instructions.  The codes' conversion to
 // fp16 (2 instructions per 4 E4M3 codes, 5 per 4 int8) is the largest part of
 // the rest.
-template <int D, int KV, int NH>
+//
+// ONE: a CTA has one pair of the list to itself, its warps cut the pair's pages and
+// join through shared memory, so short sequences need no second launch.
+template <int D, int KV, int NH, bool ONE>
 __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_kernel(const __grid_constant__ AttnParams p) {
   using G = AttnGeo<D, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -482,18 +513,27 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
     fence_barrier_init();
   }
   __syncwarp();
-  page_prefix(p, prefix);
   const int HR = p.Hkv * p.row_tiles;
-  const int64_t total = (int64_t)prefix[p.B] * HR, warps = (int64_t)gridDim.x * G::kWarps;
-  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours in work on different SMs
-  const int64_t u0 = me * total / warps, u1 = (me + 1) * total / warps;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (u0 >= u1) return;
-
   // position in the work list: sequence b, head and row tile hr, page pg of nb
   struct Pos { int b, hr, pg, nb; };
   Pos cur;
-  {
+  int64_t me, u0, u1;  // this warp's place; its units (a page of a pair each)
+  if constexpr (ONE) {
+    cur.b = blockIdx.x / HR;
+    cur.hr = blockIdx.x % HR;
+    cur.nb = pages_of(p, cur.b);
+    me = warp;
+    u0 = (int64_t)warp * cur.nb / G::kWarps;
+    u1 = (int64_t)(warp + 1) * cur.nb / G::kWarps;
+    cur.pg = (int)u0;
+  } else {
+    page_prefix(p, prefix);
+    const int64_t total = (int64_t)prefix[p.B] * HR, warps = (int64_t)gridDim.x * G::kWarps;
+    me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours in work on different SMs
+    u0 = me * total / warps;
+    u1 = (me + 1) * total / warps;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (u0 >= u1) return;
     int lo = 0, hi = p.B;  // last b with prefix[b] * HR <= u0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -506,7 +546,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
     cur.pg = (int)(r % cur.nb);
   }
   auto advance = [&](Pos& x) {
-    if (++x.pg < x.nb) return;
+    if (++x.pg < x.nb || ONE) return;
     x.pg = 0;
     if (++x.hr < HR) return;
     x.hr = 0;
@@ -529,12 +569,15 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
   };
 
   Pos next = cur;
-  int64_t blk = block_of(cur), blk_next = -1;
-  if (lane == 0) {
-    issue(p.k, blk, ring, bar_k);
-    issue(p.v, blk, ring + G::kBlock, bar_v);
+  int64_t blk = -1, blk_next = -1;
+  if (!ONE || u0 < u1) {
+    blk = block_of(cur);
+    if (lane == 0) {
+      issue(p.k, blk, ring, bar_k);
+      issue(p.v, blk, ring + G::kBlock, bar_v);
+    }
+    issued_k = issued_v = 1;
   }
-  issued_k = issued_v = 1;
   float ks = blk >= 0 ? __ldg(p.ks + blk) : 0.0f, vs = blk >= 0 ? __ldg(p.vs + blk) : 0.0f;
   advance(next);
   if (u0 + 1 < u1) blk_next = block_of(next);
@@ -745,13 +788,15 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
                 out[16 * i + 8 * h + g] = r;
               }
           } else {
-            float* po = p.part_o + (slot * 16 + row) * D;
+            // ONE: in this warp's ring, which is idle now
+            float* po = ONE ? reinterpret_cast<float*>(ring) + row * D : p.part_o + (slot * 16 + row) * D;
+            float* ml = ONE ? reinterpret_cast<float*>(ring) + 16 * D + row * 2 : p.part_ml + (slot * 16 + row) * 2;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               po[16 * i + g] = o[i][n][c];
               po[16 * i + 8 + g] = o[i][n][2 + c];
             }
-            if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 16 + row) * 2) = make_float2(m[n][c], sum);
+            if (g == 0) *reinterpret_cast<float2*>(ml) = make_float2(m[n][c], sum);
           }
         }
       fresh = true;
@@ -767,6 +812,23 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
   if (!ok) {  // copies in flight must land before the CTA exits (bounded)
     mbar_wait_bounded(bar_k, (issued_k - 1) & 1, kDevErrLoadTimeout);
     mbar_wait_bounded(bar_v, (issued_v - 1) & 1, kDevErrLoadTimeout);
+  }
+  if constexpr (ONE) {
+    __syncthreads();
+    const int64_t nb = cur.nb;
+    if (nb == 1) return;  // the page's warp wrote the result
+    const int head = cur.hr / p.row_tiles, r0 = cur.hr % p.row_tiles * (8 * NH);
+    const int rows = p.G - r0 < 8 * NH ? p.G - r0 : 8 * NH;
+    for (int i = threadIdx.x; i < rows * (D / 4); i += G::kWarps * 32) {
+      const int row = i / (D / 4), d4 = i % (D / 4);
+      Joined a;
+      for (int w = 0; w < G::kWarps; ++w) {
+        if (w * nb / G::kWarps == (w + 1) * nb / G::kWarps) continue;  // it had no page
+        const float* from = reinterpret_cast<const float*>(smem + w * 2 * G::kBlock);
+        a.take(*reinterpret_cast<const float2*>(from + 16 * D + row * 2), *reinterpret_cast<const float4*>(from + row * D + d4 * 4));
+      }
+      a.store(p, (((int64_t)cur.b * p.Hkv + head) * p.G + r0 + row) * D + d4 * 4);
+    }
   }
 }
 
@@ -790,15 +852,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   asm volatile("griddepcontrol.wait;" ::: "memory");  // in every CTA: this grid ends after the one before it
   const int64_t total = (int64_t)prefix[p.B] * HR;
   const int nb = prefix[b + 1] - prefix[b];
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float m = -INFINITY, l = 0.0f;
-  auto take = [&](const float2 ml, const float4 o) {
-    const float n = fmaxf(m, ml.x), z = n == -INFINITY ? 0.0f : n;
-    const float c = exp2_fast(m - z), cw = exp2_fast(ml.x - z);
-    v = make_float4(v.x * c + o.x * cw, v.y * c + o.y * cw, v.z * c + o.z * cw, v.w * c + o.w * cw);
-    l = l * c + ml.y * cw;
-    m = n;
-  };
+  Joined a;
   if (nb > 0) {
     const int64_t u0 = (int64_t)prefix[b] * HR + (int64_t)hr * nb, u1 = u0 + nb;
     // the warp of unit u is the last w with w * total / warps <= u; with fewer
@@ -812,29 +866,18 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
       for (int i = part; i < count; i += split) {
         const int64_t w = total >= warps ? w0 + i : ((u0 + i + 1) * warps - 1) / total;
         const int64_t at = (w * 2 + (i == 0 ? first : 0)) * 16 + row;
-        take(__ldcg(reinterpret_cast<const float2*>(p.part_ml) + at), __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4));
+        a.take(__ldcg(reinterpret_cast<const float2*>(p.part_ml) + at), __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4));
       }
     }
-    s_o[threadIdx.x] = v;
-    s_ml[threadIdx.x] = make_float2(m, l);
+    s_o[threadIdx.x] = a.v;
+    s_ml[threadIdx.x] = make_float2(a.m, a.l);
     __syncthreads();
     if (part > 0) return;
-    for (int i = 1; i < split; ++i) take(s_ml[i * per + threadIdx.x], s_o[i * per + threadIdx.x]);
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    for (int i = 1; i < split; ++i) a.take(s_ml[i * per + threadIdx.x], s_o[i * per + threadIdx.x]);
   } else if (part > 0) {
     return;
   }
-  uint32_t x, y;
-  if (p.dtype == kDtBF16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y), "f"(v.x));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w), "f"(v.z));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(v.y), "f"(v.x));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(v.w), "f"(v.z));
-  }
-  const int64_t at = (((int64_t)b * p.Hkv + head) * p.G + r0 + row) * D + d4 * 4;
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(x, y);
+  a.store(p, (((int64_t)b * p.Hkv + head) * p.G + r0 + row) * D + d4 * 4);
 }
 
 // ---------------------------------------------------------------------------
@@ -857,29 +900,52 @@ static int check_cache(int kv_dtype, int64_t num_pages, int64_t Hkv, int64_t D) 
 
 static bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
-template <int D, int KV, int NH>
-static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
-  using G = AttnGeo<D, NH>;
+// Whether each (sequence, head, row tile) pair is given to one CTA, in one launch,
+// instead of cutting all pages evenly and joining in a second one: with at most a
+// CTA per SM, and at most four pages in a row for a warp by the table's width.
+// Microseconds alone / evenly, 8 cache heads of 128, groups of 4, int8: 1 sequence
+// of 300 tokens 8.5 / 12.0, of 2000 16.7 / 14.7, of 8000 41 / 29; 8 of 1000 12.6 / 14.7,
+// 32 of 1000 (256 pairs) 24.5 / 20.8; groups of 16, 1 of 2000: 20.8 / 29.0.
+static bool attention_alone(int64_t pairs, int64_t max_pages, int sms, int warps) {
+  return pairs <= sms && max_pages <= 4 * warps;
+}
+
+template <int D, int KV, int NH, bool ONE>
+static int prepare_attention() {
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(kv_attention_kernel<D, KV, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(kKvMaxSeqs));
-    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
-    if (dev >= 0 && dev < 64) attr_set[dev] = true;
-  }
+  if (dev >= 0 && dev < 64 && attr_set[dev]) return QZ_OK;
+  e = cudaFuncSetAttribute(kv_attention_kernel<D, KV, NH, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           AttnGeo<D, NH>::smem(kKvMaxSeqs));
+  if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
+  if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  return QZ_OK;
+}
+
+template <int D, int KV, int NH>
+static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
+  using G = AttnGeo<D, NH>;
   p.rows_per_tile = 8 * NH;
   p.row_tiles = (p.G + 8 * NH - 1) / (8 * NH);
-  kv_attention_kernel<D, KV, NH><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
-  int s = cuda_status(cudaGetLastError(), "kv attention launch");
+  const int64_t pairs = (int64_t)p.B * p.Hkv * p.row_tiles;
+  if (attention_alone(pairs, p.max_pages, sms, G::kWarps)) {
+    const int s = prepare_attention<D, KV, NH, true>();
+    if (s != QZ_OK) return s;
+    kv_attention_kernel<D, KV, NH, true><<<(unsigned)pairs, G::kWarps * 32, G::smem(0), st>>>(p);
+    return cuda_status(cudaGetLastError(), "kv attention launch");
+  }
+  int s = prepare_attention<D, KV, NH, false>();
   if (s != QZ_OK) return s;
+  kv_attention_kernel<D, KV, NH, false><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
+  if ((s = cuda_status(cudaGetLastError(), "kv attention launch")) != QZ_OK) return s;
   // the join may begin while the last pages are read; it waits for the kernel's end before it reads results
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.Hkv * p.row_tiles));
+  cfg.gridDim = dim3((unsigned)pairs);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = (size_t)(p.B + 1) * 4;
   cfg.stream = st;

@@ -93,6 +93,21 @@ def test_attention_shapes(dtype, D, lens, H, G):
 
 
 @pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,G", [([300], 2, 1), ([1, 0, 64, 65], 3, 5), ([2000, 7, 640], 2, 8), ([1500], 1, 16), ([0], 1, 3)])
+def test_narrow_and_wide_tables(dtype, D, lens, H, G):
+    """A table of a few pages gives a pair of sequence and head to one CTA, a wide
+    one cuts all pages evenly; the columns behind a sequence are not read."""
+    import qwantize_b200 as q
+    c, codes, table, lengths = setup(len(lens), lens, H, D, dtype, len(lens) + G)
+    wide = torch.cat([table, table.new_full((len(lens), 130), 1 << 30)], 1)
+    for t in (torch.bfloat16, torch.float16):
+        x = queries(len(lens), H * G, D, t, 4)
+        check(q.kv_cache_attention(c, x, table, lengths), x, *codes, table, lengths)
+        check(q.kv_cache_attention(c, x, wide, lengths), x, *codes, table, lengths)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
 def test_long_sequences_shared_by_many_warps(dtype):
     import qwantize_b200 as q
     c, codes, table, lengths = setup(3, [70000, 33, 9000], 1, 128, dtype, 5)
