@@ -24,6 +24,8 @@
 //   linear_pair_kernel (prompts): a pair of CTAs on 256 tokens x 256 features; the
 //   tensor cores bound it.
 //
+// A single token goes without the first launch: each CTA quantizes it for itself.
+//
 // The second launch starts before the first has ended and fetches its first
 // stages of W meanwhile.  Issuing a copy or an MMA takes about 30 clocks from an
 // elected lane of a converged warp and about 60 from a branch on the lane, so
@@ -99,6 +101,55 @@ __device__ __forceinline__ void unpack(const uint4 (&w)[VEC], float (&v)[BS]) {
   }
 }
 
+// The power of two p of a row with the largest magnitude m (fp32 bits): the
+// exponent e, smallest with max <= 1.3125 * 2^(11 + e); 0 for an all-zero row and
+// for inf / NaN.
+__device__ __forceinline__ int row_power(uint32_t m) {
+  if (m == 0 || m >= 0x7f800000u) return 0;
+  return max((int)(m >> 23) - 127 - 11 + ((m & 0x7fffffu) > 0x280000u ? 1 : 0), -120);
+}
+
+// One block of x / p (inv = 1 / p; a power of two moves no bit of a 16-bit value):
+// its scale code, its values' codes in words.
+template <int BS, int DT, int VEC>
+__device__ __forceinline__ uint32_t quantize_block(const uint4 (&w)[VEC], uint32_t largest, float inv, uint32_t (&words)[BS / 8]) {
+  const uint32_t y = __float_as_uint(__fmul_rn(__uint_as_float(largest), inv));
+  uint32_t code;
+  float s;
+  if (BS == 16) {
+    s = e4m3_snap_nonneg(__fdiv_rn(__uint_as_float(y), 6.0f));
+    code = e4m3_code(s);
+  } else {
+    code = is_nan_bits(y) ? 255u : (uint32_t)ue8m0_naive_exp(y);
+    s = code == 255u ? __uint_as_float(kMxNanBits) : pow2f((int)code - 127);
+  }
+  if (!(s > 0.0f)) return code;  // a zero (or NaN) scale keeps codes 0
+  float v[BS];
+  unpack<DT, VEC>(w, v);
+  if (DT != kDtF32) {
+    // the conversion rounds the magnitude and keeps the sign
+    const float c = __fmul_rn(__frcp_rn(s), kBiasDown);
+    const bool in_range = inv >= 0x1p-60f && inv <= 0x1p60f;  // inv * c is exact: one product per value
+    const float ci = in_range ? __fmul_rn(c, inv) : c;
+#pragma unroll
+    for (int i = 0; i < BS; i += 2) {
+      float lo = v[i], hi = v[i + 1];
+      if (!in_range) { lo = __fmul_rn(lo, inv); hi = __fmul_rn(hi, inv); }
+      words[i / 8] |= e2m1x2_rn(__fmul_rn(lo, ci), __fmul_rn(hi, ci)) << (4 * (i % 8));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < BS; ++i) {
+      const float q = __fdiv_rn(fabsf(__fmul_rn(v[i], inv)), s);
+      uint32_t n = __float_as_uint(v[i]) >> 31 << 3;
+#pragma unroll
+      for (int k = 0; k < 7; ++k) n += q > bnd(k) ? 1u : 0u;
+      words[i / 8] |= n << (4 * (i % 8));
+    }
+  }
+  return code;
+}
+
 // One CTA per row.  A thread keeps its first R blocks of BS values in registers
 // between the row's maximum and the rounding (later ones of very long rows
 // are read again, from L2): R = 1 for few rows, where the latency of one row
@@ -148,12 +199,7 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
     __syncthreads();
     m = 0;
     for (int w = 0; w < (nt >> 5); ++w) m = max(m, s_max[w]);
-    // smallest e with max <= 1.3125 * 2^(11 + e); 0 for an all-zero row and for inf / NaN
-    int e = 0;
-    if (m != 0 && m < 0x7f800000u) {
-      e = (int)(m >> 23) - 127 - 11 + ((m & 0x7fffffu) > 0x280000u ? 1 : 0);
-      e = max(e, -120);
-    }
+    const int e = row_power(m);
     inv = pow2f(-e);
     p = pow2f(e);
   }
@@ -162,43 +208,7 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256)
   auto block = [&](int64_t b, const uint4 (&w)[kVec], uint32_t largest) {
     uint32_t code = 0;
     uint32_t words[BS / 8] = {};
-    if (b < nb) {
-      // the block of x / p: a power of two moves no bit of a 16-bit value
-      const uint32_t y = __float_as_uint(__fmul_rn(__uint_as_float(largest), inv));
-      float s;
-      if (BS == 16) {
-        s = e4m3_snap_nonneg(__fdiv_rn(__uint_as_float(y), 6.0f));
-        code = e4m3_code(s);
-      } else {
-        code = is_nan_bits(y) ? 255u : (uint32_t)ue8m0_naive_exp(y);
-        s = code == 255u ? __uint_as_float(kMxNanBits) : pow2f((int)code - 127);
-      }
-      if (s > 0.0f) {  // a zero (or NaN) scale keeps codes 0
-        float v[BS];
-        unpack<DT, kVec>(w, v);
-        if (DT != kDtF32) {
-          // the conversion rounds the magnitude and keeps the sign
-          const float c = __fmul_rn(__frcp_rn(s), kBiasDown);
-          const bool in_range = inv >= 0x1p-60f && inv <= 0x1p60f;  // inv * c is exact: one product per value
-          const float ci = in_range ? __fmul_rn(c, inv) : c;
-#pragma unroll
-          for (int i = 0; i < BS; i += 2) {
-            float lo = v[i], hi = v[i + 1];
-            if (!in_range) { lo = __fmul_rn(lo, inv); hi = __fmul_rn(hi, inv); }
-            words[i / 8] |= e2m1x2_rn(__fmul_rn(lo, ci), __fmul_rn(hi, ci)) << (4 * (i % 8));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < BS; ++i) {
-            const float q = __fdiv_rn(fabsf(__fmul_rn(v[i], inv)), s);
-            uint32_t n = __float_as_uint(v[i]) >> 31 << 3;
-#pragma unroll
-            for (int k = 0; k < 7; ++k) n += q > bnd(k) ? 1u : 0u;
-            words[i / 8] |= n << (4 * (i % 8));
-          }
-        }
-      }
-    }
+    if (b < nb) code = quantize_block<BS, DT>(w, largest, inv, words);
     if (b < nb_packed) {
       if (BS == 16) *reinterpret_cast<uint2*>(packed + row * ldp + b * 8) = make_uint2(words[0], words[1]);
       else *reinterpret_cast<uint4*>(packed + row * ldp + b * 16) = make_uint4(words[0], words[1], words[BS / 16], words[BS / 8 - 1]);
@@ -256,18 +266,23 @@ struct LinearParams {
   void* out;
   int out_dtype;
   int64_t ldo;
+  const void* x;                      // the token that the product's own kernel quantizes, K elements
+  int64_t K;
   int tma_out;                        // map_out is valid (pair form, 16-bit output, 16-byte rows)
 };
 
-// The form of few tokens: A = weight rows, B = tokens.
-template <int BN, int BS>
+// The form of few tokens: A = weight rows, B = tokens.  HERE: the CTA quantizes a
+// single token itself and keeps the codes and scales of all its stages.
+constexpr int kHereStages = 16;
+template <int BN, int BS, bool HERE>
 struct LinGeo {
   static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
   static constexpr int kSf = Fmt<BS>::kSfBytes;
-  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kSf;
-  static constexpr int kMaxStages = (232448 - 1024 - 512) / kStageBytes;
+  static constexpr int kRing = HERE ? kABytes : kABytes + kBBytes, kRingSf = HERE ? kSf : 2 * kSf;  // of a stage
+  static constexpr int kKeep = HERE ? kHereStages * (kBBytes + kSf) : 0;
+  static constexpr int kMaxStages = (232448 - 1024 - 768 - kKeep) / (kRing + kRingSf);
   static constexpr int kStages = kMaxStages > 10 ? 10 : kMaxStages;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 512;
+  static constexpr int kSmem = kStages * (kRing + kRingSf) + kKeep + 1024 + 768;
   // TMEM columns: two accumulators, then kSfBufs buffers of scales (kGroups * 4 of A, as many of B)
   static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * 2;
   static constexpr int kSfBufs = 4;
@@ -407,8 +422,9 @@ struct LinOutTokens {
   int64_t ra, cb;       // output feature, first token
   bool in;
   float bias;
+  const float* scales;  // of the tile's tokens
 
-  __device__ __forceinline__ LinOutTokens(const LinearParams& q, const LinWork<true>& u) : p(q) {
+  __device__ __forceinline__ LinOutTokens(const LinearParams& q, const LinWork<true>& u, const float* here) : p(q) {
     lane = threadIdx.x & 31;
     row = (threadIdx.x >> 5 & 3) * 32 + lane;
     ra = u.a * 128 + row;
@@ -416,10 +432,11 @@ struct LinOutTokens {
     cols = p.T - cb < BN ? (int)(p.T - cb) : BN;
     in = ra < p.N;
     bias = in && p.bias ? load_any(p.bias, p.bias_dtype, ra) : 0.0f;
+    scales = here ? here : p.row_scale + cb;
   }
   // lane q: the scale of token c + q
   __device__ __forceinline__ float column(int c) const {
-    return c + lane < cols && lane < C ? __ldg(p.row_scale + cb + c + lane) * p.w_scale : 0.0f;
+    return c + lane < cols && lane < C ? scales[c + lane] * p.w_scale : 0.0f;
   }
   __device__ __forceinline__ void store(int c, float v, float scale) const {
     if (in) store_any(p.out, p.out_dtype, (cb + c) * p.ldo + ra, __fmaf_rn(v, scale, bias));
@@ -500,26 +517,79 @@ struct LinOutRows {
 
 constexpr int kLinThreads = 224;
 
-template <int BN, int BS>
+// One token's codes and scales of stages [s0, s1), in the layout that TMA and the
+// bulk copies would give the stages of a ring, by the 128 threads of warps 2-5.
+// The row's maximum takes all of it, also where a cluster cuts K.
+template <int BS, int DT>
+__device__ __forceinline__ void quantize_here(const LinearParams& p, int s0, int s1, int stage_bytes, unsigned char* codes,
+                                              unsigned char* sf, float* scale, uint32_t* s_max) {
+  constexpr int kVec = BS * Elem<DT>::kSize / 16, kBlocks = Fmt<BS>::kBlocks, kMost = kHereStages * kBlocks / 128;
+  const int tid = threadIdx.x - 64, nb = (int)(p.K / BS), blocks = (s1 - s0) * kBlocks;
+  const uint4* row = static_cast<const uint4*>(p.x);
+  uint4 w[kMost][kVec];
+#pragma unroll
+  for (int i = 0; i < kMost; ++i)
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const int j = tid + i * 128, b = s0 * kBlocks + j;
+      w[i][v] = j < blocks && b < nb ? __ldg(row + b * kVec + v) : make_uint4(0, 0, 0, 0);
+    }
+  int e = 0;
+  if (BS == 16) {
+    uint32_t m = 0;
+#pragma unroll 4
+    for (int v = tid; v < nb * kVec; v += 128) m = abs_max<DT>(m, __ldg(row + v));
+    m = __reduce_max_sync(0xffffffffu, abs_bits<DT>(m));
+    if ((tid & 31) == 0) s_max[tid >> 5] = m;
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
+    e = row_power(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+  }
+  const float inv = pow2f(-e);
+  if (tid == 0) *scale = pow2f(e);
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int j = tid + i * 128, kb = j % kBlocks;
+    if (j >= blocks) break;
+    uint32_t m = 0, words[BS / 8] = {}, code = 0;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) m = abs_max<DT>(m, w[i][v]);
+    if (s0 * kBlocks + j < nb) code = quantize_block<BS, DT>(w[i], abs_bits<DT>(m), inv, words);
+    unsigned char* to = codes + j / kBlocks * stage_bytes;  // row 0 of the swizzle: in order
+    if constexpr (BS == 16) *reinterpret_cast<uint2*>(to + kb * 8) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint4*>(to + kb * 16) = make_uint4(words[0], words[1], words[BS / 16], words[BS / 8 - 1]);
+    sf[j / kBlocks * Fmt<BS>::kSfBytes + kb / 4 * kGroupBytes + kb % 4] = (uint8_t)code;
+  }
+  fence_proxy_async_smem();
+  asm volatile("barrier.sync 1, 128;" ::: "memory");  // the scale
+}
+
+// HERE: the type of the one token that this kernel quantizes itself (-1: an earlier launch does)
+template <int BN, int BS, int HERE>
 __global__ void __launch_bounds__(kLinThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ LinearParams p) {
   // 224 threads: warp 0 feeds the ring, warp 6 copies a stage's scales to TMEM (tcgen05.cp), warp 1 issues its four
   // block-scaled MMAs of K = 64, warps 2-5 drain the accumulator
-  using G = LinGeo<BN, BS>;
+  constexpr bool kHere = HERE >= 0;
+  using G = LinGeo<BN, BS, kHere>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // operands (1024-byte swizzle atoms), the scales of all stages, barriers
-  unsigned char* smem_sf = smem + G::kStages * (G::kABytes + G::kBBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::kStages * G::kStageBytes);
+  unsigned char* smem_x = smem + G::kStages * G::kRing;  // kHere: the token's codes, then its scales (the other 15 rows of B are whatever is there)
+  unsigned char* smem_xsf = smem_x + kHereStages * G::kBBytes;
+  unsigned char* smem_sf = smem_x + G::kKeep;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_sf + G::kStages * G::kRingSf);
   uint64_t* empty = full + G::kStages;
   uint64_t* tfull = empty + G::kStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* sf_full = tempty + 2;
   uint64_t* mma_done = sf_full + G::kSfBufs;
   uint64_t* sf_done = mma_done + 1;
-  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(sf_done + 1);
+  uint64_t* x_here = sf_done + 1;  // kHere: the token is in shared memory
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(x_here + 1);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+  float* scale_here = reinterpret_cast<float*>(tmem_base_s + 2);
+  uint32_t* s_max = reinterpret_cast<uint32_t*>(scale_here + 1);
   constexpr int C = LinOutTokens<BN>::C;
   float* part = reinterpret_cast<float*>(smem);  // (BN, 128) fp32, over the ring's first stages
   const int warp = threadIdx.x >> 5;
@@ -530,6 +600,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     for (int b = 0; b < G::kSfBufs; ++b) mbar_init(sf_full + b, 1);
     mbar_init(mma_done, 1);
     mbar_init(sf_done, 1);
+    mbar_init(x_here, 128);
     *abort_s = 0;
     fence_barrier_init();
   }
@@ -556,13 +627,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   if (warp == 0) {
     // ---------------- producer (the warp stays converged: one elected lane issues) ----------------
     auto load_w = [&](const LinWork<true>& u, int ks, int s) {
-      mbar_arrive_expect_tx(full + s, G::kStageBytes);
-      tma_load_2d(smem + s * (G::kABytes + G::kBBytes), &map_a, ks * 128, (int)(u.a * 128), full + s);
-      bulk_load(smem_sf + s * 2 * G::kSf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+      mbar_arrive_expect_tx(full + s, G::kRing + G::kRingSf);
+      tma_load_2d(smem + s * G::kRing, &map_a, ks * 128, (int)(u.a * 128), full + s);
+      bulk_load(smem_sf + s * G::kRingSf, p.sf_a + (u.a * p.n_steps + ks) * G::kSf, G::kSf, full + s);
     };
     auto load_x = [&](const LinWork<true>& u, int ks, int s) {
-      tma_load_2d(smem + s * (G::kABytes + G::kBBytes) + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
-      bulk_load(smem_sf + (s * 2 + 1) * G::kSf, p.sf_b + (u.b * p.n_steps + ks) * G::kSf, G::kSf, full + s);
+      if (kHere) return;
+      tma_load_2d(smem + s * G::kRing + G::kABytes, &map_b, ks * 128, (int)(u.b * BN), full + s);
+      bulk_load(smem_sf + s * G::kRingSf + G::kSf, p.sf_b + (u.b * p.n_steps + ks) * G::kSf, G::kSf, full + s);
     };
     // the first ring of weights does not wait for the quantization launch
     uint32_t ahead = 0;
@@ -571,7 +643,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         if (elect_one()) load_w(u, ks, ahead);
         __syncwarp();
       }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!kHere) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t it = 0, s = 0, ph = 1;
     bool ok = true;
     for (LinWork<true> u(p); ok && u.next();) {
@@ -594,11 +666,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer (the warp waits together, one lane issues) ----------------
     // low words of the descriptors of stage 0; a stage further is an addition
-    const uint32_t lo_a = smem_u32(smem) >> 4, lo_b = lo_a + (G::kABytes >> 4);
+    const uint32_t lo_a = smem_u32(smem) >> 4, lo_b = kHere ? smem_u32(smem_x) >> 4 : lo_a + (G::kABytes >> 4);
+    const bool ready = !kHere || wait(x_here, 0, kDevErrMmaTimeout);
     uint32_t lt = 0, s = 0, ph = 0, sb = 0, sph = 0;  // stage, scale buffer, their phases
     for (LinWork<true> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1;
-      bool ok = wait(tempty + acc, (lt >> 1 & 1) ^ 1, kDevErrMmaTimeout);
+      bool ok = ready && wait(tempty + acc, (lt >> 1 & 1) ^ 1, kDevErrMmaTimeout);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + acc * BN;
@@ -607,7 +680,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t da = lo_a + s * ((G::kABytes + G::kBBytes) >> 4), db = lo_b + s * ((G::kABytes + G::kBBytes) >> 4);
+        const uint32_t da = lo_a + s * (G::kRing >> 4), db = lo_b + (kHere ? (ks - u.s0) * (G::kBBytes >> 4) : s * (G::kRing >> 4));
         const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
         const uint32_t first = ks > u.s0 ? 1u : 0u;
         if (elect_one()) {
@@ -635,7 +708,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     // ---------------- scales to TMEM ----------------
     const uint32_t lo_sf = smem_u32(smem_sf) >> 4;
     uint32_t s = 0, ph = 0, sb = 0, warm = 0;  // warm: scale buffers used so far, up to kSfBufs
-    bool ok = true;
+    const uint32_t lo_xsf = smem_u32(smem_xsf) >> 4;
+    bool ok = !kHere || __all_sync(0xffffffffu, wait(x_here, 0, kDevErrMmaTimeout));
     for (LinWork<true> u(p); ok && u.next();) {
       for (int ks = u.s0; ks < u.s1; ++ks) {
         ok = wait(full + s, ph, kDevErrMmaTimeout);
@@ -649,13 +723,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ds = lo_sf + s * (2 * G::kSf >> 4);
+        const uint32_t ds = lo_sf + s * (G::kRingSf >> 4);
+        const uint32_t ds_b = kHere ? lo_xsf + (ks - u.s0) * (G::kSf >> 4) : ds + (G::kSf >> 4);
         const uint32_t t_sfa = tmem_base + G::kAccCols + sb * G::kSfCols, t_sfb = t_sfa + Fmt<BS>::kGroups * 4;
         if (elect_one()) {
 #pragma unroll
           for (int q = 0; q < Fmt<BS>::kGroups; ++q) {
             tmem_cp_scales(t_sfa + 4 * q, ds + q * (kGroupBytes >> 4));
-            tmem_cp_scales(t_sfb + 4 * q, ds + ((G::kSf + q * kGroupBytes) >> 4));
+            tmem_cp_scales(t_sfb + 4 * q, ds_b + q * (kGroupBytes >> 4));
           }
           umma_commit(sf_full + sb);
         }
@@ -671,11 +746,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     mbar_wait_bounded(sf_done, 0u, kDevErrMmaTimeout);
   } else {
     // ---------------- epilogue (warps 2-5) ----------------
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales are the quantization launch's
+    if constexpr (kHere) {
+      LinWork<true> u(p);
+      quantize_here<BS, HERE>(p, u.s0, u.s1, G::kBBytes, smem_x, smem_xsf, scale_here, s_max);
+      mbar_arrive(x_here);
+    } else {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // row scales are the quantization launch's
+    }
     uint32_t lt = 0;
     for (LinWork<true> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
-      LinOutTokens<BN> out(p, u);
+      LinOutTokens<BN> out(p, u, kHere ? scale_here : nullptr);
       if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * BN;
@@ -707,7 +788,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       LinWork<true> u(p);
       if (u.next()) {
         // rank r finishes columns [r, r + 1) * BN / split
-        LinOutTokens<BN> out(p, u);
+        LinOutTokens<BN> out(p, u, kHere ? scale_here : nullptr);
         const int rank = blockIdx.x % p.split, per = BN / p.split;
         const float col = out.column(rank * per / C * C);
         const uint32_t at = smem_u32(part) + out.row * 4;
@@ -724,7 +805,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
             for (int w = 1; w < 8; ++w) v += x[q][w];
             const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
-                                         : (c0 + q < c_end ? __ldg(p.row_scale + u.b * BN + c0 + q) * p.w_scale : 0.0f);
+                                         : (c0 + q < c_end ? out.scales[c0 + q] * p.w_scale : 0.0f);
             if (c0 + q < c_end) out.store(c0 + q, v, scale);
           }
         }
@@ -1134,7 +1215,8 @@ static int out_map(CUtensorMap* m, void* base, uint64_t N, uint64_t T, uint64_t 
 // Tile form and cluster size of one call, and its workspace.
 struct LinPlan {
   int bn, split, n_steps;
-  int gran;  // rows of a tile of x's scales
+  int gran;   // rows of a tile of x's scales
+  bool here;  // the product's kernel quantizes the token itself
   int64_t tiles_a, tiles_b, ldp;
   int64_t off_sf, off_scale, bytes;
 };
@@ -1178,6 +1260,10 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     }
   }
   best.n_steps = n_steps;
+  // a single token, quantized by every CTA for itself: no first launch.  On the device 8.6 us instead of 10.6
+  // (MXFP4) and 10.6 instead of 10.6 (NVFP4) at 2560 x 9728, and a launch less for the host; with 2 tokens 10.6 and
+  // 11.6 instead of 10.6, with 8 12.9 and 20.9, in a form for several.
+  best.here = best.bn == 16 && T == 1 && (n_steps + best.split - 1) / best.split <= kHereStages;
   best.ldp = up(K, 32) / 2;
   best.gran = best.bn < 128 ? best.bn : 128;
   const int64_t sf_tiles = best.bn == 256 ? best.tiles_a * 2 : best.tiles_b;
@@ -1215,23 +1301,28 @@ static cudaError_t launch_quantize_rows(const QuantizeRows& q, cudaStream_t st) 
   return cudaGetLastError();
 }
 
-template <int BN, int BS>
+template <int BN, int BS, int HERE>
 static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p, int sms, cudaStream_t st) {
-  using G = LinGeo<BN, BS>;
+  using G = LinGeo<BN, BS, (HERE >= 0)>;
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(linear_kernel<BN, BS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+    e = cudaFuncSetAttribute(linear_kernel<BN, BS, HERE>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   cudaLaunchAttribute at[2] = {};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim = {(unsigned)p.split, 1, 1};
+  int n = 0;
+  if (HERE < 0) {  // the quantization launch is before it
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.split > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n++].val.clusterDim = {(unsigned)p.split, 1, 1};
+  }
   const int64_t ctas = p.tiles_a * p.tiles_b * p.split;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(ctas < sms ? ctas : sms));
@@ -1239,8 +1330,8 @@ static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const Linea
   cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS>, a, b, p), "linear launch");
+  cfg.numAttrs = n;
+  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS, HERE>, a, b, p), "linear launch");
 }
 
 template <int BS>
@@ -1274,11 +1365,17 @@ template <int BS>
 static int run_linear(int bn, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
                       cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_linear<16, BS>(a, b, p, sms, st);
-    case 32: return launch_linear<32, BS>(a, b, p, sms, st);
-    case 64: return launch_linear<64, BS>(a, b, p, sms, st);
+    case 16: return launch_linear<16, BS, -1>(a, b, p, sms, st);
+    case 32: return launch_linear<32, BS, -1>(a, b, p, sms, st);
+    case 64: return launch_linear<64, BS, -1>(a, b, p, sms, st);
     default: return launch_pair<BS>(a, b, o, p, sms, st);
   }
+}
+template <int BS>
+static int run_linear_here(int x_dtype, const CUtensorMap& a, const LinearParams& p, int sms, cudaStream_t st) {
+  if (x_dtype == kDtBF16) return launch_linear<16, BS, kDtBF16>(a, a, p, sms, st);
+  if (x_dtype == kDtF16) return launch_linear<16, BS, kDtF16>(a, a, p, sms, st);
+  return launch_linear<16, BS, kDtF32>(a, a, p, sms, st);
 }
 
 static int check_sizes(int64_t T, int64_t K, int64_t N, int format, int* bs) {
@@ -1370,6 +1467,8 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
   p.bias = bias; p.bias_dtype = bias_dtype;
   p.out = out; p.out_dtype = out_dtype; p.ldo = ldo;
   p.tma_out = !swap && out_dtype != QZ_DTYPE_F32 && ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  p.x = x; p.K = K;
+  if (pl.here) return bs == 16 ? run_linear_here<16>(x_dtype, mw, p, sms, st) : run_linear_here<32>(x_dtype, mw, p, sms, st);
   CUtensorMap mo = mx;
   if (p.tma_out && (s = out_map(&mo, out, (uint64_t)N, (uint64_t)T, (uint64_t)ldo)) != QZ_OK) return s;
   const QuantizeRows q{x, x_dtype, ldx, T, K, ws, pl.ldp, ws + pl.off_sf, pl.gran, pl.n_steps,

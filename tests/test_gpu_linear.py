@@ -96,6 +96,29 @@ def test_nvfp4_odd_block_counts(T, K):
     check(q.fp4_linear(x, w, out_dtype=torch.float32), x, codes, packed, "nvfp4", 0.125)
 
 
+@pytest.mark.parametrize("fmt,K", [("nvfp4", 16), ("nvfp4", 272), ("nvfp4", 9744), ("mxfp4", 32), ("mxfp4", 2592), ("mxfp4", 9728), ("nvfp4", 40960)])
+@pytest.mark.parametrize("N", [77, 1500])
+def test_a_single_token_like_a_row_of_two(fmt, K, N):
+    """One token is quantized by the product's own kernel: the same bits as from
+    the row in a batch, whatever the type, the magnitude and what is not finite."""
+    import qwantize_b200 as q
+    codes, packed = make_weight(N, K, fmt, K + N)
+    w = q.FP4Weight(codes, packed, fmt)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = acts(2, K, dtype, K).to(DEV)
+        check(q.fp4_linear(x[:1], w), x[:1], codes, packed, fmt)
+        rows = [x[0], x[0] * 0, x[0] * 2.0**-10, x[0] * 2.0**5]
+        if dtype != torch.float16:
+            rows += [x[0] * 2.0**70, x[0] * 2.0**-70]
+        for bad in (float("inf"), float("nan")):
+            rows.append(x[0].clone())
+            rows[-1][K // 2] = bad
+        for r in rows:
+            pair = torch.stack([r, x[1]])
+            one, two = q.fp4_linear(pair[:1], w), q.fp4_linear(pair, w)[:1]
+            assert torch.equal(one.isnan(), two.isnan()) and torch.equal(one.nan_to_num(), two.nan_to_num())
+
+
 def test_many_tiles_and_bands():
     """More tiles than SMs, several bands of token tiles, a ragged last one."""
     import qwantize_b200 as q
