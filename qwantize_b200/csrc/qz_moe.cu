@@ -630,6 +630,25 @@ __device__ __forceinline__ void chunk_product(const uint8_t* codes, const uint8_
   }
 }
 
+// The weighted results of token t's experts, columns 4 h .. + 3, added in order and rounded once.
+__device__ __forceinline__ void add_experts(const MoeParams& p, int t, int h) {
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int k = 0; k < p.top; ++k) {
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.y + (int64_t)(t * p.top + k) * p.H) + h);
+    v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+  }
+  uint32_t lo, hi;
+  if (p.dtype == kDtBF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
+  }
+  reinterpret_cast<uint2*>(p.out)[(int64_t)t * (p.H / 4) + h] = make_uint2(lo, hi);
+}
+
 // The ring of one warp: pieces of up to kMoePiece chunks.
 template <int BS>
 struct MoeRing {
@@ -696,8 +715,10 @@ struct MoeWalk {
 
 // One phase: every group times its units.  UP: gate / up and the activation from
 // x; else: down from the activations (in PARTS addends), weighted.
-template <int BS, bool UP, int PARTS>
-__device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint8_t* ring, uint32_t& it) {
+// ready: called once when the first copies are on their way, waits for the
+// phase's other operand.
+template <int BS, bool UP, int PARTS, class Ready>
+__device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint8_t* ring, uint32_t& it, Ready ready) {
   using R = MoeRing<BS>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint8_t* codes = UP ? p.up_codes : p.down_codes;
@@ -724,7 +745,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
     __syncwarp();
     if (ahead.advance()) locate();
   }
-  bool ok = true;
+  bool ok = ready();
   auto unit_of = [&](auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
     const int u = w.unit, count = s.g_count[w.group], share = w.whole ? 1 : w.share, part = w.part;
@@ -878,29 +899,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_experts_kernel(const __gri
   }
   route(p, s);
   uint32_t it = 0;  // pieces this warp has consumed
-  run_phase<BS, true, 1>(p, s, ring, it);
-  if (!grid_barrier(p.barrier, s)) return;
-  run_phase<BS, false, PARTS>(p, s, ring, it);
+  run_phase<BS, true, 1>(p, s, ring, it, [] { return true; });
+  run_phase<BS, false, PARTS>(p, s, ring, it, [&] { return grid_barrier(p.barrier, s); });
   if (!grid_barrier(p.barrier + 1, s)) return;
   const int h4 = p.H / 4;
-  for (int i = blockIdx.x * kMoeThreads + threadIdx.x; i < p.T * h4; i += gridDim.x * kMoeThreads) {
-    const int t = i / h4, h = i % h4;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int k = 0; k < p.top; ++k) {
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.y + (int64_t)(t * p.top + k) * p.H) + h);
-      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-    }
-    uint32_t lo, hi;
-    if (p.dtype == kDtBF16) {
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
-    } else {
-      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(v.y), "f"(v.x));
-      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.w), "f"(v.z));
-    }
-    reinterpret_cast<uint2*>(p.out)[i] = make_uint2(lo, hi);
-  }
+  for (int i = blockIdx.x * kMoeThreads + threadIdx.x; i < p.T * h4; i += gridDim.x * kMoeThreads) add_experts(p, i / h4, i % h4);
 }
 
 // ---------------------------------------------------------------------------
