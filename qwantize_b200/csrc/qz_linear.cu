@@ -1164,6 +1164,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  // the last of the leader's signals: all before it have come
+  if (warp == 1 && rank == 1) mbar_wait_bounded(mma_done, 0u, kDevErrMmaTimeout);
+  __syncthreads();
   cluster_sync();  // neither CTA's memory is read or signalled any more
   if (warp == 1) {
     tc_fence_after();
