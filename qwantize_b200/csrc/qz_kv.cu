@@ -9,7 +9,8 @@
 //              of a group sharing one head of the cache
 //
 // The attention reads each code once and is bound by HBM: 2 D bytes per token and
-// head.  Layout inside a (page, head) block of 64 D bytes, so that a warp's
+// head (32 sequences up to 32768 tokens, 8 heads of 128, E4M3: 1.09 GB in 180 us,
+// 6.0 TB/s).  Layout inside a (page, head) block of 64 D bytes, so that a warp's
 // 16-byte loads are contiguous and are the A fragments of mma.m16n8k16 after an
 // exact conversion to fp16 (int8 and E4M3 both fit):
 //   keys    token n = 16 t + 2 j + e, value d at ((j D/64 + d/64) 8 + 2 t + e) 64 + d % 64
@@ -161,7 +162,9 @@ __device__ __forceinline__ uint32_t abs_max16(uint32_t m, uint32_t w) {
 // kept in registers; the block is rebuilt in shared memory and written whole.  A
 // decode step is one such round trip.  Threads own 8 values of a token (keys) or
 // two values of 4 neighbouring slots (values), so that a word of the block has one
-// owner.
+// owner.  Prompts are bound by instructions, 16 per value: 8 of 1900 tokens, 8 heads
+// of 128, E4M3, in 26 us (69% of the issue slots).  64 single tokens: 12.5 us, most
+// of it the chain of reads: length, table, block.
 template <int KV, int D, int DT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kStride = 68;  // bytes between value rows in shared memory: words of neighbouring rows in different banks
@@ -329,7 +332,8 @@ __device__ __forceinline__ void store16or32(void* out, int64_t i, float v) {
 }
 
 // One CTA per (page of the list, head, keys or values): codes times scale, (n,
-// Hkv, 64, D).  Bound by the writes: four times the codes' bytes for fp32.
+// Hkv, 64, D).  Bound by the writes: four times the codes' bytes for fp32 (91 MB in
+// 17.2 us).
 template <int KV, int D, int DT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
                                                       const float* __restrict__ ks, const float* __restrict__ vs,

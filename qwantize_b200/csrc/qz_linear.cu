@@ -20,6 +20,7 @@
 //   the ring once: the bytes of W bound it.  Where the tiles leave SMs idle, a
 //   cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
 //   through distributed shared memory, each CTA finishing its share of the columns.
+//   1 x 2560 x 9728: 9.5 us, 1 x 8192 x 28672: 31 us (132 MB).
 //
 //   linear_pair_kernel (prompts): a pair of CTAs on 256 tokens x 256 features; the
 //   tensor cores bound it.
@@ -488,29 +489,64 @@ struct LinOutRows {
 #pragma unroll
       for (int q = 0; q < C; ++q) v[q] = __fmul_rn(v[q], scale);
     }
-    if (p.tma_out) {
-      if (ra0 + (row & ~31) >= p.T) return;
-      // 32 rows of 64 bytes, 64-byte swizzle; the tensor map clips rows and columns beyond the result
-      unsigned char* stage = smem_out + (row >> 5) * 2048;
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      __syncwarp();
+    // 32 rows of 64 bytes per warp, 16-byte pieces swizzled: a row at a time leaves for memory from here, since
+    // lanes that each write their own row touch 32 sectors with every store (3841 x 1424 x 2630: 140 us with the call,
+    // 39 this way, 29 with 16-byte rows and TMA)
+    const int64_t r0 = ra0 + (row & ~31);
+    if (r0 >= p.T) return;
+    unsigned char* stage = smem_out + (row >> 5) * 2048;
+    auto piece = [&](int r, int q) { return stage + r * 64 + ((q ^ (r >> 1 & 3)) << 4); };
+    if (p.out_dtype == kDtF32) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
-            make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
-                       pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
+      for (int half = 0; half < 2; ++half) {
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(piece(lane, q)) =
+              make_float4(v[16 * half + 4 * q], v[16 * half + 4 * q + 1], v[16 * half + 4 * q + 2], v[16 * half + 4 * q + 3]);
+        __syncwarp();
+        const int k = lane & 15, col = c + 16 * half + k;
+        float* to = static_cast<float*>(p.out) + (r0 + (lane >> 4)) * p.ldo + cb + col;
+#pragma unroll 1
+        for (int r = lane >> 4; r < 32; r += 16) {
+          float x[8];  // all loads before the first store
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float*>(piece(r + 2 * i, k >> 2) + (k & 3) * 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i, to += 2 * p.ldo)
+            if (r0 + r + 2 * i < p.T && col < cols) *to = x[i];
+        }
+      }
+      return;
+    }
+    if (p.tma_out && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4*>(piece(lane, q)) =
+          make_uint4(pack16(v[8 * q], v[8 * q + 1], p.out_dtype), pack16(v[8 * q + 2], v[8 * q + 3], p.out_dtype),
+                     pack16(v[8 * q + 4], v[8 * q + 5], p.out_dtype), pack16(v[8 * q + 6], v[8 * q + 7], p.out_dtype));
+    if (p.tma_out) {  // the tensor map clips rows and columns beyond the result
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_out),
-                     "r"((int)cb + c), "r"((int)ra0 + (row & ~31)), "r"(smem_u32(stage))
+                     "r"((int)cb + c), "r"((int)r0), "r"(smem_u32(stage))
                      : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
-    } else if (in) {
+    } else {  // rows that are not 16-byte aligned
+      __syncwarp();
+      uint16_t* to = static_cast<uint16_t*>(p.out) + r0 * p.ldo + cb + c + lane;
+#pragma unroll 1
+      for (int r = 0; r < 32; r += 8) {
+        uint16_t x[8];  // all loads before the first store
 #pragma unroll
-      for (int q = 0; q < C; ++q)
-        if (c + q < cols) store_any(p.out, p.out_dtype, ra * p.ldo + cb + c + q, v[q]);
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint16_t*>(piece(r + i, lane >> 3) + (lane & 7) * 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i, to += p.ldo)
+          if (r0 + r + i < p.T && c + lane < cols) *to = x[i];
+      }
     }
   }
 };
@@ -830,7 +866,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 // own tokens; the tensor cores of both read both halves of B.  A stage is then
 // 38 KB per SM for 512 clocks of MMAs, where one CTA on 128 x 256 needs 55 KB: the
 // SMs take about 64 bytes per clock from L2, and that bounded a form of one CTA
-// per tile (945 clocks a stage, 829 us for 8192 x 8192 x 28672; this one 610).
+// per tile (945 clocks a stage, 829 us for 8192 x 8192 x 28672).  This one: 610 clocks
+// a stage, 673 us alone (5.7 PFLOP/s, tensor pipe 82% active); in a row the board
+// reaches its power limit and the clock falls, 820 us.
 //
 // 320 threads: warp 0 feeds this CTA's ring; its tiles signal the leader (rank 0),
 // its scales this CTA.  Warps 6-9 put a stage's scales in this CTA's TMEM (its

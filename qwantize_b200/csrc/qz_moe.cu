@@ -37,6 +37,13 @@
 // instruction and 16-bit operands in shared memory; with 1 to 32 tokens per expert
 // the matrix work is a tenth of what mma.sync can do while HBM delivers the codes.
 //
+// Measured, router and experts: 1 token, 8 of 128 experts of 2048 x 768, NVFP4: 8.9
+// and 22.9 us (21 MB; latency of launches, routing and barriers); 64 tokens, 8 of 64
+// of 2560 x 1280: 10.3 and 111 us (354 MB, 3.2 TB/s).  There a warp spends about 120
+// instructions on a chunk of 64 columns, half of them on unpacking and scaling,
+// and four warps per scheduler cover the latencies between them to 43% of the
+// issue slots; more warps leave too few registers (12, 16, 20 and 24 were tried).
+//
 // fp16 operands: a bf16 token is scaled by the power of two that puts its
 // largest magnitude in [2^14, 2^15), exact for values within 2^-28 of it.  An
 // activation row is scaled by a power of two from the bound |silu(g) u| <= |g| |u|
@@ -415,7 +422,8 @@ __device__ __forceinline__ bool grid_barrier(int* counter, MoeShared& s) {
   return s.ok != 0;
 }
 
-// Relative time of a unit with one or two tiles of 8 tokens.
+// Relative time of a unit with one or two tiles of 8 tokens: a chunk's unpacking is
+// shared, its products are not (about 110 and 135 instructions).
 __device__ __forceinline__ int unit_cost(int tokens) { return tokens <= 8 ? 4 : 5; }
 
 __device__ __forceinline__ void route(const MoeParams& p, MoeShared& s) {
