@@ -141,8 +141,9 @@ def kv_cache_read(cache, pages, dtype=torch.float32):
     assert dtype in L.DTYPE_CODES, f"unsupported dtype {dtype}"
     n = pages.shape[0]
     shape = (n, cache.kv_heads, PAGE, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.device)
+    rows = PAGE * cache.head_dim
+    strides = (cache.kv_heads * rows, rows, cache.head_dim, 1)
+    k, v = L.empty(shape, strides, dtype, cache.device), L.empty(shape, strides, dtype, cache.device)
     with L.on_device(cache.device) as stream:
         st = cache.lib.qz_kv_read(*cache.args, pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), L.DTYPE_CODES[dtype], stream)
     if st:
@@ -166,7 +167,7 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     q, q0, q1 = _rows16(q, "q", (Hq, D), dev)
     assert B <= 4096, f"{B} sequences, expected at most 4096"
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+        out = L.empty((B, Hq, D), (Hq * D, D, 1), q.dtype, dev)
     else:
         assert tuple(out.shape) == (B, Hq, D) and out.dtype == q.dtype and out.device == dev and out.is_contiguous(), (
             f"out must be a contiguous {q.dtype} tensor of shape {(B, Hq, D)} on {dev}")

@@ -156,7 +156,7 @@ def fp4_linear(x, weight, bias=None, out_dtype=None, out=None):
         bias = bias.to(dev).contiguous()
         bias_ptr, bias_code = bias.data_ptr(), codes[bias.dtype]
     if out is None:
-        y = torch.empty(shape, dtype=out_dtype, device=dev)
+        y = L.empty(shape, (N, 1), out_dtype, dev) if len(shape) == 2 else torch.empty(shape, dtype=out_dtype, device=dev)
     else:
         y = out
         assert tuple(y.shape) == shape and y.dtype == out_dtype and y.device == dev and y.is_contiguous(), (

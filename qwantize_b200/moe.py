@@ -109,15 +109,17 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     if r.data_ptr() % 16:
         r = r.clone()
     if out is None:
-        y = torch.empty(x.shape, dtype=dtype, device=dev)
+        y = L.empty(x.shape, (H, 1), dtype, dev) if x.ndim == 2 else torch.empty(x.shape, dtype=dtype, device=dev)
     else:
         y = out
         assert y.shape == x.shape and y.dtype == dtype and y.device == dev and y.is_contiguous(), (
             f"out must be a contiguous {dtype} tensor of shape {tuple(x.shape)} on {dev}")
     ids = weights = None
     if return_routing:
-        ids = torch.empty((*x.shape[:-1], top_k), dtype=torch.int32, device=dev)
-        weights = torch.empty((*x.shape[:-1], top_k), dtype=torch.float32, device=dev)
+        ids = L.empty((T, top_k), (top_k, 1), torch.int32, dev)
+        weights = L.empty((T, top_k), (top_k, 1), torch.float32, dev)
+        if x.ndim != 2:
+            ids, weights = ids.view(*x.shape[:-1], top_k), weights.view(*x.shape[:-1], top_k)
     if T:
         n = experts.workspace_bytes(T, top_k)
         with L.on_device(dev) as stream:
