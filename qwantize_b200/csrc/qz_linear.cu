@@ -20,7 +20,7 @@
 //   the ring once: the bytes of W bound it.  Where the tiles leave SMs idle, a
 //   cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
 //   through distributed shared memory, each CTA finishing its share of the columns.
-//   1 x 2560 x 9728: 9.5 us, 1 x 8192 x 28672: 31 us (132 MB).
+//   1 x 2560 x 9728: 9.5 us, 1 x 8192 x 28672: 28 us (132 MB), with the quantization.
 //
 //   linear_pair_kernel (prompts): a pair of CTAs on 256 tokens x 256 features; the
 //   tensor cores bound it.
@@ -273,22 +273,25 @@ struct LinearParams {
 };
 
 // The form of few tokens: A = weight rows, B = tokens.  HERE: the CTA quantizes a
-// single token itself and keeps the codes and scales of all its stages.
+// single token itself and keeps the codes and scales of all its stages.  CTAS per SM:
+// two where there are more tiles than SMs (16 and 32 tokens; for 64 the ring would
+// be too short): all stream at once instead of in one full wave and one that is not.
+// 4 x 8192 x 28672: 32.5 us with one, 28.4 with two; 4 x 2560 x 19456: 14.2, 10.6.
 constexpr int kHereStages = 16;
-template <int BN, int BS, bool HERE>
+template <int BN, int BS, bool HERE, int CTAS>
 struct LinGeo {
   static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
   static constexpr int kSf = Fmt<BS>::kSfBytes;
   static constexpr int kRing = HERE ? kABytes : kABytes + kBBytes, kRingSf = HERE ? kSf : 2 * kSf;  // of a stage
   static constexpr int kKeep = HERE ? kHereStages * (kBBytes + kSf) : 0;
-  static constexpr int kMaxStages = (232448 - 1024 - 768 - kKeep) / (kRing + kRingSf);
+  static constexpr int kMaxStages = ((CTAS == 1 ? 232448 : 115712) - 1024 - 768 - kKeep) / (kRing + kRingSf);
   static constexpr int kStages = kMaxStages > 10 ? 10 : kMaxStages;
   static constexpr int kSmem = kStages * (kRing + kRingSf) + kKeep + 1024 + 768;
   // TMEM columns: two accumulators, then kSfBufs buffers of scales (kGroups * 4 of A, as many of B)
   static constexpr int kSfCols = Fmt<BS>::kGroups * 4 * 2;
   static constexpr int kSfBufs = 4;
-  static constexpr int kAccCols = 2 * BN;
-  static_assert(kAccCols + kSfBufs * kSfCols <= 512, "TMEM columns");
+  static constexpr int kAccCols = 2 * BN, kTmemCols = 512 / CTAS;
+  static_assert(kAccCols + kSfBufs * kSfCols <= kTmemCols && kStages >= kSfBufs, "TMEM columns");
 };
 
 // Block-scaled MMA, E2M1 x E2M1 -> fp32, K = 64, scales of A and B in TMEM:
@@ -600,14 +603,14 @@ __device__ __forceinline__ void quantize_here(const LinearParams& p, int s0, int
 }
 
 // HERE: the type of the one token that this kernel quantizes itself (-1: an earlier launch does)
-template <int BN, int BS, int HERE>
-__global__ void __launch_bounds__(kLinThreads, 1)
+template <int BN, int BS, int HERE, int CTAS>
+__global__ void __launch_bounds__(kLinThreads, CTAS)
     linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ LinearParams p) {
   // 224 threads: warp 0 feeds the ring, warp 6 copies a stage's scales to TMEM (tcgen05.cp), warp 1 issues its four
   // block-scaled MMAs of K = 64, warps 2-5 drain the accumulator
   constexpr bool kHere = HERE >= 0;
-  using G = LinGeo<BN, BS, kHere>;
+  using G = LinGeo<BN, BS, kHere, CTAS>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // operands (1024-byte swizzle atoms), the scales of all stages, barriers
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     *abort_s = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(tmem_base_s, 512);
+  if (warp == 1) tmem_alloc(tmem_base_s, G::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -854,7 +857,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    tmem_dealloc(tmem_base, G::kTmemCols);
   }
 }
 
@@ -1258,6 +1261,7 @@ struct LinPlan {
   int bn, split, n_steps;
   int gran;   // rows of a tile of x's scales
   bool here;  // the product's kernel quantizes the token itself
+  bool two;   // two CTAs per SM
   int64_t tiles_a, tiles_b, ldp;
   int64_t off_sf, off_scale, bytes;
 };
@@ -1265,15 +1269,16 @@ struct LinPlan {
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Chooses the form by an estimate in microseconds: waves of tiles x stages x time
-// of a stage, what follows the last stage, and a cluster's exchange of sums.
-// The times were fitted to measurements of every form at 1 .. 2048 tokens and
-// (K, N) = (1024, 1024), (2560, 9728), (9728, 2560), (4096, 4096) and
-// (8192, 28672); the choice is the fastest or within 10% of it in all.  Some, in
-// microseconds with the quantization: 2560 x 9728, 64 tokens: 64 columns 13.4, 32
-// (two waves) 14.7, pair 14.5; 128 tokens: 16.8, 18.6, pair 14.8; 2048 tokens: 128
-// columns 84.4, pair 36.2.  9728 x 2560, 1 token: clusters of 4, 2, 1: 12.7, 14.8,
-// 18.9; 64 tokens: 64 columns and clusters of 4 16.8, 16 columns alone 20.9.
-// 128 columns were never the fastest by more than 8% and are not built.
+// of a stage (1.4 of it where two CTAs share an SM), what follows the last stage,
+// and a cluster's exchange of sums.  The times were fitted to measurements of every
+// form at 1 .. 2048 tokens and (K, N) = (1024, 1024), (2560, 9728), (9728, 2560),
+// (4096, 4096), (2560, 19456) and (8192, 28672); the choice is the fastest or within
+// 10% of it in all.  Some, in microseconds with the quantization: 2560 x 9728, 64
+// tokens: 32 columns (two CTAs per SM) 12.5, 64 13.2, 16 14.5, pair 14.5; 192 tokens:
+// 16.8, 18.9, pair 14.8.  9728 x 2560, 1 token: clusters of 4, 2, 1: 12.7, 14.8, 18.9;
+// 64 tokens: 64 columns and clusters of 4 16.8, 16 columns alone 20.9.  8192 x 28672, 64
+// tokens: 64 columns 35.2, 32 43.4, pair 37.2.  128 columns were never the fastest by
+// more than 8% (2560 x 9728, 2048 tokens: 84.4, pair 36.2) and are not built.
 struct LinForm {
   int bn;               // tokens of a tile (256: the pair form)
   double stage, last, join;
@@ -1289,14 +1294,15 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     if (!pair && T > 8 * f.bn) continue;  // W would pass through L2 more than eight times
     const int64_t ta = pair ? (T + 255) / 256 : (N + 127) / 128;
     const int64_t tb = pair ? (N + 255) / 256 : (T + f.bn - 1) / f.bn;
-    const int64_t slots = pair ? sms / 2 : sms;
     for (int split : {1, 2, 4, 8}) {
       if (split > 1 && (pair || split > n_steps || ta * tb * split > sms)) break;
-      const double waves = (double)((ta * tb * split + slots - 1) / slots);
+      const bool two = f.bn <= 32 && ta * tb > sms;
+      const int64_t slots = pair ? sms / 2 : two ? sms * 2 : sms;
+      const double waves = (double)((ta * tb * split + slots - 1) / slots) * (two ? 1.4 : 1.0);
       const double cost = waves * ((n_steps + split - 1) / split) * f.stage + f.last + (split > 1 ? f.join : 0.0);
       if (best_cost < 0 || cost < best_cost) {
         best_cost = cost;
-        best.bn = f.bn; best.split = split; best.tiles_a = ta; best.tiles_b = tb;
+        best.bn = f.bn; best.split = split; best.two = two; best.tiles_a = ta; best.tiles_b = tb;
       }
     }
   }
@@ -1304,7 +1310,7 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
   // a single token, quantized by every CTA for itself: no first launch.  On the device 8.6 us instead of 10.6
   // (MXFP4) and 10.6 instead of 10.6 (NVFP4) at 2560 x 9728, and a launch less for the host; with 2 tokens 10.6 and
   // 11.6 instead of 10.6, with 8 12.9 and 20.9, in a form for several.
-  best.here = best.bn == 16 && T == 1 && (n_steps + best.split - 1) / best.split <= kHereStages;
+  best.here = best.bn == 16 && T == 1 && !best.two && (n_steps + best.split - 1) / best.split <= kHereStages;
   best.ldp = up(K, 32) / 2;
   best.gran = best.bn < 128 ? best.bn : 128;
   const int64_t sf_tiles = best.bn == 256 ? best.tiles_a * 2 : best.tiles_b;
@@ -1342,15 +1348,15 @@ static cudaError_t launch_quantize_rows(const QuantizeRows& q, cudaStream_t st) 
   return cudaGetLastError();
 }
 
-template <int BN, int BS, int HERE>
+template <int BN, int BS, int HERE, int CTAS>
 static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p, int sms, cudaStream_t st) {
-  using G = LinGeo<BN, BS, (HERE >= 0)>;
+  using G = LinGeo<BN, BS, (HERE >= 0), CTAS>;
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(linear_kernel<BN, BS, HERE>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+    e = cudaFuncSetAttribute(linear_kernel<BN, BS, HERE, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
@@ -1366,13 +1372,13 @@ static int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const Linea
   }
   const int64_t ctas = p.tiles_a * p.tiles_b * p.split;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(ctas < sms ? ctas : sms));
+  cfg.gridDim = dim3((unsigned)(ctas < sms * CTAS ? ctas : sms * CTAS));
   cfg.blockDim = dim3(kLinThreads);
   cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = n;
-  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS, HERE>, a, b, p), "linear launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, linear_kernel<BN, BS, HERE, CTAS>, a, b, p), "linear launch");
 }
 
 template <int BS>
@@ -1403,20 +1409,20 @@ static int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtenso
 }
 
 template <int BS>
-static int run_linear(int bn, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
+static int run_linear(int bn, bool two, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const LinearParams& p, int sms,
                       cudaStream_t st) {
   switch (bn) {
-    case 16: return launch_linear<16, BS, -1>(a, b, p, sms, st);
-    case 32: return launch_linear<32, BS, -1>(a, b, p, sms, st);
-    case 64: return launch_linear<64, BS, -1>(a, b, p, sms, st);
+    case 16: return two ? launch_linear<16, BS, -1, 2>(a, b, p, sms, st) : launch_linear<16, BS, -1, 1>(a, b, p, sms, st);
+    case 32: return two ? launch_linear<32, BS, -1, 2>(a, b, p, sms, st) : launch_linear<32, BS, -1, 1>(a, b, p, sms, st);
+    case 64: return launch_linear<64, BS, -1, 1>(a, b, p, sms, st);
     default: return launch_pair<BS>(a, b, o, p, sms, st);
   }
 }
 template <int BS>
 static int run_linear_here(int x_dtype, const CUtensorMap& a, const LinearParams& p, int sms, cudaStream_t st) {
-  if (x_dtype == kDtBF16) return launch_linear<16, BS, kDtBF16>(a, a, p, sms, st);
-  if (x_dtype == kDtF16) return launch_linear<16, BS, kDtF16>(a, a, p, sms, st);
-  return launch_linear<16, BS, kDtF32>(a, a, p, sms, st);
+  if (x_dtype == kDtBF16) return launch_linear<16, BS, kDtBF16, 1>(a, a, p, sms, st);
+  if (x_dtype == kDtF16) return launch_linear<16, BS, kDtF16, 1>(a, a, p, sms, st);
+  return launch_linear<16, BS, kDtF32, 1>(a, a, p, sms, st);
 }
 
 static int check_sizes(int64_t T, int64_t K, int64_t N, int format, int* bs) {
@@ -1520,5 +1526,5 @@ extern "C" int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T,
                   "quantize rows launch");
   if (s != QZ_OK) return s;
   const CUtensorMap &ma = swap ? mw : mx, &mb = swap ? mx : mw;
-  return bs == 16 ? run_linear<16>(pl.bn, ma, mb, mo, p, sms, st) : run_linear<32>(pl.bn, ma, mb, mo, p, sms, st);
+  return bs == 16 ? run_linear<16>(pl.bn, pl.two, ma, mb, mo, p, sms, st) : run_linear<32>(pl.bn, pl.two, ma, mb, mo, p, sms, st);
 }
