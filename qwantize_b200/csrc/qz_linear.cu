@@ -18,7 +18,7 @@
 //   linear_kernel (few tokens; BN = 16, 32 or 64): 128 rows of W are A and BN tokens
 //   are B, so that a decode step multiplies few padded rows, and W streams through
 //   the ring once: the bytes of W bound it.  Where the tiles leave SMs idle, a
-//   cluster of 2, 4 or 8 CTAs cuts K among them and adds the fp32 parts, in order,
+//   cluster of 2 or 4 CTAs cuts K among them and adds the fp32 parts, in order,
 //   through distributed shared memory, each CTA finishing its share of the columns.
 //   1 x 2560 x 9728: 9.5 us, 1 x 8192 x 28672: 28 us (132 MB), with the quantization.
 //
@@ -833,16 +833,16 @@ __global__ void __launch_bounds__(kLinThreads, CTAS)
         const uint32_t at = smem_u32(part) + out.row * 4;
         const int c_end = (rank + 1) * per < out.cols ? (rank + 1) * per : out.cols;
         for (int c0 = rank * per; c0 < c_end; c0 += 4) {
-          float x[4][8];  // all loads of four columns before the first sum
+          float x[4][4];  // all loads of four columns before the first sum
 #pragma unroll
-          for (int w = 0; w < 8; ++w)
+          for (int w = 0; w < 4; ++w)
 #pragma unroll
             for (int q = 0; q < 4; ++q) x[q][w] = w < p.split && c0 + q < c_end ? load_peer(at + (c0 + q) * 512, w) : 0.0f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float v = x[q][0];
 #pragma unroll
-            for (int w = 1; w < 8; ++w) v += x[q][w];
+            for (int w = 1; w < 4; ++w) v += x[q][w];
             const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
                                          : (c0 + q < c_end ? out.scales[c0 + q] * p.w_scale : 0.0f);
             if (c0 + q < c_end) out.store(c0 + q, v, scale);
@@ -1276,8 +1276,10 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // 10% of it in all.  Some, in microseconds with the quantization: 2560 x 9728, 64
 // tokens: 32 columns (two CTAs per SM) 12.5, 64 13.2, 16 14.5, pair 14.5; 192 tokens:
 // 16.8, 18.9, pair 14.8.  9728 x 2560, 1 token: clusters of 4, 2, 1: 12.7, 14.8, 18.9;
-// 64 tokens: 64 columns and clusters of 4 16.8, 16 columns alone 20.9.  8192 x 28672, 64
-// tokens: 64 columns 35.2, 32 43.4, pair 37.2.  128 columns were never the fastest by
+// 64 tokens, clusters of 4: 32 columns (two CTAs per SM) 14.8, 64 columns 16.8; 16
+// alone 20.9.  Clusters of 8 gained 10% or lost 30%, as they found room on the GPU
+// (8192 x 2048, 17 tokens: 10.6 against 12.5 with 4; 32 tokens: 16.8 against 12.5).
+// 8192 x 28672, 64 tokens: 64 columns 35.2, 32 43.4, pair 37.2.  128 columns were never the fastest by
 // more than 8% (2560 x 9728, 2048 tokens: 84.4, pair 36.2) and are not built.
 struct LinForm {
   int bn;               // tokens of a tile (256: the pair form)
@@ -1294,9 +1296,9 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     if (!pair && T > 8 * f.bn) continue;  // W would pass through L2 more than eight times
     const int64_t ta = pair ? (T + 255) / 256 : (N + 127) / 128;
     const int64_t tb = pair ? (N + 255) / 256 : (T + f.bn - 1) / f.bn;
-    for (int split : {1, 2, 4, 8}) {
-      if (split > 1 && (pair || split > n_steps || ta * tb * split > sms)) break;
-      const bool two = f.bn <= 32 && ta * tb > sms;
+    for (int split : {1, 2, 4}) {
+      const bool two = f.bn <= 32 && ta * tb * split > sms;
+      if (split > 1 && (pair || split > n_steps || ta * tb * split > (f.bn <= 32 ? 2 * sms : sms))) break;
       const int64_t slots = pair ? sms / 2 : two ? sms * 2 : sms;
       const double waves = (double)((ta * tb * split + slots - 1) / slots) * (two ? 1.4 : 1.0);
       const double cost = waves * ((n_steps + split - 1) / split) * f.stage + f.last + (split > 1 ? f.join : 0.0);
