@@ -838,22 +838,25 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
 
 // Joins the partial results of the (sequence, head, row tile) pairs that several
 // warps share, in the order of their pages; writes zeros for empty sequences.
-// One CTA per pair: a thread owns four values of one row and one of `split`
-// interleaved shares of the partial results (a long sequence has hundreds),
-// which then meet in shared memory.
-constexpr int kJoinThreads = 512;
+// One CTA per pair and kJoinRows rows: a thread owns four values of one row and one
+// of `split` interleaved shares of the partial results (a long sequence has
+// hundreds), which then meet in shared memory.
+constexpr int kJoinThreads = 512, kJoinRows = 4;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps) {
   extern __shared__ int prefix[];
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   const int HR = p.Hkv * p.row_tiles;
-  const int b = blockIdx.x / HR, hr = blockIdx.x % HR, head = hr / p.row_tiles, r0 = hr % p.row_tiles * p.rows_per_tile;
-  const int rows = p.G - r0 < p.rows_per_tile ? p.G - r0 : p.rows_per_tile;
+  const int b = blockIdx.x / HR, hr = blockIdx.x % HR, head = hr / p.row_tiles, rt = hr % p.row_tiles * p.rows_per_tile;
+  const int first_row = blockIdx.y * kJoinRows, r0 = rt + first_row;  // of the row tile; of the head's group
+  const int last = rt + p.rows_per_tile < p.G ? rt + p.rows_per_tile : p.G;
+  const int rows = last - r0 < kJoinRows ? last - r0 : kJoinRows;
+  if (rows <= 0) return;
   const int per = rows * (D / 4), split = kJoinThreads / per;
   const int part = threadIdx.x / per, row = threadIdx.x % per / (D / 4), d4 = threadIdx.x % (D / 4);
   page_prefix(p, prefix);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every CTA: this grid ends after the one before it
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // in every CTA with rows: this grid ends after the one before it
   const int64_t total = (int64_t)prefix[p.B] * HR;
   const int nb = prefix[b + 1] - prefix[b];
   Joined a;
@@ -869,7 +872,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 #pragma unroll 4
       for (int i = part; i < count; i += split) {
         const int64_t w = total >= warps ? w0 + i : ((u0 + i + 1) * warps - 1) / total;
-        const int64_t at = (w * 2 + (i == 0 ? first : 0)) * 16 + row;
+        const int64_t at = (w * 2 + (i == 0 ? first : 0)) * 16 + first_row + row;
         a.take(__ldcg(reinterpret_cast<const float2*>(p.part_ml) + at), __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4));
       }
     }
@@ -949,7 +952,7 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)pairs);
+  cfg.gridDim = dim3((unsigned)pairs, (unsigned)((p.rows_per_tile + kJoinRows - 1) / kJoinRows));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = (size_t)(p.B + 1) * 4;
   cfg.stream = st;
