@@ -395,6 +395,7 @@ struct AttnParams {
   int64_t num_pages;
   int B, Hkv, G;                 // G query heads per cache head ...
   int row_tiles, rows_per_tile;  // ... in row_tiles tiles of 8 or 16
+  int join_rows;                 // rows of a CTA of the joining launch
   const uint16_t* q;             // (B, Hkv * G, D), strides in elements
   int64_t q_seq, q_head;
   int dtype;
@@ -838,10 +839,10 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
 
 // Joins the partial results of the (sequence, head, row tile) pairs that several
 // warps share, in the order of their pages; writes zeros for empty sequences.
-// One CTA per pair and kJoinRows rows: a thread owns four values of one row and one
+// One CTA per pair and join_rows rows: a thread owns four values of one row and one
 // of `split` interleaved shares of the partial results (a long sequence has
 // hundreds), which then meet in shared memory.
-constexpr int kJoinThreads = 512, kJoinRows = 4;
+constexpr int kJoinThreads = 512;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttnParams p, int64_t warps) {
   extern __shared__ int prefix[];
@@ -849,9 +850,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   __shared__ float2 s_ml[kJoinThreads];
   const int HR = p.Hkv * p.row_tiles;
   const int b = blockIdx.x / HR, hr = blockIdx.x % HR, head = hr / p.row_tiles, rt = hr % p.row_tiles * p.rows_per_tile;
-  const int first_row = blockIdx.y * kJoinRows, r0 = rt + first_row;  // of the row tile; of the head's group
+  const int first_row = blockIdx.y * p.join_rows, r0 = rt + first_row;  // of the row tile; of the head's group
   const int last = rt + p.rows_per_tile < p.G ? rt + p.rows_per_tile : p.G;
-  const int rows = last - r0 < kJoinRows ? last - r0 : kJoinRows;
+  const int rows = last - r0 < p.join_rows ? last - r0 : p.join_rows;
   if (rows <= 0) return;
   const int per = rows * (D / 4), split = kJoinThreads / per;
   const int part = threadIdx.x / per, row = threadIdx.x % per / (D / 4), d4 = threadIdx.x % (D / 4);
@@ -909,12 +910,12 @@ static bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 !=
 
 // Whether each (sequence, head, row tile) pair is given to one CTA, in one launch,
 // instead of cutting all pages evenly and joining in a second one: with at most a
-// CTA per SM, and at most four pages in a row for a warp by the table's width.
+// CTA per SM, and at most two pages in a row for a warp by the table's width.
 // Microseconds alone / evenly, 8 cache heads of 128, groups of 4, int8: 1 sequence
-// of 300 tokens 8.5 / 12.0, of 2000 16.7 / 14.7, of 8000 41 / 29; 8 of 1000 12.6 / 14.7,
-// 32 of 1000 (256 pairs) 24.5 / 20.8; groups of 16, 1 of 2000: 20.8 / 29.0.
+// of 300 tokens 8.5 / 12.0, of 1000 12.6 / 12.6, of 2000 16.7 / 14.7, of 8000 41 / 27; 8 of
+// 1000 12.6 / 14.7, 32 of 1000 (256 pairs) 24.5 / 20.8.
 static bool attention_alone(int64_t pairs, int64_t max_pages, int sms, int warps) {
-  return pairs <= sms && max_pages <= 4 * warps;
+  return pairs <= sms && max_pages <= 2 * warps;
 }
 
 template <int D, int KV, int NH, bool ONE>
@@ -943,6 +944,9 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
     kv_attention_kernel<D, KV, NH, true><<<(unsigned)pairs, G::kWarps * 32, G::smem(0), st>>>(p);
     return cuda_status(cudaGetLastError(), "kv attention launch");
   }
+  // few pairs have many partial results each: more CTAs share a pair's (1 sequence of 4528 tokens, 128 heads on 8: 47
+  // us with 16 rows per CTA, 22.5 with 4; 32 of 300 tokens, the same heads: 20.8 and 28.8)
+  p.join_rows = pairs <= sms ? 4 : p.rows_per_tile;
   int s = prepare_attention<D, KV, NH, false>();
   if (s != QZ_OK) return s;
   kv_attention_kernel<D, KV, NH, false><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
@@ -952,7 +956,7 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)pairs, (unsigned)((p.rows_per_tile + kJoinRows - 1) / kJoinRows));
+  cfg.gridDim = dim3((unsigned)pairs, (unsigned)(p.rows_per_tile / p.join_rows));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = (size_t)(p.B + 1) * 4;
   cfg.stream = st;
