@@ -324,10 +324,10 @@ QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int6
  * over them (renormalize != 0) or over all experts as weights c, and
  * out = sum c * D_e (silu(G_e x) * (U_e x)), fp32 sums, one rounding to x's type.
  *   x        (T, H) bf16 or fp16, rows ldx elements apart, 16-byte aligned
- *   router   (E, H) fp32, bf16 or fp16;  E <= 512, top_k <= 16
+ *   router   (E, H) fp32, bf16 or fp16, 16-byte aligned;  E <= 512, top_k <= 16
  *   *_codes, *_scales, up_norms, *_tensor_scale: from qz_moe_layout; gate / up (2 I, H) and
  *            down (H, I), I and H multiples of 32
- *   out      (T, H) of x's type;  ids (T, top_k) and weights (T, top_k): the
+ *   out      (T, H) of x's type, 8-byte aligned;  ids (T, top_k) and weights (T, top_k): the
  *            routing, descending logits (NULL: not written)
  *   workspace  qz_moe_workspace bytes, 256-byte aligned, not shared by calls
  *            that can overlap

@@ -1009,8 +1009,9 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   if (ldx < H || ldx % 8) return fail(QZ_ERR_INVALID, "rows of x must be at least H apart and 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(up_codes) |
        reinterpret_cast<uintptr_t>(up_scales) | reinterpret_cast<uintptr_t>(down_codes) |
-       reinterpret_cast<uintptr_t>(down_scales)) % 16 || reinterpret_cast<uintptr_t>(workspace) % 256)
-    return fail(QZ_ERR_INVALID, "inputs must be 16-byte aligned, workspace 256-byte");
+       reinterpret_cast<uintptr_t>(down_scales)) % 16 || reinterpret_cast<uintptr_t>(workspace) % 256 ||
+      (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(up_norms)) % 8)  // pairs of norms, four results at once
+    return fail(QZ_ERR_INVALID, "inputs must be 16-byte aligned, up_norms and out 8-byte, workspace 256-byte");
   const MoeWorkspace w = moe_workspace(T, H, I, top_k);
   if (workspace_bytes < w.bytes)
     return fail(QZ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.bytes);

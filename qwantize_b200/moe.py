@@ -114,6 +114,8 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
         y = out
         assert y.shape == x.shape and y.dtype == dtype and y.device == dev and y.is_contiguous(), (
             f"out must be a contiguous {dtype} tensor of shape {tuple(x.shape)} on {dev}")
+        if y.data_ptr() % 8:  # a view at an odd offset: the kernel stores four values at once
+            y = torch.empty(x.shape, dtype=dtype, device=dev)
     ids = weights = None
     if return_routing:
         ids = L.empty((T, top_k), (top_k, 1), torch.int32, dev)
@@ -133,6 +135,8 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
                 L.give_scratch(ws)
         if st:
             L.check(st, "qz_moe")
+    if out is not None and y is not out:
+        y = out.copy_(y)
     res = (y, ids, weights) if return_routing else (y,)
     if not x.is_cuda and out is None:
         res = to_host_like(res, x.device, dev)
