@@ -412,7 +412,7 @@ struct AttnParams {
 __device__ __forceinline__ int pages_of(const AttnParams& p, int b) {
   const int len = p.lengths[b];
   if (len <= 0) return 0;
-  const int nb = (len + kPage - 1) / kPage;
+  const int nb = (len - 1) / kPage + 1;  // any length of 32 bits, also one that stands for "all"
   return nb < p.max_pages ? nb : p.max_pages;
 }
 

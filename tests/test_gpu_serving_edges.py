@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tests.test_gpu_kv_cache import CACHES, check, queries, setup
 from tests.test_gpu_moe import make, router_of, tokens
 
 pytestmark = pytest.mark.gpu
@@ -23,3 +24,18 @@ def test_moe_into_a_view_at_an_odd_offset(dtype):
         assert torch.equal(out, want) and bool((buf[:off] == 7).all()) and bool((buf[off + x.numel():] == 7).all())
         got, ids, _ = q.fp4_moe(x, r, ex, 2, return_routing=True, out=out)
         assert got is out and ids.shape == (3, 2)
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("extra", [0, 130])
+def test_attention_lengths_up_to_the_largest_int32(dtype, extra):
+    """A length beyond the table means all of it, up to 2^31 - 1 (rounding it up to
+    whole pages must not wrap); extra columns take the form of wide tables."""
+    import qwantize_b200 as q
+    c, codes, table, _ = setup(3, [128] * 3, 2, 64, dtype, 41)
+    full = torch.cat([table, table.new_full((3, extra), -1)], 1)
+    x = queries(3, 8, 64, torch.bfloat16, 42)
+    have = torch.tensor([128, 70, 128], dtype=torch.int32, device=DEV)
+    for big in (2**31 - 1, 2**31 - 2, 2**31 - 63, 2**31 - 64, 2**31 - 65):
+        lengths = torch.tensor([big, 70, big], dtype=torch.int32, device=DEV)
+        check(q.kv_cache_attention(c, x, full, lengths), x, *codes, table, have)
