@@ -991,6 +991,7 @@ extern "C" int qz_kv_append(uint8_t* k, float* k_scale, uint8_t* v, float* v_sca
     return fail(QZ_ERR_INVALID, "caches and rows of new tokens must be 16-byte aligned");
   int sms = 0;
   if ((s = current_sms(&sms)) != QZ_OK) return s;
+  if (max_new > N) max_new = N;
   // a run of max_new tokens touches at most this many pages, wherever it starts
   int64_t touched = (max_new + kPage - 2) / kPage + 1;
   if (touched > max_pages) touched = max_pages;

@@ -39,3 +39,19 @@ def test_attention_lengths_up_to_the_largest_int32(dtype, extra):
     for big in (2**31 - 1, 2**31 - 2, 2**31 - 63, 2**31 - 64, 2**31 - 65):
         lengths = torch.tensor([big, 70, big], dtype=torch.int32, device=DEV)
         check(q.kv_cache_attention(c, x, full, lengths), x, *codes, table, have)
+
+
+def test_append_takes_any_upper_limit():
+    """max_new is an upper limit: one beyond the new tokens, up to 2^63 - 1, changes nothing."""
+    import qwantize_b200 as q
+    g = torch.Generator().manual_seed(43)
+    k = torch.randn(70, 2, 64, generator=g).to(torch.bfloat16).to(DEV)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([3, 0], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 69, 70], dtype=torch.int32, device=DEV)
+    caches = []
+    for most in (69, None, 1 << 40, 2**63 - 1):
+        caches.append(q.KVCache8(4, 2, 64))
+        q.kv_cache_append(caches[-1], k, k, table, lengths, cu_new=cu, max_new=most)
+    assert caches[0].k[1].any()
+    assert all(torch.equal(c.k, caches[0].k) and torch.equal(c.v_scale, caches[0].v_scale) for c in caches[1:])
