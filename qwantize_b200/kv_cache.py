@@ -86,17 +86,27 @@ def _table(block_table, lengths, cache):
     return table, lengths, B, pages, ld
 
 
+def _strides(x):
+    """The strides of x (n, heads, D), with those of single elements, which torch
+    keeps as they were cut, also through contiguous(), as in contiguous rows."""
+    s0, s1, s2 = x.stride()
+    n, heads, D = x.shape
+    if heads <= 1 or n == 0:
+        s1 = D
+    return heads * D if n <= 1 else s0, s1, s2
+
+
 def _rows16(x, name, shape_tail, dev):
     """x (n, heads, D) of 16 bits with contiguous, 16-byte aligned rows, and its strides."""
     assert x.ndim == 3 and x.shape[1:] == shape_tail, f"{name} is {tuple(x.shape)}, expected (n, {shape_tail[0]}, {shape_tail[1]})"
     assert x.dtype == torch.bfloat16 or x.dtype == torch.float16, f"unsupported dtype {x.dtype}, expected bfloat16 or float16"
     assert x.device == dev, f"{name} is on {x.device}, the cache on {dev}"
-    s0, s1, s2 = x.stride()
+    s0, s1, s2 = _strides(x)
     if s2 != 1 or s1 % 8 or s0 % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        s0, s1, _ = x.stride()
+        s0, s1, _ = _strides(x)
     return x, s0, s1
 
 

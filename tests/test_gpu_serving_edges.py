@@ -55,3 +55,18 @@ def test_append_takes_any_upper_limit():
         q.kv_cache_append(caches[-1], k, k, table, lengths, cu_new=cu, max_new=most)
     assert caches[0].k[1].any()
     assert all(torch.equal(c.k, caches[0].k) and torch.equal(c.v_scale, caches[0].v_scale) for c in caches[1:])
+
+
+def test_one_sequence_of_one_head_cut_from_odd_rows():
+    import qwantize_b200 as q
+    c, codes, table, lengths = setup(1, [100], 1, 64, torch.int8, 44)
+    wide = queries(2, 1, 68, torch.bfloat16, 45)
+    for first in (0, 4):
+        x = wide[:1, :, first: first + 64]
+        check(q.kv_cache_attention(c, x, table, lengths), x, *codes, table, lengths)
+        a, b = q.KVCache8(2, 1, 64), q.KVCache8(2, 1, 64)
+        n = torch.zeros(1, dtype=torch.int32, device=DEV)
+        t = torch.ones(1, 1, dtype=torch.int32, device=DEV)
+        q.kv_cache_append(a, x, x, t, n)
+        q.kv_cache_append(b, x.clone(), x.clone(), t, n)
+        assert a.k.any() and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
