@@ -483,6 +483,13 @@ struct Joined {
   }
 };
 
+// Probabilities go to the value product as fp16 at 2^15 times their value over the
+// largest so far: one above 2^-29 of the largest keeps 11 bits, and none is off by
+// more than 2^-40 of it (at their own value: 2^-14 and 2^-25, and where the largest
+// has a small value, thousands of small ones make up the result).  Their sum is of
+// the unrounded ones, in fp32.
+constexpr float kProbUp = 0x1p15f, kProbDown = 0x1p-15f;
+
 // NH tiles of 8 query heads share the warp's pass over a page.  Warps per SM:
 // what the registers allow (D = 128: 12 of at most 168 with one tile; two tiles
 // keep twice the sums: 8) and the ring, one page of keys and values per warp.
@@ -722,7 +729,9 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
         for (int c = 0; c < 4; ++c) s[i][n][c] = exp2_fast(s[i][n][c] - z[c & 1]);
         sum[0] += s[i][n][0] + s[i][n][2];
         sum[1] += s[i][n][1] + s[i][n][3];
-        const __half2 x = __floats2half2_rn(s[i][n][0], s[i][n][1]), y = __floats2half2_rn(s[i][n][2], s[i][n][3]);
+        const float2 up = make_float2(kProbUp, kProbUp);
+        const __half2 x = __float22half2_rn(mul2(make_float2(s[i][n][0], s[i][n][1]), up));
+        const __half2 y = __float22half2_rn(mul2(make_float2(s[i][n][2], s[i][n][3]), up));
         pb[i][n][0] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
         pb[i][n][1] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
       }
@@ -730,6 +739,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
       l[n][1] = fmaf(l[n][1], corr[n][1], sum[1]);
     }
     if (!mbar_wait_bounded(bar_v, parity, kDevErrLoadTimeout)) { ok = false; break; }
+    const float v_scale = vs * kProbDown;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const uint4 w0 = *reinterpret_cast<const uint4*>(ring + G::kBlock + i * 1024 + lane * 16);
@@ -757,7 +767,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
 #pragma unroll
       for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][n][c] = fmaf(d[n][c], vs, o[i][n][c] * corr[n][c & 1]);
+        for (int c = 0; c < 4; ++c) o[i][n][c] = fmaf(d[n][c], v_scale, o[i][n][c] * corr[n][c & 1]);
     }
     __syncwarp();  // every lane has read its values
     if (more) {

@@ -167,8 +167,10 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     q (B, heads, head_dim) bf16 or fp16, heads a multiple of the cache's (a
     group of neighbouring query heads shares one); the first lengths[b] tokens
     behind block_table[b] are attended to (an empty sequence gives zeros); scale
-    defaults to 1 / sqrt(head_dim).  Products of 16-bit operands (codes fit fp16
-    exactly), softmax and sums in fp32, rounded once to q's type."""
+    defaults to 1 / sqrt(head_dim).  Products of 16-bit operands: codes fit fp16
+    exactly, probabilities are rounded to it (2^-11 of their value, at most 2^-40 of
+    the largest beside that).  Softmax and sums are fp32, the result is rounded once
+    to q's type."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
     D, dev = cache.head_dim, cache.device
     assert q.ndim == 3 and q.shape[0] == B, f"q is {tuple(q.shape)}, expected ({B}, heads, {D})"
