@@ -486,7 +486,10 @@ struct Joined {
 // Probabilities go to the value product as fp16 at 2^15 times their value over the
 // largest so far: one above 2^-29 of the largest keeps 11 bits, and none is off by
 // more than 2^-40 of it (at their own value: 2^-14 and 2^-25, and where the largest
-// has a small value, thousands of small ones make up the result).  Their sum is of
+// has a small value, thousands of small ones make up the result).  For fp16 results,
+// whose own rounding is no coarser, the remainder is a second fp16 operand (PARTS = 2:
+// 2^-22 of a probability; 32 sequences of 16384 tokens, 8 heads of 128, int8, groups
+// of 8: 169-171 us, as without, groups of 16: 260 instead of 213).  Their sum is of
 // the unrounded ones, in fp32.
 constexpr float kProbUp = 0x1p15f, kProbDown = 0x1p-15f;
 
@@ -510,7 +513,7 @@ constexpr int kAttnMaxWarps = 16;
 //
 // ONE: a CTA has one pair of the list to itself, its warps cut the pair's pages and
 // join through shared memory, so short sequences need no second launch.
-template <int D, int KV, int NH, bool ONE>
+template <int D, int KV, int NH, bool ONE, int PARTS>
 __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_kernel(const __grid_constant__ AttnParams p) {
   using G = AttnGeo<D, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -697,7 +700,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
       ++issued_k;
     }
     float corr[NH][2];
-    uint32_t pb[4][NH][2];  // probabilities, fp16: the B fragments of the value product
+    uint32_t pb[PARTS][4][NH][2];  // probabilities, fp16: the B fragments of the value product
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       float z[2], sum[2] = {0.0f, 0.0f};
@@ -730,10 +733,17 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
         sum[0] += s[i][n][0] + s[i][n][2];
         sum[1] += s[i][n][1] + s[i][n][3];
         const float2 up = make_float2(kProbUp, kProbUp);
-        const __half2 x = __float22half2_rn(mul2(make_float2(s[i][n][0], s[i][n][1]), up));
-        const __half2 y = __float22half2_rn(mul2(make_float2(s[i][n][2], s[i][n][3]), up));
-        pb[i][n][0] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
-        pb[i][n][1] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 f = mul2(make_float2(s[i][n][2 * h], s[i][n][2 * h + 1]), up);
+          const __half2 x = __float22half2_rn(f);
+          pb[0][i][n][h] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&x));
+          if constexpr (PARTS == 2) {
+            const float2 b = __half22float2(x);
+            const __half2 y = __floats2half2_rn(f.x - b.x, f.y - b.y);
+            pb[1][i][n][h] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&y));
+          }
+        }
       }
       l[n][0] = fmaf(l[n][0], corr[n][0], sum[0]);
       l[n][1] = fmaf(l[n][1], corr[n][1], sum[1]);
@@ -762,7 +772,9 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
         codes_to_f16<KV>(x0[q], a0, a2);
         codes_to_f16<KV>(x1[q], a1, a3);
 #pragma unroll
-        for (int n = 0; n < NH; ++n) mma_16816(d[n], a0, a1, a2, a3, pb[q][n]);
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_16816(d[n], a0, a1, a2, a3, pb[part][q][n]);
       }
 #pragma unroll
       for (int n = 0; n < NH; ++n)
@@ -928,38 +940,38 @@ static bool attention_alone(int64_t pairs, int64_t max_pages, int sms, int warps
   return pairs <= sms && max_pages <= 2 * warps;
 }
 
-template <int D, int KV, int NH, bool ONE>
+template <int D, int KV, int NH, bool ONE, int PARTS>
 static int prepare_attention() {
   static bool attr_set[64] = {false};  // per device (a benign race: every thread sets the same value)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
   if (dev >= 0 && dev < 64 && attr_set[dev]) return QZ_OK;
-  e = cudaFuncSetAttribute(kv_attention_kernel<D, KV, NH, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  e = cudaFuncSetAttribute(kv_attention_kernel<D, KV, NH, ONE, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            AttnGeo<D, NH>::smem(kKvMaxSeqs));
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute");
   if (dev >= 0 && dev < 64) attr_set[dev] = true;
   return QZ_OK;
 }
 
-template <int D, int KV, int NH>
+template <int D, int KV, int NH, int PARTS>
 static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
   using G = AttnGeo<D, NH>;
   p.rows_per_tile = 8 * NH;
   p.row_tiles = (p.G + 8 * NH - 1) / (8 * NH);
   const int64_t pairs = (int64_t)p.B * p.Hkv * p.row_tiles;
   if (attention_alone(pairs, p.max_pages, sms, G::kWarps)) {
-    const int s = prepare_attention<D, KV, NH, true>();
+    const int s = prepare_attention<D, KV, NH, true, PARTS>();
     if (s != QZ_OK) return s;
-    kv_attention_kernel<D, KV, NH, true><<<(unsigned)pairs, G::kWarps * 32, G::smem(0), st>>>(p);
+    kv_attention_kernel<D, KV, NH, true, PARTS><<<(unsigned)pairs, G::kWarps * 32, G::smem(0), st>>>(p);
     return cuda_status(cudaGetLastError(), "kv attention launch");
   }
   // few pairs have many partial results each: more CTAs share a pair's (1 sequence of 4528 tokens, 128 heads on 8: 47
   // us with 16 rows per CTA, 22.5 with 4; 32 of 300 tokens, the same heads: 20.8 and 28.8)
   p.join_rows = pairs <= sms ? 4 : p.rows_per_tile;
-  int s = prepare_attention<D, KV, NH, false>();
+  int s = prepare_attention<D, KV, NH, false, PARTS>();
   if (s != QZ_OK) return s;
-  kv_attention_kernel<D, KV, NH, false><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
+  kv_attention_kernel<D, KV, NH, false, PARTS><<<sms, G::kWarps * 32, G::smem(p.B), st>>>(p);
   if ((s = cuda_status(cudaGetLastError(), "kv attention launch")) != QZ_OK) return s;
   // the join may begin while the last pages are read; it waits for the kernel's end before it reads results
   cudaLaunchAttribute at{};
@@ -977,7 +989,8 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
 
 template <int D, int KV>
 static int run_attention(const AttnParams& p, int sms, cudaStream_t st) {
-  return p.G <= 8 ? launch_attention<D, KV, 1>(p, sms, st) : launch_attention<D, KV, 2>(p, sms, st);
+  if (p.dtype == kDtF16) return p.G <= 8 ? launch_attention<D, KV, 1, 2>(p, sms, st) : launch_attention<D, KV, 2, 2>(p, sms, st);
+  return p.G <= 8 ? launch_attention<D, KV, 1, 1>(p, sms, st) : launch_attention<D, KV, 2, 1>(p, sms, st);
 }
 
 }  // namespace qz

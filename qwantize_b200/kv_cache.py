@@ -168,8 +168,8 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     group of neighbouring query heads shares one); the first lengths[b] tokens
     behind block_table[b] are attended to (an empty sequence gives zeros); scale
     defaults to 1 / sqrt(head_dim).  Products of 16-bit operands: codes fit fp16
-    exactly, probabilities are rounded to it (2^-11 of their value, at most 2^-40 of
-    the largest beside that).  Softmax and sums are fp32, the result is rounded once
+    exactly, probabilities are rounded to it (2^-11 of their value for bf16 results,
+    2^-22 for fp16, at most 2^-40 of the largest beside that).  Softmax and sums are fp32, the result is rounded once
     to q's type."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
     D, dev = cache.head_dim, cache.device

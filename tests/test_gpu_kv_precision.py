@@ -76,3 +76,27 @@ def test_one_dominant_token_and_many_small_ones(dtype, D, n, extra, last, gap):
         x[0, 1] *= 0.97
         out = q.kv_cache_attention(c, x, wide, lengths)
         check(out, *limits(x, k, ks, v, vs, table, n, 2.0**-11))
+
+
+@pytest.mark.parametrize("dtype", CACHES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,extra", [(2, 0), (70, 0), (2, 200), (2000, 200)])
+@pytest.mark.parametrize("heads", [5, 16])
+def test_fp16_results_of_values_that_nearly_cancel(dtype, D, n, extra, heads):
+    """fp16 results keep 11 bits, as many as a probability rounded to fp16: there the
+    remainder counts too, which leaves 2^-22 of it.  Two tokens of nearly the same
+    weight and opposite values show it."""
+    import qwantize_b200 as q
+    c, table, wide, lengths, g = cached(D, n, dtype, n + heads, extra)
+    P = c.num_pages
+    k = torch.zeros(P, 1, 64, D)
+    ks = torch.full((P, 1), 0.02 / (8 * D**0.5))  # a score is 0.0025 a code
+    v, vs = torch.zeros(P, 1, 64, D), torch.full((P, 1), 0.25)
+    value = torch.tensor([64.0, -80, 96, 112])[torch.randint(4, (D,), generator=g)]
+    for i, code, sign in ((0, 96.0, 1), (n - 1, 88.0, -1)):
+        page, slot = int(table[0, i // 64]), i % 64
+        k[page, 0, slot], v[page, 0, slot] = code, sign * value
+    k, v = encode(k, dtype), encode(v, dtype)
+    c.load_codes(k, ks, v, vs)
+    x = (torch.linspace(0.5, 2.5, heads)[:, None] * torch.ones(D)).to(torch.float16)[None].to(DEV)
+    check(q.kv_cache_attention(c, x, wide, lengths), *limits(x, k, ks, v, vs, table, n, 2.0**-22))
