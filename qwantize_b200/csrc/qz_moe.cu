@@ -59,6 +59,7 @@
 #include "../../include/qwantize_b200.h"
 #include "qz_common.cuh"
 #include "qz_kernels.h"
+#include "qz_moe_walk.cuh"
 #include "qz_ptx.cuh"
 #include "qz_tc.cuh"
 
@@ -69,11 +70,11 @@ int cuda_status(cudaError_t e, const char* what);
 int current_sms(int* sms);
 
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTop = 16;
-constexpr int kMoeWarps = 16, kMoeThreads = kMoeWarps * 32;
+constexpr int kMoeThreads = kMoeWarps * 32;
 constexpr int kMoeMaxSlots = kMoeMaxTokens * kMoeMaxTop;
 constexpr int kMoeGroup = 16;                                                  // tokens of a unit
 constexpr int kMoeMaxGroups = kMoeMaxExperts + kMoeMaxSlots / kMoeGroup;
-constexpr int kMoePiece = 4, kMoeStages = 2;                                   // chunks per bulk copy, copies in flight per warp
+constexpr int kMoeStages = 2;                                                  // copies in flight per warp
 
 struct MoeParams {
   int T, H, I, E, top;
@@ -666,61 +667,16 @@ struct MoeRing {
   static constexpr int kBytes = kMoeWarps * kMoeStages * kStage;
 };
 
-// This warp's part of a phase: `whole` units of its own, kMoeWarps apart, then
-// perhaps a share of one more.
-struct MoeWalk {
-  int group, unit;             // current group and unit in it
-  int units, chunks;           // per group; per unit
-  int left;                    // units after the current one
-  int c, c0, c1;               // current chunk; this warp's chunks of the current unit
-  int share, part;             // warps that share the last unit, this warp's place among them; 0: no last unit
-  int last_group, last_unit;
-  bool whole;                  // the current unit is this warp's alone
-
-  __device__ __forceinline__ MoeWalk(const int* bound, int units_, int chunks_) : units(units_), chunks(chunks_) {
-    const int warp = threadIdx.x >> 5;
-    const int begin = bound[0], end = bound[1];
-    const int rounds = (end - begin) / kMoeWarps, rest = (end - begin) % kMoeWarps;
-    share = rest ? kMoeWarps / rest : 1;
-    share = share < 8 ? share : 8;
-    share = share < chunks ? share : chunks;
-    const int last = begin + rounds * kMoeWarps + warp / share;
-    if (last < end) {
-      part = warp % share;
-      last_group = last / units;
-      last_unit = last % units;
-    } else {
-      share = 0;
-    }
-    left = rounds + (share ? 1 : 0);
-    whole = true;
-    c0 = 0;
-    c1 = chunks;
-    group = (begin + warp) / units;
-    unit = (begin + warp) % units;
-    enter();
-  }
-  __device__ __forceinline__ bool done() const { return left < 0; }
-  __device__ __forceinline__ void enter() {  // the next unit's first chunk
-    if (--left == 0 && share) {
-      whole = share == 1;
-      group = last_group;
-      unit = last_unit;
-      c0 = part * chunks / share;
-      c1 = (part + 1) * chunks / share;
-    }
-    c = c0;
-  }
-  __device__ __forceinline__ int piece() const { return c1 - c < kMoePiece ? c1 - c : kMoePiece; }
-  __device__ __forceinline__ bool advance() {  // true: a new unit
-    c += kMoePiece;
-    if (c < c1) return false;
-    unit += kMoeWarps;
-    while (unit >= units) { unit -= units; ++group; }
-    enter();
-    return true;
-  }
-};
+// `warps` neighbouring warps wait for each other at barrier `id`: whether all are well.
+__device__ __forceinline__ bool meet(bool ok, int id, int warps) {
+  uint32_t go = ok ? 1u : 0u;
+  asm volatile(
+      "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, %1, %2, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+      : "+r"(go)
+      : "r"(id), "r"(warps * 32)
+      : "memory");
+  return go != 0;
+}
 
 // One phase: every group times its units.  UP: gate / up and the activation from
 // x; else: down from the activations (in PARTS addends), weighted.
@@ -733,7 +689,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
   const uint8_t* codes = UP ? p.up_codes : p.down_codes;
   const uint8_t* scales = UP ? p.up_scales : p.down_scales;
   const int units = UP ? p.I / 16 : p.H / 32, chunks = UP ? p.hc : p.ic;
-  MoeWalk w(s.bound + (UP ? 0 : 2), units, chunks), ahead = w;
+  MoeWalk w(s.bound + (UP ? 0 : 2), units, chunks, warp), ahead = w;
   uint8_t* mine = ring + warp * kMoeStages * R::kStage;
   uint64_t* full = s.full + warp * kMoeStages;
   int64_t at_unit = 0;  // first chunk of the unit that is loaded
@@ -829,13 +785,8 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
 #pragma unroll
             for (int c = 0; c < 4; ++c) mem[((r * NT + n) * 4 + c) * 32 + lane] = acc[r][n][c];
       }
-      uint32_t go = __all_sync(0xffffffffu, ok) ? 1u : 0u;
-      asm volatile(
-          "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n barrier.cta.red.and.aligned.pred b, %1, %2, a;\n selp.u32 %0, 1, 0, b;\n}\n"
-          : "+r"(go)
-          : "r"(1 + warp / share), "r"(share * 32)
-          : "memory");
-      ok = go != 0;
+      w.met = true;
+      ok = meet(__all_sync(0xffffffffu, ok), 1 + warp / share, share);
       if (!ok) return;
       if (part == 0) {
         for (int q = 1; q < share; ++q)
@@ -893,6 +844,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
     if (s.g_count[w.group] <= 8) unit_of(std::integral_constant<int, 1>());
     else unit_of(std::integral_constant<int, 2>());
   }
+  if (!ok && w.owes_meeting()) meet(false, 1 + warp / w.share, w.share);
   if (!ok)  // copies in flight must land before the CTA exits (bounded)
     for (; it < issued; ++it) mbar_wait_bounded(full + it % kMoeStages, it / kMoeStages & 1, kDevErrLoadTimeout);
   return ok;
