@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
 #pragma unroll
           for (int c = 0; c < 4; ++c) o[i][n][c] = 0.0f;
     }
-    if (!mbar_wait_bounded(bar_k, parity, kDevErrLoadTimeout)) { ok = false; break; }
+    if (!mbar_wait_warp(bar_k, parity, kDevErrLoadTimeout)) { ok = false; break; }
     // scores: 4 tiles of 16 tokens; row g (g + 8) of tile i is token 16 (g / 2) + 4 i + g % 2 (+ 2)
     float s[4][NH][4];
 #pragma unroll
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(AttnGeo<D, NH>::kWarps * 32, 1) kv_attention_k
       l[n][0] = fmaf(l[n][0], corr[n][0], sum[0]);
       l[n][1] = fmaf(l[n][1], corr[n][1], sum[1]);
     }
-    if (!mbar_wait_bounded(bar_v, parity, kDevErrLoadTimeout)) { ok = false; break; }
+    if (!mbar_wait_warp(bar_v, parity, kDevErrLoadTimeout)) { ok = false; break; }
     const float v_scale = vs * kProbDown;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {

@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(kLinThreads, CTAS)
     for (LinWork<true> u(p); u.next(); ++lt) {
       const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
       LinOutTokens<BN> out(p, u, kHere ? scale_here : nullptr);
-      if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
+      if (!__all_sync(0xffffffffu, wait(tfull + acc, phase, kDevErrEpilogueTimeout))) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * BN;
       float col = out.column(0);
@@ -1175,7 +1175,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint32_t acc = lt & 1, phase = lt >> 1 & 1;
       u.a = u.a * 2 + rank;  // this CTA's 128 rows
       LinOutRows out(p, u);
-      if (!wait(tfull + acc, phase, kDevErrEpilogueTimeout)) break;
+      if (!__all_sync(0xffffffffu, wait(tfull + acc, phase, kDevErrEpilogueTimeout))) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * (BN - G::kOverlap);
       // the columns shared with the next tile's accumulator come first

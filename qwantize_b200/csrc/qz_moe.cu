@@ -751,7 +751,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
     bool more = true;
     while (more) {
       const int st = it % kMoeStages, pieces = w.piece();
-      if (!mbar_wait_bounded(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
+      if (!mbar_wait_warp(full + st, it / kMoeStages & 1, kDevErrLoadTimeout)) { ok = false; break; }
       const uint8_t* at = mine + st * R::kStage;
 #pragma unroll 1
       for (int k = 0; k < pieces; k += kBuffers) {
@@ -786,7 +786,7 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
             for (int c = 0; c < 4; ++c) mem[((r * NT + n) * 4 + c) * 32 + lane] = acc[r][n][c];
       }
       w.met = true;
-      ok = meet(__all_sync(0xffffffffu, ok), 1 + warp / share, share);
+      ok = meet(ok, 1 + warp / share, share);
       if (!ok) return;
       if (part == 0) {
         for (int q = 1; q < share; ++q)
@@ -800,7 +800,6 @@ __device__ __forceinline__ bool run_phase(const MoeParams& p, MoeShared& s, uint
       asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / share), "r"(share * 32) : "memory");
       if (part > 0) return;
     }
-    ok = __all_sync(0xffffffffu, ok);
     if (!ok) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n)

@@ -75,6 +75,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return true;
 }
 
+// The same for a converged warp: true only if no lane gave up, so that all lanes take
+// the same way past instructions that need the whole warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned err) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err));
+}
+
 // 1-D bulk copy global -> shared, completion counted on `bar` (bytes and both
 // addresses 16-byte aligned; no multicast).
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
