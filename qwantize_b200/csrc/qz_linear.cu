@@ -826,7 +826,8 @@ __global__ void __launch_bounds__(kLinThreads, CTAS)
     if (warp >= 2 && warp < 6) {
       LinWork<true> u(p);
       if (u.next()) {
-        // rank r finishes columns [r, r + 1) * BN / split
+        // rank r finishes columns [r, r + 1) * BN / split, which lie in one group of C
+        static_assert(BN / 2 <= C, "columns of a rank");
         LinOutTokens<BN> out(p, u, kHere ? scale_here : nullptr);
         const int rank = blockIdx.x % p.split, per = BN / p.split;
         const float col = out.column(rank * per / C * C);
@@ -843,8 +844,7 @@ __global__ void __launch_bounds__(kLinThreads, CTAS)
             float v = x[q][0];
 #pragma unroll
             for (int w = 1; w < 4; ++w) v += x[q][w];
-            const float scale = per <= C ? __shfl_sync(0xffffffffu, col, (c0 + q) % C)
-                                         : (c0 + q < c_end ? out.scales[c0 + q] * p.w_scale : 0.0f);
+            const float scale = __shfl_sync(0xffffffffu, col, (c0 + q) % C);
             if (c0 + q < c_end) out.store(c0 + q, v, scale);
           }
         }

@@ -79,7 +79,6 @@ constexpr int kMoeStages = 2;                                                  /
 struct MoeParams {
   int T, H, I, E, top;
   int hc, ic;                       // 64-column chunks of H and I
-  int renorm;
   int dtype;                        // of x and out
   const int* choice;                // (T, top) experts
   const float* choice_weight;       // (T, top)
@@ -973,7 +972,7 @@ extern "C" int qz_moe(const void* x, int dtype, int64_t ldx, int64_t T, int64_t 
   MoeParams p{};
   p.T = (int)T; p.H = (int)H; p.I = (int)I; p.E = (int)E; p.top = (int)top_k;
   p.hc = (int)((H + 63) / 64); p.ic = (int)((I + 63) / 64);
-  p.renorm = renormalize; p.dtype = dtype;
+  p.dtype = dtype;
   if (!ids) ids = reinterpret_cast<int*>(ws + w.choice);
   if (!weights) weights = reinterpret_cast<float*>(ws + w.weight);
   p.choice = ids; p.choice_weight = weights;
