@@ -480,7 +480,8 @@ struct LinOutRows {
     cb = u.b * BN;
     cols = p.N - cb < BN ? (int)(p.N - cb) : BN;
     in = ra < p.T;
-    scale = in ? __ldg(p.row_scale + ra) * p.w_scale : 0.0f;
+    // an ordinary load: the launch before this one may still write them when this one begins
+    scale = in ? p.row_scale[ra] * p.w_scale : 0.0f;
   }
   // C columns from c: scale, bias, round once, store
   __device__ __forceinline__ void finish(int c, float (&v)[C], const CUtensorMap& map_out, unsigned char* smem_out) const {
