@@ -141,6 +141,14 @@ take_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
 give_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
 
 
+def no_gradient(**tensors):
+    """Refuse what a backward pass would be expected of: the serving operators have
+    none, and a result without a gradient function would drop it silently."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            assert t is None or not t.requires_grad, (
+                f"{name} requires a gradient, which this operator does not have: call it under torch.no_grad()")
+
 
 def empty(shape, strides, dtype, device):
     """An uninitialised contiguous tensor: with its strides given, torch takes 1.4

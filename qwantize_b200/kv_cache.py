@@ -4,7 +4,8 @@
 page and head, for keys and values apart.  ``kv_cache_append`` puts new tokens
 in (a prompt's or one per sequence), ``kv_cache_attention`` attends one query
 token per sequence to them, ``kv_cache_read`` gives pages back as numbers.  Block
-tables and lengths are the caller's, device tensors of int32."""
+tables and lengths are the caller's, device tensors of int32.  None has a gradient:
+inputs that require one are refused outside torch.no_grad()."""
 from __future__ import annotations
 
 import ctypes
@@ -121,6 +122,7 @@ def kv_cache_append(cache, k, v, block_table, lengths, cu_new=None, max_new=None
     over to the larger scale, and slots behind the last token become zero.  A
     page must belong to one of the sequences only.  ``lengths`` stays as it is."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
+    L.no_gradient(k=k, v=v)
     tail = (cache.kv_heads, cache.head_dim)
     k, k0, k1 = _rows16(k, "k", tail, cache.device)
     v, v0, v1 = _rows16(v, "v", tail, cache.device)
@@ -172,6 +174,7 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     2^-22 for fp16, at most 2^-40 of the largest beside that).  Softmax and sums are fp32, the result is rounded once
     to q's type."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
+    L.no_gradient(q=q, out=out)
     D, dev = cache.head_dim, cache.device
     assert q.ndim == 3 and q.shape[0] == B, f"q is {tuple(q.shape)}, expected ({B}, heads, {D})"
     Hq = q.shape[1]

@@ -128,10 +128,12 @@ def fp4_linear(x, weight, bias=None, out_dtype=None, out=None):
     rule; NVFP4 rows carry a power of two, so any magnitude fits), products and
     sums run on the block-scaled tensor cores in fp32, and the result is rounded
     once to out_dtype (default: x's).  ``out`` may supply the result's buffer, a
-    contiguous (..., N) tensor."""
+    contiguous (..., N) tensor.  No gradient: inputs that require one are refused
+    outside torch.no_grad()."""
     assert isinstance(weight, FP4Weight), "weight must be an FP4Weight"
     dtype, codes = x.dtype, L.DTYPE_CODES
     assert dtype in codes, f"unsupported dtype {dtype}, expected one of {_DTYPES}"
+    L.no_gradient(x=x, bias=bias, out=out)
     K, N, dev = weight.K, weight.N, weight.device
     assert x.ndim >= 1 and x.shape[-1] == K, f"x has {x.shape[-1] if x.ndim else 0} columns, the weight {K}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the weight on {dev}"

@@ -80,7 +80,8 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     fp32; a token goes to the top_k largest (ties: the lowest index), weighted by
     the softmax over those (renormalize=True) or over all experts.  The
     activations stay in 16 bits, sums in fp32, the result is rounded once to x's
-    type.  With return_routing: (out, ids int32 (..., top_k), weights fp32)."""
+    type.  With return_routing: (out, ids int32 (..., top_k), weights fp32).  No
+    gradient: inputs that require one are refused outside torch.no_grad()."""
     assert isinstance(experts, FP4Experts), "experts must be an FP4Experts"
     dev, H, E = experts.device, experts.H, experts.E
     dtype, codes = x.dtype, L.DTYPE_CODES
@@ -88,6 +89,7 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     assert x.ndim >= 1 and x.shape[-1] == H, f"x has {x.shape[-1] if x.ndim else 0} columns, the experts {H}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the experts on {dev}"
     r = router_weight
+    L.no_gradient(x=x, router_weight=r, out=out)
     assert tuple(r.shape) == (E, H), f"router_weight {tuple(r.shape)}, expected {(E, H)}"
     assert r.dtype in codes, f"unsupported dtype {r.dtype}"
     top_k = int(top_k)

@@ -70,3 +70,23 @@ def test_one_sequence_of_one_head_cut_from_odd_rows():
         q.kv_cache_append(a, x, x, t, n)
         q.kv_cache_append(b, x.clone(), x.clone(), t, n)
         assert a.k.any() and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+
+
+def test_gradients_are_refused_not_dropped():
+    import qwantize_b200 as q
+    up, down, t = make(4, 64, 32, "nvfp4", 46)
+    ex, w = q.FP4Experts(up, down), q.FP4Weight(up[0][0], up[1][0])
+    r, x, b = router_of(4, 64, torch.bfloat16, 47), tokens(2, 64, torch.bfloat16, 48), torch.ones(64, device=DEV)
+    c, _, table, n = setup(2, [5, 6], 1, 64, torch.int8, 49)
+    kv = x.reshape(2, 1, 64)
+    need = lambda v: v.clone().requires_grad_()  # noqa: E731
+    for call in (lambda f: q.fp4_linear(f(x), w), lambda f: q.fp4_linear(x, w, bias=f(b)), lambda f: q.fp4_moe(f(x), r, ex, 2),
+                 lambda f: q.fp4_moe(x, f(r), ex, 2), lambda f: q.kv_cache_attention(c, f(kv), table, n),
+                 lambda f: q.kv_cache_append(c, f(kv), kv, table, n), lambda f: q.kv_cache_append(c, kv, f(kv), table, n)):
+        with pytest.raises(AssertionError, match="no_grad"):
+            call(need)
+        want = call(lambda v: v)
+        with torch.no_grad():
+            got = call(need)
+        assert want is None or torch.equal(want, got)
+        call(lambda v: need(v).detach())
