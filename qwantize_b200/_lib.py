@@ -141,6 +141,21 @@ take_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
 give_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
 
 
+class Bound:
+    """An object that keeps what every call passes on (the library, pointers) beside
+    its tensors: the attributes that ``_bind`` sets.  Copies and pickles carry the
+    tensors and bind themselves again."""
+
+    _bound = ()  # the attributes that _bind sets
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in self._bound}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
+
+
 def no_gradient(**tensors):
     """Refuse what a backward pass would be expected of: the serving operators have
     none, and a result without a gradient function would drop it silently."""

@@ -13,20 +13,23 @@ import ctypes
 import torch
 
 from . import _lib as L
+from .core import cuda_device
 
 PAGE = 64
 _KV = {torch.int8: L.KV_INT8, torch.float8_e4m3fn: L.KV_E4M3}
 _workspace = {}  # (device, D) -> bytes
 
 
-class KVCache8:
+class KVCache8(L.Bound):
     """num_pages pages of 64 tokens for kv_heads heads of head_dim (64 or 128)
     values, in dtype torch.int8 or torch.float8_e4m3fn.
 
     k, v: (num_pages, kv_heads, 64 * head_dim) bytes in the order the kernels
-    read; k_scale, v_scale: (num_pages, kv_heads) fp32."""
+    read; k_scale, v_scale: (num_pages, kv_heads) fp32.  Can be copied, pickled and
+    saved."""
 
     page = PAGE
+    _bound = ("device", "lib", "args")
 
     def __init__(self, num_pages, kv_heads, head_dim, dtype=torch.int8, device="cuda"):
         assert dtype in _KV, f"dtype={dtype}, expected torch.int8 or torch.float8_e4m3fn"
@@ -39,11 +42,16 @@ class KVCache8:
         self.v = torch.zeros_like(self.k)
         self.k_scale = torch.zeros(num_pages, kv_heads, dtype=torch.float32, device=device)
         self.v_scale = torch.zeros_like(self.k_scale)
-        self.device = self.k.device
+        self._bind()
+
+    def _bind(self):
+        self.device = dev = cuda_device(self.k)
+        for name in ("k", "v", "k_scale", "v_scale"):
+            setattr(self, name, getattr(self, name).to(dev))
         self.lib = L.load()
         # the pointers and sizes that every call passes on
-        self.args = (self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), _KV[dtype],
-                     num_pages, kv_heads, head_dim)
+        self.args = (self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), _KV[self.dtype],
+                     self.num_pages, self.kv_heads, self.head_dim)
 
     def load_codes(self, k, k_scale, v, v_scale):
         """Set the whole cache from codes (num_pages, kv_heads, 64, head_dim) of its

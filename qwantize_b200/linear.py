@@ -63,20 +63,22 @@ def quantize_weight(W, fmt, method, X=None):
     return codes, packed, t
 
 
-class FP4Weight:
+class FP4Weight(L.Bound):
     """A weight (N, K) in packed FP4, ready for ``fp4_linear``.
 
     scale_codes, packed: as ``nvfp4_quantize_packed`` / ``mxfp4_quantize_packed``
     return them for W.reshape(N, K / bs, bs) (bs 16 / 32); W stands for
     tensor_scale times their value.  The codes are used where they are when
     their rows are 16-byte aligned, else copied with padded rows; the scales
-    are laid out once, here."""
+    are laid out once, here.  Can be copied, pickled and saved."""
+
+    _bound = ("device", "lib", "fmt_code", "packed_ptr", "scales_ptr", "_workspace")
 
     def __init__(self, scale_codes, packed, fmt="nvfp4", tensor_scale=1.0):
         self.block, self.K, flat = check_packed(scale_codes, packed, fmt)
         assert scale_codes.ndim == 2, "an FP4Weight is one matrix (N, K)"
         self.fmt, self.N, self.tensor_scale = fmt, scale_codes.shape[0], float(tensor_scale)
-        self.device = dev = cuda_device(packed)
+        dev = cuda_device(packed)
         self.scale_codes = scale_codes.to(dev).contiguous()
         p = packed.to(dev).reshape(flat).contiguous()
         self.ldp = (self.K + 31) // 32 * 16
@@ -91,7 +93,12 @@ class FP4Weight:
             self.scales = torch.empty(n.value, dtype=torch.uint8, device=dev)
             L.check(L.load().qz_fp4_scale_layout(L.ptr(self.scale_codes), self.N, self.K, _FMT[fmt], L.ptr(self.scales),
                                                  L.stream_ptr(dev)), "qz_fp4_scale_layout")
-        self.lib, self.fmt_code = L.load(), _FMT[fmt]
+        self._bind()
+
+    def _bind(self):
+        self.device = dev = cuda_device(self.packed)
+        self.scale_codes, self.packed, self.scales = self.scale_codes.to(dev), self.packed.to(dev), self.scales.to(dev)
+        self.lib, self.fmt_code = L.load(), _FMT[self.fmt]
         self.packed_ptr, self.scales_ptr = self.packed.data_ptr(), self.scales.data_ptr()
         self._workspace = {}  # tokens -> bytes
 

@@ -33,16 +33,19 @@ def _lay_out(codes, packed, fmt, gate_up, dev):
     return c, s, norms, E, rows, K
 
 
-class FP4Experts:
+class FP4Experts(L.Bound):
     """The experts of one layer: E gated feed-forward blocks in packed FP4.
 
     gate_up, down: (scale_codes, packed) as ``*_quantize_packed`` return them for
     weights (E, 2 I, H) -- the I gate rows, then the I up rows -- and (E, H, I);
     the weights stand for tensor_scales times their values.  H and I are
-    multiples of 32.  Laid out once, here; the inputs are not kept."""
+    multiples of 32.  Laid out once, here; the inputs are not kept.  Can be copied,
+    pickled and saved."""
+
+    _bound = ("device", "lib", "weight_args", "_workspace")
 
     def __init__(self, gate_up, down, fmt="nvfp4", tensor_scales=(1.0, 1.0)):
-        self.device = dev = cuda_device(gate_up[0])
+        dev = cuda_device(gate_up[0])
         self.up_codes, self.up_scales, self.up_norms, self.E, rows, self.H = _lay_out(*gate_up, fmt, True, dev)
         self.down_codes, self.down_scales, _, E, H, self.I = _lay_out(*down, fmt, False, dev)
         assert (E, H, 2 * self.I) == (self.E, self.H, rows), (
@@ -50,8 +53,14 @@ class FP4Experts:
         assert self.E <= 512, f"{self.E} experts, expected at most 512"
         self.fmt = fmt
         self.tensor_scales = float(tensor_scales[0]), float(tensor_scales[1])
+        self._bind()
+
+    def _bind(self):
+        self.device = dev = cuda_device(self.up_codes)
+        for name in ("up_codes", "up_scales", "up_norms", "down_codes", "down_scales"):
+            setattr(self, name, getattr(self, name).to(dev))
         self.lib = L.load()
-        self.weight_args = (_FMT[fmt], self.up_codes.data_ptr(), self.up_scales.data_ptr(), self.up_norms.data_ptr(),
+        self.weight_args = (_FMT[self.fmt], self.up_codes.data_ptr(), self.up_scales.data_ptr(), self.up_norms.data_ptr(),
                             self.tensor_scales[0], self.down_codes.data_ptr(), self.down_scales.data_ptr(),
                             self.tensor_scales[1])
         self._workspace = {}

@@ -1,4 +1,8 @@
 """Calls of the serving operators at the edges of what they take."""
+import copy
+import io
+import pickle
+
 import pytest
 import torch
 
@@ -90,3 +94,32 @@ def test_gradients_are_refused_not_dropped():
             got = call(need)
         assert want is None or torch.equal(want, got)
         call(lambda v: need(v).detach())
+
+
+def saved(obj, where):
+    f = io.BytesIO()
+    torch.save(obj, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False, map_location=where)
+
+
+@pytest.mark.parametrize("keep", [copy.copy, copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o)), lambda o: saved(o, None), lambda o: saved(o, "cpu")],
+                         ids=["copy", "deepcopy", "pickle", "save", "save to cpu"])
+def test_weights_experts_and_caches_can_be_kept(keep):
+    import qwantize_b200 as q
+    up, down, t = make(4, 64, 32, "nvfp4", 50)
+    r, x = router_of(4, 64, torch.bfloat16, 51), tokens(5, 64, torch.bfloat16, 52)
+    ex, w = q.FP4Experts(up, down, tensor_scales=(t, t)), q.FP4Weight(up[0][1], up[1][1], tensor_scale=t)
+    odd = q.FP4Weight(down[0][0][:, :1], down[1][0][:, :1])  # K = 16: padded rows
+    c, _, table, n = setup(2, [5, 70], 1, 64, torch.float8_e4m3fn, 53)
+    kv = tokens(2, 64, torch.bfloat16, 54).reshape(2, 1, 64)
+    for obj, call in ((w, lambda o: q.fp4_linear(x, o)), (odd, lambda o: q.fp4_linear(x[:, :16], o)), (w, lambda o: o.dequantize()),
+                      (ex, lambda o: q.fp4_moe(x, r, o, 2)), (c, lambda o: q.kv_cache_attention(o, kv, table, n))):
+        want = call(obj)
+        other = keep(obj)
+        assert torch.equal(call(other), want) and torch.equal(call(obj), want)
+    # a copy is its own, but for the shallow one
+    other = keep(c)
+    before = c.k.clone()
+    q.kv_cache_append(other, kv, kv, table, n)
+    assert torch.equal(c.k, before) == (keep is not copy.copy) and not torch.equal(other.k, before)
