@@ -34,6 +34,7 @@ class KVCache8(L.Bound):
     def __init__(self, num_pages, kv_heads, head_dim, dtype=torch.int8, device="cuda"):
         assert dtype in _KV, f"dtype={dtype}, expected torch.int8 or torch.float8_e4m3fn"
         assert head_dim in (64, 128), f"head_dim={head_dim}, expected 64 or 128"
+        assert torch.device(device).type == "cuda", f"device={device}, a cache lives on a CUDA device"
         assert num_pages >= 0 and 1 <= kv_heads <= 1024, "need num_pages >= 0 and 1 to 1024 kv_heads"
         if not torch.cuda.is_available():
             raise RuntimeError("qwantize_b200 needs a CUDA (sm_100a) device; none is available")

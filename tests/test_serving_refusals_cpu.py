@@ -27,3 +27,9 @@ def test_moe_out_off_the_8_bytes_that_are_stored_at_once(off):
 
 def test_moe_norms_off_the_8_bytes_that_are_loaded_at_once():
     refused(moe(un=256 + 4), b"aligned")
+
+
+def test_a_cache_in_host_memory_is_refused():
+    import qwantize_b200 as q
+    with pytest.raises(AssertionError, match="CUDA device"):
+        q.KVCache8(4, 2, 64, device="cpu")
