@@ -312,7 +312,8 @@ QZ_API int qz_fp4_linear(const void* x, int x_dtype, int64_t ldx, int64_t T, int
  * (once per weight; rows and K multiples of 32).  gate_up != 0: rows are the
  * gate rows, then as many up rows.  codes_out: E * rows * up(K, 64) / 2 bytes,
  * scales_out: E * rows * up(K, 64) / bs bytes, both 16-byte aligned.  norms_out
- * (gate_up only): (E, 2) fp32, the largest norms of a gate and of an up row.
+ * (gate_up only): (E, 2) fp32, 8-byte aligned, two factors of a bound of the
+ * product of a gate row's norm and its up row's.
  */
 QZ_API int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, int64_t E, int64_t rows, int64_t K,
                          int format, int gate_up, uint8_t* codes_out, uint8_t* scales_out, float* norms_out,

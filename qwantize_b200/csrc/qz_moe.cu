@@ -47,9 +47,13 @@
 // fp16 operands: a bf16 token is scaled by the power of two that puts its
 // largest magnitude in [2^14, 2^15), exact for values within 2^-28 of it.  An
 // activation row is scaled by a power of two from the bound |silu(g) u| <= |g| |u|
-// <= |x|^2 max|G row| max|U row| (row norms kept with the weights), so it cannot
-// overflow whatever the data, and rounded to 11 bits; for fp16 outputs, whose
-// own rounding is no coarser, the remainder is kept as a second fp16 operand.
+// <= |x|^2 max(|G row| |U row|) over its outputs (kept with the weights), so it cannot
+// overflow whatever the data, and rounded to 11 bits, or to 2^-40 of the bound where
+// that is more; for fp16 outputs, whose own rounding is no coarser, the remainder is
+// kept as a second fp16 operand.  The largest activation of normal data lies near
+// 2^-14 of the bound; where a token's norm comes from a channel that the weights
+// suppress, it lies lower, and the first bit goes at about 2^-26 (a channel 10,000
+// times the others, its weights as much smaller; at 100,000 seven bits are left).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -84,7 +88,7 @@ struct MoeParams {
   const float* choice_weight;       // (T, top)
   const uint8_t *up_codes, *up_scales;      // (E, I / 16 units, hc chunks, 2 tiles) 512 and 8 * 2 * 64 / bs bytes
   const uint8_t *down_codes, *down_scales;  // (E, H / 32 units, ic chunks, 2 tiles)
-  const float* norms;               // (E, 2): largest row norm of gate and of up, without the tensor scale
+  const float* norms;               // (E, 2): factors of the bound of |G row| |U row|, without the tensor scale
   float up_scale, down_scale;       // tensor scales
   const __half* xh;                 // (T, hc, 64) in fragment order
   const int2* xp;                   // (T): power of two of the token, exponent bound of its scaled squared norm
@@ -130,30 +134,48 @@ __global__ void moe_layout_kernel(const uint8_t* __restrict__ packed, const uint
   }
 }
 
-// Largest row norms of the gate and of the up rows, one warp per row.
+// A bound of every output's |G row| |U row|, a warp per pair of rows: the largest sum of
+// the two norms' exponent bounds (the row of one output and the row of another do not
+// meet, so neither do their norms), as whole numbers in the first word of `norms`.
+// Rows of zeros and rows that are not finite count for nothing: their activations are
+// zero, or spoil the token whatever its scale.
 template <int BS>
-__global__ void moe_norm_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales, int64_t E,
-                                int64_t rows, int64_t K, float* __restrict__ norms) {
+__global__ void moe_bound_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales, int64_t E, int64_t rows,
+                                 int64_t K, int* __restrict__ norms) {
   const int lane = threadIdx.x & 31;
-  const int64_t n_warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < E * rows; r += n_warps) {
-    float sum = 0.0f;
-    for (int64_t b = lane; b < K / BS; b += 32) {
-      const uint32_t c = scales[r * (K / BS) + b];
-      const float s = BS == 32 ? (c == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(c == 0 ? 0x00400000u : c << 23))
-                    : c == 127 ? __uint_as_float(0x7fffffffu) : e4m3_value((int)c);
-      float q2 = 0.0f;
-      for (int k = 0; k < BS / 2; ++k) {
-        const float2 v = e2m1x2_to_float2(packed[r * (K / 2) + b * (BS / 2) + k]);
-        q2 += v.x * v.x + v.y * v.y;
+  const int64_t n_warps = (int64_t)gridDim.x * (blockDim.x >> 5), outputs = rows / 2;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < E * outputs; i += n_warps) {
+    int both = 0;
+    bool counts = true;
+    for (int h = 0; h < 2; ++h) {
+      const int64_t r = i / outputs * rows + h * outputs + i % outputs;
+      double sum = 0.0;
+      for (int64_t b = lane; b < K / BS; b += 32) {
+        const uint32_t c = scales[r * (K / BS) + b];
+        const float s = BS == 32 ? (c == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(c == 0 ? 0x00400000u : c << 23))
+                      : c == 127 ? __uint_as_float(0x7fffffffu) : e4m3_value((int)c);
+        float q2 = 0.0f;
+        for (int k = 0; k < BS / 2; ++k) {
+          const float2 v = e2m1x2_to_float2(packed[r * (K / 2) + b * (BS / 2) + k]);
+          q2 += v.x * v.x + v.y * v.y;
+        }
+        sum += (double)q2 * s * s;  // an MXFP4 scale's square does not fit in fp32
       }
-      sum += q2 * s * s;
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0)  // non-negative floats order like their bits, NaN above all
-      atomicMax(reinterpret_cast<unsigned*>(norms) + r / rows * 2 + (r % rows >= rows / 2), __float_as_uint(sqrtf(sum)) & 0x7fffffffu);
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (sum > 0.0 && isfinite(sum)) both += ilogb(sqrt(sum)) + 1;
+      else counts = false;
+    }
+    if (lane == 0 && counts) atomicMax(norms + i / outputs * 2, both);
   }
+}
+// ... as two powers of two whose exponent bounds add up to it.
+__global__ void moe_factors_kernel(float2* norms, int64_t E) {
+  const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= E) return;
+  // below (2^-126)^2 nothing is left of an activation in fp32
+  const int both = min(max(__float_as_int(norms[e].x), -250), 256), half = both >> 1;
+  norms[e] = make_float2(ldexpf(1.0f, half - 1), ldexpf(1.0f, both - half - 1));
 }
 
 // ---------------------------------------------------------------------------
@@ -918,8 +940,9 @@ extern "C" int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, 
   if (E < 1 || E > kMoeMaxExperts || rows <= 0 || rows % 32 || K <= 0 || K % 32)
     return fail(QZ_ERR_INVALID, "need 1 to %d experts, rows and K positive multiples of 32", kMoeMaxExperts);
   if (!scale_codes || !packed || !codes_out || !scales_out || (gate_up && !norms_out)) return fail(QZ_ERR_INVALID, "NULL pointer");
-  if ((reinterpret_cast<uintptr_t>(codes_out) | reinterpret_cast<uintptr_t>(scales_out)) % 16)
-    return fail(QZ_ERR_INVALID, "codes_out and scales_out must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(codes_out) | reinterpret_cast<uintptr_t>(scales_out)) % 16 ||
+      (gate_up && reinterpret_cast<uintptr_t>(norms_out) % 8))
+    return fail(QZ_ERR_INVALID, "codes_out and scales_out must be 16-byte aligned, norms_out 8-byte");
   int sms = 0;
   const int s = current_sms(&sms);
   if (s != QZ_OK) return s;
@@ -929,10 +952,14 @@ extern "C" int qz_moe_layout(const uint8_t* scale_codes, const uint8_t* packed, 
   else moe_layout_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, gate_up, co, scales_out);
   int r = cuda_status(cudaGetLastError(), "moe layout launch");
   if (r != QZ_OK || !gate_up) return r;
-  if ((r = cuda_status(cudaMemsetAsync(norms_out, 0, (size_t)E * 8, st), "cudaMemsetAsync")) != QZ_OK) return r;
-  if (format == QZ_FMT_NVFP4) moe_norm_kernel<16><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms_out);
-  else moe_norm_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms_out);
-  return cuda_status(cudaGetLastError(), "moe norm launch");
+  // 0x80 in every byte: below any bound
+  if ((r = cuda_status(cudaMemsetAsync(norms_out, 0x80, (size_t)E * 8, st), "cudaMemsetAsync")) != QZ_OK) return r;
+  int* norms = reinterpret_cast<int*>(norms_out);
+  if (format == QZ_FMT_NVFP4) moe_bound_kernel<16><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms);
+  else moe_bound_kernel<32><<<sms * 8, 256, 0, st>>>(packed, scale_codes, E, rows, K, norms);
+  if ((r = cuda_status(cudaGetLastError(), "moe bound launch")) != QZ_OK) return r;
+  moe_factors_kernel<<<(unsigned)((E + 127) / 128), 128, 0, st>>>(reinterpret_cast<float2*>(norms_out), E);
+  return cuda_status(cudaGetLastError(), "moe bound launch");
 }
 
 extern "C" int qz_moe_workspace(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k, int64_t* bytes) {
