@@ -163,8 +163,10 @@ __device__ __forceinline__ uint32_t abs_max16(uint32_t m, uint32_t w) {
 // decode step is one such round trip.  Threads own 8 values of a token (keys) or
 // two values of 4 neighbouring slots (values), so that a word of the block has one
 // owner.  Prompts are bound by instructions, 16 per value: 8 of 1900 tokens, 8 heads
-// of 128, E4M3, in 26 us (69% of the issue slots).  64 single tokens: 12.5 us, most
-// of it the chain of reads: length, table, block.
+// of 128, E4M3, in 26 us (69% of the issue slots).  64 single tokens: 12.5 to 13.7 us
+// for 1024 CTAs in 1.4 waves; a warp's 630 instructions, nearly all of them on the
+// page's older codes, take half of the issue slots, and of the stalls half are waits
+// for the reads (length, table, block) and at the CTA's barriers.
 template <int KV, int D, int DT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kStride = 68;  // bytes between value rows in shared memory: words of neighbouring rows in different banks
@@ -933,9 +935,13 @@ static bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 !=
 // Whether each (sequence, head, row tile) pair is given to one CTA, in one launch,
 // instead of cutting all pages evenly and joining in a second one: with at most a
 // CTA per SM, and at most two pages in a row for a warp by the table's width.
-// Microseconds alone / evenly, 8 cache heads of 128, groups of 4, int8: 1 sequence
-// of 300 tokens 8.5 / 12.0, of 1000 12.6 / 12.6, of 2000 16.7 / 14.7, of 8000 41 / 27; 8 of
-// 1000 12.6 / 14.7, 32 of 1000 (256 pairs) 24.5 / 20.8.
+// Microseconds alone / evenly (a call in a graph of 60), 8 cache heads of 128, groups
+// of 4, int8: 1 sequence of 300 tokens 7.4 / 9.5, of 1000 10.6 / 10.6, of 2000 14.4 / 12.4, of
+// 8000 41 / 26; 8 of 1000 11.7 / 13.7, 32 of 1000 (256 pairs) 24.6 / 21.7.  With heads of 64 and
+// 128, groups of 1, 4 and 16, both cache types and 16 batches from 1 x 60 to 32 x 1000 the
+// rule is within 12% of the faster (worst: 1 of 1000, groups of 1: 10.5 / 9.3).  The width
+// stands for the lengths, which the host does not know: in a wide table short
+// sequences pay for the second launch.
 static bool attention_alone(int64_t pairs, int64_t max_pages, int sms, int warps) {
   return pairs <= sms && max_pages <= 2 * warps;
 }
@@ -966,8 +972,8 @@ static int launch_attention(AttnParams p, int sms, cudaStream_t st) {
     kv_attention_kernel<D, KV, NH, true, PARTS><<<(unsigned)pairs, G::kWarps * 32, G::smem(0), st>>>(p);
     return cuda_status(cudaGetLastError(), "kv attention launch");
   }
-  // few pairs have many partial results each: more CTAs share a pair's (1 sequence of 4528 tokens, 128 heads on 8: 47
-  // us with 16 rows per CTA, 22.5 with 4; 32 of 300 tokens, the same heads: 20.8 and 28.8)
+  // few pairs have many partial results each: more CTAs share a pair's (1 sequence of 4528 tokens, 128 heads on 8: 43.4
+  // us with 16 rows per CTA, 19.5 with 4; 16 of 2000: 28.8 and 29.6; 32 of 300: 19.6 and 26.7)
   p.join_rows = pairs <= sms ? 4 : p.rows_per_tile;
   int s = prepare_attention<D, KV, NH, false, PARTS>();
   if (s != QZ_OK) return s;

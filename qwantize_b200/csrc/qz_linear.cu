@@ -20,7 +20,7 @@
 //   the ring once: the bytes of W bound it.  Where the tiles leave SMs idle, a
 //   cluster of 2 or 4 CTAs cuts K among them and adds the fp32 parts, in order,
 //   through distributed shared memory, each CTA finishing its share of the columns.
-//   1 x 2560 x 9728: 9.5 us, 1 x 8192 x 28672: 28 us (132 MB), with the quantization.
+//   1 x 2560 x 9728: 8.1 us, 1 x 8192 x 28672: 27 us (132 MB), with the quantization.
 //
 //   linear_pair_kernel (prompts): a pair of CTAs on 256 tokens x 256 features; the
 //   tensor cores bound it.
@@ -276,7 +276,8 @@ struct LinearParams {
 // single token itself and keeps the codes and scales of all its stages.  CTAS per SM:
 // two where there are more tiles than SMs (16 and 32 tokens; for 64 the ring would
 // be too short): all stream at once instead of in one full wave and one that is not.
-// 4 x 8192 x 28672: 32.5 us with one, 28.4 with two; 4 x 2560 x 19456: 14.2, 10.6.
+// 4 x 8192 x 28672: 29.8 us with one, 27.0 with two; 4 x 2560 x 19456: 14.7, 11.3;
+// 48 x 9728 x 2560: 14.5, 12.3; 17 x 4096 x 4096, the one loss seen: 9.5, 10.0.
 constexpr int kHereStages = 16;
 template <int BN, int BS, bool HERE, int CTAS>
 struct LinGeo {
@@ -872,7 +873,8 @@ __global__ void __launch_bounds__(kLinThreads, CTAS)
 // SMs take about 64 bytes per clock from L2, and that bounded a form of one CTA
 // per tile (945 clocks a stage, 829 us for 8192 x 8192 x 28672).  This one: 610 clocks
 // a stage, 673 us alone (5.7 PFLOP/s, tensor pipe 82% active); in a row the board
-// reaches its power limit and the clock falls, 820 us.
+// reaches its power limit and the clock falls: 770 to 885 us a call, as long as it
+// lasts.
 //
 // 320 threads: warp 0 feeds this CTA's ring; its tiles signal the leader (rank 0),
 // its scales this CTA.  Warps 6-9 put a stage's scales in this CTA's TMEM (its
@@ -1271,17 +1273,22 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Chooses the form by an estimate in microseconds: waves of tiles x stages x time
 // of a stage (1.4 of it where two CTAs share an SM), what follows the last stage,
-// and a cluster's exchange of sums.  The times were fitted to measurements of every
-// form at 1 .. 2048 tokens and (K, N) = (1024, 1024), (2560, 9728), (9728, 2560),
-// (4096, 4096), (2560, 19456) and (8192, 28672); the choice is the fastest or within
-// 10% of it in all.  Some, in microseconds with the quantization: 2560 x 9728, 64
-// tokens: 32 columns (two CTAs per SM) 12.5, 64 13.2, 16 14.5, pair 14.5; 192 tokens:
-// 16.8, 18.9, pair 14.8.  9728 x 2560, 1 token: clusters of 4, 2, 1: 12.7, 14.8, 18.9;
-// 64 tokens, clusters of 4: 32 columns (two CTAs per SM) 14.8, 64 columns 16.8; 16
-// alone 20.9.  Clusters of 8 gained 10% or lost 30%, as they found room on the GPU
-// (8192 x 2048, 17 tokens: 10.6 against 12.5 with 4; 32 tokens: 16.8 against 12.5).
-// 8192 x 28672, 64 tokens: 64 columns 35.2, 32 43.4, pair 37.2.  128 columns were never the fastest by
-// more than 8% (2560 x 9728, 2048 tokens: 84.4, pair 36.2) and are not built.
+// and a cluster's exchange of sums.  Checked against every form that can run, at 16
+// numbers of tokens from 1 to 2048 and (K, N) = (1024, 1024), (2560, 9728), (9728, 2560),
+// (4096, 4096), (2560, 1000), (8192, 1024), (2560, 19456), (8192, 2048) and (8192, 28672),
+// MXFP4 at the first three (per call in a graph of 100, over weights that exceed L2
+// together; repeats agree within 0.1 us): the choice is the fastest or within 10% of
+// it in 179 of 189.  The others: 64 tokens of 1024 x 1024 (10.3%), and 333 to 1024 tokens
+// of weights with about 1000 features and K up to 2560, which the limit of eight
+// passes over W keeps from the narrow forms (1024 x 1024, 333 tokens: 9.8 us, 16
+// columns 7.8; 2560 x 1000: 13.2, 10.8).
+// Some, in microseconds with the quantization: 2560 x 9728, 64 tokens: 32 columns (two
+// CTAs per SM) 11.1, 64 13.0, 16 14.0, pair 13.0; 192 tokens: 15.7, 17.5, 21.8, pair 13.3.
+// 9728 x 2560, 1 token: clusters of 4, 2, 1: 9.9, 13.0, 17.8; 64 tokens, clusters of 4: 32
+// columns (two CTAs per SM) 12.6, 64 columns 13.6; 16 alone 18.2.  8192 x 28672, 64
+// tokens: 64 columns 33.4, 32 42.1, pair 35.3.  Not built: clusters of 8, which gained 10%
+// or lost 30% as they found room on the GPU (8192 x 2048, 17 and 32 tokens), and 128
+// columns, never the fastest by more than 8% (both from a timer with steps of 2 us).
 struct LinForm {
   int bn;               // tokens of a tile (256: the pair form)
   double stage, last, join;
@@ -1310,9 +1317,10 @@ static LinPlan plan_linear(int64_t T, int64_t K, int64_t N, int bs, int sms) {
     }
   }
   best.n_steps = n_steps;
-  // a single token, quantized by every CTA for itself: no first launch.  On the device 8.6 us instead of 10.6
-  // (MXFP4) and 10.6 instead of 10.6 (NVFP4) at 2560 x 9728, and a launch less for the host; with 2 tokens 10.6 and
-  // 11.6 instead of 10.6, with 8 12.9 and 20.9, in a form for several.
+  // a single token, quantized by every CTA for itself: no first launch.  On the device 8.1 us instead of 10.3
+  // (NVFP4) and 7.8 instead of 9.7 (MXFP4) at 2560 x 9728, 9.9 instead of 10.7 at 9728 x 2560, 5.9 instead of 6.9 at
+  // 2560 x 1000, and a launch less for the host.  A form of it for several tokens gained nothing from 2 on, and took 13
+  // (MXFP4) and 21 us (NVFP4) for 8, where two launches take 10.3.
   best.here = best.bn == 16 && T == 1 && !best.two && (n_steps + best.split - 1) / best.split <= kHereStages;
   best.ldp = up(K, 32) / 2;
   best.gran = best.bn < 128 ? best.bn : 128;
