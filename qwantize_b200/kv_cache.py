@@ -80,7 +80,7 @@ def _index(t, name, dev, ndim):
     assert t.ndim == ndim and (t.dtype == torch.int32 or t.dtype == torch.int64), f"{name} must be a {ndim}-d int32 tensor"
     assert t.device == dev, f"{name} is on {t.device}, the cache on {dev}"
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        t = t.clamp(-(2**31), 2**31 - 1).to(torch.int32)  # beyond 32 bits: still beyond the cache
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 

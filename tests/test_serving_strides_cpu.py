@@ -31,3 +31,11 @@ def test_what_is_aligned_is_not_copied():
     buf = torch.zeros(4, 12, 64, dtype=torch.float16)
     for x in (buf, buf[:, 2:10], buf[1:2, 3:4], buf[::2]):
         assert rows(x).data_ptr() == x.data_ptr()
+
+
+@pytest.mark.parametrize("value,kept", [(2**31 - 1, 2**31 - 1), (2**31, 2**31 - 1), (2**32, 2**31 - 1), (2**63 - 1, 2**31 - 1), (-1, -1), (-(2**31) - 1, -(2**31)),
+                                        (-(2**40), -(2**31)), (7, 7)])
+def test_indices_of_64_bits_do_not_wrap(value, kept):
+    """A length that stands for "all", or a page that no cache has, stays what it is."""
+    t = kv_cache._index(torch.tensor([value, 3]), "lengths", CPU, 1)
+    assert t.dtype == torch.int32 and t.tolist() == [kept, 3]
