@@ -289,7 +289,8 @@ QZ_API int qz_fp4_scale_layout(const uint8_t* scale_codes, int64_t N, int64_t K,
  * counterpart in the reference, whose quantized weights are only dequantized.
  *   x            rows ldx elements apart, 16-byte aligned.  A row is quantized
  *                by the naive rule of qz_quantize; for NVFP4 after division by
- *                the smallest power of two p with max|row| <= 448 * 6 * p.
+ *                the smallest power of two p with max|row| <= 448 * 6 * p (at
+ *                least 2^-120: a row below 2^-110 or so keeps fewer bits).
  *   packed       N rows of up(K, 32) / 2 bytes, ldp bytes apart (a multiple of
  *                16; codes beyond K zero); element 2i in the low nibble
  *   scales       from qz_fp4_scale_layout

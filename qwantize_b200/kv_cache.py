@@ -4,7 +4,8 @@
 page and head, for keys and values apart.  ``kv_cache_append`` puts new tokens
 in (a prompt's or one per sequence), ``kv_cache_attention`` attends one query
 token per sequence to them, ``kv_cache_read`` gives pages back as numbers.  Block
-tables and lengths are the caller's, device tensors of int32.  None has a gradient:
+tables and lengths are the caller's, device tensors of int32 (int64 is converted on
+each call, two small kernels a tensor).  None has a gradient:
 inputs that require one are refused outside torch.no_grad()."""
 from __future__ import annotations
 
