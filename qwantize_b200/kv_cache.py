@@ -112,12 +112,14 @@ def _rows16(x, name, shape_tail, dev):
     assert x.ndim == 3 and x.shape[1:] == shape_tail, f"{name} is {tuple(x.shape)}, expected (n, {shape_tail[0]}, {shape_tail[1]})"
     assert x.dtype == torch.bfloat16 or x.dtype == torch.float16, f"unsupported dtype {x.dtype}, expected bfloat16 or float16"
     assert x.device == dev, f"{name} is on {x.device}, the cache on {dev}"
-    s0, s1, s2 = _strides(x)
+    s0, s1, s2 = x.stride()
     if s2 != 1 or s1 % 8 or s0 % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-        s0, s1, _ = _strides(x)
+        s0, s1, s2 = _strides(x)
+        if s2 != 1 or s1 % 8 or s0 % 8 or x.data_ptr() % 16:
+            x = x.contiguous()
+            if x.data_ptr() % 16:
+                x = x.clone()
+            s0, s1, _ = _strides(x)
     return x, s0, s1
 
 
@@ -132,7 +134,8 @@ def kv_cache_append(cache, k, v, block_table, lengths, cu_new=None, max_new=None
     over to the larger scale, and slots behind the last token become zero.  A
     page must belong to one of the sequences only.  ``lengths`` stays as it is."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
-    L.no_gradient(k=k, v=v)
+    if k.requires_grad or v.requires_grad:
+        L.no_gradient(k=k, v=v)
     tail = (cache.kv_heads, cache.head_dim)
     k, k0, k1 = _rows16(k, "k", tail, cache.device)
     v, v0, v1 = _rows16(v, "v", tail, cache.device)
@@ -184,7 +187,8 @@ def kv_cache_attention(cache, q, block_table, lengths, scale=None, out=None):
     2^-22 for fp16, at most 2^-40 of the largest beside that).  Softmax and sums are fp32, the result is rounded once
     to q's type."""
     table, lengths, B, pages, ld = _table(block_table, lengths, cache)
-    L.no_gradient(q=q, out=out)
+    if q.requires_grad or (out is not None and out.requires_grad):
+        L.no_gradient(q=q, out=out)
     D, dev = cache.head_dim, cache.device
     assert q.ndim == 3 and q.shape[0] == B, f"q is {tuple(q.shape)}, expected ({B}, heads, {D})"
     Hq = q.shape[1]

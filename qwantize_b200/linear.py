@@ -140,7 +140,8 @@ def fp4_linear(x, weight, bias=None, out_dtype=None, out=None):
     assert isinstance(weight, FP4Weight), "weight must be an FP4Weight"
     dtype, codes = x.dtype, L.DTYPE_CODES
     assert dtype in codes, f"unsupported dtype {dtype}, expected one of {_DTYPES}"
-    L.no_gradient(x=x, bias=bias, out=out)
+    if x.requires_grad or (bias is not None and bias.requires_grad) or (out is not None and out.requires_grad):
+        L.no_gradient(x=x, bias=bias, out=out)
     K, N, dev = weight.K, weight.N, weight.device
     assert x.ndim >= 1 and x.shape[-1] == K, f"x has {x.shape[-1] if x.ndim else 0} columns, the weight {K}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the weight on {dev}"

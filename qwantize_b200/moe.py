@@ -98,7 +98,8 @@ def fp4_moe(x, router_weight, experts, top_k, renormalize=True, return_routing=F
     assert x.ndim >= 1 and x.shape[-1] == H, f"x has {x.shape[-1] if x.ndim else 0} columns, the experts {H}"
     assert x.device == dev or x.device.type == "cpu", f"x is on {x.device}, the experts on {dev}"
     r = router_weight
-    L.no_gradient(x=x, router_weight=r, out=out)
+    if x.requires_grad or r.requires_grad or (out is not None and out.requires_grad):
+        L.no_gradient(x=x, router_weight=r, out=out)
     assert tuple(r.shape) == (E, H), f"router_weight {tuple(r.shape)}, expected {(E, H)}"
     assert r.dtype in codes, f"unsupported dtype {r.dtype}"
     top_k = int(top_k)
